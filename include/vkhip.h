@@ -551,6 +551,43 @@ vkh_status vkh_fa_backward_from_o(const vkh_attn_params *p, const void *q, const
                                   const float *lse, float *d, float *dq, float *dk, float *dv,
                                   void *workspace, vkh_stream stream);
 
+/* Attention with a sliding window and a few first keys that stay visible, any number of queries
+ * up to the keys (one: the next token against a cache), padded batches.  The reference has the
+ * unlimited causal form only.
+ *
+ * Sequence b has kv_len[b] keys and q_len[b] query rows (device arrays [n_batch], values beyond
+ * n_kv and n_q taken as those; NULL: all n_kv, all n_q).  Its query row r is at position
+ * t = r + kv_len[b] - q_len[b], the last one at the last key, and sees key j where j <= t and
+ * (j > t - window or j < n_sink).  Pairs that are not seen take no part, whatever their rows
+ * hold.  Rows that see no key (r >= q_len[b], or t < 0) get O = 0, LSE = -inf and no gradient;
+ * keys from kv_len[b] on get gradients of 0. */
+typedef struct vkh_window_params {
+    uint32_t n_batch;    /* 0 means 1 */
+    uint32_t n_q, n_kv;  /* rows per sequence, n_q <= n_kv */
+    uint32_t n_heads, n_kv_heads, head_dim; /* head_dim up to 256; 64 and 128 on aligned rows are the fast form */
+    uint32_t window;     /* keys up to and with the query's own; 0: no limit */
+    uint32_t n_sink;
+    float inv_sqrt_dim;
+    uint32_t dtype;      /* vkh_dtype of q, k, v, dO */
+    uint32_t out_dtype;  /* of O, dQ, dK, dV: dtype or VKH_F32 */
+    uint32_t ld_q, ld_k, ld_v, ld_o, ld_do, ld_dq, ld_dk, ld_dv; /* row strides in elements; 0: dense */
+} vkh_window_params;
+/* O, and LSE [rows, n_heads] fp32 if non-NULL.  `workspace` (16-byte aligned, may be NULL) holds
+ * vkh_fa_window_forward_workspace_bytes(p) bytes: the partial results of calls whose few queries
+ * have their keys split between blocks.  Without it the call takes the library's per-stream
+ * scratch, and where that is not to be had (a stream under capture) runs unsplit. */
+size_t vkh_fa_window_forward_workspace_bytes(const vkh_window_params *p);
+vkh_status vkh_fa_window_forward(const vkh_window_params *p, const void *q, const void *k,
+                                 const void *v, void *o, float *lse, const uint32_t *q_len,
+                                 const uint32_t *kv_len, void *workspace, vkh_stream stream);
+/* dQ, dK, dV (overwrite) from the forward's O and LSE; d [rows, n_heads] fp32 receives
+ * D = rowsum(O dO).  Workspace as above. */
+size_t vkh_fa_window_backward_workspace_bytes(const vkh_window_params *p);
+vkh_status vkh_fa_window_backward(const vkh_window_params *p, const void *q, const void *k,
+                                  const void *v, const void *o, const void *dout, const float *lse,
+                                  float *d, void *dq, void *dk, void *dv, const uint32_t *q_len,
+                                  const uint32_t *kv_len, void *workspace, vkh_stream stream);
+
 /* shaders/matmul_nt_v2.comp (MatmulPush {m, n, k}): y[M,N] = x[M,K] w[N,K]^T. */
 vkh_status vkh_matmul_nt(const float *x, const float *w, float *y, uint32_t M, uint32_t N,
                          uint32_t K, uint32_t precision, vkh_stream stream);
@@ -697,6 +734,86 @@ vkh_status vkh_qk_rope_forward(const vkh_rope_params *p, const float *q_in, floa
                                const float *k_in, float *k_out, vkh_stream stream);
 vkh_status vkh_qk_rope_backward(const vkh_rope_params *p, const float *dq_out, float *dq_in,
                                 const float *dk_out, float *dk_in, vkh_stream stream);
+/* Rotary positions in the forms that the calls above do not take: neighbouring pairs,
+ * positions of the caller's, frequencies scaled for contexts longer than they were made for,
+ * bf16 rows and row strides.  The reference has the half layout, row positions and plain
+ * frequencies only (qk_rope_partial_batched.comp).
+ *
+ * Pair i of the rotary_dim / 2 pairs of a head is turned by position * f_i radians:
+ *   UNSCALED  f_i = theta^(-2 i / rotary_dim)
+ *   LINEAR    f_i / factor
+ *   NTK       theta' = theta * factor^(rotary_dim / (rotary_dim - 2)) in theta's place
+ *   YARN      f_i (1 - u) + (f_i / factor) u with u = clamp((i - lo) / (hi - lo), 0, 1), lo and hi
+ *             the pairs (rounded down and up, kept in [0, rotary_dim - 1]) that make beta_fast and
+ *             beta_slow turns in orig_len positions; attn_factor defaults to 0.1 ln(factor) + 1
+ *   BANDS     the same blend with 1 - u = clamp((n_i - low_freq) / (high_freq - low_freq), 0, 1),
+ *             n_i = orig_len f_i / (2 pi) the pair's turns in orig_len positions
+ * and the turned values are multiplied by attn_factor. */
+typedef enum vkh_rotary_layout {
+    VKH_ROTARY_HALF = 0,       /* pairs (i, i + rotary_dim / 2) */
+    VKH_ROTARY_INTERLEAVED = 1 /* pairs (2 i, 2 i + 1) */
+} vkh_rotary_layout;
+typedef enum vkh_rotary_scaling {
+    VKH_ROTARY_UNSCALED = 0, VKH_ROTARY_LINEAR = 1, VKH_ROTARY_NTK = 2, VKH_ROTARY_YARN = 3,
+    VKH_ROTARY_BANDS = 4
+} vkh_rotary_scaling;
+typedef struct vkh_rotary_spec {
+    uint32_t rotary_dim; /* even, at most 256; 0: nothing is turned */
+    uint32_t layout, scaling;
+    uint32_t orig_len;          /* YARN (over 2 pi beta_fast), BANDS */
+    float theta;                /* over 1 */
+    float factor;               /* over 0; all but UNSCALED */
+    float beta_fast, beta_slow; /* YARN: 0 means 32 and 1 */
+    float low_freq, high_freq;  /* BANDS: 0 means 1 and 4 */
+    float attn_factor;          /* 0: the scaling's own (1 but for YARN) */
+} vkh_rotary_spec;
+#define VKH_ROTARY_MAX_PAIRS 128
+/* A plan is plain data of the caller's (one of its own making serves as well); the calls copy it. */
+typedef struct vkh_rotary_plan {
+    uint32_t rotary_dim, layout;
+    float attn_factor;
+    uint32_t reserved;
+    double turns[VKH_ROTARY_MAX_PAIRS]; /* f_i / (2 pi) */
+} vkh_rotary_plan;
+/* Host only. */
+vkh_status vkh_rotary_plan_init(const vkh_rotary_spec *spec, vkh_rotary_plan *out);
+
+/* Query and key head rows of one call, x -> y forward, dy -> dx backward.  Row strides are in
+ * elements, 0 for dense rows.  y may be x, and dx may be dy or x, where type and stride are the
+ * same.  n_q_heads or n_kv_heads may be 0, its pointers NULL.  head_dim up to 256; rows and
+ * pointers aligned to 16 bytes with head_dim and rotary_dim multiples of 16 are the fast form. */
+typedef struct vkh_rotary_params {
+    uint32_t n_rows, n_q_heads, n_kv_heads, head_dim;
+    uint32_t seq_len, pos0; /* without positions: row r is at pos0 + r % seq_len (0: n_rows) */
+    float eps;              /* of the norm */
+    uint32_t gemma_quirk;   /* of the norm: gains are 1 + w */
+    uint32_t x_dtype, y_dtype, dy_dtype, dx_dtype; /* vkh_dtype */
+    uint32_t ld_xq, ld_xk, ld_yq, ld_yk, ld_dyq, ld_dyk, ld_dxq, ld_dxk;
+} vkh_rotary_params;
+/* positions [n_rows] on the device, or NULL.  The backward turns dy back: dx = attn_factor R^T dy. */
+vkh_status vkh_rotary_forward(const vkh_rotary_params *p, const vkh_rotary_plan *plan,
+                              const uint32_t *positions, const void *q_in, void *q_out,
+                              const void *k_in, void *k_out, vkh_stream stream);
+vkh_status vkh_rotary_backward(const vkh_rotary_params *p, const vkh_rotary_plan *plan,
+                               const uint32_t *positions, const void *dq_out, void *dq_in,
+                               const void *dk_out, void *dk_in, vkh_stream stream);
+/* RMSNorm of each query and key head (gains wq, wk [head_dim] fp32) and the rotation in one
+ * pass: rmsnorm.comp over the heads, then qk_rope_partial_batched.comp, of which
+ * vkh_qkv_project* has the form behind its projection. */
+vkh_status vkh_qk_norm_rotary_forward(const vkh_rotary_params *p, const vkh_rotary_plan *plan,
+                                      const uint32_t *positions, const float *wq, const float *wk,
+                                      const void *q_in, void *q_out, const void *k_in, void *k_out,
+                                      vkh_stream stream);
+/* Its backward from the same inputs: dq_in, dk_in, and dwq, dwk [head_dim] fp32 (overwrite, summed
+ * in a fixed order; either may be NULL).  `workspace` (16-byte aligned) holds
+ * vkh_qk_norm_rotary_workspace_bytes(p) bytes; NULL takes the library's per-stream scratch, which a
+ * call with gain gradients on a stream under capture may not (VKH_ERR_INVALID_ARGUMENT). */
+size_t vkh_qk_norm_rotary_workspace_bytes(const vkh_rotary_params *p);
+vkh_status vkh_qk_norm_rotary_backward(const vkh_rotary_params *p, const vkh_rotary_plan *plan,
+                                       const uint32_t *positions, const float *wq, const float *wk,
+                                       const void *q_in, const void *k_in, const void *dq_out,
+                                       const void *dk_out, void *dq_in, void *dk_in, float *dwq,
+                                       float *dwk, void *workspace, vkh_stream stream);
 /* The bf16 step's q|k|v projection and attention operand: y[n_pos, (Hq + 2 Hkv) hd]
  * = x[n_pos, K] w^T (bf16 operands, fp32 y: the backward's pre-norm values) and
  * out = bf16 of the q and k heads Q/K-RMSNorm'd (qk_norm, gains wq / wk, eps) and

@@ -105,6 +105,35 @@ class RopeParams(C.Structure):
                 ("seq_len", C.c_uint32)]
 
 
+class RotarySpec(C.Structure):
+    _fields_ = [("rotary_dim", C.c_uint32), ("layout", C.c_uint32), ("scaling", C.c_uint32),
+                ("orig_len", C.c_uint32), ("theta", C.c_float), ("factor", C.c_float),
+                ("beta_fast", C.c_float), ("beta_slow", C.c_float), ("low_freq", C.c_float),
+                ("high_freq", C.c_float), ("attn_factor", C.c_float)]
+
+
+class RotaryPlan(C.Structure):
+    _fields_ = [("rotary_dim", C.c_uint32), ("layout", C.c_uint32), ("attn_factor", C.c_float),
+                ("reserved", C.c_uint32), ("turns", C.c_double * 128)]
+
+
+class RotaryParams(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("n_rows", "n_q_heads", "n_kv_heads", "head_dim", "seq_len",
+                                          "pos0")]
+    _fields_ += [("eps", C.c_float)]
+    _fields_ += [(n, C.c_uint32) for n in ("gemma_quirk", "x_dtype", "y_dtype", "dy_dtype", "dx_dtype",
+                                           "ld_xq", "ld_xk", "ld_yq", "ld_yk", "ld_dyq", "ld_dyk",
+                                           "ld_dxq", "ld_dxk")]
+
+
+class WindowParams(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("n_batch", "n_q", "n_kv", "n_heads", "n_kv_heads",
+                                          "head_dim", "window", "n_sink")]
+    _fields_ += [("inv_sqrt_dim", C.c_float)]
+    _fields_ += [(n, C.c_uint32) for n in ("dtype", "out_dtype", "ld_q", "ld_k", "ld_v", "ld_o",
+                                           "ld_do", "ld_dq", "ld_dk", "ld_dv")]
+
+
 class TrainBudget(C.Structure):
     _fields_ = [("mode", C.c_uint32), ("steps", C.c_uint32), ("microseconds", C.c_uint64)]
 
@@ -239,6 +268,16 @@ SIGNATURES = [
     ("vkh_swiglu_backward", ST, [P, P, P, P, P, SZ, P]),
     ("vkh_qk_rope_forward", ST, [C.POINTER(RopeParams), P, P, P, P, P]),
     ("vkh_qk_rope_backward", ST, [C.POINTER(RopeParams), P, P, P, P, P]),
+    ("vkh_rotary_plan_init", ST, [C.POINTER(RotarySpec), C.POINTER(RotaryPlan)]),
+    ("vkh_rotary_forward", ST, [C.POINTER(RotaryParams), C.POINTER(RotaryPlan), P, P, P, P, P, P]),
+    ("vkh_rotary_backward", ST, [C.POINTER(RotaryParams), C.POINTER(RotaryPlan), P, P, P, P, P, P]),
+    ("vkh_qk_norm_rotary_forward", ST, [C.POINTER(RotaryParams), C.POINTER(RotaryPlan), P, P, P, P, P, P, P, P]),
+    ("vkh_qk_norm_rotary_workspace_bytes", SZ, [C.POINTER(RotaryParams)]),
+    ("vkh_qk_norm_rotary_backward", ST, [C.POINTER(RotaryParams), C.POINTER(RotaryPlan), P, P, P, P, P, P, P, P, P, P, P, P, P]),
+    ("vkh_fa_window_forward_workspace_bytes", SZ, [C.POINTER(WindowParams)]),
+    ("vkh_fa_window_forward", ST, [C.POINTER(WindowParams), P, P, P, P, P, P, P, P, P]),
+    ("vkh_fa_window_backward_workspace_bytes", SZ, [C.POINTER(WindowParams)]),
+    ("vkh_fa_window_backward", ST, [C.POINTER(WindowParams), P, P, P, P, P, P, P, P, P, P, P, P, P, P]),
     ("vkh_embed_lookup", ST, [P, P, P, U32, U32, F, P]),
     ("vkh_embedding_backward", ST, [P, P, P, U32, U32, U32, P]),
     ("vkh_adam_step", ST, [P, P, P, P, SZ, F, F, F, F, U32, F, P]),

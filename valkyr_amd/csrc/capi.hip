@@ -8,11 +8,13 @@
 
 #include <algorithm>
 #include <atomic>
+#include <initializer_list>
 #include <iterator>
 #include <map>
 #include <memory>
 #include <mutex>
 #include <tuple>
+#include <utility>
 #include <vector>
 
 #include "internal.hpp"
@@ -486,6 +488,98 @@ static bool capturing(hipStream_t st) {
         return true;
     }
     return cs != hipStreamCaptureStatusNone;
+}
+
+// ── windowed attention ─────────────────────────────────────────────────
+
+static vkh_status window_args(const vkh_window_params *p, WindowArgs &a) {
+    CHECK_ARG(p, "null params");
+    CHECK_ARG(p->n_heads && p->n_kv_heads && p->head_dim && p->n_q && p->n_kv, "zero attention dimension");
+    CHECK_ARG(p->n_heads % p->n_kv_heads == 0, "n_heads % n_kv_heads != 0");
+    CHECK_ARG(p->n_q <= p->n_kv, "windowed attention needs n_q <= n_kv");
+    CHECK_ARG(p->dtype <= VKH_BF16 && (p->out_dtype == p->dtype || p->out_dtype == VKH_F32), "dtype");
+    if (p->head_dim > 256) return fail(VKH_ERR_UNSUPPORTED, "head_dim > 256");
+    const uint64_t nb = p->n_batch ? p->n_batch : 1, lim = 1ull << 31;
+    if (p->n_kv >= (1u << 30) || p->n_heads >= (1u << 16) || nb >= lim || nb * p->n_q >= lim || nb * p->n_kv >= lim ||
+        nb * p->n_q * p->n_heads >= lim || nb * p->n_kv * p->n_kv_heads >= lim)
+        return fail(VKH_ERR_UNSUPPORTED, "2^31 or more head rows");
+    const uint32_t qd = p->n_heads * p->head_dim, kd = p->n_kv_heads * p->head_dim;
+    auto ld = [](uint32_t l, uint32_t dense) { return (long)(l ? l : dense); };
+    a = WindowArgs{};
+    a.n_batch = (int)nb; a.n_q = (int)p->n_q; a.n_kv = (int)p->n_kv;
+    a.n_heads = (int)p->n_heads; a.n_kv_heads = (int)p->n_kv_heads; a.hd = (int)p->head_dim;
+    a.window = (int)(p->window ? std::min(p->window, p->n_kv) : p->n_kv);
+    a.n_sink = (int)std::min(p->n_sink, p->n_kv);
+    a.scale = p->inv_sqrt_dim;
+    a.dt = p->dtype == VKH_BF16 ? DType::BF16 : DType::F32;
+    a.odt = p->out_dtype == VKH_BF16 ? DType::BF16 : DType::F32;
+    a.ldq = ld(p->ld_q, qd); a.ldo = ld(p->ld_o, qd); a.lddo = ld(p->ld_do, qd); a.lddq = ld(p->ld_dq, qd);
+    a.ldk = ld(p->ld_k, kd); a.ldv = ld(p->ld_v, kd); a.lddk = ld(p->ld_dk, kd); a.lddv = ld(p->ld_dv, kd);
+    CHECK_ARG(std::min({a.ldq, a.ldo, a.lddo, a.lddq}) >= (long)qd && std::min({a.ldk, a.ldv, a.lddk, a.lddv}) >= (long)kd,
+              "a row stride is less than its heads");
+    return VKH_OK;
+}
+static bool aligned_to(const void *x, DType t) { return (uintptr_t)x % (t == DType::F32 ? 4 : 2) == 0; }
+
+// The caller's workspace, else the stream's scratch; none (ws = null) under capture or where
+// there is no memory for it.
+static vkh_status optional_ws(void *workspace, size_t bytes, ScratchLease &lease, hipStream_t st, float **ws) {
+    *ws = nullptr;
+    if (!bytes) return VKH_OK;
+    CHECK_ARG((uintptr_t)workspace % 16 == 0, "the workspace is not 16-byte aligned");
+    void *w = workspace;
+    if (!w && !capturing(st)) {
+        const vkh_status got = lease.acquire(bytes, st, &w);
+        if (got == VKH_ERR_OUT_OF_MEMORY) w = nullptr;
+        else VKH_TRY(got);
+    }
+    *ws = (float *)w;
+    return VKH_OK;
+}
+
+size_t vkh_fa_window_forward_workspace_bytes(const vkh_window_params *p) {
+    WindowArgs a;
+    return window_args(p, a) == VKH_OK ? window_fwd_ws_bytes(a) : 0;
+}
+
+vkh_status vkh_fa_window_forward(const vkh_window_params *p, const void *q, const void *k,
+                                 const void *v, void *o, float *lse, const uint32_t *q_len,
+                                 const uint32_t *kv_len, void *workspace, vkh_stream stream) {
+    WindowArgs a;
+    VKH_TRY(window_args(p, a));
+    CHECK_ARG(q && k && v && o, "null pointer");
+    CHECK_ARG(aligned_to(q, a.dt) && aligned_to(k, a.dt) && aligned_to(v, a.dt) && aligned_to(o, a.odt) &&
+                  aligned_to(lse, DType::F32),
+              "a pointer is not aligned to its type");
+    a.q = q; a.k = k; a.v = v; a.o = o; a.lse = lse; a.q_len = q_len; a.kv_len = kv_len;
+    ScratchLease lease;
+    VKH_TRY(optional_ws(workspace, window_fwd_ws_bytes(a), lease, S(stream), &a.ws));
+    VKH_HIP(window_forward(a, S(stream)));
+    return VKH_OK;
+}
+
+size_t vkh_fa_window_backward_workspace_bytes(const vkh_window_params *p) {
+    WindowArgs a;
+    return window_args(p, a) == VKH_OK ? window_bwd_ws_bytes(a) : 0;
+}
+
+vkh_status vkh_fa_window_backward(const vkh_window_params *p, const void *q, const void *k,
+                                  const void *v, const void *o, const void *dout, const float *lse,
+                                  float *d, void *dq, void *dk, void *dv, const uint32_t *q_len,
+                                  const uint32_t *kv_len, void *workspace, vkh_stream stream) {
+    WindowArgs a;
+    VKH_TRY(window_args(p, a));
+    CHECK_ARG(q && k && v && o && dout && lse && d && dq && dk && dv, "null pointer");
+    CHECK_ARG(aligned_to(q, a.dt) && aligned_to(k, a.dt) && aligned_to(v, a.dt) && aligned_to(dout, a.dt) &&
+                  aligned_to(o, a.odt) && aligned_to(dq, a.odt) && aligned_to(dk, a.odt) && aligned_to(dv, a.odt) &&
+                  aligned_to(lse, DType::F32) && aligned_to(d, DType::F32),
+              "a pointer is not aligned to its type");
+    a.q = q; a.k = k; a.v = v; a.o = (void *)o; a.dout = dout; a.lse = (float *)lse; a.d = d;
+    a.dq = dq; a.dk = dk; a.dv = dv; a.q_len = q_len; a.kv_len = kv_len;
+    ScratchLease lease;
+    VKH_TRY(optional_ws(workspace, window_bwd_ws_bytes(a), lease, S(stream), &a.ws));
+    VKH_HIP(window_backward(a, S(stream)));
+    return VKH_OK;
 }
 
 // One contraction of a linear layer.  Operands that need a packed copy (fp32
@@ -1028,6 +1122,173 @@ vkh_status vkh_qk_rope_forward(const vkh_rope_params *p, const float *q_in, floa
 vkh_status vkh_qk_rope_backward(const vkh_rope_params *p, const float *dq_out, float *dq_in,
                                 const float *dk_out, float *dk_in, vkh_stream stream) {
     return rope_common(p, dq_out, dq_in, dk_out, dk_in, true, stream);
+}
+
+// ── rotary positions, Q/K norm with rotation ───────────────────────────
+
+vkh_status vkh_rotary_plan_init(const vkh_rotary_spec *sp, vkh_rotary_plan *out) {
+    CHECK_ARG(sp && out, "null pointer");
+    const uint32_t r = sp->rotary_dim;
+    CHECK_ARG(r % 2 == 0 && r <= 2 * VKH_ROTARY_MAX_PAIRS, "rotary_dim: even, at most 256");
+    CHECK_ARG(sp->layout <= VKH_ROTARY_INTERLEAVED, "layout");
+    CHECK_ARG(sp->scaling <= VKH_ROTARY_BANDS, "scaling");
+    CHECK_ARG(isfinite(sp->theta) && sp->theta > 1.f, "theta must be over 1");
+    CHECK_ARG(isfinite(sp->attn_factor) && sp->attn_factor >= 0.f, "attn_factor");
+    const bool scaled = sp->scaling != VKH_ROTARY_UNSCALED;
+    CHECK_ARG(!scaled || (isfinite(sp->factor) && sp->factor > 0.f), "factor must be over 0");
+    CHECK_ARG(sp->scaling != VKH_ROTARY_NTK || r != 2, "ntk scaling needs more than one pair");
+    const double two_pi = 6.283185307179586476925, s = scaled ? sp->factor : 1.0, L = sp->orig_len;
+    const double fast = sp->beta_fast != 0.f ? sp->beta_fast : 32.0, slow = sp->beta_slow != 0.f ? sp->beta_slow : 1.0;
+    const double low = sp->low_freq != 0.f ? sp->low_freq : 1.0, high = sp->high_freq != 0.f ? sp->high_freq : 4.0;
+    double theta = sp->theta, lo = 0, hi = 0, attn = 1.0;
+    if (sp->scaling == VKH_ROTARY_NTK && r) theta *= pow(s, r / (r - 2.0));
+    if (sp->scaling == VKH_ROTARY_YARN) {
+        CHECK_ARG(isfinite(fast) && slow > 0 && fast > slow, "beta_fast must be over beta_slow, both over 0");
+        CHECK_ARG(L > two_pi * fast, "yarn scaling needs orig_len over 2 pi beta_fast");
+        auto pair_of = [&](double turns) { return r * log(L / (turns * two_pi)) / (2.0 * log(theta)); };
+        lo = floor(pair_of(fast));
+        hi = std::max(std::min(ceil(pair_of(slow)), r - 1.0), lo);
+        if (hi == lo) hi += 1e-3;
+        if (s > 1.0) attn = 0.1 * log(s) + 1.0;
+    }
+    if (sp->scaling == VKH_ROTARY_BANDS) {
+        CHECK_ARG(isfinite(high) && low > 0 && high > low, "high_freq must be over low_freq, both over 0");
+        CHECK_ARG(sp->orig_len, "bands scaling needs orig_len");
+    }
+    vkh_rotary_plan pl = {};
+    pl.rotary_dim = r;
+    pl.layout = sp->layout;
+    pl.attn_factor = sp->attn_factor != 0.f ? sp->attn_factor : (float)attn;
+    for (uint32_t i = 0; i < r / 2; ++i) {
+        double f = pow(theta, -2.0 * i / r), u = 0.0;  // u: how much of the stretched frequency
+        if (sp->scaling == VKH_ROTARY_LINEAR) u = 1.0;
+        if (sp->scaling == VKH_ROTARY_YARN) u = (i - lo) / (hi - lo);
+        if (sp->scaling == VKH_ROTARY_BANDS) u = 1.0 - (L * f / two_pi - low) / (high - low);
+        u = std::min(1.0, std::max(0.0, u));
+        pl.turns[i] = (f * (1.0 - u) + f / s * u) / two_pi;
+    }
+    *out = pl;
+    return VKH_OK;
+}
+
+static inline DType DT(uint32_t d) { return d == VKH_BF16 ? DType::BF16 : DType::F32; }
+
+static vkh_status rotary_args(const vkh_rotary_params *p, const vkh_rotary_plan *pl, const uint32_t *positions,
+                              RotaryArgs &a) {
+    CHECK_ARG(p, "null params");
+    CHECK_ARG(p->head_dim && (p->n_q_heads || p->n_kv_heads), "zero dimension");
+    CHECK_ARG(p->x_dtype <= VKH_BF16 && p->y_dtype <= VKH_BF16 && p->dy_dtype <= VKH_BF16 && p->dx_dtype <= VKH_BF16, "dtype");
+    if (p->head_dim > 256) return fail(VKH_ERR_UNSUPPORTED, "head_dim > 256");
+    if (p->n_rows >= (1u << 31) || p->n_q_heads >= (1u << 16) || p->n_kv_heads >= (1u << 16))
+        return fail(VKH_ERR_UNSUPPORTED, "2^31 rows or 2^16 heads");
+    a = RotaryArgs{};
+    const uint32_t lds[2][4] = {{p->ld_xq, p->ld_yq, p->ld_dyq, p->ld_dxq}, {p->ld_xk, p->ld_yk, p->ld_dyk, p->ld_dxk}};
+    for (int k = 0; k < 2; ++k) {
+        a.nh[k] = (int)(k ? p->n_kv_heads : p->n_q_heads);
+        const uint32_t dense = a.nh[k] * p->head_dim;
+        for (uint32_t l : lds[k]) CHECK_ARG(!l || l >= dense, "a row stride is less than its heads");
+        auto ld = [&](int i) { return (long)(lds[k][i] ? lds[k][i] : dense); };
+        a.s[k].ldx = ld(0); a.s[k].ldy = ld(1); a.s[k].lddy = ld(2); a.s[k].lddx = ld(3);
+    }
+    a.n_rows = p->n_rows; a.hd = (int)p->head_dim;
+    a.seq = p->seq_len ? p->seq_len : std::max(1u, p->n_rows);
+    a.pos0 = p->pos0; a.pos = positions;
+    a.eps = p->eps; a.quirk = p->gemma_quirk ? 1.f : 0.f;
+    if (!pl) return VKH_OK;  // (the workspace's size)
+    CHECK_ARG(pl->rotary_dim % 2 == 0 && pl->rotary_dim <= 2 * VKH_ROTARY_MAX_PAIRS && pl->layout <= VKH_ROTARY_INTERLEAVED, "plan");
+    CHECK_ARG(pl->rotary_dim <= p->head_dim, "rotary_dim > head_dim");
+    CHECK_ARG((uintptr_t)positions % 4 == 0, "a pointer is not aligned to its type");
+    a.rot = (int)pl->rotary_dim; a.interleaved = pl->layout == VKH_ROTARY_INTERLEAVED;
+    a.scale = pl->attn_factor; a.sign = 1.f;
+    memcpy(a.turns, pl->turns, pl->rotary_dim / 2 * sizeof(double));
+    return VKH_OK;
+}
+// one side's pointers: all there and aligned to their types, or no heads
+static bool side_ok(int nh, std::initializer_list<std::pair<const void *, DType>> ptrs) {
+    for (auto &x : ptrs)
+        if (nh && (!x.first || !aligned_to(x.first, x.second))) return false;
+    return true;
+}
+
+static vkh_status rotary_call(const vkh_rotary_params *p, const vkh_rotary_plan *plan, const uint32_t *positions,
+                              bool norm, const float *wq, const float *wk, bool back, const void *qi, void *qo,
+                              const void *ki, void *ko, vkh_stream stream) {
+    CHECK_ARG(plan, "null plan");
+    RotaryArgs a;
+    VKH_TRY(rotary_args(p, plan, positions, a));
+    const DType xt = DT(back ? p->dy_dtype : p->x_dtype), yt = DT(back ? p->dx_dtype : p->y_dtype);
+    if (!a.n_rows) return VKH_OK;
+    CHECK_ARG(side_ok(a.nh[0], {{qi, xt}, {qo, yt}}) && side_ok(a.nh[1], {{ki, xt}, {ko, yt}}),
+              "null pointer, or one not aligned to its type");
+    CHECK_ARG(!norm || (side_ok(a.nh[0], {{wq, DType::F32}}) && side_ok(a.nh[1], {{wk, DType::F32}})), "norm gains");
+    a.s[0].x = qi; a.s[0].y = qo; a.s[0].w = wq;
+    a.s[1].x = ki; a.s[1].y = ko; a.s[1].w = wk;
+    if (back) {
+        a.sign = -1.f;
+        for (auto &s : a.s) s.ldx = s.lddy, s.ldy = s.lddx;
+    }
+    VKH_HIP(rotary_forward(a, norm, xt, yt, S(stream)));
+    return VKH_OK;
+}
+
+vkh_status vkh_rotary_forward(const vkh_rotary_params *p, const vkh_rotary_plan *plan,
+                              const uint32_t *positions, const void *q_in, void *q_out,
+                              const void *k_in, void *k_out, vkh_stream stream) {
+    return rotary_call(p, plan, positions, false, nullptr, nullptr, false, q_in, q_out, k_in, k_out, stream);
+}
+
+vkh_status vkh_rotary_backward(const vkh_rotary_params *p, const vkh_rotary_plan *plan,
+                               const uint32_t *positions, const void *dq_out, void *dq_in,
+                               const void *dk_out, void *dk_in, vkh_stream stream) {
+    return rotary_call(p, plan, positions, false, nullptr, nullptr, true, dq_out, dq_in, dk_out, dk_in, stream);
+}
+
+vkh_status vkh_qk_norm_rotary_forward(const vkh_rotary_params *p, const vkh_rotary_plan *plan,
+                                      const uint32_t *positions, const float *wq, const float *wk,
+                                      const void *q_in, void *q_out, const void *k_in, void *k_out,
+                                      vkh_stream stream) {
+    return rotary_call(p, plan, positions, true, wq, wk, false, q_in, q_out, k_in, k_out, stream);
+}
+
+size_t vkh_qk_norm_rotary_workspace_bytes(const vkh_rotary_params *p) {
+    RotaryArgs a;
+    if (rotary_args(p, nullptr, nullptr, a) != VKH_OK) return 0;
+    return (size_t)rotary_parts(a) * 2 * a.hd * sizeof(float);
+}
+
+vkh_status vkh_qk_norm_rotary_backward(const vkh_rotary_params *p, const vkh_rotary_plan *plan,
+                                       const uint32_t *positions, const float *wq, const float *wk,
+                                       const void *q_in, const void *k_in, const void *dq_out,
+                                       const void *dk_out, void *dq_in, void *dk_in, float *dwq,
+                                       float *dwk, void *workspace, vkh_stream stream) {
+    CHECK_ARG(plan, "null plan");
+    RotaryArgs a;
+    VKH_TRY(rotary_args(p, plan, positions, a));
+    const DType xt = DT(p->x_dtype), gt = DT(p->dy_dtype), dt = DT(p->dx_dtype);
+    hipStream_t st = S(stream);
+    CHECK_ARG(aligned_to(dwq, DType::F32) && aligned_to(dwk, DType::F32), "a pointer is not aligned to its type");
+    if (!a.n_rows) {  // empty sums
+        if (dwq) VKH_HIP(fill_f32(dwq, a.hd, 0.f, st));
+        if (dwk) VKH_HIP(fill_f32(dwk, a.hd, 0.f, st));
+        return VKH_OK;
+    }
+    CHECK_ARG(side_ok(a.nh[0], {{q_in, xt}, {dq_out, gt}, {dq_in, dt}, {wq, DType::F32}}) &&
+                  side_ok(a.nh[1], {{k_in, xt}, {dk_out, gt}, {dk_in, dt}, {wk, DType::F32}}),
+              "null pointer, or one not aligned to its type");
+    a.s[0].x = q_in; a.s[0].dy = dq_out; a.s[0].dx = dq_in; a.s[0].w = wq;
+    a.s[1].x = k_in; a.s[1].dy = dk_out; a.s[1].dx = dk_in; a.s[1].w = wk;
+    a.sign = -1.f;
+    float *partial = nullptr;
+    ScratchLease lease;
+    if (dwq || dwk) {
+        CHECK_ARG((uintptr_t)workspace % 16 == 0, "the workspace is not 16-byte aligned");
+        CHECK_ARG(workspace || !capturing(st), "gain gradients on a stream under capture need a workspace");
+        void *w = workspace;
+        if (!w) VKH_TRY(lease.acquire((size_t)rotary_parts(a) * 2 * a.hd * sizeof(float), st, &w));
+        partial = (float *)w;
+    }
+    VKH_HIP(rotary_norm_backward(a, xt, gt, dt, partial, dwq, dwk, st));
+    return VKH_OK;
 }
 
 vkh_status vkh_qkv_project_bf16(const vkh_rope_params *p, uint32_t K, float eps, int qk_norm,

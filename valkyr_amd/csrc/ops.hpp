@@ -249,6 +249,36 @@ hipError_t qk_rope(const float *q_in, long ldq_in, float *q_out, long ldq_out, c
                    int n_kv_heads, int head_dim, int rotary_dim, int seq_len, const float2 *tab,
                    bool backward, hipStream_t st);
 
+// ── rotary positions (k_rotary.hip) ───────────────────────────────────
+// q (side 0) and k (side 1) rows of nh heads: x -> y forward, dy -> dx backward; strides in
+// elements.  A side of no heads is left out.
+struct RotarySide {
+    const void *x = nullptr;
+    void *y = nullptr;
+    const void *dy = nullptr;
+    void *dx = nullptr;
+    long ldx = 0, ldy = 0, lddy = 0, lddx = 0;
+    const float *w = nullptr;  // norm gain [hd]
+};
+struct RotaryArgs {
+    RotarySide s[2];
+    int nh[2];
+    long n_rows;
+    int hd, rot, interleaved;
+    unsigned seq, pos0;         // position of row r without `pos`: pos0 + r % seq
+    const uint32_t *pos;
+    float eps, quirk;           // quirk 1: gains are 1 + w
+    float scale, sign;          // sign -1: turned back
+    double turns[128];          // turns per position of each pair
+};
+// y = rotation of x, or (norm) of x rstd w; any head_dim up to 256.
+hipError_t rotary_forward(const RotaryArgs &a, bool norm, DType xt, DType yt, hipStream_t st);
+// dx of the norm and rotation (a.sign = -1), and with `partial` (rotary_parts(a) rows of 2 hd
+// floats) the gain gradients dwq / dwk (overwrite; either may be null).
+hipError_t rotary_norm_backward(const RotaryArgs &a, DType xt, DType gt, DType dt, float *partial,
+                                float *dwq, float *dwk, hipStream_t st);
+int rotary_parts(const RotaryArgs &a);
+
 // Fused per-head Q/K RMSNorm + RoPE forward, emitting the attention
 // operands (fp32 or bf16) for q, k and (copy/cast of) v.
 struct QkvLayout {
@@ -422,6 +452,34 @@ int fa_bw_v4_kv_blocks(const AttnShape &s);
 bool fa_bw_qk_epi_ok(const AttnShape &s, int rotary_dim);
 size_t fa_bw_ws_bytes(const AttnShape &s, bool v4);
 hipError_t fa_bw_fused(const AttnShape &s, const AttnPtrs &p, bf16 *ds_ws, bool v4, hipStream_t st);
+
+// ── windowed attention (k_attn_window.hip) ───────────────────────────
+// Sequence b has kl = min(kv_len[b], n_kv) keys and ql = min(q_len[b], n_q) query rows (all of
+// them without the arrays); its row r is at position r + kl - ql and sees key j where
+// j <= position and (j > position - window or j < n_sink).
+struct WindowArgs {
+    int n_batch, n_q, n_kv, n_heads, n_kv_heads, hd;
+    int window, n_sink;  // 1 <= window <= n_kv, n_sink <= n_kv
+    float scale;         // of the scores
+    DType dt, odt;       // of q, k, v, dO; of O, dQ, dK, dV
+    const void *q, *k, *v;
+    long ldq, ldk, ldv;
+    void *o;
+    long ldo;
+    float *lse;
+    const uint32_t *q_len, *kv_len;
+    const void *dout;
+    long lddo;
+    float *d;
+    void *dq, *dk, *dv;
+    long lddq, lddk, lddv;
+    float *ws;           // split partial sums (null: no split)
+};
+size_t window_fwd_ws_bytes(const WindowArgs &a);
+size_t window_bwd_ws_bytes(const WindowArgs &a);
+hipError_t window_forward(const WindowArgs &a, hipStream_t st);
+// d (= rowsum(O dO)), dQ, dK, dV (overwrite)
+hipError_t window_backward(const WindowArgs &a, hipStream_t st);
 
 // ── cut cross-entropy (k_cce.hip) ────────────────────────────────────
 struct CceShape {

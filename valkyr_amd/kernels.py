@@ -10,9 +10,12 @@ from __future__ import annotations
 import ctypes as C
 import math
 
-from ._lib import AttnParams, CceParams, LoraAdapter, RopeParams, check, lib
+from ._lib import (AttnParams, CceParams, LoraAdapter, RopeParams, RotaryParams, RotaryPlan,
+                   RotarySpec, WindowParams, check, lib)
 
 F32, BF16 = 0, 1
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
+ROTARY_UNSCALED, ROTARY_LINEAR, ROTARY_NTK, ROTARY_YARN, ROTARY_BANDS = range(5)
 PRECISION_FP32, PRECISION_BF16 = 0, 1
 
 
@@ -78,6 +81,40 @@ def fa_backward_from_o(p, q, k, v, o16, dout16, lse, d, dq, dk, dv, workspace=No
     check(lib().vkh_fa_backward_from_o(C.byref(p), _p(q), _p(k), _p(v), _p(o16), _p(dout16),
                                        _p(lse), _p(d), _p(dq), _p(dk), _p(dv), _p(workspace),
                                        _s(stream)))
+
+
+def window_params(n_q, n_kv, n_heads, n_kv_heads, head_dim, window=0, n_sink=0, n_batch=1, dtype=F32,
+                  out_dtype=None, inv_sqrt_dim=None, ld_q=0, ld_k=0, ld_v=0, ld_o=0, ld_do=0, ld_dq=0,
+                  ld_dk=0, ld_dv=0):
+    """Attention over the last `window` keys (0: all) and the first n_sink; O and gradients are
+    stored as out_dtype (None: dtype); row strides in elements, 0 for dense rows."""
+    return WindowParams(n_batch, n_q, n_kv, n_heads, n_kv_heads, head_dim, window, n_sink,
+                        inv_sqrt_dim if inv_sqrt_dim is not None else 1.0 / math.sqrt(head_dim), dtype,
+                        dtype if out_dtype is None else out_dtype, ld_q, ld_k, ld_v, ld_o, ld_do, ld_dq,
+                        ld_dk, ld_dv)
+
+
+def fa_window_forward_workspace_bytes(p):
+    return lib().vkh_fa_window_forward_workspace_bytes(C.byref(p))
+
+
+def fa_window_forward(p, q, k, v, o, lse=None, q_len=None, kv_len=None, workspace=None, stream=None):
+    """O (and LSE) of windowed attention; q_len, kv_len: each sequence's rows and keys (uint32
+    [n_batch] on the device), None for all."""
+    check(lib().vkh_fa_window_forward(C.byref(p), _p(q), _p(k), _p(v), _p(o), _p(lse), _p(q_len),
+                                      _p(kv_len), _p(workspace), _s(stream)))
+
+
+def fa_window_backward_workspace_bytes(p):
+    return lib().vkh_fa_window_backward_workspace_bytes(C.byref(p))
+
+
+def fa_window_backward(p, q, k, v, o, dout, lse, d, dq, dk, dv, q_len=None, kv_len=None,
+                       workspace=None, stream=None):
+    """dQ, dK, dV from the forward's O and LSE; D = rowsum(O dO) is written to d."""
+    check(lib().vkh_fa_window_backward(C.byref(p), _p(q), _p(k), _p(v), _p(o), _p(dout), _p(lse),
+                                       _p(d), _p(dq), _p(dk), _p(dv), _p(q_len), _p(kv_len),
+                                       _p(workspace), _s(stream)))
 
 
 def matmul_nt(x, w, y, M, N, K, precision=PRECISION_FP32, stream=None):
@@ -227,6 +264,55 @@ def qk_rope_forward(p, q_in, q_out, k_in, k_out, stream=None):
 def qk_rope_backward(p, dq_out, dq_in, dk_out, dk_in, stream=None):
     check(lib().vkh_qk_rope_backward(C.byref(p), _p(dq_out), _p(dq_in), _p(dk_out), _p(dk_in),
                                      _s(stream)))
+
+
+def rotary_plan(rotary_dim, theta, layout=ROTARY_HALF, scaling=ROTARY_UNSCALED, factor=1.0, orig_len=0,
+                beta_fast=0.0, beta_slow=0.0, low_freq=0.0, high_freq=0.0, attn_factor=0.0):
+    """The frequencies of a rotation (vkh_rotary_spec), as plain data for the calls below."""
+    plan = RotaryPlan()
+    spec = RotarySpec(rotary_dim, layout, scaling, orig_len, theta, factor, beta_fast, beta_slow,
+                      low_freq, high_freq, attn_factor)
+    check(lib().vkh_rotary_plan_init(C.byref(spec), C.byref(plan)))
+    return plan
+
+
+def rotary_params(n_rows, n_q_heads, n_kv_heads, head_dim, seq_len=0, pos0=0, eps=1e-6,
+                  gemma_quirk=False, x_dtype=F32, y_dtype=F32, dy_dtype=F32, dx_dtype=F32, ld_xq=0,
+                  ld_xk=0, ld_yq=0, ld_yk=0, ld_dyq=0, ld_dyk=0, ld_dxq=0, ld_dxk=0):
+    return RotaryParams(n_rows, n_q_heads, n_kv_heads, head_dim, seq_len, pos0, eps, int(gemma_quirk),
+                        x_dtype, y_dtype, dy_dtype, dx_dtype, ld_xq, ld_xk, ld_yq, ld_yk, ld_dyq,
+                        ld_dyk, ld_dxq, ld_dxk)
+
+
+def rotary_forward(p, plan, q_in, q_out, k_in=None, k_out=None, positions=None, stream=None):
+    """Query and key heads turned by their positions (uint32 [n_rows] on the device, or None for
+    pos0 + row % seq_len)."""
+    check(lib().vkh_rotary_forward(C.byref(p), C.byref(plan), _p(positions), _p(q_in), _p(q_out),
+                                   _p(k_in), _p(k_out), _s(stream)))
+
+
+def rotary_backward(p, plan, dq_out, dq_in, dk_out=None, dk_in=None, positions=None, stream=None):
+    check(lib().vkh_rotary_backward(C.byref(p), C.byref(plan), _p(positions), _p(dq_out), _p(dq_in),
+                                    _p(dk_out), _p(dk_in), _s(stream)))
+
+
+def qk_norm_rotary_forward(p, plan, wq, wk, q_in, q_out, k_in=None, k_out=None, positions=None,
+                           stream=None):
+    """RMSNorm of each query and key head and the rotation in one pass."""
+    check(lib().vkh_qk_norm_rotary_forward(C.byref(p), C.byref(plan), _p(positions), _p(wq), _p(wk),
+                                           _p(q_in), _p(q_out), _p(k_in), _p(k_out), _s(stream)))
+
+
+def qk_norm_rotary_workspace_bytes(p):
+    return lib().vkh_qk_norm_rotary_workspace_bytes(C.byref(p))
+
+
+def qk_norm_rotary_backward(p, plan, wq, wk, q_in, k_in, dq_out, dk_out, dq_in, dk_in, dwq=None,
+                            dwk=None, positions=None, workspace=None, stream=None):
+    """dq_in, dk_in and the gain gradients of qk_norm_rotary_forward."""
+    check(lib().vkh_qk_norm_rotary_backward(C.byref(p), C.byref(plan), _p(positions), _p(wq), _p(wk),
+                                            _p(q_in), _p(k_in), _p(dq_out), _p(dk_out), _p(dq_in),
+                                            _p(dk_in), _p(dwq), _p(dwk), _p(workspace), _s(stream)))
 
 
 def embed_lookup(embed, ids, out, n_pos, dim, scale=1.0, stream=None):
