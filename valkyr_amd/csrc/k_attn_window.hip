@@ -15,25 +15,13 @@
 // the weighted sum with the head's values over the lanes.
 #include <algorithm>
 
-#include "ops.hpp"
+#include "window.hpp"
 
 namespace vkh {
 namespace {
 
 constexpr int WNT = 256, WPB = WNT / 64;
 constexpr int WE = 4;  // values of a head row per lane (head_dim <= 256)
-
-// Query rows, keys and the first row's position of a sequence.
-struct Span {
-    int ql, kl, off;
-};
-VKH_DEV Span span_of(const WindowArgs &a, int b) {
-    Span s;
-    s.ql = a.q_len ? (int)min(a.q_len[b], (unsigned)a.n_q) : a.n_q;
-    s.kl = a.kv_len ? (int)min(a.kv_len[b], (unsigned)a.n_kv) : a.n_kv;
-    s.off = s.kl - s.ql;
-    return s;
-}
 
 // dot product of a row with `hd` values in LDS
 template <class T>
@@ -208,9 +196,10 @@ unsigned row_blocks(long rows) { return (unsigned)((rows + WPB - 1) / WPB); }
 }  // namespace
 
 size_t window_fwd_ws_bytes(const WindowArgs &) { return 0; }
-size_t window_bwd_ws_bytes(const WindowArgs &) { return 0; }
+size_t window_bwd_ws_bytes(const WindowArgs &a) { return window16_bwd_ws_bytes(a); }
 
 hipError_t window_forward(const WindowArgs &a, hipStream_t st) {
+    if (window16_forward(a, st)) return hipGetLastError();
     by_types(a, [&](auto t, auto o) {
         hipLaunchKernelGGL((window_fwd_any_k<decltype(t), decltype(o)>),
                            dim3(row_blocks((long)a.n_batch * a.n_q * a.n_heads)), dim3(WNT), 0, st, a);
@@ -219,6 +208,7 @@ hipError_t window_forward(const WindowArgs &a, hipStream_t st) {
 }
 
 hipError_t window_backward(const WindowArgs &a, hipStream_t st) {
+    if (window16_backward(a, st)) return hipGetLastError();
     by_types(a, [&](auto t, auto o) {
         hipLaunchKernelGGL((window_dq_any_k<decltype(t), decltype(o)>),
                            dim3(row_blocks((long)a.n_batch * a.n_q * a.n_heads)), dim3(WNT), 0, st, a);

@@ -1,0 +1,920 @@
+// Windowed attention on bf16 operands: the tile kernels (64- and 128-wide heads, aligned rows) of
+// the operator that k_attn_window.hip describes.
+//
+// v_mfma_f32_16x16x32_bf16 with fp32 accumulation; scores are formed transposed where that lets P
+// and dS go from the accumulators straight into the next product as its B operand:
+//   forward  S^T = K Q^T, O^T += V^T P^T          dQ  S^T, dP^T = V dO^T, dQ^T += K^T dS^T
+//   dK/dV    S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS
+// P and dS are rounded to bf16 for those products, as their other operands are (the sum of P that
+// divides O is of the unrounded values); everything else is fp32.
+//
+// A block walks only the tiles of its window and, before them, those of the sinks.  Tiles come
+// by DMA into swizzled LDS rows, through a buffer resource that is set on the tile's first row:
+// its offsets stay small however long the cache is, a lane's offset is the same for every tile,
+// and rows past a sequence's end read as zero by the range check.  Masks cost nothing in tiles
+// that every row sees in full.  In the others a masked pair has P = dS = 0, selected, and since
+// 0 times an infinity or a NaN is NaN, the tile that multiplies them is scanned for such values;
+// a tile that holds one (none, in a healthy run) is left out, and after the others its products are
+// added pair by pair, seen pairs only.
+#include <algorithm>
+
+#include "attn16.hpp"
+#include "window.hpp"
+
+namespace vkh {
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr int kAll = 0x7fffffff;  // the window of a sink
+
+// Whether position t sees key j (t = -1: a row that sees none).
+VKH_DEV bool sees(const WindowArgs &a, int t, int j) {
+    return (unsigned)(t - j) < (unsigned)(j < a.n_sink ? kAll : a.window);
+}
+// Whether all positions ta .. tb see all keys j0 .. j1, or none sees any.
+VKH_DEV bool all_seen(const WindowArgs &a, int ta, int tb, int j0, int j1) {
+    return j1 <= ta && (j0 > tb - a.window || j1 < a.n_sink);
+}
+VKH_DEV bool none_seen(const WindowArgs &a, int ta, int tb, int j0, int j1) {
+    return tb < ta || j0 > tb || (j1 <= ta - a.window && j0 >= a.n_sink);
+}
+
+VKH_DEV bool not_finite(uint4 v) {
+    bool bad = false;
+#pragma unroll
+    for (unsigned w : {v.x, v.y, v.z, v.w})
+        bad |= (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+    return bad;
+}
+// whether any of the thread's share of `bytes` of LDS holds an infinity or a NaN
+template <int BYTES, int NT>
+VKH_DEV bool scan(const char *lds, int tid) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < (BYTES + 16 * NT - 1) / (16 * NT); ++i)
+        if ((i + 1) * 16 * NT <= BYTES || (i * NT + tid) * 16 < BYTES)
+            bad |= not_finite(*reinterpret_cast<const uint4 *>(lds + (i * NT + tid) * 16));
+    return bad;
+}
+
+// The resource of rows row0 .. row0 + rows - 1 of one head (rows <= 0: of none).
+template <int HD>
+VKH_DEV sgpr4 head_rows(const void *p, long row0, long ld, int col, int rows) {
+    return rsrc4((const bf16 *)p + row0 * ld + col, rows > 0 ? (unsigned)(((rows - 1) * (int)ld + HD) * 2) : 0u);
+}
+// A lane's byte offset in a DMA of 1 KB: row r0 + lane / (HD / 8) of the tile, its chunk swizzled.
+template <int HD>
+VKH_DEV unsigned dma_off(int r0, int lane, int ld) {
+    const int r = r0 + lane / (HD / 8), c = (lane % (HD / 8)) ^ TileRows<HD>::swz(r);
+    return (unsigned)((r * ld + 8 * c) * 2);
+}
+
+// acc[i][r] += sum over the tile's rows x that `see` names of T[x][16 i + 4 g + r] w[x], where w is
+// held as a B operand: element 4 u + e of w[s] is row 32 s + 16 u + 4 g + e.  `wl` is the wave's own
+// LDS (1 KB for each s) that w goes through, so that the loop over rows need not be unrolled.
+template <int HD, int NS, class See>
+VKH_DEV void add_pairs(f32x4 (&acc)[HD / 16], const char *T, const bf16x8 (&w)[NS], bf16x8 *wl, int lane, See see) {
+    const int g = lane / 16, c16 = lane % 16;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) wl[64 * s + lane] = w[s];
+#pragma unroll 1
+    for (int x = 0; x < 32 * NS; ++x) {
+        const bf16 *wp = reinterpret_cast<const bf16 *>(wl + 64 * (x / 32) + x % 16 / 4 * 16 + c16);
+        const float wx = (float)wp[x % 32 / 16 * 4 + x % 4];
+        if (!see(x)) continue;
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) {
+            const bf16x4 t = *reinterpret_cast<const bf16x4 *>(T + TileRows<HD>::toff(x, 16 * i + 4 * g));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][r] = fmaf((float)t[r], wx, acc[i][r]);
+        }
+    }
+}
+
+VKH_DEV void store4(float *p, float x, float y, float z, float w) {
+    *reinterpret_cast<float4 *>(p) = make_float4(x, y, z, w);
+}
+VKH_DEV void store4(bf16 *p, float x, float y, float z, float w) {
+    bf16x4 o;
+    o[0] = (bf16)x; o[1] = (bf16)y; o[2] = (bf16)z; o[3] = (bf16)w;
+    *reinterpret_cast<bf16x4 *>(p) = o;
+}
+
+// The key tiles (of BN keys) that a block of query rows r0 .. r1 - 1 walks: those of the sinks that
+// lie before its window, then its window's.
+struct KeyTiles {
+    int ta, tb;     // live positions (tb < ta: none)
+    int n_sink, w0, n;
+    VKH_DEV int tile(int it) const { return it < n_sink ? it : w0 + it - n_sink; }
+};
+template <int BN>
+VKH_DEV KeyTiles key_tiles(const WindowArgs &a, const Span &s, int r0, int r1) {
+    KeyTiles k;
+    k.ta = max(0, r0 + s.off);
+    k.tb = min(r1, s.ql) - 1 + s.off;
+    k.w0 = max(0, k.ta - a.window + 1) / BN;
+    k.n_sink = min((a.n_sink + BN - 1) / BN, k.w0);
+    k.n = k.tb >= k.ta ? k.n_sink + k.tb / BN - k.w0 + 1 : 0;
+    return k;
+}
+
+// ── forward ──────────────────────────────────────────────────────────────
+// Block = 64 QS query rows of one head, 4 waves of 16 QS; 64-key tiles, two buffers.  Block ids run
+// over (sequence, KV head) first, so the blocks of one KV head sit on one XCD and share its
+// tiles there, and the heaviest (last) rows start first.
+template <int HD, int QS, class TO>
+__global__ __launch_bounds__(256, 2) void window_fwd16_k(WindowArgs a) {
+    using R = TileRows<HD>;
+    constexpr int DS = HD / 32, DSUB = HD / 16, BM = 64 * QS, BN = 64, KT = BN * HD * 2;
+    constexpr int RPI = 512 / HD, IPW = 16 / RPI;  // rows per DMA, DMAs per wave and tile
+    __shared__ __attribute__((aligned(16))) char Ks[2][KT], Vs[2][KT];
+    __shared__ bf16x8 wl[4][128];
+    __shared__ int odd[2];  // odd[buffer] = step + 1 where V is to be added pair by pair
+    const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, nqt = (a.n_q + BM - 1) / BM;
+    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
+    const int h = kvh * grp + blockIdx.x / nbk % grp, qt = nqt - 1 - (int)(blockIdx.x / nbk / grp);
+    const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c16 = lane % 16;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const Span s = span_of(a, b);
+    const int r0 = qt * BM, qw0 = r0 + wave * 16 * QS;
+    const KeyTiles kt = key_tiles<BN>(a, s, r0, r0 + BM);
+    const int wta = max(0, qw0 + s.off), wtb = min(qw0 + 16 * QS, s.ql) - 1 + s.off;
+    const float c2 = a.scale * LOG2E;
+    const long row0 = (long)b * a.n_q, key0 = (long)b * a.n_kv;
+
+    bf16x8 qf[QS][DS];
+    int pos[QS];
+#pragma unroll
+    for (int qs = 0; qs < QS; ++qs) {
+        const int r = qw0 + 16 * qs + c16;
+        pos[qs] = r < s.ql ? max(-1, r + s.off) : -1;
+        const bf16 *qr = (const bf16 *)a.q + (row0 + r) * a.ldq + h * HD + 8 * g;
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds) qf[qs][ds] = pos[qs] >= 0 ? ld_frag(qr + 32 * ds) : bf16x8{};
+    }
+    unsigned ko[IPW], vo[IPW];
+#pragma unroll
+    for (int i = 0; i < IPW; ++i) {
+        ko[i] = dma_off<HD>(16 * wave + RPI * i, lane, (int)a.ldk);
+        vo[i] = dma_off<HD>(16 * wave + RPI * i, lane, (int)a.ldv);
+    }
+    if (tid < 2) odd[tid] = 0;
+    wait_vm0();  // Q fragments are in registers before any DMA is queued
+    auto dma = [&](int it, int buf) {
+        const int k0 = kt.tile(it) * BN, rows = min(BN, s.kl - k0);
+        const sgpr4 rk = head_rows<HD>(a.k, key0 + k0, a.ldk, kvh * HD, rows);
+        const sgpr4 rv = head_rows<HD>(a.v, key0 + k0, a.ldv, kvh * HD, rows);
+#pragma unroll
+        for (int i = 0; i < IPW; ++i) {
+            dma16_async(rk, Ks[buf] + (16 * wave + RPI * i) * HD * 2, ko[i]);
+            dma16_async(rv, Vs[buf] + (16 * wave + RPI * i) * HD * 2, vo[i]);
+        }
+    };
+    f32x4 oacc[QS][DSUB];
+    float m[QS], l[QS];  // running maximum in log2 units; this lane's share of the sum
+#pragma unroll
+    for (int qs = 0; qs < QS; ++qs) {
+        m[qs] = -INFINITY;
+        l[qs] = 0.f;
+#pragma unroll
+        for (int i = 0; i < DSUB; ++i) oacc[qs][i] = f32x4{0, 0, 0, 0};
+    }
+    bool any_odd = false;
+    auto step = [&](const int it, const int buf, auto pairsc) {
+        constexpr bool PAIRS = decltype(pairsc)::value;
+        const int k0 = kt.tile(it) * BN;
+        wait_vm0();
+        lds_barrier();  // tile `it` landed; everyone is done with the other buffer
+        if (!PAIRS && it + 1 < kt.n) dma(it + 1, buf ^ 1);
+        const char *Kb = Ks[buf], *Vb = Vs[buf];
+        if (!all_seen(a, kt.ta, kt.tb, k0, k0 + BN - 1)) {
+            if (scan<KT, 256>(Vb, tid)) odd[buf] = it + 1;
+            lds_barrier();
+            const bool pairs = odd[buf] == it + 1;
+            any_odd |= pairs;
+            if (pairs != PAIRS) return;
+        } else if (PAIRS) {
+            return;
+        }
+        if (none_seen(a, wta, wtb, k0, k0 + BN - 1)) return;
+
+        f32x4 st[4][QS];
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int qs = 0; qs < QS; ++qs) st[ks][qs] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds)
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                const bf16x8 kf = R::frag_row(Kb, 16 * ks + c16, 32 * ds + 8 * g);
+#pragma unroll
+                for (int qs = 0; qs < QS; ++qs) st[ks][qs] = mfma16x16x32(kf, qf[qs][ds], st[ks][qs]);
+            }
+        const bool full = all_seen(a, wta, wtb, k0, k0 + BN - 1) && qw0 + 16 * QS <= s.ql && qw0 + s.off >= 0;
+        bf16x8 pf[QS][2];
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs) {
+            if (!full) {
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (!sees(a, pos[qs], k0 + 16 * ks + 4 * g + r)) st[ks][qs][r] = -INFINITY;
+            }
+            float mt = -INFINITY;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) mt = fmaxf(mt, st[ks][qs][r]);
+            // The maximum that P is taken against moves only when a row's scores pass it by more
+            // than 8 (in log2 units): P stays under 2^8, where bf16 and fp32 hold it as exactly,
+            // and the accumulators are rescaled in few tiles after the first.  A row's decision
+            // is its own.
+            if (__any(mt * c2 > m[qs] + 8.f)) {
+                const float mn = xrow_max(mt) * c2;
+                const float mo = m[qs];
+                if (mn > mo + 8.f) m[qs] = mn;
+                const float so = m[qs] == mo ? 1.f : __builtin_amdgcn_exp2f(mo - m[qs]);
+                l[qs] *= so;
+#pragma unroll
+                for (int i = 0; i < DSUB; ++i) oacc[qs][i] *= so;
+            }
+            const float ms = m[qs] == -INFINITY ? 0.f : m[qs];  // no score above -inf yet: P = 0
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(st[ks][qs][r], c2, -ms));
+                    st[ks][qs][r] = p;
+                    l[qs] += p;
+                }
+            pf[qs][0] = frag_acc(st[0][qs], st[1][qs]);
+            pf[qs][1] = frag_acc(st[2][qs], st[3][qs]);
+        }
+        if constexpr (PAIRS) {
+#pragma unroll
+            for (int qs = 0; qs < QS; ++qs)
+                add_pairs<HD>(oacc[qs], Vb, pf[qs], wl[wave], lane, [&](int x) { return sees(a, pos[qs], k0 + x); });
+            return;
+        }
+#pragma unroll
+        for (int kst = 0; kst < 2; ++kst)
+#pragma unroll
+            for (int i = 0; i < DSUB; ++i) {
+                const bf16x8 vf = R::frag_t(Vb, 16 * i, 32 * kst, g, c16);
+#pragma unroll
+                for (int qs = 0; qs < QS; ++qs) oacc[qs][i] = mfma16x16x32(vf, pf[qs][kst], oacc[qs][i]);
+            }
+    };
+    if (kt.n > 0) dma(0, 0);
+    for (int it = 0; it < kt.n; ++it) step(it, it & 1, std::false_type{});
+    if (any_odd)  // (the same for all waves)
+#pragma unroll 1
+        for (int it = 0; it < kt.n; ++it) {
+            __syncthreads();
+            if (tid == 0) odd[0] = 0;
+            dma(it, 0);
+            step(it, 0, std::true_type{});
+        }
+#pragma unroll
+    for (int qs = 0; qs < QS; ++qs) {
+        const int r = qw0 + 16 * qs + c16;
+        const float lt = xrow_sum(l[qs]);
+        if (r >= a.n_q) continue;
+        const bool dead = lt == 0.f;
+        const float inv = 1.0f / lt;
+        TO *o = (TO *)a.o + (row0 + r) * a.ldo + h * HD + 4 * g;
+#pragma unroll
+        for (int i = 0; i < DSUB; ++i) {
+            const f32x4 x = dead ? f32x4{0, 0, 0, 0} : oacc[qs][i] * inv;
+            store4(o + 16 * i, x[0], x[1], x[2], x[3]);
+        }
+        if (a.lse && g == 0)
+            a.lse[(row0 + r) * a.n_heads + h] = dead ? -INFINITY : (m[qs] + log2f(lt)) * LN2;
+    }
+}
+
+// ── backward: D and dQ ───────────────────────────────────────────────────
+// Block = BQ query rows of one head on NWV waves of 16 QSUB rows, whose Q and dO fragments stay in
+// registers; 32-key tiles of K and V through three buffers (two in flight, the wait counted).
+// D = rowsum(O dO) of the block's rows is formed first (fp64 sums of the bf16 products) and
+// stored for the dK/dV kernel, which runs after this one.
+template <int HD, int NWV, int BQ, class TO>
+__global__ __launch_bounds__(NWV * 64, 1) void window_dq16_k(WindowArgs a) {
+    using R = TileRows<HD>;
+    constexpr int QSUB = BQ / 16 / NWV, BN = 32, KS = 2, NBUF = 3, TILE = BN * HD * 2;
+    constexpr int DS = HD / 32, DSUB = HD / 16, NF = 2 * DS;
+    constexpr int RPI = 512 / HD, IPT = BN / RPI, C = 2 * IPT / NWV;  // DMAs per tile and tensor, per wave
+    static_assert(C >= 1 && C * NWV == 2 * IPT, "DMA share");
+    __shared__ __attribute__((aligned(16))) char Kt[NBUF][TILE], Vt[NBUF][TILE];
+    __shared__ bf16x8 wl[NWV][64];
+    __shared__ int odd[NBUF];
+    const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, nqb = (a.n_q + BQ - 1) / BQ;
+    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
+    const int h = kvh * grp + blockIdx.x / nbk % grp, qb = nqb - 1 - (int)(blockIdx.x / nbk / grp);
+    const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c16 = lane % 16;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const Span s = span_of(a, b);
+    const int r0 = qb * BQ, qw0 = r0 + wave * 16 * QSUB;
+    const KeyTiles kt = key_tiles<BN>(a, s, r0, r0 + BQ);
+    const int wta = max(0, qw0 + s.off), wtb = min(qw0 + 16 * QSUB, s.ql) - 1 + s.off;
+    const float c2 = a.scale * LOG2E;
+    const long row0 = (long)b * a.n_q, key0 = (long)b * a.n_kv;
+
+    bf16x8 qr[QSUB][DS], orr[QSUB][DS];
+    float lq[QSUB], dd[QSUB];
+    int pos[QSUB];
+#pragma unroll
+    for (int j = 0; j < QSUB; ++j) {
+        const int r = qw0 + 16 * j + c16;
+        const long t = row0 + r;
+        const float l = r < s.ql && r + s.off >= 0 ? a.lse[t * a.n_heads + h] : -INFINITY;
+        const bool live = l != -INFINITY;  // no gradient for a row whose scores are all -inf either
+        pos[j] = live ? r + s.off : -1;
+        lq[j] = l * LOG2E;
+        const bf16 *qp = (const bf16 *)a.q + t * a.ldq + h * HD + 8 * g;
+        const bf16 *gp = (const bf16 *)a.dout + t * a.lddo + h * HD + 8 * g;
+        const TO *op = (const TO *)a.o + t * a.ldo + h * HD + 8 * g;
+        double acc = 0;
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds) {
+            qr[j][ds] = live ? ld_frag(qp + 32 * ds) : bf16x8{};
+            orr[j][ds] = live ? ld_frag(gp + 32 * ds) : bf16x8{};
+            if (live) {
+                typedef TO vec __attribute__((ext_vector_type(8)));
+                const vec o = *reinterpret_cast<const vec *>(op + 32 * ds);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc += (double)(float)o[e] * (double)(float)orr[j][ds][e];
+            }
+        }
+        acc += __shfl_xor(acc, 16, 64);
+        acc += __shfl_xor(acc, 32, 64);
+        dd[j] = (float)acc;
+        if (r < a.n_q && g == 0) a.d[t * a.n_heads + h] = dd[j];
+    }
+    // the wave's DMAs: number q = C wave + i of the 2 IPT of a tile, K's first
+    unsigned off[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        const int q = C * wave + i;
+        off[i] = dma_off<HD>(q % IPT * RPI, lane, (int)(q < IPT ? a.ldk : a.ldv));
+    }
+    if (tid < NBUF) odd[tid] = 0;
+    wait_vm0();
+    auto dma = [&](int it, int buf) {
+        const int k0 = kt.tile(it) * BN, rows = min(BN, s.kl - k0);
+        const sgpr4 rk = head_rows<HD>(a.k, key0 + k0, a.ldk, kvh * HD, rows);
+        const sgpr4 rv = head_rows<HD>(a.v, key0 + k0, a.ldv, kvh * HD, rows);
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int q = C * wave + i;
+            if (q < IPT) dma16_async(rk, Kt[buf] + q * 1024, off[i]);
+            else dma16_async(rv, Vt[buf] + (q - IPT) * 1024, off[i]);
+        }
+    };
+    f32x4 acc[QSUB][DSUB];
+#pragma unroll
+    for (int j = 0; j < QSUB; ++j)
+#pragma unroll
+        for (int i = 0; i < DSUB; ++i) acc[j][i] = f32x4{0, 0, 0, 0};
+    if (kt.n > 0) dma(0, 0);
+    if (kt.n > 1) dma(1, 1);
+    // unrolled over the three buffers: every LDS address is a lane's base plus a constant
+    bool any_odd = false;
+    auto step = [&](const int it, auto bufc, auto pairsc) {
+        constexpr int buf = decltype(bufc)::value;
+        constexpr bool PAIRS = decltype(pairsc)::value;
+        if (!PAIRS && it + 1 < kt.n) __builtin_amdgcn_s_waitcnt(0x0f70 | C);
+        else wait_vm0();
+        lds_barrier();
+        if (!PAIRS && it + 2 < kt.n) dma(it + 2, (buf + 2) % NBUF);
+        const int k0 = kt.tile(it) * BN;
+        const char *Kb = Kt[buf], *Vb = Vt[buf];
+        if (!all_seen(a, kt.ta, kt.tb, k0, k0 + BN - 1)) {
+            if (scan<TILE, NWV * 64>(Kb, tid)) odd[buf] = it + 1;
+            lds_barrier();
+            const bool pairs = odd[buf] == it + 1;
+            any_odd |= pairs;
+            if (pairs != PAIRS) return;
+        } else if (PAIRS) {
+            return;
+        }
+        if (none_seen(a, wta, wtb, k0, k0 + BN - 1)) return;
+        // the dP^T accumulators start at -D (one query per lane), so they end as dP^T - D
+        f32x4 st[KS][QSUB], dpt[KS][QSUB];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int j = 0; j < QSUB; ++j) {
+                st[ks][j] = f32x4{0, 0, 0, 0};
+                dpt[ks][j] = f32x4{-dd[j], -dd[j], -dd[j], -dd[j]};
+            }
+        // The three phases walk their operand fragments in one sequence (K rows for S^T, V rows
+        // for dP^T, transposed K for dQ^T), each slot's LDS read issued PD slots ahead of its MFMAs.
+        constexpr int PD = 2, RING = PD + 1;
+        auto ldslot = [&](int n) -> bf16x8 {
+            if (n < NF) return R::frag_row(Kb, 16 * (n % 2) + c16, 32 * (n / 2) + 8 * g);
+            if (n < 2 * NF) return R::frag_row(Vb, 16 * ((n - NF) % 2) + c16, 32 * ((n - NF) / 2) + 8 * g);
+            return R::frag_t(Kb, 16 * (n - 2 * NF), 0, g, c16);
+        };
+        bf16x8 fr[RING];
+#pragma unroll
+        for (int n = 0; n < PD; ++n) fr[n] = ldslot(n);
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            fr[(f + PD) % RING] = ldslot(f + PD);
+#pragma unroll
+            for (int j = 0; j < QSUB; ++j) st[f % 2][j] = mfma16x16x32(fr[f % RING], qr[j][f / 2], st[f % 2][j]);
+        }
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            const int n = NF + f;
+            fr[(n + PD) % RING] = ldslot(n + PD);
+#pragma unroll
+            for (int j = 0; j < QSUB; ++j) dpt[f % 2][j] = mfma16x16x32(fr[n % RING], orr[j][f / 2], dpt[f % 2][j]);
+            // P^T = exp2(S^T c - lse) of one (ks, j) tile rides along
+            constexpr int EVERY = NF / (KS * QSUB);
+            static_assert(EVERY >= 1 && EVERY * KS * QSUB == NF, "exp schedule");
+            if (f % EVERY == 0) {
+                const int t2 = f / EVERY, ks2 = t2 / QSUB, j2 = t2 % QSUB;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    st[ks2][j2][r] = __builtin_amdgcn_exp2f(fmaf(st[ks2][j2][r], c2, -lq[j2]));
+            }
+        }
+        bool whole = all_seen(a, wta, wtb, k0, k0 + BN - 1);
+        bool live = true;
+#pragma unroll
+        for (int j = 0; j < QSUB; ++j) live = live && pos[j] >= 0;
+        whole = whole && __all(live);
+        bf16x8 sb[QSUB][1];
+#pragma unroll
+        for (int j = 0; j < QSUB; ++j) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) dpt[ks][j][r] = st[ks][j][r] * dpt[ks][j][r];
+            if (!whole) {
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (!sees(a, pos[j], k0 + 16 * ks + 4 * g + r)) dpt[ks][j][r] = 0.f;
+            }
+            sb[j][0] = frag_acc(dpt[0][j], dpt[1][j]);
+        }
+        if constexpr (PAIRS) {
+#pragma unroll
+            for (int j = 0; j < QSUB; ++j)
+                add_pairs<HD>(acc[j], Kb, sb[j], wl[wave], lane, [&](int x) { return sees(a, pos[j], k0 + x); });
+            return;
+        }
+        // dQ^T += K^T dS^T
+#pragma unroll
+        for (int i = 0; i < DSUB; ++i) {
+            const int n = 2 * NF + i;
+            if (n + PD < 2 * NF + DSUB) fr[(n + PD) % RING] = ldslot(n + PD);
+#pragma unroll
+            for (int j = 0; j < QSUB; ++j) acc[j][i] = mfma16x16x32(fr[n % RING], sb[j][0], acc[j][i]);
+        }
+    };
+    for (int t0 = 0; t0 < kt.n; t0 += NBUF) {
+        step(t0, std::integral_constant<int, 0>{}, std::false_type{});
+        if (t0 + 1 < kt.n) step(t0 + 1, std::integral_constant<int, 1>{}, std::false_type{});
+        if (t0 + 2 < kt.n) step(t0 + 2, std::integral_constant<int, 2>{}, std::false_type{});
+    }
+    if (any_odd)  // (the same for all waves)
+#pragma unroll 1
+        for (int it = 0; it < kt.n; ++it) {
+            __syncthreads();
+            if (tid == 0) odd[0] = 0;
+            dma(it, 0);
+            step(it, std::integral_constant<int, 0>{}, std::true_type{});
+        }
+#pragma unroll
+    for (int j = 0; j < QSUB; ++j) {
+        const int r = qw0 + 16 * j + c16;
+        if (r >= a.n_q) continue;
+        TO *dq = (TO *)a.dq + (row0 + r) * a.lddq + h * HD + 4 * g;
+#pragma unroll
+        for (int i = 0; i < DSUB; ++i) {
+            const f32x4 x = pos[j] >= 0 ? acc[j][i] * a.scale : f32x4{0, 0, 0, 0};
+            store4(dq + 16 * i, x[0], x[1], x[2], x[3]);
+        }
+    }
+}
+
+// ── backward: dK and dV ──────────────────────────────────────────────────
+// Block = 128 keys of one KV head; 8 waves = 4 slices of 32 keys x 2 groups.  A wave holds K of its
+// slice in registers (V of the block sits in LDS) and takes 32-query tiles of the query heads that
+// share the KV head: group 0 every other head, group 1 the rest, or for an odd number of heads
+// alternate query tiles of every head.  Each group streams its Q and dO tiles through three
+// buffers.  Query tiles run from the first row that sees the block's first key to the last in
+// its window, or to the last row of all where the block holds sinks; such a block has a share of
+// work as many times the others' as the sequence is longer than the window, and is split between
+// `parts` blocks, as all blocks are where they are too few for the chip.  Parts write fp32 sums
+// to their slots of a.ws, which window_dkv_sum16_k adds in order.
+struct DkvPlan {
+    int key_blocks, sink_blocks;   // per KV head; the first sink_blocks hold sinks
+    int sink_parts, parts;         // blocks per sink block, per other block
+    __host__ __device__ int blocks() const { return sink_blocks * sink_parts + (key_blocks - sink_blocks) * parts; }
+    // slots of partial sums per KV head: a split block's parts
+    __host__ __device__ int slots() const { return (sink_parts > 1 ? sink_blocks * sink_parts : 0) + (parts > 1 ? (key_blocks - sink_blocks) * parts : 0); }
+};
+VKH_DEV void dkv_block(const DkvPlan &p, int y, int &kb, int &z, int &parts, int &slot) {
+    const int s = p.sink_blocks * p.sink_parts;
+    if (y < s) {
+        kb = y / p.sink_parts; z = y % p.sink_parts; parts = p.sink_parts;
+        slot = y;
+    } else {
+        kb = p.sink_blocks + (y - s) / p.parts; z = (y - s) % p.parts; parts = p.parts;
+        slot = (p.sink_parts > 1 ? s : 0) + y - s;
+    }
+}
+
+template <int HD, class TO>
+__global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan plan) {
+    using R = TileRows<HD>;
+    constexpr int NS = 4, BM = 32, BN = 128, KW = 32, KS = 2, QS = 2, NBUF = 3, TILE = BM * HD * 2;
+    constexpr int STREAM = NBUF * 2 * TILE, DS = HD / 32, DSUB = HD / 16, NF = 2 * DS;
+    constexpr int XSLOT = DSUB * KS * 64 * 16;  // one wave's dK^T or dV^T
+    constexpr int LDS = 8 * XSLOT > 2 * STREAM + BN * HD * 2 ? 8 * XSLOT : 2 * STREAM + BN * HD * 2;
+    constexpr int RPI = 512 / HD, C = 16 / RPI;  // rows per DMA; a wave's DMAs per tile (16 rows)
+    __shared__ __attribute__((aligned(16))) char smem[LDS];
+    __shared__ __attribute__((aligned(16))) float Ls[2][NBUF][64], Dd[2][NBUF][64];
+    __shared__ bf16x8 wl[8][64];
+    __shared__ int odd[2][NBUF];
+
+    const int nbk = a.n_batch * a.n_kv_heads;
+    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
+    int kb, zpart, zparts, slot;
+    dkv_block(plan, blockIdx.x / nbk, kb, zpart, zparts, slot);
+    const int hpk = a.n_heads / a.n_kv_heads;
+    const bool alt = hpk & 1;
+    const int nh = alt ? hpk : hpk / 2;  // heads per group
+    const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c16 = lane % 16;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int sl = wave % NS, hg = wave / NS;
+    const bool tdo = sl >= NS / 2;  // this wave moves dO and D (else Q and LSE), rows 16 part ..
+    const int part = sl % (NS / 2);
+    const Span s = span_of(a, b);
+    const int k0 = kb * BN, kw0 = k0 + sl * KW;
+    const float c2 = a.scale * LOG2E;
+    const long row0 = (long)b * a.n_q, key0 = (long)b * a.n_kv;
+
+    // K of the slice as B operands (keys past the end read the last row: not stored)
+    bf16x8 kr[KS][DS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        const bf16 *kp = (const bf16 *)a.k + (key0 + min(kw0 + 16 * ks + c16, a.n_kv - 1)) * a.ldk + kvh * HD + 8 * g;
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds) kr[ks][ds] = ld_frag(kp + 32 * ds);
+    }
+    char *vsl = smem + 2 * STREAM + sl * KW * HD * 2;
+    if (hg == 0) {
+        const sgpr4 rv = head_rows<HD>(a.v, key0 + kw0, a.ldv, kvh * HD, min(KW, s.kl - kw0));
+#pragma unroll
+        for (int i = 0; i < KW / RPI; ++i) dma16_async(rv, vsl + i * 1024, dma_off<HD>(RPI * i, lane, (int)a.ldv));
+    }
+    if (tid < 2 * NBUF) odd[tid / NBUF][tid % NBUF] = 0;
+    wait_vm0();
+    __syncthreads();
+    f32x4 dvt[KS][DSUB], dkt[KS][DSUB];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < DSUB; ++i) dvt[ks][i] = dkt[ks][i] = f32x4{0, 0, 0, 0};
+
+    const int k1 = min(k0 + BN, s.kl) - 1;  // the block's last key
+    const int qstart = max(0, k0 - s.off);
+    const int qend = k0 < a.n_sink ? s.ql : (int)min((long)s.ql, (long)k1 + a.window - s.off);
+    const int nqt = k1 >= k0 && qend > qstart ? (qend - qstart + BM - 1) / BM : 0;
+    const int nsteps = nh * (alt ? (nqt + 1) / 2 : nqt);
+    const int niter = max(0, (nsteps - zpart + zparts - 1) / zparts);
+    char *strm = smem + hg * STREAM;
+    const void *tp = tdo ? a.dout : a.q;
+    const long ldt = tdo ? a.lddo : a.ldq;
+    const float *sp = tdo ? a.d : a.lse;
+    unsigned off[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) off[i] = dma_off<HD>(16 * part + RPI * i, lane, (int)ldt);
+    auto tile_of = [&](int it, int grp, int &h, int &q0) {
+        it = it * zparts + zpart;
+        if (alt) {
+            h = kvh * hpk + it % nh;
+            q0 = qstart + ((nqt + 1) / 2 * 2 - 1 - 2 * (it / nh) - grp) * BM;
+            return;
+        }
+        h = kvh * hpk + grp + 2 * (it % nh);
+        q0 = qstart + (nqt - 1 - it / nh) * BM;
+    };
+    // C DMAs per wave and tile, and one more for the waves that move LSE or D
+    auto dma = [&](int it, int buf) {
+        int h, q0;
+        tile_of(it, hg, h, q0);
+        const int rows = min(BM, s.ql - q0);
+        const sgpr4 rt = head_rows<HD>(tp, row0 + q0, ldt, h * HD, rows);
+        char *dst = strm + buf * 2 * TILE + (tdo ? TILE : 0) + part * 16 * HD * 2;
+#pragma unroll
+        for (int i = 0; i < C; ++i) dma16_async(rt, dst + i * 1024, off[i]);
+        if (part == 0) {
+            const sgpr4 rs = rsrc4(sp + (row0 + q0) * a.n_heads + h, rows > 0 ? (unsigned)(((rows - 1) * a.n_heads + 1) * 4) : 0u);
+            const unsigned so = lane < BM ? (unsigned)(lane * a.n_heads * 4) : kOOB;
+            if (tdo) dma4_async(rs, Dd[hg][buf], so);
+            else dma4_async(rs, Ls[hg][buf], so);
+        }
+    };
+    if (niter > 0) dma(0, 0);
+    if (niter > 1) dma(1, 1);
+    bool any_odd = false;
+    auto step = [&](const int it, auto bufc, auto pairsc) {
+        constexpr int buf = decltype(bufc)::value;
+        constexpr bool PAIRS = decltype(pairsc)::value;
+        if (!PAIRS && it + 1 < niter) {
+            if (part == 0) __builtin_amdgcn_s_waitcnt(0x0f70 | (C + 1));
+            else __builtin_amdgcn_s_waitcnt(0x0f70 | C);
+        } else {
+            wait_vm0();
+        }
+        lds_barrier();
+        if (!PAIRS && it + 2 < niter) dma(it + 2, (buf + 2) % NBUF);
+        int h, q0, hx, qx;
+        tile_of(it, hg, h, q0);
+        tile_of(it, 1 - hg, hx, qx);
+        const char *Qb = strm + buf * 2 * TILE, *Ob = Qb + TILE;
+        // the tile's live positions, and both groups' together (the block decides as one)
+        const int ta = q0 + s.off, tb = min(q0 + BM, s.ql) - 1 + s.off;
+        if (!all_seen(a, min(q0, qx) + s.off, max(q0, qx) + BM - 1 + s.off, k0, k0 + BN - 1)) {
+            if (scan<2 * TILE, 256>(Qb, tid % 256)) odd[hg][buf] = it + 1;
+            lds_barrier();
+            const bool mine = odd[hg][buf] == it + 1;
+            any_odd |= mine || odd[1 - hg][buf] == it + 1;
+            if (mine != PAIRS) return;
+        } else if (PAIRS) {
+            return;
+        }
+        if (none_seen(a, ta, tb, kw0, kw0 + KW - 1)) return;
+        auto dval = [&](int qs, int r) { return Dd[hg][buf][16 * qs + 4 * g + r]; };
+        auto prob = [&](float x, int qs, int r) {
+            return __builtin_amdgcn_exp2f(fmaf(x, c2, -(Ls[hg][buf][16 * qs + 4 * g + r] * LOG2E)));
+        };
+        // the dP accumulators start at -D, so they end as dP - D
+        f32x4 sc[QS][KS], dp[QS][KS];
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs) {
+            const f32x4 nd{-dval(qs, 0), -dval(qs, 1), -dval(qs, 2), -dval(qs, 3)};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                sc[qs][ks] = f32x4{0, 0, 0, 0};
+                dp[qs][ks] = nd;
+            }
+        }
+        // each phase's next fragment is read ahead of this one's MFMAs; the arithmetic of one score
+        // tile rides along with each step of the phase after it
+        bf16x8 fr[2];
+        fr[0] = R::frag_row(Qb, c16, 8 * g);
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            const int ds = f / 2, qs = f % 2, n = f + 1;
+            fr[n & 1] = n < NF ? R::frag_row(Qb, 16 * (n % 2) + c16, 32 * (n / 2) + 8 * g) : R::frag_row(Ob, c16, 8 * g);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) sc[qs][ks] = mfma16x16x32(fr[f & 1], kr[ks][ds], sc[qs][ks]);
+        }
+        bf16x8 vf[KS];
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            const int ds = f / 2, qs = f % 2, n = f + 1;
+            if (qs == 0)
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) vf[ks] = R::frag_row(vsl, 16 * ks + c16, 32 * ds + 8 * g);
+            fr[n & 1] = n < NF ? R::frag_row(Ob, 16 * (n % 2) + c16, 32 * (n / 2) + 8 * g) : R::frag_t(Ob, 0, 0, g, c16);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) dp[qs][ks] = mfma16x16x32(fr[f & 1], vf[ks], dp[qs][ks]);
+            constexpr int EVERY = NF / (QS * KS);
+            static_assert(EVERY >= 1 && EVERY * QS * KS == NF, "exp schedule");
+            if (f % EVERY == 0) {
+                const int t2 = f / EVERY, qs2 = t2 / KS, ks2 = t2 % KS;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sc[qs2][ks2][r] = prob(sc[qs2][ks2][r], qs2, r);
+            }
+        }
+        const bool dead = __any(lane < BM && Ls[hg][buf][lane % BM] == -INFINITY);  // a row of no gradient
+        if (dead || q0 + BM > s.ql || !all_seen(a, ta, tb, kw0, kw0 + KW - 1)) {
+#pragma unroll
+            for (int qs = 0; qs < QS; ++qs)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = q0 + 16 * qs + 4 * g + r;
+                    const bool live = row < s.ql && Ls[hg][buf][16 * qs + 4 * g + r] != -INFINITY;
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks)
+                        if (!sees(a, live ? row + s.off : -1, kw0 + 16 * ks + c16)) sc[qs][ks][r] = dp[qs][ks][r] = 0.f;
+                }
+        }
+        bf16x8 pb[KS][1];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) pb[ks][0] = frag_acc(sc[0][ks], sc[1][ks]);
+        if constexpr (PAIRS) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                auto see = [&](int x) {
+                    return sees(a, q0 + x < s.ql && Ls[hg][buf][x] != -INFINITY ? q0 + x + s.off : -1, kw0 + 16 * ks + c16);
+                };
+#pragma unroll
+                for (int qs = 0; qs < QS; ++qs)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) dp[qs][ks][r] *= sc[qs][ks][r];
+                const bf16x8 sb[1] = {frag_acc(dp[0][ks], dp[1][ks])};
+                add_pairs<HD>(dvt[ks], Ob, pb[ks], wl[wave], lane, see);
+                add_pairs<HD>(dkt[ks], Qb, sb, wl[wave], lane, see);
+            }
+            return;
+        }
+        // dV^T += dO^T P, with dS = P (dP - D)
+#pragma unroll
+        for (int i = 0; i < DSUB; ++i) {
+            const int n = i + 1;
+            fr[n & 1] = n < DSUB ? R::frag_t(Ob, 16 * n, 0, g, c16) : R::frag_t(Qb, 0, 0, g, c16);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) dvt[ks][i] = mfma16x16x32(fr[i & 1], pb[ks][0], dvt[ks][i]);
+            constexpr int EVERY = DSUB / (QS * KS);
+            static_assert(EVERY >= 1 && EVERY * QS * KS == DSUB, "dS schedule");
+            if (i % EVERY == 0) {
+                const int t2 = i / EVERY, qs2 = t2 / KS, ks2 = t2 % KS;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) dp[qs2][ks2][r] = sc[qs2][ks2][r] * dp[qs2][ks2][r];
+            }
+        }
+        // dK^T += Q^T dS
+        bf16x8 sb[KS];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) sb[ks] = frag_acc(dp[0][ks], dp[1][ks]);
+#pragma unroll
+        for (int i = 0; i < DSUB; ++i) {
+            if (i + 1 < DSUB) fr[(i + 1) & 1] = R::frag_t(Qb, 16 * (i + 1), 0, g, c16);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) dkt[ks][i] = mfma16x16x32(fr[i & 1], sb[ks], dkt[ks][i]);
+        }
+    };
+    for (int it0 = 0; it0 < niter; it0 += NBUF) {
+        step(it0, std::integral_constant<int, 0>{}, std::false_type{});
+        if (it0 + 1 < niter) step(it0 + 1, std::integral_constant<int, 1>{}, std::false_type{});
+        if (it0 + 2 < niter) step(it0 + 2, std::integral_constant<int, 2>{}, std::false_type{});
+    }
+    if (any_odd)  // (the same for all waves)
+#pragma unroll 1
+        for (int it = 0; it < niter; ++it) {
+            __syncthreads();
+            if (tid < 2) odd[tid][0] = 0;
+            dma(it, 0);
+            step(it, std::integral_constant<int, 0>{}, std::true_type{});
+        }
+    // the two groups' sums through the (now idle) tile arena: group 0 hands over dK^T and keeps dV^T
+    wait_vm0();
+    __syncthreads();
+    f32x4 *xs = reinterpret_cast<f32x4 *>(smem + (sl * 2 + hg) * XSLOT);
+    const f32x4 *xp = reinterpret_cast<const f32x4 *>(smem + (sl * 2 + (1 - hg)) * XSLOT);
+    auto give = [&](const f32x4 (&x)[KS][DSUB]) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int i = 0; i < DSUB; ++i) xs[(i * KS + ks) * 64 + lane] = x[ks][i];
+    };
+    if (hg == 0) give(dkt);
+    else give(dvt);
+    __syncthreads();
+    auto keep = [&](const f32x4 (&x)[KS][DSUB], auto *base, long ld, bool raw, float mul) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int key = sl * KW + 16 * ks + c16;  // of the block
+            if (!raw && k0 + key >= a.n_kv) continue;
+            const bool live = k0 + key < s.kl;
+            auto *out = base + key * ld + 4 * g;
+#pragma unroll
+            for (int i = 0; i < DSUB; ++i) {
+                const f32x4 v = live ? (x[ks][i] + xp[(i * KS + ks) * 64 + lane]) * mul : f32x4{0, 0, 0, 0};
+                store4(out + 16 * i, v[0], v[1], v[2], v[3]);
+            }
+        }
+    };
+    if (zparts > 1) {
+        float *ws = a.ws + ((long)bk * plan.slots() + slot) * (2 * BN * HD);
+        if (hg == 0) keep(dvt, ws + BN * HD, HD, true, 1.f);
+        else keep(dkt, ws, HD, true, a.scale);
+        return;
+    }
+    if (hg == 0) keep(dvt, (TO *)a.dv + (key0 + k0) * a.lddv + kvh * HD, a.lddv, false, 1.f);
+    else keep(dkt, (TO *)a.dk + (key0 + k0) * a.lddk + kvh * HD, a.lddk, false, a.scale);
+}
+
+// dK and dV of the split key blocks: their parts added in order, four values a thread.
+template <int HD, class TO>
+__global__ __launch_bounds__(256) void window_dkv_sum16_k(WindowArgs a, DkvPlan plan) {
+    const int nbk = a.n_batch * a.n_kv_heads;
+    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
+    const int kb = blockIdx.x / nbk + (plan.sink_parts > 1 ? 0 : plan.sink_blocks);
+    const bool sink = kb < plan.sink_blocks;
+    const int parts = sink ? plan.sink_parts : plan.parts;
+    const int first = sink ? kb * parts : (plan.sink_parts > 1 ? plan.sink_blocks * plan.sink_parts : 0) + (kb - plan.sink_blocks) * parts;
+    const float *ws = a.ws + ((long)bk * plan.slots() + first) * (2 * 128 * HD);
+    const int x = (blockIdx.y * 256 + threadIdx.x) * 4;  // of dK [128][HD], then dV
+    f32x4 t{0, 0, 0, 0};
+    for (int p = 0; p < parts; ++p) t += *reinterpret_cast<const f32x4 *>(ws + (long)p * 2 * 128 * HD + x);
+    const bool v = x >= 128 * HD;
+    const int y = v ? x - 128 * HD : x, key = kb * 128 + y / HD;
+    if (key >= a.n_kv) return;
+    const long row = (long)b * a.n_kv + key;
+    TO *out = v ? (TO *)a.dv + row * a.lddv : (TO *)a.dk + row * a.lddk;
+    store4(out + kvh * HD + y % HD, t[0], t[1], t[2], t[3]);
+}
+
+DkvPlan dkv_plan(const WindowArgs &a, bool ws) {
+    DkvPlan p;
+    p.key_blocks = (a.n_kv + 127) / 128;
+    p.sink_blocks = a.window < a.n_kv ? std::min(p.key_blocks, (a.n_sink + 127) / 128) : 0;
+    p.sink_parts = p.parts = 1;
+    if (!ws) return p;
+    const long nbk = (long)a.n_batch * a.n_kv_heads, blocks = nbk * p.key_blocks, hpk = a.n_heads / a.n_kv_heads;
+    const long most = hpk * ((a.n_q + 31) / 32), usual = std::min(most, hpk * ((std::min<long>(a.n_kv, a.window) + 159) / 32));
+    // towards one block per CU, with at least four steps of both groups each
+    p.parts = (int)std::max(1l, std::min({8l, 256 / blocks, usual / 8}));
+    // a sink block's steps over the usual block's; at most 256 MiB of partial sums
+    p.sink_parts = (int)std::max<long>(p.parts, std::min<long>(64, (most * p.parts + usual - 1) / usual));
+    const long slot = 2 * 128 * a.hd * 4;
+    while (p.sink_parts > 1 && p.sink_blocks * nbk * slot * p.sink_parts > (192l << 20)) --p.sink_parts;
+    while (p.parts > 1 && blocks * slot * p.parts > (64l << 20)) --p.parts;
+    return p;
+}
+
+bool al(const void *x, long ld, int align, int es) { return (uintptr_t)x % align == 0 && ld * es % align == 0; }
+// Heads of 64 or 128 values in rows of aligned 16-byte chunks, a tile's rows within 31 bits of
+// offset, and a scale that keeps the order of the scores.
+bool shape_ok(const WindowArgs &a) {
+    return a.dt == DType::BF16 && (a.hd == 64 || a.hd == 128) && a.scale > 0.f && a.scale < INFINITY &&
+           std::max({a.ldq, a.ldk, a.ldv, a.lddo}) < (1l << 23) && a.n_heads < (1 << 16);
+}
+bool fwd_ok(const WindowArgs &a) {
+    const int es = a.odt == DType::F32 ? 4 : 2;
+    return shape_ok(a) && al(a.q, a.ldq, 16, 2) && al(a.k, a.ldk, 16, 2) && al(a.v, a.ldv, 16, 2) && al(a.o, a.ldo, 4 * es, es);
+}
+bool bwd_ok(const WindowArgs &a) {
+    const int es = a.odt == DType::F32 ? 4 : 2;
+    return fwd_ok(a) && al(a.dout, a.lddo, 16, 2) && al(a.o, a.ldo, 16, es) && al(a.dq, a.lddq, 4 * es, es) &&
+           al(a.dk, a.lddk, 4 * es, es) && al(a.dv, a.lddv, 4 * es, es);
+}
+
+}  // namespace
+
+size_t window16_bwd_ws_bytes(const WindowArgs &a) {
+    if (!shape_ok(a)) return 0;
+    return (size_t)a.n_batch * a.n_kv_heads * dkv_plan(a, true).slots() * 2 * 128 * a.hd * sizeof(float);
+}
+
+bool window16_forward(const WindowArgs &a, hipStream_t st) {
+    if (!fwd_ok(a)) return false;
+    const long per = (long)a.n_heads * a.n_batch;
+    auto go = [&](auto kernel, int bm) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(per * ((a.n_q + bm - 1) / bm))), dim3(256), 0, st, a);
+    };
+    // grids of 128-row blocks that leave the CUs one block each or fewer take 64 rows, two per CU
+    const bool small = per * ((a.n_q + 127) / 128) <= cu_count();
+    auto by = [&](auto to) {
+        using TO = decltype(to);
+        if (a.hd == 128) small ? go(window_fwd16_k<128, 1, TO>, 64) : go(window_fwd16_k<128, 2, TO>, 128);
+        else small ? go(window_fwd16_k<64, 1, TO>, 64) : go(window_fwd16_k<64, 2, TO>, 128);
+    };
+    a.odt == DType::F32 ? by(float{}) : by(bf16{});
+    return true;
+}
+
+bool window16_backward(const WindowArgs &a, hipStream_t st) {
+    if (!bwd_ok(a)) return false;
+    const long per = (long)a.n_heads * a.n_batch, nbk = (long)a.n_batch * a.n_kv_heads;
+    // 256-row dQ blocks where they fill the chip, else 128, else 64 (as the dense backward)
+    const int bq = per * ((a.n_q + 255) / 256) >= 256 ? 256 : per * ((a.n_q + 127) / 128) >= 256 ? 128 : 64;
+    const DkvPlan plan = dkv_plan(a, a.ws != nullptr);
+    auto by = [&](auto hd, auto to) {
+        constexpr int HD = decltype(hd)::value;
+        using TO = decltype(to);
+        auto dq = [&](auto kernel, int nt) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)(per * ((a.n_q + bq - 1) / bq))), dim3(nt), 0, st, a);
+        };
+        if (bq == 256) dq(window_dq16_k<HD, 8, 256, TO>, 512);
+        else if (bq == 128) dq(window_dq16_k<HD, 8, 128, TO>, 512);
+        else dq(window_dq16_k<HD, 4, 64, TO>, 256);
+        hipLaunchKernelGGL((window_dkv16_k<HD, TO>), dim3((unsigned)(nbk * plan.blocks())), dim3(512), 0, st, a, plan);
+        const int split = (plan.sink_parts > 1 ? plan.sink_blocks : 0) + (plan.parts > 1 ? plan.key_blocks - plan.sink_blocks : 0);
+        if (split)
+            hipLaunchKernelGGL((window_dkv_sum16_k<HD, TO>), dim3((unsigned)(nbk * split), HD / 4), dim3(256), 0, st, a, plan);
+    };
+    auto by_head = [&](auto to) {
+        if (a.hd == 128) by(std::integral_constant<int, 128>{}, to);
+        else by(std::integral_constant<int, 64>{}, to);
+    };
+    a.odt == DType::F32 ? by_head(float{}) : by_head(bf16{});
+    return true;
+}
+
+}  // namespace vkh
