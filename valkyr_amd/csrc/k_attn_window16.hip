@@ -13,9 +13,9 @@
 // its offsets stay small however long the cache is, a lane's offset is the same for every tile,
 // and rows past a sequence's end read as zero by the range check.  Masks cost nothing in tiles
 // that every row sees in full.  In the others a masked pair has P = dS = 0, selected, and since
-// 0 times an infinity or a NaN is NaN, the tile that multiplies them is scanned for such values;
-// a tile that holds one (none, in a healthy run) is left out, and after the others its products are
-// added pair by pair, seen pairs only.
+// 0 times an infinity or a NaN is NaN, the tile that multiplies them is scanned for such values: a
+// block that meets one (none does, in a healthy run) forms its rows anew one at a time, from seen
+// pairs only.
 #include <algorithm>
 
 #include "attn16.hpp"
@@ -70,28 +70,6 @@ VKH_DEV unsigned dma_off(int r0, int lane, int ld) {
     return (unsigned)((r * ld + 8 * c) * 2);
 }
 
-// acc[i][r] += sum over the tile's rows x that `see` names of T[x][16 i + 4 g + r] w[x], where w is
-// held as a B operand: element 4 u + e of w[s] is row 32 s + 16 u + 4 g + e.  `wl` is the wave's own
-// LDS (1 KB for each s) that w goes through, so that the loop over rows need not be unrolled.
-template <int HD, int NS, class See>
-VKH_DEV void add_pairs(f32x4 (&acc)[HD / 16], const char *T, const bf16x8 (&w)[NS], bf16x8 *wl, int lane, See see) {
-    const int g = lane / 16, c16 = lane % 16;
-#pragma unroll
-    for (int s = 0; s < NS; ++s) wl[64 * s + lane] = w[s];
-#pragma unroll 1
-    for (int x = 0; x < 32 * NS; ++x) {
-        const bf16 *wp = reinterpret_cast<const bf16 *>(wl + 64 * (x / 32) + x % 16 / 4 * 16 + c16);
-        const float wx = (float)wp[x % 32 / 16 * 4 + x % 4];
-        if (!see(x)) continue;
-#pragma unroll
-        for (int i = 0; i < HD / 16; ++i) {
-            const bf16x4 t = *reinterpret_cast<const bf16x4 *>(T + TileRows<HD>::toff(x, 16 * i + 4 * g));
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[i][r] = fmaf((float)t[r], wx, acc[i][r]);
-        }
-    }
-}
-
 VKH_DEV void store4(float *p, float x, float y, float z, float w) {
     *reinterpret_cast<float4 *>(p) = make_float4(x, y, z, w);
 }
@@ -119,6 +97,52 @@ VKH_DEV KeyTiles key_tiles(const WindowArgs &a, const Span &s, int r0, int r1) {
     return k;
 }
 
+// A kernel's first argument, read anew from where the launch put it (the kernel arguments begin
+// with it): its values need not stay in registers for the calls below.
+VKH_DEV const WindowArgs &args_again() {
+    unsigned long p = (unsigned long)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *reinterpret_cast<const WindowArgs *>(p);
+}
+// A block's rows one at a time, for blocks that met an infinity or a NaN in a tile which some of
+// their rows do not see in full (0 times either is NaN).  Out of line: their registers are not the
+// tile loops'.
+template <class TO>
+__device__ __attribute__((noinline)) void fwd_rows(const WindowArgs &a, int b, int r, int end, int step, int h, float *q,
+                                                   int lane) {
+    for (; r < end; r += step) window_fwd_row<bf16, TO>(a, b, r, h, q, lane);
+}
+template <class TO>
+__device__ __attribute__((noinline)) void dq_rows(const WindowArgs &a, int b, int r, int end, int step, int h, float *q,
+                                                  float *g, int lane) {
+    for (; r < end; r += step) window_dq_row<bf16, TO>(a, b, r, h, q, g, lane);
+}
+// The (query tile, head) steps of one part of a key block, as window_dkv16_k walks them.
+struct Steps {
+    int head0, qstart, top, nh;
+    bool alt;
+    int zpart, zparts;
+    VKH_DEV bool mine(int h, int row) const {
+        const int t = top - (row - qstart) / 32;
+        return ((alt ? t / 2 : t) * nh + (alt ? h - head0 : (h - head0) / 2)) % zparts == zpart;
+    }
+};
+template <int HD, class TO>
+__device__ __attribute__((noinline)) void dkv_rows(const WindowArgs &a, const Steps &st, int b, int kvh, int k0, int wave,
+                                                   float *ws, float *k, float *v, int lane) {
+    auto mine = [&](int h, int row) { return st.mine(h, row); };
+    for (int x = wave; x < 128; x += 8) {
+        if (k0 + x >= a.n_kv) {  // (their slots are read)
+            for (int d = lane; ws && d < HD; d += 64) ws[x * HD + d] = ws[(128 + x) * HD + d] = 0.f;
+            continue;
+        }
+        const long row = (long)b * a.n_kv + k0 + x;
+        if (ws) window_dkv_row<bf16>(a, b, k0 + x, kvh, k, v, ws + x * HD, ws + (128 + x) * HD, lane, mine);
+        else window_dkv_row<bf16>(a, b, k0 + x, kvh, k, v, (TO *)a.dk + row * a.lddk + kvh * HD,
+                                  (TO *)a.dv + row * a.lddv + kvh * HD, lane, mine);
+    }
+}
+
 // ── forward ──────────────────────────────────────────────────────────────
 // Block = 64 QS query rows of one head, 4 waves of 16 QS; 64-key tiles, two buffers.  Block ids run
 // over (sequence, KV head) first, so the blocks of one KV head sit on one XCD and share its
@@ -129,8 +153,6 @@ __global__ __launch_bounds__(256, 2) void window_fwd16_k(WindowArgs a) {
     constexpr int DS = HD / 32, DSUB = HD / 16, BM = 64 * QS, BN = 64, KT = BN * HD * 2;
     constexpr int RPI = 512 / HD, IPW = 16 / RPI;  // rows per DMA, DMAs per wave and tile
     __shared__ __attribute__((aligned(16))) char Ks[2][KT], Vs[2][KT];
-    __shared__ bf16x8 wl[4][128];
-    __shared__ int odd[2];  // odd[buffer] = step + 1 where V is to be added pair by pair
     const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, nqt = (a.n_q + BM - 1) / BM;
     const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
     const int h = kvh * grp + blockIdx.x / nbk % grp, qt = nqt - 1 - (int)(blockIdx.x / nbk / grp);
@@ -159,7 +181,6 @@ __global__ __launch_bounds__(256, 2) void window_fwd16_k(WindowArgs a) {
         ko[i] = dma_off<HD>(16 * wave + RPI * i, lane, (int)a.ldk);
         vo[i] = dma_off<HD>(16 * wave + RPI * i, lane, (int)a.ldv);
     }
-    if (tid < 2) odd[tid] = 0;
     wait_vm0();  // Q fragments are in registers before any DMA is queued
     auto dma = [&](int it, int buf) {
         const int k0 = kt.tile(it) * BN, rows = min(BN, s.kl - k0);
@@ -180,22 +201,15 @@ __global__ __launch_bounds__(256, 2) void window_fwd16_k(WindowArgs a) {
 #pragma unroll
         for (int i = 0; i < DSUB; ++i) oacc[qs][i] = f32x4{0, 0, 0, 0};
     }
-    bool any_odd = false;
-    auto step = [&](const int it, const int buf, auto pairsc) {
-        constexpr bool PAIRS = decltype(pairsc)::value;
+    bool odd = false;  // an infinity or a NaN in V of a tile that is not seen in full
+    auto step = [&](const int it, const int buf) {
         const int k0 = kt.tile(it) * BN;
         wait_vm0();
         lds_barrier();  // tile `it` landed; everyone is done with the other buffer
-        if (!PAIRS && it + 1 < kt.n) dma(it + 1, buf ^ 1);
+        if (it + 1 < kt.n) dma(it + 1, buf ^ 1);
         const char *Kb = Ks[buf], *Vb = Vs[buf];
         if (!all_seen(a, kt.ta, kt.tb, k0, k0 + BN - 1)) {
-            if (scan<KT, 256>(Vb, tid)) odd[buf] = it + 1;
-            lds_barrier();
-            const bool pairs = odd[buf] == it + 1;
-            any_odd |= pairs;
-            if (pairs != PAIRS) return;
-        } else if (PAIRS) {
-            return;
+            if (scan<KT, 256>(Vb, tid)) odd = true;
         }
         if (none_seen(a, wta, wtb, k0, k0 + BN - 1)) return;
 
@@ -253,12 +267,6 @@ __global__ __launch_bounds__(256, 2) void window_fwd16_k(WindowArgs a) {
             pf[qs][0] = frag_acc(st[0][qs], st[1][qs]);
             pf[qs][1] = frag_acc(st[2][qs], st[3][qs]);
         }
-        if constexpr (PAIRS) {
-#pragma unroll
-            for (int qs = 0; qs < QS; ++qs)
-                add_pairs<HD>(oacc[qs], Vb, pf[qs], wl[wave], lane, [&](int x) { return sees(a, pos[qs], k0 + x); });
-            return;
-        }
 #pragma unroll
         for (int kst = 0; kst < 2; ++kst)
 #pragma unroll
@@ -269,15 +277,11 @@ __global__ __launch_bounds__(256, 2) void window_fwd16_k(WindowArgs a) {
             }
     };
     if (kt.n > 0) dma(0, 0);
-    for (int it = 0; it < kt.n; ++it) step(it, it & 1, std::false_type{});
-    if (any_odd)  // (the same for all waves)
-#pragma unroll 1
-        for (int it = 0; it < kt.n; ++it) {
-            __syncthreads();
-            if (tid == 0) odd[0] = 0;
-            dma(it, 0);
-            step(it, 0, std::true_type{});
-        }
+    for (int it = 0; it < kt.n; ++it) step(it, it & 1);
+    if (__syncthreads_or(odd)) {
+        fwd_rows<TO>(args_again(), b, r0 + wave, min(r0 + BM, a.n_q), 4, h, (float *)Ks + wave * HD, lane);
+        return;
+    }
 #pragma unroll
     for (int qs = 0; qs < QS; ++qs) {
         const int r = qw0 + 16 * qs + c16;
@@ -309,8 +313,6 @@ __global__ __launch_bounds__(NWV * 64, 1) void window_dq16_k(WindowArgs a) {
     constexpr int RPI = 512 / HD, IPT = BN / RPI, C = 2 * IPT / NWV;  // DMAs per tile and tensor, per wave
     static_assert(C >= 1 && C * NWV == 2 * IPT, "DMA share");
     __shared__ __attribute__((aligned(16))) char Kt[NBUF][TILE], Vt[NBUF][TILE];
-    __shared__ bf16x8 wl[NWV][64];
-    __shared__ int odd[NBUF];
     const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, nqb = (a.n_q + BQ - 1) / BQ;
     const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
     const int h = kvh * grp + blockIdx.x / nbk % grp, qb = nqb - 1 - (int)(blockIdx.x / nbk / grp);
@@ -361,7 +363,6 @@ __global__ __launch_bounds__(NWV * 64, 1) void window_dq16_k(WindowArgs a) {
         const int q = C * wave + i;
         off[i] = dma_off<HD>(q % IPT * RPI, lane, (int)(q < IPT ? a.ldk : a.ldv));
     }
-    if (tid < NBUF) odd[tid] = 0;
     wait_vm0();
     auto dma = [&](int it, int buf) {
         const int k0 = kt.tile(it) * BN, rows = min(BN, s.kl - k0);
@@ -382,24 +383,17 @@ __global__ __launch_bounds__(NWV * 64, 1) void window_dq16_k(WindowArgs a) {
     if (kt.n > 0) dma(0, 0);
     if (kt.n > 1) dma(1, 1);
     // unrolled over the three buffers: every LDS address is a lane's base plus a constant
-    bool any_odd = false;
-    auto step = [&](const int it, auto bufc, auto pairsc) {
+    bool odd = false;  // an infinity or a NaN in K of a tile that is not seen in full
+    auto step = [&](const int it, auto bufc) {
         constexpr int buf = decltype(bufc)::value;
-        constexpr bool PAIRS = decltype(pairsc)::value;
-        if (!PAIRS && it + 1 < kt.n) __builtin_amdgcn_s_waitcnt(0x0f70 | C);
+        if (it + 1 < kt.n) __builtin_amdgcn_s_waitcnt(0x0f70 | C);
         else wait_vm0();
         lds_barrier();
-        if (!PAIRS && it + 2 < kt.n) dma(it + 2, (buf + 2) % NBUF);
+        if (it + 2 < kt.n) dma(it + 2, (buf + 2) % NBUF);
         const int k0 = kt.tile(it) * BN;
         const char *Kb = Kt[buf], *Vb = Vt[buf];
         if (!all_seen(a, kt.ta, kt.tb, k0, k0 + BN - 1)) {
-            if (scan<TILE, NWV * 64>(Kb, tid)) odd[buf] = it + 1;
-            lds_barrier();
-            const bool pairs = odd[buf] == it + 1;
-            any_odd |= pairs;
-            if (pairs != PAIRS) return;
-        } else if (PAIRS) {
-            return;
+            if (scan<TILE, NWV * 64>(Kb, tid)) odd = true;
         }
         if (none_seen(a, wta, wtb, k0, k0 + BN - 1)) return;
         // the dP^T accumulators start at -D (one query per lane), so they end as dP^T - D
@@ -449,7 +443,7 @@ __global__ __launch_bounds__(NWV * 64, 1) void window_dq16_k(WindowArgs a) {
 #pragma unroll
         for (int j = 0; j < QSUB; ++j) live = live && pos[j] >= 0;
         whole = whole && __all(live);
-        bf16x8 sb[QSUB][1];
+        bf16x8 sb[QSUB];
 #pragma unroll
         for (int j = 0; j < QSUB; ++j) {
 #pragma unroll
@@ -463,13 +457,7 @@ __global__ __launch_bounds__(NWV * 64, 1) void window_dq16_k(WindowArgs a) {
                     for (int r = 0; r < 4; ++r)
                         if (!sees(a, pos[j], k0 + 16 * ks + 4 * g + r)) dpt[ks][j][r] = 0.f;
             }
-            sb[j][0] = frag_acc(dpt[0][j], dpt[1][j]);
-        }
-        if constexpr (PAIRS) {
-#pragma unroll
-            for (int j = 0; j < QSUB; ++j)
-                add_pairs<HD>(acc[j], Kb, sb[j], wl[wave], lane, [&](int x) { return sees(a, pos[j], k0 + x); });
-            return;
+            sb[j] = frag_acc(dpt[0][j], dpt[1][j]);
         }
         // dQ^T += K^T dS^T
 #pragma unroll
@@ -477,22 +465,19 @@ __global__ __launch_bounds__(NWV * 64, 1) void window_dq16_k(WindowArgs a) {
             const int n = 2 * NF + i;
             if (n + PD < 2 * NF + DSUB) fr[(n + PD) % RING] = ldslot(n + PD);
 #pragma unroll
-            for (int j = 0; j < QSUB; ++j) acc[j][i] = mfma16x16x32(fr[n % RING], sb[j][0], acc[j][i]);
+            for (int j = 0; j < QSUB; ++j) acc[j][i] = mfma16x16x32(fr[n % RING], sb[j], acc[j][i]);
         }
     };
     for (int t0 = 0; t0 < kt.n; t0 += NBUF) {
-        step(t0, std::integral_constant<int, 0>{}, std::false_type{});
-        if (t0 + 1 < kt.n) step(t0 + 1, std::integral_constant<int, 1>{}, std::false_type{});
-        if (t0 + 2 < kt.n) step(t0 + 2, std::integral_constant<int, 2>{}, std::false_type{});
+        step(t0, std::integral_constant<int, 0>{});
+        if (t0 + 1 < kt.n) step(t0 + 1, std::integral_constant<int, 1>{});
+        if (t0 + 2 < kt.n) step(t0 + 2, std::integral_constant<int, 2>{});
     }
-    if (any_odd)  // (the same for all waves)
-#pragma unroll 1
-        for (int it = 0; it < kt.n; ++it) {
-            __syncthreads();
-            if (tid == 0) odd[0] = 0;
-            dma(it, 0);
-            step(it, std::integral_constant<int, 0>{}, std::true_type{});
-        }
+    if (__syncthreads_or(odd)) {
+        float *sh = (float *)Kt + wave * 2 * HD;
+        dq_rows<TO>(args_again(), b, r0 + wave, min(r0 + BQ, a.n_q), NWV, h, sh, sh + HD, lane);
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < QSUB; ++j) {
         const int r = qw0 + 16 * j + c16;
@@ -544,8 +529,6 @@ __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan p
     constexpr int RPI = 512 / HD, C = 16 / RPI;  // rows per DMA; a wave's DMAs per tile (16 rows)
     __shared__ __attribute__((aligned(16))) char smem[LDS];
     __shared__ __attribute__((aligned(16))) float Ls[2][NBUF][64], Dd[2][NBUF][64];
-    __shared__ bf16x8 wl[8][64];
-    __shared__ int odd[2][NBUF];
 
     const int nbk = a.n_batch * a.n_kv_heads;
     const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
@@ -578,7 +561,6 @@ __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan p
 #pragma unroll
         for (int i = 0; i < KW / RPI; ++i) dma16_async(rv, vsl + i * 1024, dma_off<HD>(RPI * i, lane, (int)a.ldv));
     }
-    if (tid < 2 * NBUF) odd[tid / NBUF][tid % NBUF] = 0;
     wait_vm0();
     __syncthreads();
     f32x4 dvt[KS][DSUB], dkt[KS][DSUB];
@@ -597,64 +579,58 @@ __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan p
     const void *tp = tdo ? a.dout : a.q;
     const long ldt = tdo ? a.lddo : a.ldq;
     const float *sp = tdo ? a.d : a.lse;
-    unsigned off[C];
-#pragma unroll
-    for (int i = 0; i < C; ++i) off[i] = dma_off<HD>(16 * part + RPI * i, lane, (int)ldt);
-    auto tile_of = [&](int it, int grp, int &h, int &q0) {
-        it = it * zparts + zpart;
-        if (alt) {
-            h = kvh * hpk + it % nh;
-            q0 = qstart + ((nqt + 1) / 2 * 2 - 1 - 2 * (it / nh) - grp) * BM;
-            return;
-        }
-        h = kvh * hpk + grp + 2 * (it % nh);
-        q0 = qstart + (nqt - 1 - it / nh) * BM;
+    // A cursor runs over the block's steps zpart, zpart + zparts, ... of (query tile, head), heads
+    // inner; the group's tile and head of a step.
+    struct Cursor {
+        int head, tile;
     };
+    const int dh = zparts % nh, dt = zparts / nh;
+    auto advance = [&](Cursor &c) {
+        c.head += dh;
+        c.tile += dt;
+        if (c.head >= nh) c.head -= nh, ++c.tile;
+    };
+    const int top = alt ? (nqt + 1) / 2 * 2 - 1 : nqt - 1;  // the last tile (alt: of a pair)
+    auto head_of = [&](const Cursor &c) { return kvh * hpk + (alt ? c.head : hg + 2 * c.head); };
+    auto row_of = [&](const Cursor &c) { return qstart + (top - (alt ? 2 * c.tile + hg : c.tile)) * BM; };
+    Cursor ahead{zpart % nh, zpart / nh}, now = ahead;
     // C DMAs per wave and tile, and one more for the waves that move LSE or D
-    auto dma = [&](int it, int buf) {
-        int h, q0;
-        tile_of(it, hg, h, q0);
-        const int rows = min(BM, s.ql - q0);
+    // (the lane id is laundered so that the offsets are recomputed here rather than held in
+    // registers across the loop: spilled, their reloads would wait for the DMA in flight)
+    auto dma = [&](int buf) {
+        const int h = head_of(ahead), q0 = row_of(ahead), rows = min(BM, s.ql - q0);
+        advance(ahead);
         const sgpr4 rt = head_rows<HD>(tp, row0 + q0, ldt, h * HD, rows);
         char *dst = strm + buf * 2 * TILE + (tdo ? TILE : 0) + part * 16 * HD * 2;
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
 #pragma unroll
-        for (int i = 0; i < C; ++i) dma16_async(rt, dst + i * 1024, off[i]);
+        for (int i = 0; i < C; ++i) dma16_async(rt, dst + i * 1024, dma_off<HD>(16 * part + RPI * i, ln, (int)ldt));
         if (part == 0) {
             const sgpr4 rs = rsrc4(sp + (row0 + q0) * a.n_heads + h, rows > 0 ? (unsigned)(((rows - 1) * a.n_heads + 1) * 4) : 0u);
-            const unsigned so = lane < BM ? (unsigned)(lane * a.n_heads * 4) : kOOB;
+            const unsigned so = ln < BM ? (unsigned)(ln * a.n_heads * 4) : kOOB;
             if (tdo) dma4_async(rs, Dd[hg][buf], so);
             else dma4_async(rs, Ls[hg][buf], so);
         }
     };
-    if (niter > 0) dma(0, 0);
-    if (niter > 1) dma(1, 1);
-    bool any_odd = false;
-    auto step = [&](const int it, auto bufc, auto pairsc) {
+    if (niter > 0) dma(0);
+    if (niter > 1) dma(1);
+    bool odd = false;  // an infinity or a NaN in Q or dO of a tile whose rows do not all see all keys
+    auto step = [&](const int it, auto bufc) {
         constexpr int buf = decltype(bufc)::value;
-        constexpr bool PAIRS = decltype(pairsc)::value;
-        if (!PAIRS && it + 1 < niter) {
+        if (it + 1 < niter) {
             if (part == 0) __builtin_amdgcn_s_waitcnt(0x0f70 | (C + 1));
             else __builtin_amdgcn_s_waitcnt(0x0f70 | C);
         } else {
             wait_vm0();
         }
         lds_barrier();
-        if (!PAIRS && it + 2 < niter) dma(it + 2, (buf + 2) % NBUF);
-        int h, q0, hx, qx;
-        tile_of(it, hg, h, q0);
-        tile_of(it, 1 - hg, hx, qx);
+        if (it + 2 < niter) dma((buf + 2) % NBUF);
+        const int q0 = row_of(now);
+        advance(now);
         const char *Qb = strm + buf * 2 * TILE, *Ob = Qb + TILE;
-        // the tile's live positions, and both groups' together (the block decides as one)
-        const int ta = q0 + s.off, tb = min(q0 + BM, s.ql) - 1 + s.off;
-        if (!all_seen(a, min(q0, qx) + s.off, max(q0, qx) + BM - 1 + s.off, k0, k0 + BN - 1)) {
-            if (scan<2 * TILE, 256>(Qb, tid % 256)) odd[hg][buf] = it + 1;
-            lds_barrier();
-            const bool mine = odd[hg][buf] == it + 1;
-            any_odd |= mine || odd[1 - hg][buf] == it + 1;
-            if (mine != PAIRS) return;
-        } else if (PAIRS) {
-            return;
-        }
+        const int ta = q0 + s.off, tb = min(q0 + BM, s.ql) - 1 + s.off;  // the tile's live positions
+        if (!all_seen(a, ta, tb, k0, k0 + BN - 1)) odd |= scan<2 * TILE, 256>(Qb, tid % 256);
         if (none_seen(a, ta, tb, kw0, kw0 + KW - 1)) return;
         auto dval = [&](int qs, int r) { return Dd[hg][buf][16 * qs + 4 * g + r]; };
         auto prob = [&](float x, int qs, int r) {
@@ -713,32 +689,16 @@ __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan p
                         if (!sees(a, live ? row + s.off : -1, kw0 + 16 * ks + c16)) sc[qs][ks][r] = dp[qs][ks][r] = 0.f;
                 }
         }
-        bf16x8 pb[KS][1];
+        bf16x8 pb[KS];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) pb[ks][0] = frag_acc(sc[0][ks], sc[1][ks]);
-        if constexpr (PAIRS) {
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                auto see = [&](int x) {
-                    return sees(a, q0 + x < s.ql && Ls[hg][buf][x] != -INFINITY ? q0 + x + s.off : -1, kw0 + 16 * ks + c16);
-                };
-#pragma unroll
-                for (int qs = 0; qs < QS; ++qs)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) dp[qs][ks][r] *= sc[qs][ks][r];
-                const bf16x8 sb[1] = {frag_acc(dp[0][ks], dp[1][ks])};
-                add_pairs<HD>(dvt[ks], Ob, pb[ks], wl[wave], lane, see);
-                add_pairs<HD>(dkt[ks], Qb, sb, wl[wave], lane, see);
-            }
-            return;
-        }
+        for (int ks = 0; ks < KS; ++ks) pb[ks] = frag_acc(sc[0][ks], sc[1][ks]);
         // dV^T += dO^T P, with dS = P (dP - D)
 #pragma unroll
         for (int i = 0; i < DSUB; ++i) {
             const int n = i + 1;
             fr[n & 1] = n < DSUB ? R::frag_t(Ob, 16 * n, 0, g, c16) : R::frag_t(Qb, 0, 0, g, c16);
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) dvt[ks][i] = mfma16x16x32(fr[i & 1], pb[ks][0], dvt[ks][i]);
+            for (int ks = 0; ks < KS; ++ks) dvt[ks][i] = mfma16x16x32(fr[i & 1], pb[ks], dvt[ks][i]);
             constexpr int EVERY = DSUB / (QS * KS);
             static_assert(EVERY >= 1 && EVERY * QS * KS == DSUB, "dS schedule");
             if (i % EVERY == 0) {
@@ -759,18 +719,17 @@ __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan p
         }
     };
     for (int it0 = 0; it0 < niter; it0 += NBUF) {
-        step(it0, std::integral_constant<int, 0>{}, std::false_type{});
-        if (it0 + 1 < niter) step(it0 + 1, std::integral_constant<int, 1>{}, std::false_type{});
-        if (it0 + 2 < niter) step(it0 + 2, std::integral_constant<int, 2>{}, std::false_type{});
+        step(it0, std::integral_constant<int, 0>{});
+        if (it0 + 1 < niter) step(it0 + 1, std::integral_constant<int, 1>{});
+        if (it0 + 2 < niter) step(it0 + 2, std::integral_constant<int, 2>{});
     }
-    if (any_odd)  // (the same for all waves)
-#pragma unroll 1
-        for (int it = 0; it < niter; ++it) {
-            __syncthreads();
-            if (tid < 2) odd[tid][0] = 0;
-            dma(it, 0);
-            step(it, std::integral_constant<int, 0>{}, std::true_type{});
-        }
+    float *ws = zparts > 1 ? a.ws + ((long)bk * plan.slots() + slot) * (2 * BN * HD) : nullptr;
+    if (__syncthreads_or(odd)) {
+        float *sh = (float *)smem + wave * 2 * HD;
+        const Steps st{kvh * hpk, qstart, top, nh, alt, zpart, zparts};
+        dkv_rows<HD, TO>(args_again(), st, b, kvh, k0, wave, ws, sh, sh + HD, lane);
+        return;
+    }
     // the two groups' sums through the (now idle) tile arena: group 0 hands over dK^T and keeps dV^T
     wait_vm0();
     __syncthreads();
@@ -800,7 +759,6 @@ __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan p
         }
     };
     if (zparts > 1) {
-        float *ws = a.ws + ((long)bk * plan.slots() + slot) * (2 * BN * HD);
         if (hg == 0) keep(dvt, ws + BN * HD, HD, true, 1.f);
         else keep(dkt, ws, HD, true, a.scale);
         return;
