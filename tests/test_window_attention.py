@@ -221,6 +221,9 @@ SHAPES = [
     (1, 300, 300, 2, 2, 64, 0, 0),
     (1, 321, 400, 4, 2, 128, 500, 3),
     (1, 330, 330, 4, 2, 64, 90, 600),
+    (1, 13, 1200, 8, 1, 64, 500, 2),
+    (2, 16, 300, 6, 2, 128, 40, 35),
+    (1, 17, 300, 6, 2, 128, 40, 35),
     # other head widths
     (1, 37, 50, 4, 2, 32, 20, 2),
     (2, 33, 33, 2, 1, 80, 9, 1),

@@ -58,11 +58,11 @@ unsigned row_blocks(long rows) { return (unsigned)((rows + WPB - 1) / WPB); }
 
 }  // namespace
 
-size_t window_fwd_ws_bytes(const WindowArgs &) { return 0; }
-size_t window_bwd_ws_bytes(const WindowArgs &a) { return window16_bwd_ws_bytes(a); }
+size_t window_fwd_ws_bytes(const WindowArgs &a) { return window16_fwd_ws_bytes(a) + window32_fwd_ws_bytes(a); }
+size_t window_bwd_ws_bytes(const WindowArgs &a) { return window16_bwd_ws_bytes(a) + window32_bwd_ws_bytes(a); }
 
 hipError_t window_forward(const WindowArgs &a, hipStream_t st) {
-    if (window16_forward(a, st)) return hipGetLastError();
+    if (window16_forward(a, st) || window32_forward(a, st)) return hipGetLastError();
     by_types(a, [&](auto t, auto o) {
         hipLaunchKernelGGL((window_fwd_any_k<decltype(t), decltype(o)>),
                            dim3(row_blocks((long)a.n_batch * a.n_q * a.n_heads)), dim3(WNT), 0, st, a);
@@ -71,7 +71,7 @@ hipError_t window_forward(const WindowArgs &a, hipStream_t st) {
 }
 
 hipError_t window_backward(const WindowArgs &a, hipStream_t st) {
-    if (window16_backward(a, st)) return hipGetLastError();
+    if (window16_backward(a, st) || window32_backward(a, st)) return hipGetLastError();
     by_types(a, [&](auto t, auto o) {
         hipLaunchKernelGGL((window_dq_any_k<decltype(t), decltype(o)>),
                            dim3(row_blocks((long)a.n_batch * a.n_q * a.n_heads)), dim3(WNT), 0, st, a);

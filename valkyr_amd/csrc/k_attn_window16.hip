@@ -24,22 +24,6 @@
 namespace vkh {
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LN2 = 0.6931471805599453f;
-constexpr int kAll = 0x7fffffff;  // the window of a sink
-
-// Whether position t sees key j (t = -1: a row that sees none).
-VKH_DEV bool sees(const WindowArgs &a, int t, int j) {
-    return (unsigned)(t - j) < (unsigned)(j < a.n_sink ? kAll : a.window);
-}
-// Whether all positions ta .. tb see all keys j0 .. j1, or none sees any.
-VKH_DEV bool all_seen(const WindowArgs &a, int ta, int tb, int j0, int j1) {
-    return j1 <= ta && (j0 > tb - a.window || j1 < a.n_sink);
-}
-VKH_DEV bool none_seen(const WindowArgs &a, int ta, int tb, int j0, int j1) {
-    return tb < ta || j0 > tb || (j1 <= ta - a.window && j0 >= a.n_sink);
-}
-
 VKH_DEV bool not_finite(uint4 v) {
     bool bad = false;
 #pragma unroll
@@ -70,40 +54,6 @@ VKH_DEV unsigned dma_off(int r0, int lane, int ld) {
     return (unsigned)((r * ld + 8 * c) * 2);
 }
 
-VKH_DEV void store4(float *p, float x, float y, float z, float w) {
-    *reinterpret_cast<float4 *>(p) = make_float4(x, y, z, w);
-}
-VKH_DEV void store4(bf16 *p, float x, float y, float z, float w) {
-    bf16x4 o;
-    o[0] = (bf16)x; o[1] = (bf16)y; o[2] = (bf16)z; o[3] = (bf16)w;
-    *reinterpret_cast<bf16x4 *>(p) = o;
-}
-
-// The key tiles (of BN keys) that a block of query rows r0 .. r1 - 1 walks: those of the sinks that
-// lie before its window, then its window's.
-struct KeyTiles {
-    int ta, tb;     // live positions (tb < ta: none)
-    int n_sink, w0, n;
-    VKH_DEV int tile(int it) const { return it < n_sink ? it : w0 + it - n_sink; }
-};
-template <int BN>
-VKH_DEV KeyTiles key_tiles(const WindowArgs &a, const Span &s, int r0, int r1) {
-    KeyTiles k;
-    k.ta = max(0, r0 + s.off);
-    k.tb = min(r1, s.ql) - 1 + s.off;
-    k.w0 = max(0, k.ta - a.window + 1) / BN;
-    k.n_sink = min((a.n_sink + BN - 1) / BN, k.w0);
-    k.n = k.tb >= k.ta ? k.n_sink + k.tb / BN - k.w0 + 1 : 0;
-    return k;
-}
-
-// A kernel's first argument, read anew from where the launch put it (the kernel arguments begin
-// with it): its values need not stay in registers for the calls below.
-VKH_DEV const WindowArgs &args_again() {
-    unsigned long p = (unsigned long)__builtin_amdgcn_kernarg_segment_ptr();
-    asm volatile("" : "+s"(p));
-    return *reinterpret_cast<const WindowArgs *>(p);
-}
 // A block's rows one at a time, for blocks that met an infinity or a NaN in a tile which some of
 // their rows do not see in full (0 times either is NaN).  Out of line: their registers are not the
 // tile loops'.
@@ -117,16 +67,6 @@ __device__ __attribute__((noinline)) void dq_rows(const WindowArgs &a, int b, in
                                                   float *g, int lane) {
     for (; r < end; r += step) window_dq_row<bf16, TO>(a, b, r, h, q, g, lane);
 }
-// The (query tile, head) steps of one part of a key block, as window_dkv16_k walks them.
-struct Steps {
-    int head0, qstart, top, nh;
-    bool alt;
-    int zpart, zparts;
-    VKH_DEV bool mine(int h, int row) const {
-        const int t = top - (row - qstart) / 32;
-        return ((alt ? t / 2 : t) * nh + (alt ? h - head0 : (h - head0) / 2)) % zparts == zpart;
-    }
-};
 template <int HD, class TO>
 __device__ __attribute__((noinline)) void dkv_rows(const WindowArgs &a, const Steps &st, int b, int kvh, int k0, int wave,
                                                    float *ws, float *k, float *v, int lane) {
@@ -298,6 +238,190 @@ __global__ __launch_bounds__(256, 2) void window_fwd16_k(WindowArgs a) {
         if (a.lse && g == 0)
             a.lse[(row0 + r) * a.n_heads + h] = dead ? -INFINITY : (m[qs] + log2f(lt)) * LN2;
     }
+}
+
+// ── forward of a few rows ────────────────────────────────────────────────
+// One new token against a cache, or a few: bound by reading K and V.  The rows of all query heads
+// of a KV head (row m = query row m / group, head m % group) share each key that is read, 16 at a
+// time; each of the 4 waves streams 32-key tiles of its own (two in LDS, no barrier between the
+// waves), every fourth of the block's, and their results are joined at the end.  `splits` blocks
+// share a KV head's tiles; their results (maximum, sum, O in fp32) go to a.ws and
+// window_join_k joins them in order.
+template <int N>
+VKH_DEV void wait_vm() {
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4 << 14));
+}
+// acc[i][r] += sum over the tile's rows x that `see` names of T[x][16 i + 4 g + r] w[x], where w is
+// held as a B operand: element 4 u + e is row 16 u + 4 g + e.  It goes through `wl`, 1 KB of the
+// wave's own LDS.
+template <int HD, class See>
+VKH_DEV void add_pairs(f32x4 (&acc)[HD / 16], const char *T, const bf16x8 &w, bf16x8 *wl, int lane, See see) {
+    const int g = lane / 16, c16 = lane % 16;
+    wl[lane] = w;
+    wave_lds();
+#pragma unroll 1
+    for (int x = 0; x < 32; ++x) {
+        const float wx = (float)reinterpret_cast<const bf16 *>(wl + x % 16 / 4 * 16 + c16)[x / 16 * 4 + x % 4];
+        if (!see(x)) continue;
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) {
+            const bf16x4 t = *reinterpret_cast<const bf16x4 *>(T + TileRows<HD>::toff(x, 16 * i + 4 * g));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][r] = fmaf((float)t[r], wx, acc[i][r]);
+        }
+    }
+}
+template <int HD, class TO>
+__global__ __launch_bounds__(256, 1) void window_step16_k(WindowArgs a, int splits) {
+    using R = TileRows<HD>;
+    constexpr int DS = HD / 32, DSUB = HD / 16, BN = 32, TILE = BN * HD * 2, RPI = 512 / HD, IPT = BN / RPI;
+    constexpr int RL = HD + 4;  // floats of a result row in LDS
+    __shared__ __attribute__((aligned(16))) char tiles[4][2][2][TILE];
+    __shared__ bf16x8 wl[4][64];
+    __shared__ float ml[4][2][16];
+    static_assert(16 * RL * 4 <= 4 * TILE, "a wave's result fits its tiles");
+    const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, M = a.n_q * grp, RT = (M + 15) / 16;
+    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
+    const int rt = blockIdx.x / nbk % RT, split = blockIdx.x / nbk / RT;
+    const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c16 = lane % 16;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const Span s = span_of(a, b);
+    const KeyTiles kt = key_tiles<BN>(a, s, rt * 16 / grp, (min(M, rt * 16 + 16) - 1) / grp + 1);
+    const int per = (kt.n + splits - 1) / splits, last = min(kt.n, (split + 1) * per);
+    const float c2 = a.scale * LOG2E;
+    const long key0 = (long)b * a.n_kv;
+    char *Kt = tiles[wave][0][0], *Vt = tiles[wave][1][0];
+
+    const int m16 = rt * 16 + c16, row = m16 / grp, h = kvh * grp + m16 % grp;
+    const int pos = m16 < M && row < s.ql ? max(-1, row + s.off) : -1;
+    bf16x8 qf[DS];
+    {
+        const bf16 *qr = (const bf16 *)a.q + ((long)b * a.n_q + row) * a.ldq + h * HD + 8 * g;
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds) qf[ds] = pos >= 0 ? ld_frag(qr + 32 * ds) : bf16x8{};
+    }
+    unsigned ko[IPT], vo[IPT];
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) {
+        ko[i] = dma_off<HD>(RPI * i, lane, (int)a.ldk);
+        vo[i] = dma_off<HD>(RPI * i, lane, (int)a.ldv);
+    }
+    const bool live = __all(pos >= 0);
+    wait_vm0();
+    auto dma = [&](int it, int buf) {
+        const int k0 = kt.tile(it) * BN, rows = min(BN, s.kl - k0);
+        const sgpr4 rk = head_rows<HD>(a.k, key0 + k0, a.ldk, kvh * HD, rows);
+        const sgpr4 rv = head_rows<HD>(a.v, key0 + k0, a.ldv, kvh * HD, rows);
+#pragma unroll
+        for (int i = 0; i < IPT; ++i) dma16_async(rk, Kt + buf * TILE + i * 1024, ko[i]);
+#pragma unroll
+        for (int i = 0; i < IPT; ++i) dma16_async(rv, Vt + buf * TILE + i * 1024, vo[i]);
+    };
+    f32x4 acc[DSUB];
+#pragma unroll
+    for (int i = 0; i < DSUB; ++i) acc[i] = f32x4{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.f;
+    const int it0 = split * per + wave;
+    if (it0 < last) dma(it0, 0);
+    if (it0 + 4 < last) dma(it0 + 4, 1);
+    for (int it = it0, buf = 0; it < last; it += 4, buf ^= 1) {
+        const int k0 = kt.tile(it) * BN;
+        const char *Kb = Kt + buf * TILE, *Vb = Vt + buf * TILE;
+        // its K and V are here (the next tile's may still be on their way)
+        if (it + 4 < last) wait_vm<2 * IPT>();
+        else wait_vm0();
+        asm volatile("" ::: "memory");
+        const bool whole = live && all_seen(a, kt.ta, kt.tb, k0, k0 + BN - 1);
+        f32x4 st[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+                st[ks] = mfma16x16x32(R::frag_row(Kb, 16 * ks + c16, 32 * ds + 8 * g), qf[ds], st[ks]);
+        if (!whole) {
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (!sees(a, pos, k0 + 16 * ks + 4 * g + r)) st[ks][r] = -INFINITY;
+        }
+        float mt = -INFINITY;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mt = fmaxf(mt, st[ks][r]);
+        if (__any(mt * c2 > m + 8.f)) {  // (as in the forward above)
+            const float mn = xrow_max(mt) * c2, mo = m;
+            if (mn > mo + 8.f) m = mn;
+            const float so = m == mo ? 1.f : __builtin_amdgcn_exp2f(mo - m);
+            l *= so;
+#pragma unroll
+            for (int i = 0; i < DSUB; ++i) acc[i] *= so;
+        }
+        const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(st[ks][r], c2, -ms));
+                st[ks][r] = p;
+                l += p;
+            }
+        const bf16x8 pf = frag_acc(st[0], st[1]);
+        if (!whole && __any(scan<TILE, 64>(Vb, lane))) {
+            add_pairs<HD>(acc, Vb, pf, wl[wave], lane, [&](int x) { return sees(a, pos, k0 + x); });
+        } else {
+#pragma unroll
+            for (int i = 0; i < DSUB; ++i) acc[i] = mfma16x16x32(R::frag_t(Vb, 16 * i, 0, g, c16), pf, acc[i]);
+        }
+        if (it + 8 < last) {
+            wave_lds();  // this buffer's reads are done
+            dma(it + 8, buf);
+        }
+    }
+    // the four waves' results: rows of HD floats over their own tiles, maximum and sum beside them
+    wave_lds();
+    float *res = reinterpret_cast<float *>(tiles[wave]);
+    const float lt = xrow_sum(l);
+#pragma unroll
+    for (int i = 0; i < DSUB; ++i) *reinterpret_cast<f32x4 *>(res + c16 * RL + 16 * i + 4 * g) = acc[i];
+    if (g == 0) ml[wave][0][c16] = m, ml[wave][1][c16] = lt;
+    __syncthreads();
+    constexpr int E = HD / 16;  // values per thread
+    const int r = tid / 16, d0 = tid % 16 * E;
+    float mx = -INFINITY, sum = 0.f, o[E] = {};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mx = fmaxf(mx, ml[w][0][r]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float lw = ml[w][1][r], f = lw == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[w][0][r] - (mx == -INFINITY ? 0.f : mx));
+        if (lw == 0.f) continue;
+        sum = fmaf(lw, f, sum);
+        const float *src = reinterpret_cast<const float *>(tiles[w]) + r * RL + d0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(src[e], f, o[e]);
+    }
+    const int mr = rt * 16 + r;
+    if (mr >= M) return;
+    const long orow = (long)b * a.n_q + mr / grp;
+    const int oh = kvh * grp + mr % grp;
+    if (splits > 1) {  // [split][row][head]: HD values; behind them all, maximum and sum
+        const long rows = (long)a.n_batch * a.n_q * a.n_heads, at = (split * rows) + orow * a.n_heads + oh;
+        float *dst = a.ws + at * HD + d0;
+#pragma unroll
+        for (int e = 0; e < E; e += 4) store4(dst + e, o[e], o[e + 1], o[e + 2], o[e + 3]);
+        if (d0 == 0) {
+            float *st = a.ws + splits * rows * HD + at * 2;
+            st[0] = mx;
+            st[1] = sum;
+        }
+        return;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    TO *out = (TO *)a.o + orow * a.ldo + oh * HD + d0;
+#pragma unroll
+    for (int e = 0; e < E; e += 4) store4(out + e, o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+    if (a.lse && d0 == 0) a.lse[orow * a.n_heads + oh] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * LN2;
 }
 
 // ── backward: D and dQ ───────────────────────────────────────────────────
@@ -500,25 +624,7 @@ __global__ __launch_bounds__(NWV * 64, 1) void window_dq16_k(WindowArgs a) {
 // its window, or to the last row of all where the block holds sinks; such a block has a share of
 // work as many times the others' as the sequence is longer than the window, and is split between
 // `parts` blocks, as all blocks are where they are too few for the chip.  Parts write fp32 sums
-// to their slots of a.ws, which window_dkv_sum16_k adds in order.
-struct DkvPlan {
-    int key_blocks, sink_blocks;   // per KV head; the first sink_blocks hold sinks
-    int sink_parts, parts;         // blocks per sink block, per other block
-    __host__ __device__ int blocks() const { return sink_blocks * sink_parts + (key_blocks - sink_blocks) * parts; }
-    // slots of partial sums per KV head: a split block's parts
-    __host__ __device__ int slots() const { return (sink_parts > 1 ? sink_blocks * sink_parts : 0) + (parts > 1 ? (key_blocks - sink_blocks) * parts : 0); }
-};
-VKH_DEV void dkv_block(const DkvPlan &p, int y, int &kb, int &z, int &parts, int &slot) {
-    const int s = p.sink_blocks * p.sink_parts;
-    if (y < s) {
-        kb = y / p.sink_parts; z = y % p.sink_parts; parts = p.sink_parts;
-        slot = y;
-    } else {
-        kb = p.sink_blocks + (y - s) / p.parts; z = (y - s) % p.parts; parts = p.parts;
-        slot = (p.sink_parts > 1 ? s : 0) + y - s;
-    }
-}
-
+// to their slots of a.ws, which window_dkv_sum_k adds in order.
 template <int HD, class TO>
 __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan plan) {
     using R = TileRows<HD>;
@@ -726,7 +832,7 @@ __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan p
     float *ws = zparts > 1 ? a.ws + ((long)bk * plan.slots() + slot) * (2 * BN * HD) : nullptr;
     if (__syncthreads_or(odd)) {
         float *sh = (float *)smem + wave * 2 * HD;
-        const Steps st{kvh * hpk, qstart, top, nh, alt, zpart, zparts};
+        const Steps st{kvh * hpk, qstart, top, nh, alt, 2, zpart, zparts};
         dkv_rows<HD, TO>(args_again(), st, b, kvh, k0, wave, ws, sh, sh + HD, lane);
         return;
     }
@@ -767,46 +873,6 @@ __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan p
     else keep(dkt, (TO *)a.dk + (key0 + k0) * a.lddk + kvh * HD, a.lddk, false, a.scale);
 }
 
-// dK and dV of the split key blocks: their parts added in order, four values a thread.
-template <int HD, class TO>
-__global__ __launch_bounds__(256) void window_dkv_sum16_k(WindowArgs a, DkvPlan plan) {
-    const int nbk = a.n_batch * a.n_kv_heads;
-    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
-    const int kb = blockIdx.x / nbk + (plan.sink_parts > 1 ? 0 : plan.sink_blocks);
-    const bool sink = kb < plan.sink_blocks;
-    const int parts = sink ? plan.sink_parts : plan.parts;
-    const int first = sink ? kb * parts : (plan.sink_parts > 1 ? plan.sink_blocks * plan.sink_parts : 0) + (kb - plan.sink_blocks) * parts;
-    const float *ws = a.ws + ((long)bk * plan.slots() + first) * (2 * 128 * HD);
-    const int x = (blockIdx.y * 256 + threadIdx.x) * 4;  // of dK [128][HD], then dV
-    f32x4 t{0, 0, 0, 0};
-    for (int p = 0; p < parts; ++p) t += *reinterpret_cast<const f32x4 *>(ws + (long)p * 2 * 128 * HD + x);
-    const bool v = x >= 128 * HD;
-    const int y = v ? x - 128 * HD : x, key = kb * 128 + y / HD;
-    if (key >= a.n_kv) return;
-    const long row = (long)b * a.n_kv + key;
-    TO *out = v ? (TO *)a.dv + row * a.lddv : (TO *)a.dk + row * a.lddk;
-    store4(out + kvh * HD + y % HD, t[0], t[1], t[2], t[3]);
-}
-
-DkvPlan dkv_plan(const WindowArgs &a, bool ws) {
-    DkvPlan p;
-    p.key_blocks = (a.n_kv + 127) / 128;
-    p.sink_blocks = a.window < a.n_kv ? std::min(p.key_blocks, (a.n_sink + 127) / 128) : 0;
-    p.sink_parts = p.parts = 1;
-    if (!ws) return p;
-    const long nbk = (long)a.n_batch * a.n_kv_heads, blocks = nbk * p.key_blocks, hpk = a.n_heads / a.n_kv_heads;
-    const long most = hpk * ((a.n_q + 31) / 32), usual = std::min(most, hpk * ((std::min<long>(a.n_kv, a.window) + 159) / 32));
-    // towards one block per CU, with at least four steps of both groups each
-    p.parts = (int)std::max(1l, std::min({8l, 256 / blocks, usual / 8}));
-    // a sink block's steps over the usual block's; at most 256 MiB of partial sums
-    p.sink_parts = (int)std::max<long>(p.parts, std::min<long>(64, (most * p.parts + usual - 1) / usual));
-    const long slot = 2 * 128 * a.hd * 4;
-    while (p.sink_parts > 1 && p.sink_blocks * nbk * slot * p.sink_parts > (192l << 20)) --p.sink_parts;
-    while (p.parts > 1 && blocks * slot * p.parts > (64l << 20)) --p.parts;
-    return p;
-}
-
-bool al(const void *x, long ld, int align, int es) { return (uintptr_t)x % align == 0 && ld * es % align == 0; }
 // Heads of 64 or 128 values in rows of aligned 16-byte chunks, a tile's rows within 31 bits of
 // offset, and a scale that keeps the order of the scores.
 bool shape_ok(const WindowArgs &a) {
@@ -815,23 +881,47 @@ bool shape_ok(const WindowArgs &a) {
 }
 bool fwd_ok(const WindowArgs &a) {
     const int es = a.odt == DType::F32 ? 4 : 2;
-    return shape_ok(a) && al(a.q, a.ldq, 16, 2) && al(a.k, a.ldk, 16, 2) && al(a.v, a.ldv, 16, 2) && al(a.o, a.ldo, 4 * es, es);
+    return shape_ok(a) && aligned_rows(a.q, a.ldq, 16, 2) && aligned_rows(a.k, a.ldk, 16, 2) && aligned_rows(a.v, a.ldv, 16, 2) && aligned_rows(a.o, a.ldo, 4 * es, es);
 }
 bool bwd_ok(const WindowArgs &a) {
     const int es = a.odt == DType::F32 ? 4 : 2;
-    return fwd_ok(a) && al(a.dout, a.lddo, 16, 2) && al(a.o, a.ldo, 16, es) && al(a.dq, a.lddq, 4 * es, es) &&
-           al(a.dk, a.lddk, 4 * es, es) && al(a.dv, a.lddv, 4 * es, es);
+    return fwd_ok(a) && aligned_rows(a.dout, a.lddo, 16, 2) && aligned_rows(a.o, a.ldo, 16, es) && aligned_rows(a.dq, a.lddq, 4 * es, es) &&
+           aligned_rows(a.dk, a.lddk, 4 * es, es) && aligned_rows(a.dv, a.lddv, 4 * es, es);
 }
+
+// Few rows: the tile kernel would give a KV head's keys to one block per head.
+bool few_rows(const WindowArgs &a) { return a.n_q <= kFewRows; }
+// two rounds of one block per CU
+int splits16(const WindowArgs &a) { return step_splits(a, 32, 512); }
+// dK/dV: one block per CU, at least four steps of both groups each
+DkvPlan plan16(const WindowArgs &a, bool ws) { return dkv_plan(a, ws, 128, 256, 8, 8); }
 
 }  // namespace
 
+size_t window16_fwd_ws_bytes(const WindowArgs &a) { return shape_ok(a) && few_rows(a) ? step_ws_bytes(a, splits16(a)) : 0; }
 size_t window16_bwd_ws_bytes(const WindowArgs &a) {
     if (!shape_ok(a)) return 0;
-    return (size_t)a.n_batch * a.n_kv_heads * dkv_plan(a, true).slots() * 2 * 128 * a.hd * sizeof(float);
+    return dkv_ws_bytes(a, plan16(a, true));
 }
 
 bool window16_forward(const WindowArgs &a, hipStream_t st) {
     if (!fwd_ok(a)) return false;
+    if (few_rows(a)) {
+        const int grp = a.n_heads / a.n_kv_heads, rt = (a.n_q * grp + 15) / 16, splits = a.ws ? splits16(a) : 1;
+        const long blocks = (long)a.n_batch * a.n_kv_heads * rt * splits;
+        auto by = [&](auto hd, auto to) {
+            constexpr int HD = decltype(hd)::value;
+            using TO = decltype(to);
+            hipLaunchKernelGGL((window_step16_k<HD, TO>), dim3((unsigned)blocks), dim3(256), 0, st, a, splits);
+            if (splits > 1) launch_join<HD, TO>(a, splits, st);
+        };
+        auto by_head = [&](auto to) {
+            if (a.hd == 128) by(std::integral_constant<int, 128>{}, to);
+            else by(std::integral_constant<int, 64>{}, to);
+        };
+        a.odt == DType::F32 ? by_head(float{}) : by_head(bf16{});
+        return true;
+    }
     const long per = (long)a.n_heads * a.n_batch;
     auto go = [&](auto kernel, int bm) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)(per * ((a.n_q + bm - 1) / bm))), dim3(256), 0, st, a);
@@ -852,7 +942,7 @@ bool window16_backward(const WindowArgs &a, hipStream_t st) {
     const long per = (long)a.n_heads * a.n_batch, nbk = (long)a.n_batch * a.n_kv_heads;
     // 256-row dQ blocks where they fill the chip, else 128, else 64 (as the dense backward)
     const int bq = per * ((a.n_q + 255) / 256) >= 256 ? 256 : per * ((a.n_q + 127) / 128) >= 256 ? 128 : 64;
-    const DkvPlan plan = dkv_plan(a, a.ws != nullptr);
+    const DkvPlan plan = plan16(a, a.ws != nullptr);
     auto by = [&](auto hd, auto to) {
         constexpr int HD = decltype(hd)::value;
         using TO = decltype(to);
@@ -863,9 +953,7 @@ bool window16_backward(const WindowArgs &a, hipStream_t st) {
         else if (bq == 128) dq(window_dq16_k<HD, 8, 128, TO>, 512);
         else dq(window_dq16_k<HD, 4, 64, TO>, 256);
         hipLaunchKernelGGL((window_dkv16_k<HD, TO>), dim3((unsigned)(nbk * plan.blocks())), dim3(512), 0, st, a, plan);
-        const int split = (plan.sink_parts > 1 ? plan.sink_blocks : 0) + (plan.parts > 1 ? plan.key_blocks - plan.sink_blocks : 0);
-        if (split)
-            hipLaunchKernelGGL((window_dkv_sum16_k<HD, TO>), dim3((unsigned)(nbk * split), HD / 4), dim3(256), 0, st, a, plan);
+        launch_dkv_sum<HD, 128, TO>(a, plan, st);
     };
     auto by_head = [&](auto to) {
         if (a.hd == 128) by(std::integral_constant<int, 128>{}, to);

@@ -1,0 +1,619 @@
+// Windowed attention on fp32 operands: the tile kernels (64- and 128-wide heads, aligned rows) of the
+// operator that k_attn_window.hip describes, on v_mfma_f32_16x16x4_f32.
+//
+// Tiles of 32 keys (dK/dV: 32 queries) go through registers into LDS rows of HD + 4 floats (no bank
+// conflicts in the fragment reads), the next tile's loads in flight while one computes; each of a
+// block's 4 waves holds 16 query (key) rows in registers.  Lane (g, c) = (lane / 16, lane % 16) gives A[c][g]
+// and B[g][c] and holds C[4 g + r][c]: over the head, step (u, e) stands for value 16 u + 4 g + e (one 16-byte
+// read covers four), and an accumulator is the next product's B operand as it stands:
+//   forward  S^T = K Q^T, O^T += V^T P^T          dQ  S^T, dP^T = V dO^T, dQ^T += K^T dS^T
+//   dK/dV    S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS
+// A score is the sum of HD / 16 side-by-side chains (one chain of 128 terms rounds three times as
+// coarsely, and each product would wait for the one before).  Bound by the fp32 matrix cores, and on
+// short sequences by the few steps that each block has.
+//
+// As in the bf16 kernels, a block that meets an infinity or a NaN in a tile that its rows do not see
+// in full forms its rows anew one at a time.
+#include "attn16.hpp"
+#include "window.hpp"
+
+#pragma clang fp contract(off)
+
+namespace vkh {
+namespace {
+
+constexpr int FNT = 256, FT = 32;
+
+VKH_DEV float4 f4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+VKH_DEV f32x4 mfma4(const float4 &a, const float4 &b, f32x4 c) {
+    c = mfma16x16x4(a.x, b.x, c);
+    c = mfma16x16x4(a.y, b.y, c);
+    c = mfma16x16x4(a.z, b.z, c);
+    return mfma16x16x4(a.w, b.w, c);
+}
+VKH_DEV float xmax(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+VKH_DEV float xsum(float v) {
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+template <int NU>
+VKH_DEV f32x4 head_dot(const float *row, const float4 (&f)[NU]) {
+    f32x4 a[NU] = {};
+#pragma unroll
+    for (int u = 0; u < NU; ++u) a[u] = mfma4(f4(row + 16 * u), f[u], a[u]);
+#pragma unroll
+    for (int w = NU / 2; w; w /= 2)
+#pragma unroll
+        for (int u = 0; u < w; ++u) a[u] += a[u + w];
+    return a[0];
+}
+
+// R rows of HD floats moved by NT threads, global -> registers -> LDS (pitch HD + 4).
+template <int HD, int R, int NT>
+struct Tile32 {
+    static constexpr int P = HD + 4, N4 = R * HD / 4 / NT;
+    static_assert(N4 * NT * 4 == R * HD, "tile / thread count");
+    float4 v[N4];
+    VKH_DEV void load(const float *base, long ld, int tid, int rows) {  // rows from `rows` on are zero
+#pragma unroll
+        for (int i = 0; i < N4; ++i) {
+            const int x = tid + NT * i, r = x / (HD / 4), c = x % (HD / 4);
+            v[i] = r < rows ? f4(base + (long)r * ld + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    }
+    VKH_DEV void store(float *lds, int tid) const {
+#pragma unroll
+        for (int i = 0; i < N4; ++i) {
+            const int x = tid + NT * i, r = x / (HD / 4), c = x % (HD / 4);
+            *reinterpret_cast<float4 *>(lds + r * P + 4 * c) = v[i];
+        }
+    }
+    VKH_DEV bool odd() const {  // holds an infinity or a NaN (0 times which is NaN)
+        float z = 0.f;
+#pragma unroll
+        for (int i = 0; i < N4; ++i) {
+            z = fmaf(v[i].x, 0.f, z); z = fmaf(v[i].y, 0.f, z);
+            z = fmaf(v[i].z, 0.f, z); z = fmaf(v[i].w, 0.f, z);
+        }
+        return !(z == 0.f);
+    }
+};
+
+__device__ __attribute__((noinline)) void fwd_rows32(const WindowArgs &a, int b, int r, int end, int h, float *q, int lane) {
+    for (; r < end; r += 4) window_fwd_row<float, float>(a, b, r, h, q, lane);
+}
+__device__ __attribute__((noinline)) void dq_rows32(const WindowArgs &a, int b, int r, int end, int h, float *q, float *g, int lane) {
+    for (; r < end; r += 4) window_dq_row<float, float>(a, b, r, h, q, g, lane);
+}
+__device__ __attribute__((noinline)) void dkv_rows32(const WindowArgs &a, const Steps &st, int b, int kvh, int k0, int wave,
+                                                     float *ws, float *k, float *v, int lane) {
+    auto mine = [&](int h, int row) { return st.mine(h, row); };
+    for (int x = wave; x < 64; x += 4) {
+        if (k0 + x >= a.n_kv) {  // (their slots are read)
+            for (int d = lane; ws && d < a.hd; d += 64) ws[x * a.hd + d] = ws[(64 + x) * a.hd + d] = 0.f;
+            continue;
+        }
+        const long row = (long)b * a.n_kv + k0 + x;
+        window_dkv_row<float>(a, b, k0 + x, kvh, k, v, ws ? ws + x * a.hd : (float *)a.dk + row * a.lddk + kvh * a.hd,
+                              ws ? ws + (64 + x) * a.hd : (float *)a.dv + row * a.lddv + kvh * a.hd, lane, mine);
+    }
+}
+
+// ── forward: block = 64 query rows of one head ───────────────────────────
+template <int HD>
+__global__ __launch_bounds__(FNT, 2) void window_fwd32_k(WindowArgs a) {
+    using T = Tile32<HD, FT, FNT>;
+    constexpr int P = T::P, NU = HD / 16;
+    __shared__ __attribute__((aligned(16))) float Ks[2][FT * P], Vs[2][FT * P];
+    const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, nqt = (a.n_q + 63) / 64;
+    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
+    const int h = kvh * grp + blockIdx.x / nbk % grp, qt = nqt - 1 - (int)(blockIdx.x / nbk / grp);
+    const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const Span s = span_of(a, b);
+    const int r0 = qt * 64, qw = r0 + 16 * wave, r = qw + c;
+    const KeyTiles kt = key_tiles<FT>(a, s, r0, r0 + 64);
+    const int wta = max(0, qw + s.off), wtb = min(qw + 16, s.ql) - 1 + s.off;
+    const int pos = r < s.ql ? max(-1, r + s.off) : -1;
+    const long row = (long)b * a.n_q + r;
+    float4 qf[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+        qf[u] = pos >= 0 ? f4((const float *)a.q + row * a.ldq + h * HD + 4 * g + 16 * u) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float *kb = (const float *)a.k + (long)b * a.n_kv * a.ldk + kvh * HD;
+    const float *vb = (const float *)a.v + (long)b * a.n_kv * a.ldv + kvh * HD;
+    T tk, tv;
+    auto load = [&](int it) {
+        const int k0 = kt.tile(it) * FT;
+        tk.load(kb + (long)k0 * a.ldk, a.ldk, tid, s.kl - k0);
+        tv.load(vb + (long)k0 * a.ldv, a.ldv, tid, s.kl - k0);
+    };
+    bool odd = false;  // in V of a tile that is not seen in full
+    auto store = [&](int it) {
+        const int k0 = kt.tile(it) * FT;
+        if (!all_seen(a, kt.ta, kt.tb, k0, k0 + FT - 1)) odd |= tv.odd();
+        tk.store(Ks[it & 1], tid);
+        tv.store(Vs[it & 1], tid);
+    };
+    if (kt.n > 0) {
+        load(0);
+        store(0);
+    }
+    __syncthreads();
+    f32x4 ot[NU];  // O^T[16 j + 4 g + r][row]
+#pragma unroll
+    for (int j = 0; j < NU; ++j) ot[j] = f32x4{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.f;  // running maximum; this lane's share of the sum
+    for (int it = 0; it < kt.n; ++it) {
+        if (it + 1 < kt.n) load(it + 1);
+        const int k0 = kt.tile(it) * FT;
+        const float *Kl = Ks[it & 1], *Vl = Vs[it & 1];
+        f32x4 st[2];
+        bool live[2];
+        float tmax = -INFINITY;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            live[ks] = !none_seen(a, wta, wtb, k0 + 16 * ks, k0 + 16 * ks + 15);  // wave-uniform
+            st[ks] = f32x4{0, 0, 0, 0};
+            if (live[ks]) st[ks] = head_dot<NU>(Kl + (16 * ks + c) * P + 4 * g, qf) * a.scale;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (!sees(a, pos, k0 + 16 * ks + 4 * g + e)) st[ks][e] = -INFINITY;
+                tmax = fmaxf(tmax, st[ks][e]);
+            }
+        }
+        const float mn = fmaxf(m, xmax(tmax)), ms = mn == -INFINITY ? 0.f : mn;
+        const float alpha = expf(m - ms);
+        l *= alpha;
+#pragma unroll
+        for (int j = 0; j < NU; ++j) ot[j] *= alpha;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                st[ks][e] = expf(st[ks][e] - ms);
+                l += st[ks][e];
+            }
+        m = mn;
+        // O^T += V^T P^T: step (ks, e) is key k0 + 16 ks + 4 g + e
+#pragma unroll
+        for (int j = 0; j < NU; ++j)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                if (!live[ks]) continue;
+                const float *vr = Vl + (16 * ks + 4 * g) * P + 16 * j + c;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ot[j] = mfma16x16x4(vr[e * P], st[ks][e], ot[j]);
+            }
+        if (it + 1 < kt.n) store(it + 1);  // its buffer was last read before the previous barrier
+        __syncthreads();
+    }
+    if (__syncthreads_or(odd)) {
+        fwd_rows32(args_again(), b, r0 + wave, min(r0 + 64, a.n_q), h, Ks[0] + wave * HD, lane);
+        return;
+    }
+    l = xsum(l);
+    if (r >= a.n_q) return;
+    const bool dead = l == 0.f;
+    const float inv = 1.0f / l;
+    float *o = (float *)a.o + row * a.ldo + h * HD + 4 * g;
+#pragma unroll
+    for (int j = 0; j < NU; ++j) {
+        const f32x4 x = dead ? f32x4{0, 0, 0, 0} : ot[j] * inv;
+        store4(o + 16 * j, x[0], x[1], x[2], x[3]);
+    }
+    if (a.lse && g == 0) a.lse[row * a.n_heads + h] = dead ? -INFINITY : m + logf(l);
+}
+
+// ── forward of a few rows ────────────────────────────────────────────────
+// As in bf16 (window_step16_k), with 16-key tiles that a wave moves through its registers.
+template <int HD>
+__global__ __launch_bounds__(FNT, 2) void window_step32_k(WindowArgs a, int splits) {
+    constexpr int BN = 16, NU = HD / 16;
+    using T = Tile32<HD, BN, 64>;
+    constexpr int P = T::P;
+    __shared__ __attribute__((aligned(16))) float tiles[4][2][BN * P];
+    __shared__ float ml[4][2][16];
+    const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, M = a.n_q * grp, RT = (M + 15) / 16;
+    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
+    const int rt = blockIdx.x / nbk % RT, split = blockIdx.x / nbk / RT;
+    const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const Span s = span_of(a, b);
+    const KeyTiles kt = key_tiles<BN>(a, s, rt * 16 / grp, (min(M, rt * 16 + 16) - 1) / grp + 1);
+    const int per = (kt.n + splits - 1) / splits, last = min(kt.n, (split + 1) * per);
+    const float c2 = a.scale * LOG2E;
+    const int mi = rt * 16 + c, row = mi / grp, h = kvh * grp + mi % grp;
+    const int pos = mi < M && row < s.ql ? max(-1, row + s.off) : -1;
+    float4 qf[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+        qf[u] = pos >= 0 ? f4((const float *)a.q + ((long)b * a.n_q + row) * a.ldq + h * HD + 4 * g + 16 * u)
+                         : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float *kb = (const float *)a.k + (long)b * a.n_kv * a.ldk + kvh * HD;
+    const float *vb = (const float *)a.v + (long)b * a.n_kv * a.ldv + kvh * HD;
+    float *Kl = tiles[wave][0], *Vl = tiles[wave][1];
+    T tk, tv;
+    auto load = [&](int it) {
+        const int k0 = kt.tile(it) * BN;
+        tk.load(kb + (long)k0 * a.ldk, a.ldk, lane, s.kl - k0);
+        tv.load(vb + (long)k0 * a.ldv, a.ldv, lane, s.kl - k0);
+    };
+    f32x4 acc[NU];
+#pragma unroll
+    for (int j = 0; j < NU; ++j) acc[j] = f32x4{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.f;  // maximum in log2 units
+    int it = split * per + wave;
+    if (it < last) load(it);
+    for (; it < last; it += 4) {
+        const int k0 = kt.tile(it) * BN;
+        const bool odd = !all_seen(a, kt.ta, kt.tb, k0, k0 + BN - 1) && __any(tv.odd());
+        wave_lds();  // the last tile's reads are done
+        tk.store(Kl, lane);
+        tv.store(Vl, lane);
+        if (it + 4 < last) load(it + 4);
+        wave_lds();
+        f32x4 st = head_dot<NU>(Kl + c * P + 4 * g, qf) * c2;
+        float mt = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (!sees(a, pos, k0 + 4 * g + e)) st[e] = -INFINITY;
+            mt = fmaxf(mt, st[e]);
+        }
+        const float mn = fmaxf(m, xmax(mt)), ms = mn == -INFINITY ? 0.f : mn;
+        const float so = __builtin_amdgcn_exp2f(m - ms);
+        m = mn;
+        l *= so;
+#pragma unroll
+        for (int j = 0; j < NU; ++j) acc[j] *= so;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            st[e] = __builtin_amdgcn_exp2f(st[e] - ms);
+            l += st[e];
+        }
+        if (odd) {  // pair by pair, seen pairs only
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll 1
+                for (int g2 = 0; g2 < 4; ++g2) {
+                    const float w = __shfl(st[e], 16 * g2 + c, 64);
+                    if (!sees(a, pos, k0 + 4 * g2 + e)) continue;
+#pragma unroll
+                    for (int j = 0; j < NU; ++j)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) acc[j][x] = fmaf(Vl[(4 * g2 + e) * P + 16 * j + 4 * g + x], w, acc[j][x]);
+                }
+            continue;
+        }
+#pragma unroll
+        for (int j = 0; j < NU; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[j] = mfma16x16x4(Vl[(4 * g + e) * P + 16 * j + c], st[e], acc[j]);
+    }
+    wave_lds();
+    float *res = tiles[wave][0];  // rows of P floats
+    const float lt = xsum(l);
+#pragma unroll
+    for (int j = 0; j < NU; ++j) *reinterpret_cast<f32x4 *>(res + c * P + 16 * j + 4 * g) = acc[j];
+    if (g == 0) ml[wave][0][c] = m, ml[wave][1][c] = lt;
+    __syncthreads();
+    constexpr int E = HD / 16;
+    const int r = tid / 16, d0 = tid % 16 * E;
+    float mx = -INFINITY, sum = 0.f, o[E] = {};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mx = fmaxf(mx, ml[w][0][r]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float lw = ml[w][1][r];
+        if (lw == 0.f) continue;
+        const float f = __builtin_amdgcn_exp2f(ml[w][0][r] - (mx == -INFINITY ? 0.f : mx));
+        sum = fmaf(lw, f, sum);
+        const float *src = tiles[w][0] + r * P + d0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(src[e], f, o[e]);
+    }
+    const int mr = rt * 16 + r;
+    if (mr >= M) return;
+    const long orow = (long)b * a.n_q + mr / grp;
+    const int oh = kvh * grp + mr % grp;
+    if (splits > 1) {  // as in bf16
+        const long rows = (long)a.n_batch * a.n_q * a.n_heads, at = (split * rows) + orow * a.n_heads + oh;
+        float *dst = a.ws + at * HD + d0;
+#pragma unroll
+        for (int e = 0; e < E; e += 4) store4(dst + e, o[e], o[e + 1], o[e + 2], o[e + 3]);
+        if (d0 == 0) {
+            float *st = a.ws + splits * rows * HD + at * 2;
+            st[0] = mx;
+            st[1] = sum;
+        }
+        return;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    float *out = (float *)a.o + orow * a.ldo + oh * HD + d0;
+#pragma unroll
+    for (int e = 0; e < E; e += 4) store4(out + e, o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+    if (a.lse && d0 == 0) a.lse[orow * a.n_heads + oh] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * LN2;
+}
+
+// ── backward: D and dQ, block = 64 query rows of one head ────────────────
+template <int HD>
+__global__ __launch_bounds__(FNT, 2) void window_dq32_k(WindowArgs a) {
+    using T = Tile32<HD, FT, FNT>;
+    constexpr int P = T::P, NU = HD / 16;
+    __shared__ __attribute__((aligned(16))) float Ks[2][FT * P], Vs[2][FT * P];
+    const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, nqt = (a.n_q + 63) / 64;
+    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
+    const int h = kvh * grp + blockIdx.x / nbk % grp, qt = nqt - 1 - (int)(blockIdx.x / nbk / grp);
+    const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const Span s = span_of(a, b);
+    const int r0 = qt * 64, qw = r0 + 16 * wave, r = qw + c;
+    const KeyTiles kt = key_tiles<FT>(a, s, r0, r0 + 64);
+    const int wta = max(0, qw + s.off), wtb = min(qw + 16, s.ql) - 1 + s.off;
+    const long row = (long)b * a.n_q + r;
+    const float lse = r < s.ql && r + s.off >= 0 ? a.lse[row * a.n_heads + h] : -INFINITY;
+    const int pos = lse == -INFINITY ? -1 : r + s.off;
+    float4 qf[NU], of[NU];
+    double acc = 0;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+        const long col = h * HD + 4 * g + 16 * u;
+        qf[u] = of[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (pos >= 0) {
+            qf[u] = f4((const float *)a.q + row * a.ldq + col);
+            of[u] = f4((const float *)a.dout + row * a.lddo + col);
+            const float4 o = f4((const float *)a.o + row * a.ldo + col);
+            acc += (double)o.x * of[u].x + (double)o.y * of[u].y + (double)o.z * of[u].z + (double)o.w * of[u].w;
+        }
+    }
+    acc += __shfl_xor(acc, 16, 64);
+    acc += __shfl_xor(acc, 32, 64);
+    const float dd = (float)acc;
+    if (r < a.n_q && g == 0) a.d[row * a.n_heads + h] = dd;
+    const float *kb = (const float *)a.k + (long)b * a.n_kv * a.ldk + kvh * HD;
+    const float *vb = (const float *)a.v + (long)b * a.n_kv * a.ldv + kvh * HD;
+    T tk, tv;
+    auto load = [&](int it) {
+        const int k0 = kt.tile(it) * FT;
+        tk.load(kb + (long)k0 * a.ldk, a.ldk, tid, s.kl - k0);
+        tv.load(vb + (long)k0 * a.ldv, a.ldv, tid, s.kl - k0);
+    };
+    bool odd = false;  // in K of a tile that is not seen in full
+    auto store = [&](int it) {
+        const int k0 = kt.tile(it) * FT;
+        if (!all_seen(a, kt.ta, kt.tb, k0, k0 + FT - 1)) odd |= tk.odd();
+        tk.store(Ks[it & 1], tid);
+        tv.store(Vs[it & 1], tid);
+    };
+    if (kt.n > 0) {
+        load(0);
+        store(0);
+    }
+    __syncthreads();
+    f32x4 dqt[NU];
+#pragma unroll
+    for (int j = 0; j < NU; ++j) dqt[j] = f32x4{0, 0, 0, 0};
+    for (int it = 0; it < kt.n; ++it) {
+        if (it + 1 < kt.n) load(it + 1);
+        const int k0 = kt.tile(it) * FT;
+        const float *Kl = Ks[it & 1], *Vl = Vs[it & 1];
+        f32x4 da[2];
+        bool live[2];
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            live[ks] = !none_seen(a, wta, wtb, k0 + 16 * ks, k0 + 16 * ks + 15);  // wave-uniform
+            da[ks] = f32x4{0, 0, 0, 0};
+            if (!live[ks]) continue;
+            const f32x4 sa = head_dot<NU>(Kl + (16 * ks + c) * P + 4 * g, qf);
+            da[ks] = head_dot<NU>(Vl + (16 * ks + c) * P + 4 * g, of);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p = expf(fmaf(sa[e], a.scale, -lse));
+                da[ks][e] = sees(a, pos, k0 + 16 * ks + 4 * g + e) ? p * (da[ks][e] - dd) : 0.f;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NU; ++j)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                if (!live[ks]) continue;
+                const float *kr = Kl + (16 * ks + 4 * g) * P + 16 * j + c;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dqt[j] = mfma16x16x4(kr[e * P], da[ks][e], dqt[j]);
+            }
+        if (it + 1 < kt.n) store(it + 1);
+        __syncthreads();
+    }
+    if (__syncthreads_or(odd)) {
+        float *sh = Ks[0] + wave * 2 * HD;
+        dq_rows32(args_again(), b, r0 + wave, min(r0 + 64, a.n_q), h, sh, sh + HD, lane);
+        return;
+    }
+    if (r >= a.n_q) return;
+    float *dq = (float *)a.dq + row * a.lddq + h * HD + 4 * g;
+#pragma unroll
+    for (int j = 0; j < NU; ++j) {
+        const f32x4 x = pos >= 0 ? dqt[j] * a.scale : f32x4{0, 0, 0, 0};
+        store4(dq + 16 * j, x[0], x[1], x[2], x[3]);
+    }
+}
+
+// ── backward: dK and dV, block = 64 keys of one KV head ──────────────────
+// Steps and parts as in bf16 (window_dkv16_k), one head a step.
+template <int HD>
+__global__ __launch_bounds__(FNT, 2) void window_dkv32_k(WindowArgs a, DkvPlan plan) {
+    using T = Tile32<HD, FT, FNT>;
+    constexpr int P = T::P, NU = HD / 16, BN = 64;
+    __shared__ __attribute__((aligned(16))) float Qs[2][FT * P], Os[2][FT * P];
+    __shared__ float Ls[2][FT], Dl[2][FT];
+    const int nbk = a.n_batch * a.n_kv_heads;
+    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
+    int kb, zpart, zparts, slot;
+    dkv_block(plan, blockIdx.x / nbk, kb, zpart, zparts, slot);
+    const int nh = a.n_heads / a.n_kv_heads;
+    const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const Span s = span_of(a, b);
+    const int k0 = kb * BN, kw = k0 + 16 * wave, key = kw + c;
+    const long krow = (long)b * a.n_kv + key, row0 = (long)b * a.n_q;
+    float4 kf[NU], vf[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+        const long col = kvh * HD + 4 * g + 16 * u;
+        kf[u] = vf[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (key < s.kl) {
+            kf[u] = f4((const float *)a.k + krow * a.ldk + col);
+            vf[u] = f4((const float *)a.v + krow * a.ldv + col);
+        }
+    }
+    const int k1 = min(k0 + BN, s.kl) - 1;  // the block's last key
+    const int qstart = max(0, k0 - s.off);
+    const int qend = k0 < a.n_sink ? s.ql : (int)min((long)s.ql, (long)k1 + a.window - s.off);
+    const int nqt = k1 >= k0 && qend > qstart ? (qend - qstart + FT - 1) / FT : 0;
+    const int niter = max(0, (nh * nqt - zpart + zparts - 1) / zparts), top = nqt - 1;
+    auto tile_of = [&](int it, int &h, int &q0) {
+        it = it * zparts + zpart;
+        h = kvh * nh + it % nh;
+        q0 = qstart + (top - it / nh) * FT;
+    };
+    T tq, to;
+    float stat = 0.f;  // LSE (threads 0..31) or D (32..63) of one tile row
+    auto load = [&](int it) {
+        int h, q0;
+        tile_of(it, h, q0);
+        const int rows = s.ql - q0;
+        tq.load((const float *)a.q + (row0 + q0) * a.ldq + h * HD, a.ldq, tid, rows);
+        to.load((const float *)a.dout + (row0 + q0) * a.lddo + h * HD, a.lddo, tid, rows);
+        if (tid < 2 * FT) {  // rows past the end: of no gradient, as rows of LSE = -inf
+            stat = tid < FT ? -INFINITY : 0.f;
+            if (tid % FT < rows) stat = (tid < FT ? a.lse : a.d)[(row0 + q0 + tid % FT) * a.n_heads + h];
+        }
+    };
+    bool odd = false;  // in Q or dO of a tile whose rows do not all see all keys
+    auto store = [&](int it) {
+        int h, q0;
+        tile_of(it, h, q0);
+        const int ta = q0 + s.off, tb = min(q0 + FT, s.ql) - 1 + s.off;
+        if (!all_seen(a, ta, tb, k0, k0 + BN - 1)) odd |= tq.odd() || to.odd();
+        tq.store(Qs[it & 1], tid);
+        to.store(Os[it & 1], tid);
+        if (tid < FT) Ls[it & 1][tid] = stat;
+        else if (tid < 2 * FT) Dl[it & 1][tid - FT] = stat;
+    };
+    f32x4 dvt[NU], dkt[NU];
+#pragma unroll
+    for (int j = 0; j < NU; ++j) dvt[j] = dkt[j] = f32x4{0, 0, 0, 0};
+    if (niter > 0) {
+        load(0);
+        store(0);
+    }
+    __syncthreads();
+    for (int it = 0; it < niter; ++it) {
+        const int buf = it & 1;
+        if (it + 1 < niter) load(it + 1);
+        int h, q0;
+        tile_of(it, h, q0);
+        const float *Ql = Qs[buf], *Ol = Os[buf];
+        f32x4 sa[2], da[2];  // S / dP[q0 + 16 qs + 4 g + e][key]
+        bool live[2];
+#pragma unroll
+        for (int qs = 0; qs < 2; ++qs) {
+            const int ta = q0 + 16 * qs + s.off, tb = min(q0 + 16 * qs + 16, s.ql) - 1 + s.off;
+            sa[qs] = da[qs] = f32x4{0, 0, 0, 0};
+            live[qs] = !none_seen(a, ta, tb, kw, kw + 15);  // wave-uniform
+            if (!live[qs]) continue;
+            sa[qs] = head_dot<NU>(Ql + (16 * qs + c) * P + 4 * g, kf);
+            da[qs] = head_dot<NU>(Ol + (16 * qs + c) * P + 4 * g, vf);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int x = 16 * qs + 4 * g + e;
+                const float l = Ls[buf][x];
+                const float p = expf(fmaf(sa[qs][e], a.scale, -l));
+                const bool on = l != -INFINITY && sees(a, q0 + x + s.off, key);
+                sa[qs][e] = on ? p : 0.f;
+                da[qs][e] = on ? p * (da[qs][e] - Dl[buf][x]) : 0.f;
+            }
+        }
+        // dV^T += dO^T P, dK^T += Q^T dS: step (qs, e) is query q0 + 16 qs + 4 g + e
+#pragma unroll
+        for (int j = 0; j < NU; ++j)
+#pragma unroll
+            for (int qs = 0; qs < 2; ++qs) {
+                if (!live[qs]) continue;
+                const float *orow = Ol + (16 * qs + 4 * g) * P + 16 * j + c, *qrow = Ql + (16 * qs + 4 * g) * P + 16 * j + c;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    dvt[j] = mfma16x16x4(orow[e * P], sa[qs][e], dvt[j]);
+                    dkt[j] = mfma16x16x4(qrow[e * P], da[qs][e], dkt[j]);
+                }
+            }
+        if (it + 1 < niter) store(it + 1);
+        __syncthreads();
+    }
+    float *ws = zparts > 1 ? a.ws + ((long)bk * plan.slots() + slot) * (2 * BN * HD) : nullptr;
+    if (__syncthreads_or(odd)) {
+        float *sh = Qs[0] + wave * 2 * HD;
+        const Steps st{kvh * nh, qstart, top, nh, false, 1, zpart, zparts};
+        dkv_rows32(args_again(), st, b, kvh, k0, wave, ws, sh, sh + HD, lane);
+        return;
+    }
+    if (!ws && key >= a.n_kv) return;
+    float *dk = ws ? ws + (16 * wave + c) * HD : (float *)a.dk + krow * a.lddk + kvh * HD;
+    float *dv = ws ? ws + (BN + 16 * wave + c) * HD : (float *)a.dv + krow * a.lddv + kvh * HD;
+    const bool live = key < s.kl;
+#pragma unroll
+    for (int j = 0; j < NU; ++j) {
+        const f32x4 x = live ? dkt[j] * a.scale : f32x4{0, 0, 0, 0}, y = live ? dvt[j] : f32x4{0, 0, 0, 0};
+        store4(dk + 16 * j + 4 * g, x[0], x[1], x[2], x[3]);
+        store4(dv + 16 * j + 4 * g, y[0], y[1], y[2], y[3]);
+    }
+}
+
+bool shape_ok(const WindowArgs &a) { return a.dt == DType::F32 && (a.hd == 64 || a.hd == 128) && a.scale > 0.f && a.scale < INFINITY; }
+bool ok(const void *p, long ld) { return aligned_rows(p, ld, 16, 4); }
+bool fwd_ok(const WindowArgs &a) { return shape_ok(a) && ok(a.q, a.ldq) && ok(a.k, a.ldk) && ok(a.v, a.ldv) && ok(a.o, a.ldo); }
+bool few_rows(const WindowArgs &a) { return a.n_q <= kFewRows; }
+int splits32(const WindowArgs &a) { return step_splits(a, 16, 1024); }
+DkvPlan plan32(const WindowArgs &a, bool ws) { return dkv_plan(a, ws, 64, 512, 16, 2); }
+
+}  // namespace
+
+size_t window32_fwd_ws_bytes(const WindowArgs &a) { return shape_ok(a) && few_rows(a) ? step_ws_bytes(a, splits32(a)) : 0; }
+size_t window32_bwd_ws_bytes(const WindowArgs &a) { return shape_ok(a) ? dkv_ws_bytes(a, plan32(a, true)) : 0; }
+
+bool window32_forward(const WindowArgs &a, hipStream_t st) {
+    if (!fwd_ok(a)) return false;
+    if (few_rows(a)) {
+        const int grp = a.n_heads / a.n_kv_heads, splits = a.ws ? splits32(a) : 1;
+        const dim3 grid((unsigned)((long)a.n_batch * a.n_kv_heads * ((a.n_q * grp + 15) / 16) * splits));
+        if (a.hd == 128) hipLaunchKernelGGL(window_step32_k<128>, grid, dim3(FNT), 0, st, a, splits);
+        else hipLaunchKernelGGL(window_step32_k<64>, grid, dim3(FNT), 0, st, a, splits);
+        if (splits > 1) a.hd == 128 ? launch_join<128, float>(a, splits, st) : launch_join<64, float>(a, splits, st);
+        return true;
+    }
+    const dim3 grid((unsigned)((long)a.n_heads * a.n_batch * ((a.n_q + 63) / 64)));
+    if (a.hd == 128) hipLaunchKernelGGL(window_fwd32_k<128>, grid, dim3(FNT), 0, st, a);
+    else hipLaunchKernelGGL(window_fwd32_k<64>, grid, dim3(FNT), 0, st, a);
+    return true;
+}
+
+bool window32_backward(const WindowArgs &a, hipStream_t st) {
+    if (!fwd_ok(a) || !ok(a.dout, a.lddo) || !ok(a.dq, a.lddq) || !ok(a.dk, a.lddk) || !ok(a.dv, a.lddv)) return false;
+    const DkvPlan plan = plan32(a, a.ws != nullptr);
+    const dim3 gq((unsigned)((long)a.n_heads * a.n_batch * ((a.n_q + 63) / 64)));
+    const dim3 gk((unsigned)((long)a.n_batch * a.n_kv_heads * plan.blocks()));
+    auto by = [&](auto hd) {
+        constexpr int HD = decltype(hd)::value;
+        hipLaunchKernelGGL(window_dq32_k<HD>, gq, dim3(FNT), 0, st, a);
+        hipLaunchKernelGGL(window_dkv32_k<HD>, gk, dim3(FNT), 0, st, a, plan);
+        launch_dkv_sum<HD, 64, float>(a, plan, st);
+    };
+    if (a.hd == 128) by(std::integral_constant<int, 128>{});
+    else by(std::integral_constant<int, 64>{});
+    return true;
+}
+
+}  // namespace vkh

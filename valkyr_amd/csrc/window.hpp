@@ -1,6 +1,8 @@
 // What the windowed attention's kernel files share.
 #pragma once
 
+#include <algorithm>
+
 #include "ops.hpp"
 
 namespace vkh {
@@ -17,6 +19,56 @@ VKH_DEV Span span_of(const WindowArgs &a, int b) {
     return s;
 }
 
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr int kAll = 0x7fffffff;  // the window of a sink
+
+// Whether position t sees key j (t = -1: a row that sees none).
+VKH_DEV bool sees(const WindowArgs &a, int t, int j) {
+    return (unsigned)(t - j) < (unsigned)(j < a.n_sink ? kAll : a.window);
+}
+// Whether all positions ta .. tb see all keys j0 .. j1, or none sees any.
+VKH_DEV bool all_seen(const WindowArgs &a, int ta, int tb, int j0, int j1) {
+    return j1 <= ta && (j0 > tb - a.window || j1 < a.n_sink);
+}
+VKH_DEV bool none_seen(const WindowArgs &a, int ta, int tb, int j0, int j1) {
+    return tb < ta || j0 > tb || (j1 <= ta - a.window && j0 >= a.n_sink);
+}
+
+VKH_DEV void store4(float *p, float x, float y, float z, float w) {
+    *reinterpret_cast<float4 *>(p) = make_float4(x, y, z, w);
+}
+VKH_DEV void store4(bf16 *p, float x, float y, float z, float w) {
+    bf16x4 o;
+    o[0] = (bf16)x; o[1] = (bf16)y; o[2] = (bf16)z; o[3] = (bf16)w;
+    *reinterpret_cast<bf16x4 *>(p) = o;
+}
+
+// The key tiles (of BN keys) that a block of query rows r0 .. r1 - 1 walks: those of the sinks that
+// lie before its window, then its window's.
+struct KeyTiles {
+    int ta, tb;     // live positions (tb < ta: none)
+    int n_sink, w0, n;
+    VKH_DEV int tile(int it) const { return it < n_sink ? it : w0 + it - n_sink; }
+};
+template <int BN>
+VKH_DEV KeyTiles key_tiles(const WindowArgs &a, const Span &s, int r0, int r1) {
+    KeyTiles k;
+    k.ta = max(0, r0 + s.off);
+    k.tb = min(r1, s.ql) - 1 + s.off;
+    k.w0 = max(0, k.ta - a.window + 1) / BN;
+    k.n_sink = min((a.n_sink + BN - 1) / BN, k.w0);
+    k.n = k.tb >= k.ta ? k.n_sink + k.tb / BN - k.w0 + 1 : 0;
+    return k;
+}
+
+// A kernel's first argument, read anew from where the launch put it (the kernel arguments begin
+// with it): its values need not stay in registers for the calls below.
+VKH_DEV const WindowArgs &args_again() {
+    unsigned long p = (unsigned long)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *reinterpret_cast<const WindowArgs *>(p);
+}
 // ── one row at a time ────────────────────────────────────────────────────
 // A wave's work on one query row (dK/dV: key row), 64 keys (queries) at a time with one dot product
 // a lane, then the weighted sum with the head's values over the lanes.  `q`, `g` (`k`, `v`) are
@@ -171,11 +223,169 @@ VKH_DEV void window_dkv_row(const WindowArgs &a, int b, int j, int kh, float *k,
         }
 }
 
+// ── joined results ───────────────────────────────────────────────────────
+struct DkvPlan {
+    int key_blocks, sink_blocks;   // per KV head, of `keys` keys; the first sink_blocks hold sinks
+    int sink_parts, parts;         // launched blocks per sink block, per other block
+    int keys;
+    __host__ __device__ int blocks() const { return sink_blocks * sink_parts + (key_blocks - sink_blocks) * parts; }
+    // slots of partial sums per KV head: a split block's parts
+    __host__ __device__ int slots() const { return (sink_parts > 1 ? sink_blocks * sink_parts : 0) + (parts > 1 ? (key_blocks - sink_blocks) * parts : 0); }
+};
+VKH_DEV void dkv_block(const DkvPlan &p, int y, int &kb, int &z, int &parts, int &slot) {
+    const int s = p.sink_blocks * p.sink_parts;
+    if (y < s) {
+        kb = y / p.sink_parts; z = y % p.sink_parts; parts = p.sink_parts;
+        slot = y;
+    } else {
+        kb = p.sink_blocks + (y - s) / p.parts; z = (y - s) % p.parts; parts = p.parts;
+        slot = (p.sink_parts > 1 ? s : 0) + y - s;
+    }
+}
+
+// The (query tile, head) steps of one part of a key block, as the dK/dV kernels walk them: tiles of
+// 32 rows from the last one (`top`) down, heads inner; per: heads (alt: tiles) that one step takes.
+struct Steps {
+    int head0, qstart, top, nh;
+    bool alt;
+    int per, zpart, zparts;
+    VKH_DEV bool mine(int h, int row) const {
+        const int t = top - (row - qstart) / 32;
+        return ((alt ? t / per : t) * nh + (alt ? h - head0 : (h - head0) / per)) % zparts == zpart;
+    }
+};
+// dK and dV of the split key blocks: their parts added in order, four values a thread.
+template <int HD, int BN, class TO>
+__global__ __launch_bounds__(256) void window_dkv_sum_k(WindowArgs a, DkvPlan plan) {
+    const int nbk = a.n_batch * a.n_kv_heads;
+    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
+    const int kb = blockIdx.x / nbk + (plan.sink_parts > 1 ? 0 : plan.sink_blocks);
+    const bool sink = kb < plan.sink_blocks;
+    const int parts = sink ? plan.sink_parts : plan.parts;
+    const int first = sink ? kb * parts : (plan.sink_parts > 1 ? plan.sink_blocks * plan.sink_parts : 0) + (kb - plan.sink_blocks) * parts;
+    const float *ws = a.ws + ((long)bk * plan.slots() + first) * (2 * BN * HD);
+    const int x = (blockIdx.y * 256 + threadIdx.x) * 4;  // of dK [BN][HD], then dV
+    f32x4 t{0, 0, 0, 0};
+    for (int p = 0; p < parts; ++p) t += *reinterpret_cast<const f32x4 *>(ws + (long)p * 2 * BN * HD + x);
+    const bool v = x >= BN * HD;
+    const int y = v ? x - BN * HD : x, key = kb * BN + y / HD;
+    if (key >= a.n_kv) return;
+    const long row = (long)b * a.n_kv + key;
+    TO *out = v ? (TO *)a.dv + row * a.lddv : (TO *)a.dk + row * a.lddk;
+    store4(out + kvh * HD + y % HD, t[0], t[1], t[2], t[3]);
+}
+
+// The splits' results of one (row, head) per 16 lanes, joined in order: lane i holds the factors of
+// splits i, i + 16, ...
+template <int HD, class TO>
+__global__ __launch_bounds__(256) void window_join_k(WindowArgs a, int splits) {
+    constexpr int E = HD / 16;
+    const int lane = threadIdx.x % 64, i16 = lane % 16;
+    const long rows = (long)a.n_batch * a.n_q * a.n_heads, at0 = (long)blockIdx.x * 16 + threadIdx.x / 16;
+    const long at = min(at0, rows - 1);
+    const float *st = a.ws + splits * rows * HD;
+    float m[4], f[4], mx = -INFINITY, sum = 0.f, o[E] = {};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const bool on = 16 * k + i16 < splits;
+        const float2 x = on ? *reinterpret_cast<const float2 *>(st + ((16 * k + i16) * rows + at) * 2) : make_float2(-INFINITY, 0.f);
+        m[k] = x.x;
+        f[k] = x.y;
+        mx = fmaxf(mx, x.x);
+    }
+    mx = row16_max(mx);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float w = f[k] == 0.f ? 0.f : __builtin_amdgcn_exp2f(m[k] - (mx == -INFINITY ? 0.f : mx));
+        sum = f[k] == 0.f ? sum : fmaf(f[k], w, sum);
+        f[k] = f[k] == 0.f ? -1.f : w;  // (a split without keys has no result)
+    }
+    sum = row16_sum(sum);
+    const float *src = a.ws + at * HD + i16 * E;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (16 * k >= splits) break;
+        f32x4 v[16][E / 4];  // all on their way at once (the last split's again past the end)
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+#pragma unroll
+            for (int e = 0; e < E / 4; ++e)
+                v[x][e] = *reinterpret_cast<const f32x4 *>(src + min(16 * k + x, splits - 1) * rows * HD + 4 * e);
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            const float w = __shfl(f[k], (lane & 48) + x, 64);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = w < 0.f ? o[e] : fmaf(v[x][e / 4][e % 4], w, o[e]);
+        }
+    }
+    if (at0 >= rows) return;
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    const long row = at / a.n_heads;
+    const int h = (int)(at % a.n_heads);
+    TO *out = (TO *)a.o + row * a.ldo + h * HD + i16 * E;
+#pragma unroll
+    for (int e = 0; e < E; e += 4) store4(out + e, o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+    if (a.lse && i16 == 0) a.lse[row * a.n_heads + h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * LN2;
+}
+
 // ── host ─────────────────────────────────────────────────────────────────
-// The tile kernels on bf16 operands (k_attn_window16.hip): false, launching nothing, for a shape,
-// stride or alignment that they do not take.
+// keys: per key block; cu_blocks: that fill the chip; least: steps that a part keeps.  At most 256
+// MiB of partial sums.
+inline DkvPlan dkv_plan(const WindowArgs &a, bool ws, int keys, long cu_blocks, long most_parts, long least) {
+    DkvPlan p;
+    p.keys = keys;
+    p.key_blocks = (a.n_kv + keys - 1) / keys;
+    p.sink_blocks = a.window < a.n_kv ? std::min(p.key_blocks, (a.n_sink + keys - 1) / keys) : 0;
+    p.sink_parts = p.parts = 1;
+    if (!ws) return p;
+    const long nbk = (long)a.n_batch * a.n_kv_heads, blocks = nbk * p.key_blocks, hpk = a.n_heads / a.n_kv_heads;
+    const long most = hpk * ((a.n_q + 31) / 32), usual = std::min(most, hpk * ((std::min<long>(a.n_kv, a.window) + keys + 31) / 32));
+    p.parts = (int)std::max(1l, std::min({most_parts, cu_blocks / blocks, usual / least}));
+    // a sink block's steps over the usual block's
+    p.sink_parts = (int)std::max<long>(p.parts, std::min<long>(64, (most * p.parts + usual - 1) / usual));
+    const long slot = 2l * keys * a.hd * 4;
+    while (p.sink_parts > 1 && p.sink_blocks * nbk * slot * p.sink_parts > (192l << 20)) --p.sink_parts;
+    while (p.parts > 1 && blocks * slot * p.parts > (64l << 20)) --p.parts;
+    return p;
+}
+inline size_t dkv_ws_bytes(const WindowArgs &a, const DkvPlan &p) {
+    return (size_t)a.n_batch * a.n_kv_heads * p.slots() * 2 * p.keys * a.hd * sizeof(float);
+}
+template <int HD, int BN, class TO>
+void launch_dkv_sum(const WindowArgs &a, const DkvPlan &p, hipStream_t st) {
+    const int split = (p.sink_parts > 1 ? p.sink_blocks : 0) + (p.parts > 1 ? p.key_blocks - p.sink_blocks : 0);
+    if (split)
+        hipLaunchKernelGGL((window_dkv_sum_k<HD, BN, TO>), dim3((unsigned)((long)a.n_batch * a.n_kv_heads * split), BN * HD / 512),
+                           dim3(256), 0, st, a, p);
+}
+
+// Blocks that share a KV head's keys where few rows see them (n_q query rows at most kFewRows):
+// towards `fill` blocks, while each of a block's four waves keeps a tile of `keys` keys.
+constexpr int kFewRows = 16;
+inline int step_splits(const WindowArgs &a, int keys, long fill) {
+    const long base = (long)a.n_batch * a.n_kv_heads * ((a.n_q * (a.n_heads / a.n_kv_heads) + 15) / 16);
+    const long tiles = (std::min<long>(a.n_kv, (long)a.window + a.n_q) + a.n_sink + 2 * keys - 1) / keys;
+    return (int)std::max(1l, std::min({64l, fill / base, (tiles + 3) / 4}));
+}
+inline size_t step_ws_bytes(const WindowArgs &a, int splits) {
+    return splits > 1 ? (size_t)splits * a.n_batch * a.n_q * a.n_heads * (a.hd + 2) * sizeof(float) : 0;
+}
+template <int HD, class TO>
+void launch_join(const WindowArgs &a, int splits, hipStream_t st) {
+    const long rows = (long)a.n_batch * a.n_q * a.n_heads;
+    hipLaunchKernelGGL((window_join_k<HD, TO>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a, splits);
+}
+inline bool aligned_rows(const void *x, long ld, int align, int es) { return (uintptr_t)x % align == 0 && ld * es % align == 0; }
+
+// The tile kernels on bf16 (k_attn_window16.hip) and fp32 operands (k_attn_window32.hip): false,
+// launching nothing, for a shape, stride or alignment that they do not take.
 bool window16_forward(const WindowArgs &a, hipStream_t st);
 bool window16_backward(const WindowArgs &a, hipStream_t st);
+size_t window16_fwd_ws_bytes(const WindowArgs &a);
 size_t window16_bwd_ws_bytes(const WindowArgs &a);
+bool window32_forward(const WindowArgs &a, hipStream_t st);
+bool window32_backward(const WindowArgs &a, hipStream_t st);
+size_t window32_fwd_ws_bytes(const WindowArgs &a);
+size_t window32_bwd_ws_bytes(const WindowArgs &a);
 
 }  // namespace vkh
