@@ -1250,10 +1250,13 @@ vkh_status vkh_qk_norm_rotary_forward(const vkh_rotary_params *p, const vkh_rota
     return rotary_call(p, plan, positions, true, wq, wk, false, q_in, q_out, k_in, k_out, stream);
 }
 
+static size_t rotary_ws_bytes(const RotaryArgs &a) {
+    const RotaryParts n = rotary_parts(a);
+    return (size_t)(n.q + n.k) * a.hd * sizeof(float);
+}
 size_t vkh_qk_norm_rotary_workspace_bytes(const vkh_rotary_params *p) {
     RotaryArgs a;
-    if (rotary_args(p, nullptr, nullptr, a) != VKH_OK) return 0;
-    return (size_t)rotary_parts(a) * 2 * a.hd * sizeof(float);
+    return rotary_args(p, nullptr, nullptr, a) == VKH_OK ? rotary_ws_bytes(a) : 0;
 }
 
 vkh_status vkh_qk_norm_rotary_backward(const vkh_rotary_params *p, const vkh_rotary_plan *plan,
@@ -1284,7 +1287,7 @@ vkh_status vkh_qk_norm_rotary_backward(const vkh_rotary_params *p, const vkh_rot
         CHECK_ARG((uintptr_t)workspace % 16 == 0, "the workspace is not 16-byte aligned");
         CHECK_ARG(workspace || !capturing(st), "gain gradients on a stream under capture need a workspace");
         void *w = workspace;
-        if (!w) VKH_TRY(lease.acquire((size_t)rotary_parts(a) * 2 * a.hd * sizeof(float), st, &w));
+        if (!w) VKH_TRY(lease.acquire(rotary_ws_bytes(a), st, &w));
         partial = (float *)w;
     }
     VKH_HIP(rotary_norm_backward(a, xt, gt, dt, partial, dwq, dwk, st));

@@ -10,11 +10,11 @@
 //                dx = rstd (w g - xh mean(xh w g)),  dw = sum over rows and heads of g xh
 //
 // The angle is formed in turns, in 64 bits (t up to 2^32 times a frequency loses whole
-// radians in 32), reduced to [-1/2, 1/2] and only then rounded to 32 bits.  A block computes
-// the cosines and sines of its rows once, in LDS, for all heads; head rows are held by
-// 2 V values a lane (both members of V pairs), so neither layout exchanges values between
-// lanes, and a lane's loads and stores are 8 or 16 bytes.  Every pass reads and writes each
-// value once: bound by HBM for long batches and by the launch for a few tokens.
+// radians in 32), reduced to [-1/2, 1/2] and only then rounded to 32 bits.  A wave computes
+// the cosines and sines of its row once for all heads; head rows are held by 2 V values a
+// lane (both members of V pairs), so neither layout exchanges values between lanes, and a
+// lane's loads and stores are 8 or 16 bytes.  Every pass reads and writes each value once: bound
+// by HBM for long batches and by the launch for a few tokens.
 #include <algorithm>
 #include <initializer_list>
 #include <utility>
@@ -26,8 +26,10 @@ namespace {
 
 constexpr int RNT = 256;
 
-VKH_DEV float2 cos_sin(const RotaryArgs &a, long row, int j) {
-    const unsigned t = a.pos ? a.pos[row] : a.pos0 + (unsigned)row % a.seq;
+VKH_DEV unsigned position(const RotaryArgs &a, long row) {
+    return a.pos ? a.pos[row] : a.pos0 + (unsigned)row % a.seq;
+}
+VKH_DEV float2 cos_sin(const RotaryArgs &a, unsigned t, int j) {
     double turn = (double)t * a.turns[j];
     turn -= rint(turn);
     float s, c;
@@ -65,10 +67,17 @@ VKH_DEV void store_v(bf16 *p, const float (&o)[V]) {
     *reinterpret_cast<vec *>(p) = f;
 }
 
+// gains (any alignment)
+template <int V>
+VKH_DEV void load_gain(const float *p, float (&o)[V], float quirk) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = p[i] + quirk;
+}
+
 // The V pairs that a lane holds as two chunks, turned.  Half layout: pair i is (a[i], b[i]);
 // interleaved: neighbours within a, then within b.
 template <int V>
-VKH_DEV void turn_pairs(float (&a)[V], float (&b)[V], const float2 *cs, bool interleaved) {
+VKH_DEV void turn_pairs(float (&a)[V], float (&b)[V], const float2 (&cs)[V], bool interleaved) {
     if (interleaved) {
 #pragma unroll
         for (int i = 0; i < V / 2; ++i) {
@@ -90,9 +99,13 @@ VKH_DEV void turn_pairs(float (&a)[V], float (&b)[V], const float2 *cs, bool int
     }
 }
 
-// sum over the LP lanes (a power of two) of a head row
+// sum over the LP lanes (a power of two, at most 32) of a head row
 VKH_DEV float row_sum(float v, int LP) {
-    for (int o = LP / 2; o; o /= 2) v += __shfl_xor(v, o, 64);
+    if (LP > 1) v += dpp_f<0xB1>(v);   // quad_perm [1,0,3,2]
+    if (LP > 2) v += dpp_f<0x4E>(v);   // quad_perm [2,3,0,1]
+    if (LP > 4) v += dpp_f<0x141>(v);  // row_half_mirror
+    if (LP > 8) v += dpp_f<0x140>(v);  // row_mirror
+    if (LP > 16) v += __shfl_xor(v, 16, 64);
     return v;
 }
 
@@ -104,169 +117,185 @@ VKH_DEV void chunks(const RotaryArgs &a, int t, int V, int &e0, int &e1) {
     if (!a.interleaved && turned) e0 = t * V, e1 = a.rot / 2 + t * V;
 }
 
-// Forward of both operators, and the rotary backward (a.sign = -1, dy in, dx out).  A block
-// takes RB rows; grid.y > 1 (RB = 1) shares a row's heads between blocks.  The next head
-// row's values are loaded before the present one is stored.
-template <class TX, class TY, int V, bool NORM>
-__global__ __launch_bounds__(RNT) void rotary_fwd_k(RotaryArgs a, int RB, int LP) {
-    extern __shared__ float2 cs[];
-    const int tid = threadIdx.x, t = tid % LP, grp = tid / LP, NG = RNT / LP;
-    const int half = a.rot / 2, hd = a.hd, H = a.nh[0] + a.nh[1];
-    const long row0 = (long)blockIdx.x * RB;
-    const int nr = (int)min((long)RB, a.n_rows - row0), items = nr * H;
-    const bool act = 2 * t * V < hd, turned = 2 * t * V < a.rot;
-    int e0, e1;
-    chunks(a, t, V, e0, e1);
-    auto src = [&](int it) {
-        const long row = row0 + it / H;
-        const int h = it % H;
-        return h < a.nh[0] ? (const TX *)a.s[0].x + row * a.s[0].ldx + (long)h * hd
-                           : (const TX *)a.s[1].x + row * a.s[1].ldx + (long)(h - a.nh[0]) * hd;
-    };
-    auto fetch = [&](int it, float (&u)[V], float (&v)[V]) {
-        if (it >= items || !act) {
+// The cosines and sines of a row for the V pairs of each lane: a wave computes one pair a lane and
+// hands them round through its own LDS (128 pairs).
+template <int V>
+VKH_DEV void row_angles(const RotaryArgs &a, unsigned pos, float2 *sh, int lane, int t, float2 (&cs)[V]) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last row's are read
+    for (int j = lane; j < a.rot / 2; j += 64) sh[j] = cos_sin(a, pos, j);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (2 * t * V < a.rot) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) u[i] = v[i] = 0.f;
-            return;
-        }
-        const TX *p = src(it);
-        load_v<V>(p + e0, u);
-        load_v<V>(p + e1, v);
-    };
-    const int step = NG * gridDim.y;
-    const int first = blockIdx.y * NG + grp, wave0 = blockIdx.y * NG + (tid - tid % 64) / LP;
-    float u[V], v[V], wg[2][2 * V];
-    fetch(first, u, v);
-    if constexpr (NORM) {
+        for (int i = 0; i < V; ++i) cs[i] = sh[t * V + i];
+    } else {
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const bool on = act && a.nh[k];
-                wg[k][i] = on ? a.s[k].w[e0 + i] + a.quirk : 0.f;
-                wg[k][V + i] = on ? a.s[k].w[e1 + i] + a.quirk : 0.f;
-            }
-    }
-    for (int i = tid; i < nr * half; i += RNT) cs[i] = cos_sin(a, row0 + i / half, i % half);
-    __syncthreads();
-    const float inv_hd = 1.0f / (float)hd;
-    for (int w0 = wave0, it = first; w0 < items; w0 += step, it += step) {
-        float nu[V], nv[V];
-        fetch(it + step, nu, nv);
-        const int h = it % H;
-        const bool isk = h >= a.nh[0];
-        if constexpr (NORM) {
-            float ss = 0.f;
-#pragma unroll
-            for (int i = 0; i < V; ++i) ss = fmaf(u[i], u[i], fmaf(v[i], v[i], ss));
-            const float r = 1.0f / sqrtf(row_sum(ss, LP) * inv_hd + a.eps);
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                u[i] = u[i] * r * (isk ? wg[1][i] : wg[0][i]);
-                v[i] = v[i] * r * (isk ? wg[1][V + i] : wg[0][V + i]);
-            }
-        }
-        if (it < items && act) {
-            const long row = row0 + it / H;
-            if (turned) turn_pairs<V>(u, v, cs + (it / H) * half + t * V, a.interleaved);
-            TY *p = isk ? (TY *)a.s[1].y + row * a.s[1].ldy + (long)(h - a.nh[0]) * hd
-                        : (TY *)a.s[0].y + row * a.s[0].ldy + (long)h * hd;
-            store_v<V>(p + e0, u);
-            store_v<V>(p + e1, v);
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) u[i] = nu[i], v[i] = nv[i];
+        for (int i = 0; i < V; ++i) cs[i] = make_float2(1.f, 0.f);
     }
 }
 
-// Backward of norm + rotary.  Blocks walk tiles of RB rows, the query heads of a tile first
-// and then its key heads, so each gain's gradient has one set of sums per lane (a lane holds
-// the same values of every head row); a block's sums go to its row of `partial`
-// ([blocks][2 hd]), which rotary_dw_k adds in block order.
+// Forward of both operators, and the rotary backward (a.sign = -1, dy in, dx out).  HS waves share
+// a row (4 where rows are few: one token's latency; 1 where they fill the chip), 64 / LP heads at a
+// time; the next heads' values are on their way while the present ones are turned.
+// 16384 rows, 32 / 8 heads of 128, bf16: 73 us a rotation with a block per 4 rows over a flat list
+// of heads; with the norm 105 us.
+template <class TX, class TY, int V, bool NORM>
+__global__ __launch_bounds__(RNT) void rotary_fwd_k(RotaryArgs a, int HS, int LP) {
+    __shared__ float2 sh[RNT / 64][128];
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int t = lane % LP, grp = lane / LP, NG = 64 / LP, hd = a.hd;
+    const long row = (long)blockIdx.x * (RNT / 64 / HS) + wave / HS;
+    if (row >= a.n_rows) return;
+    const bool act = 2 * t * V < hd;
+    const int step = NG * HS, first = wave % HS * NG;
+    int e0, e1;
+    chunks(a, t, V, e0, e1);
+    const float inv_hd = 1.0f / (float)hd;
+    float2 cs[V];
+    bool angles = false;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const RotarySide &s = a.s[k];
+        const int H = a.nh[k];
+        if (first >= H) continue;
+        const TX *x = (const TX *)s.x + row * s.ldx;
+        TY *y = (TY *)s.y + row * s.ldy;
+        auto fetch = [&](int h, float (&u)[V], float (&v)[V]) {
+            if (h < H && act) {
+                load_v<V>(x + h * hd + e0, u);
+                load_v<V>(x + h * hd + e1, v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) u[i] = v[i] = 0.f;
+            }
+        };
+        float u[V], v[V], w0[V], w1[V];
+        fetch(first + grp, u, v);
+        if constexpr (NORM) {
+            if (act) {
+                load_gain<V>(s.w + e0, w0, a.quirk);
+                load_gain<V>(s.w + e1, w1, a.quirk);
+            }
+        }
+        if (!angles) row_angles<V>(a, position(a, row), sh[wave], lane, t, cs);
+        angles = true;
+        for (int h0 = first; h0 < H; h0 += step) {
+            float nu[V], nv[V];
+            if (h0 + step < H) fetch(h0 + step + grp, nu, nv);
+            if constexpr (NORM) {
+                float ss = 0.f;
+#pragma unroll
+                for (int i = 0; i < V; ++i) ss = fmaf(u[i], u[i], fmaf(v[i], v[i], ss));
+                const float r = rsqrtf(fmaf(row_sum(ss, LP), inv_hd, a.eps));
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    u[i] = u[i] * r * w0[i];
+                    v[i] = v[i] * r * w1[i];
+                }
+            }
+            turn_pairs<V>(u, v, cs, a.interleaved);
+            if (h0 + grp < H && act) {
+                store_v<V>(y + (h0 + grp) * hd + e0, u);
+                store_v<V>(y + (h0 + grp) * hd + e1, v);
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) u[i] = nu[i], v[i] = nv[i];
+        }
+    }
+}
+
+// Backward of norm + rotary.  The first parts.q blocks take the query heads, the others the key
+// heads: a lane then has one set of sums for its gain's gradient (it holds the same values of every
+// head row), and registers for more waves.  A wave walks rows, 64 / LP heads at a time; the next
+// heads' values, also the next row's, are on their way while the present ones are worked on.  A
+// block's sums go to its row of `partial` ([blocks][hd]), which rotary_dw_k adds in block order.
 template <class TX, class TG, class TD, int V>
-__global__ __launch_bounds__(RNT) void rotary_norm_bwd_k(RotaryArgs a, int RB, int LP, float *partial) {
-    extern __shared__ float2 cs[];  // RB rot / 2 cosines and sines; afterwards NG hd gain sums
-    const int tid = threadIdx.x, t = tid % LP, grp = tid / LP, NG = RNT / LP;
-    const int half = a.rot / 2, hd = a.hd;
-    const bool act = 2 * t * V < hd, turned = 2 * t * V < a.rot;
+__global__ __launch_bounds__(RNT) void rotary_norm_bwd_k(RotaryArgs a, int LP, RotaryParts parts, float *partial) {
+    __shared__ float2 sh[RNT / 64][128];
+    extern __shared__ float sums[];  // 256 / LP head rows of hd gain sums
+    const bool isk = (int)blockIdx.x >= parts.q;
+    const RotarySide s = isk ? a.s[1] : a.s[0];
+    const int H = isk ? a.nh[1] : a.nh[0], blk = blockIdx.x - (isk ? parts.q : 0);
+    const long stride = (long)(isk ? parts.k : parts.q) * (RNT / 64);
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int t = lane % LP, grp = lane / LP, NG = 64 / LP, hd = a.hd;
+    const bool act = 2 * t * V < hd;
     const float inv_hd = 1.0f / (float)hd;
     int e0, e1;
     chunks(a, t, V, e0, e1);
-    float dw[2][2 * V] = {};
-    for (long row0 = (long)blockIdx.x * RB; row0 < a.n_rows; row0 += (long)gridDim.x * RB) {
-        const int nr = (int)min((long)RB, a.n_rows - row0);
-        __syncthreads();  // everyone is done with the last tile's angles
-        for (int i = tid; i < nr * half; i += RNT) cs[i] = cos_sin(a, row0 + i / half, i % half);
-        __syncthreads();
+    float dw[2 * V] = {}, w0[V] = {}, w1[V] = {};
+    if (act) {
+        load_gain<V>(s.w + e0, w0, a.quirk);
+        load_gain<V>(s.w + e1, w1, a.quirk);
+    }
+    float2 cs[V];
+    float x0[V], x1[V], g0[V], g1[V];
+    auto fetch = [&](long row, int h, float (&x0)[V], float (&x1)[V], float (&g0)[V], float (&g1)[V]) {
+        if (row < a.n_rows && h < H && act) {
+            const TX *x = (const TX *)s.x + row * s.ldx + h * hd;
+            const TG *dy = (const TG *)s.dy + row * s.lddy + h * hd;
+            load_v<V>(x + e0, x0);
+            load_v<V>(x + e1, x1);
+            load_v<V>(dy + e0, g0);
+            load_v<V>(dy + e1, g1);
+        } else {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const RotarySide &s = a.s[k];
-            const int H = a.nh[k], items = nr * H;
-            if (!H) continue;
-            float w[2 * V];
+            for (int i = 0; i < V; ++i) x0[i] = x1[i] = g0[i] = g1[i] = 0.f;
+        }
+    };
+    long row = (long)blk * (RNT / 64) + wave;
+    unsigned pos = row < a.n_rows ? position(a, row) : 0;
+    fetch(row, grp, x0, x1, g0, g1);
+    while (row < a.n_rows) {
+        const long next = row + stride;
+        const unsigned npos = next < a.n_rows ? position(a, next) : 0;
+        row_angles<V>(a, pos, sh[wave], lane, t, cs);
+        for (int h0 = 0; h0 < H; h0 += NG) {
+            float nx0[V], nx1[V], ng0[V], ng1[V];
+            const bool same = h0 + NG < H;
+            fetch(same ? row : next, (same ? h0 + NG : 0) + grp, nx0, nx1, ng0, ng1);
+            float ss = 0.f, dot = 0.f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) ss = fmaf(x0[i], x0[i], fmaf(x1[i], x1[i], ss));
+            turn_pairs<V>(g0, g1, cs, a.interleaved);
+            const float r = rsqrtf(fmaf(row_sum(ss, LP), inv_hd, a.eps));
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                w[i] = act ? s.w[e0 + i] + a.quirk : 0.f;
-                w[V + i] = act ? s.w[e1 + i] + a.quirk : 0.f;
+                x0[i] *= r;
+                x1[i] *= r;
+                dw[i] = fmaf(g0[i], x0[i], dw[i]);
+                dw[V + i] = fmaf(g1[i], x1[i], dw[V + i]);
+                g0[i] *= w0[i];
+                g1[i] *= w1[i];
+                dot = fmaf(x0[i], g0[i], fmaf(x1[i], g1[i], dot));
             }
-            for (int w0 = (tid - tid % 64) / LP, it = grp; w0 < items; w0 += NG, it += NG) {
-                const bool on = it < items && act;
-                const long row = row0 + it / H;
-                const long h = (long)(it % H) * hd;
-                float x0[V] = {}, x1[V] = {}, g0[V] = {}, g1[V] = {};
-                if (on) {
-                    const TX *xp = (const TX *)s.x + row * s.ldx + h;
-                    const TG *gp = (const TG *)s.dy + row * s.lddy + h;
-                    load_v<V>(xp + e0, x0);
-                    load_v<V>(xp + e1, x1);
-                    load_v<V>(gp + e0, g0);
-                    load_v<V>(gp + e1, g1);
-                }
-                float ss = 0.f;
+            const float m = row_sum(dot, LP) * inv_hd;
 #pragma unroll
-                for (int i = 0; i < V; ++i) ss = fmaf(x0[i], x0[i], fmaf(x1[i], x1[i], ss));
-                if (on && turned) turn_pairs<V>(g0, g1, cs + (it / H) * half + t * V, a.interleaved);
-                const float r = 1.0f / sqrtf(row_sum(ss, LP) * inv_hd + a.eps);
-                float dot = 0.f;
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    x0[i] *= r;
-                    x1[i] *= r;
-                    dw[k][i] = fmaf(g0[i], x0[i], dw[k][i]);
-                    dw[k][V + i] = fmaf(g1[i], x1[i], dw[k][V + i]);
-                    g0[i] *= w[i];
-                    g1[i] *= w[V + i];
-                    dot = fmaf(x0[i], g0[i], fmaf(x1[i], g1[i], dot));
-                }
-                const float m = row_sum(dot, LP) * inv_hd;
-                if (on) {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        g0[i] = (g0[i] - x0[i] * m) * r;
-                        g1[i] = (g1[i] - x1[i] * m) * r;
-                    }
-                    TD *dp = (TD *)s.dx + row * s.lddx + h;
-                    store_v<V>(dp + e0, g0);
-                    store_v<V>(dp + e1, g1);
-                }
+            for (int i = 0; i < V; ++i) {
+                g0[i] = (g0[i] - x0[i] * m) * r;
+                g1[i] = (g1[i] - x1[i] * m) * r;
             }
+            if (h0 + grp < H && act) {
+                TD *dx = (TD *)s.dx + row * s.lddx + (h0 + grp) * hd;
+                store_v<V>(dx + e0, g0);
+                store_v<V>(dx + e1, g1);
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) x0[i] = nx0[i], x1[i] = nx1[i], g0[i] = ng0[i], g1[i] = ng1[i];
         }
+        row = next;
+        pos = npos;
     }
     if (!partial) return;
-    float *sh = reinterpret_cast<float *>(cs);
+    if (act) {
+        float *mine = sums + (wave * NG + grp) * hd;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        __syncthreads();
-        if (act) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) sh[grp * hd + e0 + i] = dw[k][i], sh[grp * hd + e1 + i] = dw[k][V + i];
-        }
-        __syncthreads();
-        for (int c = tid; c < hd; c += RNT) {
-            float s = 0.f;
-            for (int g = 0; g < NG; ++g) s += sh[g * hd + c];
-            partial[(long)blockIdx.x * 2 * hd + k * hd + c] = s;
-        }
+        for (int i = 0; i < V; ++i) mine[e0 + i] = dw[i], mine[e1 + i] = dw[V + i];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < hd; c += RNT) {
+        float x = 0.f;
+        for (int g = 0; g < RNT / LP; ++g) x += sums[g * hd + c];
+        partial[(long)blockIdx.x * hd + c] = x;
     }
 }
 
@@ -312,7 +341,7 @@ __global__ __launch_bounds__(RNT) void rotary_fwd_any_k(RotaryArgs a) {
             if (e.e1 >= 0) v[i] = v[i] * r * (s.w[e.e1] + a.quirk);
         }
         if (e.e1 >= 0) {
-            const float2 c = cos_sin(a, row, lane + 64 * i);
+            const float2 c = cos_sin(a, position(a, row), lane + 64 * i);
             const float p = u[i] * c.x - v[i] * c.y;
             v[i] = v[i] * c.x + u[i] * c.y;
             u[i] = p;
@@ -322,15 +351,16 @@ __global__ __launch_bounds__(RNT) void rotary_fwd_any_k(RotaryArgs a) {
     }
 }
 template <class TX, class TG, class TD>
-__global__ __launch_bounds__(RNT) void rotary_norm_bwd_any_k(RotaryArgs a, float *partial) {
+__global__ __launch_bounds__(RNT) void rotary_norm_bwd_any_k(RotaryArgs a, RotaryParts parts, float *partial) {
     __shared__ float sh[RNT / 64][256];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-#pragma unroll 1
-    for (int k = 0; k < 2; ++k) {
-        const RotarySide &s = a.s[k];
+    {
+        const bool isk = (int)blockIdx.x >= parts.q;
+        const RotarySide s = isk ? a.s[1] : a.s[0];
+        const int H = isk ? a.nh[1] : a.nh[0], blk = blockIdx.x - (isk ? parts.q : 0);
         float du[GI] = {}, dv[GI] = {};
-        for (long it = (long)blockIdx.x * (RNT / 64) + wave; it < a.n_rows * a.nh[k]; it += (long)gridDim.x * (RNT / 64)) {
-            const long row = it / a.nh[k], h = it % a.nh[k] * a.hd;
+        for (long it = (long)blk * (RNT / 64) + wave; it < a.n_rows * H; it += (long)(isk ? parts.k : parts.q) * (RNT / 64)) {
+            const long row = it / H, h = it % H * a.hd;
             const TX *x = (const TX *)s.x + row * s.ldx + h;
             const TG *dy = (const TG *)s.dy + row * s.lddy + h;
             TD *dx = (TD *)s.dx + row * s.lddx + h;
@@ -344,7 +374,7 @@ __global__ __launch_bounds__(RNT) void rotary_norm_bwd_any_k(RotaryArgs a, float
                 q[i] = e.e1 >= 0 ? to_f32(dy[e.e1]) : 0.f;
                 ss = fmaf(u[i], u[i], fmaf(v[i], v[i], ss));
                 if (e.e1 >= 0) {
-                    const float2 c = cos_sin(a, row, lane + 64 * i);
+                    const float2 c = cos_sin(a, position(a, row), lane + 64 * i);
                     const float g = p[i] * c.x - q[i] * c.y;
                     q[i] = q[i] * c.x + p[i] * c.y;
                     p[i] = g;
@@ -371,8 +401,7 @@ __global__ __launch_bounds__(RNT) void rotary_norm_bwd_any_k(RotaryArgs a, float
                 if (e.e1 >= 0) dx[e.e1] = (TD)((q[i] - v[i] * m) * r);
             }
         }
-        if (!partial) continue;
-        __syncthreads();
+        if (!partial) return;
 #pragma unroll
         for (int i = 0; i < GI; ++i) {
             const RotItem e = rot_item(a, lane + 64 * i);
@@ -383,27 +412,34 @@ __global__ __launch_bounds__(RNT) void rotary_norm_bwd_any_k(RotaryArgs a, float
         for (int c = threadIdx.x; c < a.hd; c += RNT) {
             float t = 0.f;
             for (int w = 0; w < RNT / 64; ++w) t += sh[w][c];
-            partial[(long)blockIdx.x * 2 * a.hd + k * a.hd + c] = t;
+            partial[(long)blockIdx.x * a.hd + c] = t;
         }
     }
 }
 
-// dw of both gains: column c of the 2 hd partial sums, 16 columns a block, each added by 16
-// threads over every 16th block's row and then in thread order.
-__global__ __launch_bounds__(RNT) void rotary_dw_k(const float *partial, int parts, int hd, float *dwq, float *dwk) {
-    __shared__ float sh[16][17];
-    const int c = threadIdx.x % 16, r = threadIdx.x / 16, col = blockIdx.x * 16 + c;
-    float s = 0.f;
-    if (col < 2 * hd)
-        for (int b = r; b < parts; b += 16) s += partial[(long)b * 2 * hd + col];
-    sh[r][c] = s;
-    __syncthreads();
-    if (r || col >= 2 * hd) return;
-    float t = 0.f;
+// The gain gradients: four columns of one side's partial sums a block; thread r adds every 256th
+// block's row, then the threads' sums are added by halves.
+__global__ __launch_bounds__(RNT) void rotary_dw_k(const float *partial, RotaryParts parts, int hd, float *dwq, float *dwk) {
+    __shared__ f32x4 sh[RNT];
+    const int r = threadIdx.x, col = blockIdx.x * 4;
+    const bool isk = blockIdx.y;
+    float *out = isk ? dwk : dwq;
+    if (!out) return;
+    partial += isk ? (long)parts.q * hd : 0;
+    f32x4 s{0, 0, 0, 0};
+    for (int b = r; b < (isk ? parts.k : parts.q); b += RNT)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t += sh[i][c];
-    float *out = col < hd ? dwq : dwk;
-    if (out) out[col % hd] = t;
+        for (int i = 0; i < 4; ++i)
+            if (col + i < hd) s[i] += partial[(long)b * hd + col + i];
+    sh[r] = s;
+    for (int o = RNT / 2; o; o /= 2) {
+        __syncthreads();
+        if (r < o) sh[r] += sh[r + o];
+    }
+    if (r) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (col + i < hd) out[col + i] = sh[0][i];
 }
 
 // Chunk width: 8 values where both dtypes' rows allow 16-byte (fp32: two 16-byte) accesses,
@@ -439,12 +475,13 @@ void by_type(DType d, F f) {
 
 }  // namespace
 
-// Partial rows of the gain sums: at most kRotaryParts blocks.
-constexpr int kRotaryParts = 512;
-static int bwd_rows(const RotaryArgs &a) { return a.n_rows >= 4 * kRotaryParts ? 4 : a.n_rows >= 2 * kRotaryParts ? 2 : 1; }
-int rotary_parts(const RotaryArgs &a) {
-    const int RB = bwd_rows(a);
-    return (int)std::min<long>(kRotaryParts, (a.n_rows + RB - 1) / RB);
+// Blocks of each side: five a CU in all (as many as fit at 4-value chunks), shared by the sides'
+// heads, at most one a wave's row.  16384 rows, 32 / 8 heads of 128, bf16: 114 us; 8-value chunks fill
+// the registers with three a CU and take 123; 2048 rows, 16 / 8 heads, fp32 to bf16: 14 against 18.
+RotaryParts rotary_parts(const RotaryArgs &a) {
+    const long H = a.nh[0] + a.nh[1], rows = (a.n_rows + RNT / 64 - 1) / (RNT / 64);
+    auto of = [&](int nh) { return nh ? (int)std::max(1l, std::min(rows, 1280 * nh / H)) : 0; };
+    return RotaryParts{of(a.nh[0]), of(a.nh[1])};
 }
 
 hipError_t rotary_forward(const RotaryArgs &a, bool norm, DType xt, DType yt, hipStream_t st) {
@@ -462,16 +499,13 @@ hipError_t rotary_forward(const RotaryArgs &a, bool norm, DType xt, DType yt, hi
         });
         return hipGetLastError();
     }
-    const int LP = lanes(a.hd, V), NG = RNT / LP;
-    const int RB = a.n_rows >= 4096 ? 4 : a.n_rows >= 2048 ? 2 : 1;
-    const unsigned gy = RB == 1 && a.n_rows < 256 ? (unsigned)((H + NG - 1) / NG) : 1u;
-    const dim3 grid((unsigned)((a.n_rows + RB - 1) / RB), gy);
-    const unsigned lds = std::max(1, RB * a.rot / 2) * sizeof(float2);
+    const int LP = lanes(a.hd, V), HS = a.n_rows >= 2048 ? 1 : a.n_rows >= 1024 ? 2 : 4, per = RNT / 64 / HS;
+    const dim3 grid((unsigned)((a.n_rows + per - 1) / per));
     by_type(xt, [&](auto x) {
         by_type(yt, [&](auto y) {
             using X = decltype(x);
             using Y = decltype(y);
-            auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, dim3(RNT), lds, st, a, RB, LP); };
+            auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, dim3(RNT), 0, st, a, HS, LP); };
             if (V == 8) norm ? go(rotary_fwd_k<X, Y, 8, true>) : go(rotary_fwd_k<X, Y, 8, false>);
             else norm ? go(rotary_fwd_k<X, Y, 4, true>) : go(rotary_fwd_k<X, Y, 4, false>);
         });
@@ -482,28 +516,26 @@ hipError_t rotary_forward(const RotaryArgs &a, bool norm, DType xt, DType yt, hi
 hipError_t rotary_norm_backward(const RotaryArgs &a, DType xt, DType gt, DType dt, float *partial,
                                 float *dwq, float *dwk, hipStream_t st) {
     if (a.n_rows <= 0 || !(a.nh[0] + a.nh[1])) return hipSuccess;
-    const int V = chunk_width(a, {{xt, 0}, {gt, 2}, {dt, 3}});
-    const int parts = rotary_parts(a), RB = bwd_rows(a);
+    const bool chunked = chunk_width(a, {{xt, 0}, {gt, 2}, {dt, 3}}) != 0;
+    const RotaryParts parts = rotary_parts(a);
+    const dim3 grid(parts.q + parts.k);
     by_type(xt, [&](auto x) {
         by_type(gt, [&](auto g) {
             by_type(dt, [&](auto d) {
                 using X = decltype(x);
                 using G = decltype(g);
                 using D = decltype(d);
-                if (!V) {
-                    hipLaunchKernelGGL((rotary_norm_bwd_any_k<X, G, D>), dim3(parts), dim3(RNT), 0, st, a, partial);
+                if (!chunked) {
+                    hipLaunchKernelGGL((rotary_norm_bwd_any_k<X, G, D>), grid, dim3(RNT), 0, st, a, parts, partial);
                     return;
                 }
-                const int LP = lanes(a.hd, V);
-                const unsigned lds = std::max<unsigned>(RB * a.rot / 2 * sizeof(float2), RNT / LP * a.hd * sizeof(float));
-                auto go = [&](auto k) { hipLaunchKernelGGL(k, dim3(parts), dim3(RNT), lds, st, a, RB, LP, partial); };
-                if (V == 8) go(rotary_norm_bwd_k<X, G, D, 8>);
-                else go(rotary_norm_bwd_k<X, G, D, 4>);
+                const int LP = lanes(a.hd, 4);
+                hipLaunchKernelGGL((rotary_norm_bwd_k<X, G, D, 4>), grid, dim3(RNT), RNT / LP * a.hd * sizeof(float), st, a, LP, parts, partial);
             });
         });
     });
     if (partial)
-        hipLaunchKernelGGL(rotary_dw_k, dim3((2 * a.hd + 15) / 16), dim3(RNT), 0, st, partial, parts, a.hd, dwq, dwk);
+        hipLaunchKernelGGL(rotary_dw_k, dim3((a.hd + 3) / 4, 2), dim3(RNT), 0, st, partial, parts, a.hd, dwq, dwk);
     return hipGetLastError();
 }
 

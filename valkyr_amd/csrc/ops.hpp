@@ -273,11 +273,14 @@ struct RotaryArgs {
 };
 // y = rotation of x, or (norm) of x rstd w; any head_dim up to 256.
 hipError_t rotary_forward(const RotaryArgs &a, bool norm, DType xt, DType yt, hipStream_t st);
-// dx of the norm and rotation (a.sign = -1), and with `partial` (rotary_parts(a) rows of 2 hd
-// floats) the gain gradients dwq / dwk (overwrite; either may be null).
+// dx of the norm and rotation (a.sign = -1), and with `partial` (a row of hd floats for each of
+// rotary_parts(a)'s blocks) the gain gradients dwq / dwk (overwrite; either may be null).
 hipError_t rotary_norm_backward(const RotaryArgs &a, DType xt, DType gt, DType dt, float *partial,
                                 float *dwq, float *dwk, hipStream_t st);
-int rotary_parts(const RotaryArgs &a);
+struct RotaryParts {
+    int q, k;  // blocks on query heads, on key heads
+};
+RotaryParts rotary_parts(const RotaryArgs &a);
 
 // Fused per-head Q/K RMSNorm + RoPE forward, emitting the attention
 // operands (fp32 or bf16) for q, k and (copy/cast of) v.
