@@ -84,9 +84,8 @@ __device__ __attribute__((noinline)) void dkv_rows(const WindowArgs &a, const St
 }
 
 // ── forward ──────────────────────────────────────────────────────────────
-// Block = 64 QS query rows of one head, 4 waves of 16 QS; 64-key tiles, two buffers.  Block ids run
-// over (sequence, KV head) first, so the blocks of one KV head sit on one XCD and share its
-// tiles there, and the heaviest (last) rows start first.
+// Block = 64 QS query rows of one head, 4 waves of 16 QS; 64-key tiles, two buffers.  The
+// heaviest (last) rows start first.
 template <int HD, int QS, class TO>
 __global__ __launch_bounds__(256, 2) void window_fwd16_k(WindowArgs a) {
     using R = TileRows<HD>;
@@ -94,8 +93,8 @@ __global__ __launch_bounds__(256, 2) void window_fwd16_k(WindowArgs a) {
     constexpr int RPI = 512 / HD, IPW = 16 / RPI;  // rows per DMA, DMAs per wave and tile
     __shared__ __attribute__((aligned(16))) char Ks[2][KT], Vs[2][KT];
     const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, nqt = (a.n_q + BM - 1) / BM;
-    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
-    const int h = kvh * grp + blockIdx.x / nbk % grp, qt = nqt - 1 - (int)(blockIdx.x / nbk / grp);
+    const Pair pr = pair_of(blockIdx.x, gridDim.x, nbk, 4 * grp);
+    const int b = pr.bk / a.n_kv_heads, kvh = pr.bk % a.n_kv_heads, h = kvh * grp + pr.y % grp, qt = nqt - 1 - pr.y / grp;
     const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c16 = lane % 16;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const Span s = span_of(a, b);
@@ -281,8 +280,8 @@ __global__ __launch_bounds__(256, 1) void window_step16_k(WindowArgs a, int spli
     __shared__ float ml[4][2][16];
     static_assert(16 * RL * 4 <= 4 * TILE, "a wave's result fits its tiles");
     const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, M = a.n_q * grp, RT = (M + 15) / 16;
-    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
-    const int rt = blockIdx.x / nbk % RT, split = blockIdx.x / nbk / RT;
+    const Pair pr = pair_of(blockIdx.x, gridDim.x, nbk, 4);
+    const int b = pr.bk / a.n_kv_heads, kvh = pr.bk % a.n_kv_heads, rt = pr.y % RT, split = pr.y / RT;
     const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c16 = lane % 16;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const Span s = span_of(a, b);
@@ -425,21 +424,22 @@ __global__ __launch_bounds__(256, 1) void window_step16_k(WindowArgs a, int spli
 }
 
 // ── backward: D and dQ ───────────────────────────────────────────────────
-// Block = BQ query rows of one head on NWV waves of 16 QSUB rows, whose Q and dO fragments stay in
+// Block = BQ query rows of one head on 4 waves of 16 QSUB rows, whose Q and dO fragments stay in
 // registers; 32-key tiles of K and V through three buffers (two in flight, the wait counted).
 // D = rowsum(O dO) of the block's rows is formed first (fp64 sums of the bf16 products) and
 // stored for the dK/dV kernel, which runs after this one.
-template <int HD, int NWV, int BQ, class TO>
-__global__ __launch_bounds__(NWV * 64, 1) void window_dq16_k(WindowArgs a) {
+template <int HD, int BQ, class TO>
+__global__ __launch_bounds__(256, 2) void window_dq16_k(WindowArgs a) {
     using R = TileRows<HD>;
+    constexpr int NWV = 4;
     constexpr int QSUB = BQ / 16 / NWV, BN = 32, KS = 2, NBUF = 3, TILE = BN * HD * 2;
     constexpr int DS = HD / 32, DSUB = HD / 16, NF = 2 * DS;
     constexpr int RPI = 512 / HD, IPT = BN / RPI, C = 2 * IPT / NWV;  // DMAs per tile and tensor, per wave
     static_assert(C >= 1 && C * NWV == 2 * IPT, "DMA share");
     __shared__ __attribute__((aligned(16))) char Kt[NBUF][TILE], Vt[NBUF][TILE];
     const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, nqb = (a.n_q + BQ - 1) / BQ;
-    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
-    const int h = kvh * grp + blockIdx.x / nbk % grp, qb = nqb - 1 - (int)(blockIdx.x / nbk / grp);
+    const Pair pr = pair_of(blockIdx.x, gridDim.x, nbk, 4 * grp);
+    const int b = pr.bk / a.n_kv_heads, kvh = pr.bk % a.n_kv_heads, h = kvh * grp + pr.y % grp, qb = nqb - 1 - pr.y / grp;
     const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c16 = lane % 16;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const Span s = span_of(a, b);
@@ -637,9 +637,10 @@ __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan p
     __shared__ __attribute__((aligned(16))) float Ls[2][NBUF][64], Dd[2][NBUF][64];
 
     const int nbk = a.n_batch * a.n_kv_heads;
-    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
+    const Pair pr = pair_of(blockIdx.x, gridDim.x, nbk, 4);
+    const int bk = pr.bk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
     int kb, zpart, zparts, slot;
-    dkv_block(plan, blockIdx.x / nbk, kb, zpart, zparts, slot);
+    dkv_block(plan, pr.y, kb, zpart, zparts, slot);
     const int hpk = a.n_heads / a.n_kv_heads;
     const bool alt = hpk & 1;
     const int nh = alt ? hpk : hpk / 2;  // heads per group
@@ -829,7 +830,7 @@ __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan p
         if (it0 + 1 < niter) step(it0 + 1, std::integral_constant<int, 1>{});
         if (it0 + 2 < niter) step(it0 + 2, std::integral_constant<int, 2>{});
     }
-    float *ws = zparts > 1 ? a.ws + ((long)bk * plan.slots() + slot) * (2 * BN * HD) : nullptr;
+    float *ws = slot >= 0 ? a.ws + ((long)bk * plan.slots() + slot) * (2 * BN * HD) : nullptr;
     if (__syncthreads_or(odd)) {
         float *sh = (float *)smem + wave * 2 * HD;
         const Steps st{kvh * hpk, qstart, top, nh, alt, 2, zpart, zparts};
@@ -864,13 +865,176 @@ __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan p
             }
         }
     };
-    if (zparts > 1) {
+    if (ws) {
         if (hg == 0) keep(dvt, ws + BN * HD, HD, true, 1.f);
         else keep(dkt, ws, HD, true, a.scale);
         return;
     }
     if (hg == 0) keep(dvt, (TO *)a.dv + (key0 + k0) * a.lddv + kvh * HD, a.lddv, false, 1.f);
     else keep(dkt, (TO *)a.dk + (key0 + k0) * a.lddk + kvh * HD, a.lddk, false, a.scale);
+}
+
+// ── backward: dK and dV of the sinks from rows past their window ─────────
+// A wave holds 32 sinks' K and V in registers and streams 32-query tiles of its own (Q and dO, two
+// tiles in LDS, no barrier between the waves) from the first row past a sink's window to the last,
+// over the query heads of the KV head; the block's four waves and then the blocks' parts are added in
+// order.  The key blocks leave these pairs out: with them, the sink blocks' steps past the window, for
+// which three waves of four had nothing to do, took 1442 us of dK/dV to 1177 without (16384 tokens,
+// window 2048, 4 sinks, 32 / 8 heads of 128).
+template <int HD>
+__global__ __launch_bounds__(256, 1) void window_far16_k(WindowArgs a, DkvPlan plan) {
+    using R = TileRows<HD>;
+    constexpr int KS = 2, QS = 2, BM = 32, TILE = BM * HD * 2, DS = HD / 32, DSUB = HD / 16, RPI = 512 / HD, C = BM / RPI;
+    __shared__ __attribute__((aligned(16))) char tiles[4][2][2 * TILE];
+    __shared__ __attribute__((aligned(16))) float stat[4][2][2][64];  // LSE and D of a tile's rows
+    __shared__ bf16x8 wl[4][64];
+    const int nbk = a.n_batch * a.n_kv_heads, hpk = a.n_heads / a.n_kv_heads;
+    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
+    const int slice = blockIdx.x / nbk % plan.far_slices, part = blockIdx.x / nbk / plan.far_slices;
+    const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c16 = lane % 16;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const Span s = span_of(a, b);
+    const int k0 = 32 * slice, nk = min(min(a.n_sink, s.kl) - k0, 32);  // this slice's sinks
+    const float c2 = a.scale * LOG2E;
+    const long row0 = (long)b * a.n_q, key0 = (long)b * a.n_kv;
+    bf16x8 kr[KS][DS], vr[KS][DS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        const long row = key0 + min(k0 + 16 * ks + c16, a.n_kv - 1);
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds) {
+            kr[ks][ds] = ld_frag((const bf16 *)a.k + row * a.ldk + kvh * HD + 8 * g + 32 * ds);
+            vr[ks][ds] = ld_frag((const bf16 *)a.v + row * a.ldv + kvh * HD + 8 * g + 32 * ds);
+        }
+    }
+    unsigned qo[C], go[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        qo[i] = dma_off<HD>(RPI * i, lane, (int)a.ldq);
+        go[i] = dma_off<HD>(RPI * i, lane, (int)a.lddo);
+    }
+    const unsigned so = lane < BM ? (unsigned)(lane * a.n_heads * 4) : kOOB;
+    f32x4 dvt[KS][DSUB], dkt[KS][DSUB];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < DSUB; ++i) dvt[ks][i] = dkt[ks][i] = f32x4{0, 0, 0, 0};
+    const int qstart = max(0, k0 + a.window - s.off);  // the first row past the first sink's window
+    const int nqt = nk > 0 && s.ql > qstart ? (s.ql - qstart + BM - 1) / BM : 0, n = nqt * hpk;
+    const int step = 4 * plan.far_parts;
+    wait_vm0();
+    auto dma = [&](int it, int buf) {
+        const int h = kvh * hpk + it % hpk, q0 = qstart + it / hpk * BM, rows = min(BM, s.ql - q0);
+        const sgpr4 rq = head_rows<HD>(a.q, row0 + q0, a.ldq, h * HD, rows);
+        const sgpr4 rg = head_rows<HD>(a.dout, row0 + q0, a.lddo, h * HD, rows);
+        const long at = (row0 + q0) * a.n_heads + h;
+        const unsigned bytes = (unsigned)(((rows - 1) * a.n_heads + 1) * 4);
+#pragma unroll
+        for (int i = 0; i < C; ++i) dma16_async(rq, tiles[wave][buf] + i * 1024, qo[i]);
+#pragma unroll
+        for (int i = 0; i < C; ++i) dma16_async(rg, tiles[wave][buf] + TILE + i * 1024, go[i]);
+        dma4_async(rsrc4(a.lse + at, bytes), stat[wave][buf][0], so);
+        dma4_async(rsrc4(a.d + at, bytes), stat[wave][buf][1], so);
+    };
+    const int it0 = 4 * part + wave;
+    if (it0 < n) dma(it0, 0);
+    if (it0 + step < n) dma(it0 + step, 1);
+    for (int it = it0, buf = 0; it < n; it += step, buf ^= 1) {
+        const int q0 = qstart + it / hpk * BM;
+        const char *Qb = tiles[wave][buf], *Ob = Qb + TILE;
+        const float *L = stat[wave][buf][0], *D = stat[wave][buf][1];
+        if (it + step < n) wait_vm<2 * C + 2>();
+        else wait_vm0();
+        asm volatile("" ::: "memory");
+        // whether row q0 + x is past the window of key (ks, c16) and has a gradient
+        auto far = [&](int x, int ks) {
+            const int key = 16 * ks + c16;
+            return key < nk && q0 + x < s.ql && q0 + x + s.off - k0 - key >= a.window && L[x] != -INFINITY;
+        };
+        f32x4 sc[QS][KS], dp[QS][KS];
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) sc[qs][ks] = dp[qs][ks] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds)
+#pragma unroll
+            for (int qs = 0; qs < QS; ++qs) {
+                const bf16x8 fq = R::frag_row(Qb, 16 * qs + c16, 32 * ds + 8 * g), fo = R::frag_row(Ob, 16 * qs + c16, 32 * ds + 8 * g);
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    sc[qs][ks] = mfma16x16x32(fq, kr[ks][ds], sc[qs][ks]);
+                    dp[qs][ks] = mfma16x16x32(fo, vr[ks][ds], dp[qs][ks]);
+                }
+            }
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int x = 16 * qs + 4 * g + r;
+                const float l2 = L[x] * LOG2E, d = D[x];
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const bool on = far(x, ks);
+                    const float p = __builtin_amdgcn_exp2f(fmaf(sc[qs][ks][r], c2, -l2));
+                    sc[qs][ks][r] = on ? p : 0.f;
+                    dp[qs][ks][r] = on ? p * (dp[qs][ks][r] - d) : 0.f;
+                }
+            }
+        // the first tiles hold rows that are past some sinks' windows only
+        const bool odd = q0 + s.off < k0 + 31 + a.window && __any(scan<2 * TILE, 64>(Qb, lane));
+        bf16x8 pb[KS], sb[KS];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            pb[ks] = frag_acc(sc[0][ks], sc[1][ks]);
+            sb[ks] = frag_acc(dp[0][ks], dp[1][ks]);
+        }
+        if (odd) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                add_pairs<HD>(dvt[ks], Ob, pb[ks], wl[wave], lane, [&](int x) { return far(x, ks); });
+                wave_lds();
+                add_pairs<HD>(dkt[ks], Qb, sb[ks], wl[wave], lane, [&](int x) { return far(x, ks); });
+                wave_lds();
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < DSUB; ++i) {
+                const bf16x8 fo = R::frag_t(Ob, 16 * i, 0, g, c16), fq = R::frag_t(Qb, 16 * i, 0, g, c16);
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    dvt[ks][i] = mfma16x16x32(fo, pb[ks], dvt[ks][i]);
+                    dkt[ks][i] = mfma16x16x32(fq, sb[ks], dkt[ks][i]);
+                }
+            }
+        }
+        if (it + 2 * step < n) {
+            wave_lds();  // this buffer's reads are done
+            dma(it + 2 * step, buf);
+        }
+    }
+    // the four waves' sums, each [dK, dV][32][HD] floats over its own tiles
+    wave_lds();
+    static_assert(64 * HD * 4 <= (int)sizeof(tiles[0]), "a wave's sums fit its tiles");
+    float *mine = reinterpret_cast<float *>(tiles[wave]);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < DSUB; ++i) {
+            *reinterpret_cast<f32x4 *>(mine + (16 * ks + c16) * HD + 16 * i + 4 * g) = dkt[ks][i] * a.scale;
+            *reinterpret_cast<f32x4 *>(mine + (32 + 16 * ks + c16) * HD + 16 * i + 4 * g) = dvt[ks][i];
+        }
+    __syncthreads();
+    float *ws = a.ws + (long)nbk * plan.slots() * (2 * 128 * HD) + (((long)bk * plan.far_slices + slice) * plan.far_parts + part) * (64 * HD);
+#pragma unroll
+    for (int i = 0; i < 64 * HD / 1024; ++i) {
+        const int x = (i * 256 + tid) * 4;
+        f32x4 t{0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) t += *reinterpret_cast<const f32x4 *>(reinterpret_cast<const float *>(tiles[w]) + x);
+        if (x / HD % 32 >= nk) t = f32x4{0, 0, 0, 0};
+        *reinterpret_cast<f32x4 *>(ws + x) = t;
+    }
 }
 
 // Heads of 64 or 128 values in rows of aligned 16-byte chunks, a tile's rows within 31 bits of
@@ -894,7 +1058,7 @@ bool few_rows(const WindowArgs &a) { return a.n_q <= kFewRows; }
 // two rounds of one block per CU
 int splits16(const WindowArgs &a) { return step_splits(a, 32, 512); }
 // dK/dV: one block per CU, at least four steps of both groups each
-DkvPlan plan16(const WindowArgs &a, bool ws) { return dkv_plan(a, ws, 128, 256, 8, 8); }
+DkvPlan plan16(const WindowArgs &a, bool ws) { return dkv_plan(a, ws, 128, 256, 8, 8, true); }
 
 }  // namespace
 
@@ -940,19 +1104,25 @@ bool window16_forward(const WindowArgs &a, hipStream_t st) {
 bool window16_backward(const WindowArgs &a, hipStream_t st) {
     if (!bwd_ok(a)) return false;
     const long per = (long)a.n_heads * a.n_batch, nbk = (long)a.n_batch * a.n_kv_heads;
-    // 256-row dQ blocks where they fill the chip, else 128, else 64 (as the dense backward)
-    const int bq = per * ((a.n_q + 255) / 256) >= 256 ? 256 : per * ((a.n_q + 127) / 128) >= 256 ? 128 : 64;
+    // 128-row dQ blocks on 4 waves, two a CU (256 rows on 8 waves, one a CU, wait for each other over
+    // twice the span of masked tiles: 16384 tokens, window 2048, 996 against 881 us; 4 x 2048, window
+    // 512, 112 against 90); 64 rows where those leave CUs idle
+    const int bq = per * ((a.n_q + 127) / 128) >= 256 ? 128 : 64;
     const DkvPlan plan = plan16(a, a.ws != nullptr);
     auto by = [&](auto hd, auto to) {
         constexpr int HD = decltype(hd)::value;
         using TO = decltype(to);
-        auto dq = [&](auto kernel, int nt) {
-            hipLaunchKernelGGL(kernel, dim3((unsigned)(per * ((a.n_q + bq - 1) / bq))), dim3(nt), 0, st, a);
+        auto dq = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)(per * ((a.n_q + bq - 1) / bq))), dim3(256), 0, st, a);
         };
-        if (bq == 256) dq(window_dq16_k<HD, 8, 256, TO>, 512);
-        else if (bq == 128) dq(window_dq16_k<HD, 8, 128, TO>, 512);
-        else dq(window_dq16_k<HD, 4, 64, TO>, 256);
-        hipLaunchKernelGGL((window_dkv16_k<HD, TO>), dim3((unsigned)(nbk * plan.blocks())), dim3(512), 0, st, a, plan);
+        if (bq == 128) dq(window_dq16_k<HD, 128, TO>);
+        else dq(window_dq16_k<HD, 64, TO>);
+        WindowArgs near = a;
+        if (plan.far_parts) {
+            near.n_sink = 0;
+            hipLaunchKernelGGL((window_far16_k<HD>), dim3((unsigned)(nbk * plan.far_slices * plan.far_parts)), dim3(256), 0, st, a, plan);
+        }
+        hipLaunchKernelGGL((window_dkv16_k<HD, TO>), dim3((unsigned)(nbk * plan.blocks())), dim3(512), 0, st, near, plan);
         launch_dkv_sum<HD, 128, TO>(a, plan, st);
     };
     auto by_head = [&](auto to) {

@@ -51,6 +51,35 @@ VKH_DEV f32x4 head_dot(const float *row, const float4 (&f)[NU]) {
     return a[0];
 }
 
+// acc += T^T w over 16 rows of an LDS tile: element e of w is row 4 g + e (row0 points at the lane's row
+// 4 g).  Matrix row i of acc[4 J + j] is column 64 J + 4 i + j of the tile, so that one 16-byte read
+// feeds four products (a 4-byte read for each left them waiting on LDS: see acc_cols for the way back).
+template <int NU>
+VKH_DEV void add_rows(f32x4 (&acc)[NU], const float *row0, int P, int c, const f32x4 &w) {
+#pragma unroll
+    for (int J = 0; J < NU / 4; ++J) {
+        float4 t[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = f4(row0 + e * P + 64 * J + 4 * c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            acc[4 * J] = mfma16x16x4(t[e].x, w[e], acc[4 * J]);
+            acc[4 * J + 1] = mfma16x16x4(t[e].y, w[e], acc[4 * J + 1]);
+            acc[4 * J + 2] = mfma16x16x4(t[e].z, w[e], acc[4 * J + 2]);
+            acc[4 * J + 3] = mfma16x16x4(t[e].w, w[e], acc[4 * J + 3]);
+        }
+    }
+}
+// Four columns of the lane's item: f(first column, their values) for columns 64 J + 16 g + 4 r.
+template <int NU, class F>
+VKH_DEV void acc_cols(const f32x4 (&acc)[NU], int g, F f) {
+#pragma unroll
+    for (int J = 0; J < NU / 4; ++J)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            f(64 * J + 16 * g + 4 * r, f32x4{acc[4 * J][r], acc[4 * J + 1][r], acc[4 * J + 2][r], acc[4 * J + 3][r]});
+}
+
 // R rows of HD floats moved by NT threads, global -> registers -> LDS (pitch HD + 4).
 template <int HD, int R, int NT>
 struct Tile32 {
@@ -109,8 +138,8 @@ __global__ __launch_bounds__(FNT, 2) void window_fwd32_k(WindowArgs a) {
     constexpr int P = T::P, NU = HD / 16;
     __shared__ __attribute__((aligned(16))) float Ks[2][FT * P], Vs[2][FT * P];
     const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, nqt = (a.n_q + 63) / 64;
-    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
-    const int h = kvh * grp + blockIdx.x / nbk % grp, qt = nqt - 1 - (int)(blockIdx.x / nbk / grp);
+    const Pair pr = pair_of(blockIdx.x, gridDim.x, nbk, 4 * grp);
+    const int b = pr.bk / a.n_kv_heads, kvh = pr.bk % a.n_kv_heads, h = kvh * grp + pr.y % grp, qt = nqt - 1 - pr.y / grp;
     const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const Span s = span_of(a, b);
@@ -143,7 +172,7 @@ __global__ __launch_bounds__(FNT, 2) void window_fwd32_k(WindowArgs a) {
         store(0);
     }
     __syncthreads();
-    f32x4 ot[NU];  // O^T[16 j + 4 g + r][row]
+    f32x4 ot[NU];  // O^T, columns as acc_cols has them
 #pragma unroll
     for (int j = 0; j < NU; ++j) ot[j] = f32x4{0, 0, 0, 0};
     float m = -INFINITY, l = 0.f;  // running maximum; this lane's share of the sum
@@ -178,16 +207,10 @@ __global__ __launch_bounds__(FNT, 2) void window_fwd32_k(WindowArgs a) {
                 l += st[ks][e];
             }
         m = mn;
-        // O^T += V^T P^T: step (ks, e) is key k0 + 16 ks + 4 g + e
+        // O^T += V^T P^T
 #pragma unroll
-        for (int j = 0; j < NU; ++j)
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                if (!live[ks]) continue;
-                const float *vr = Vl + (16 * ks + 4 * g) * P + 16 * j + c;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) ot[j] = mfma16x16x4(vr[e * P], st[ks][e], ot[j]);
-            }
+        for (int ks = 0; ks < 2; ++ks)
+            if (live[ks]) add_rows<NU>(ot, Vl + (16 * ks + 4 * g) * P, P, c, st[ks]);
         if (it + 1 < kt.n) store(it + 1);  // its buffer was last read before the previous barrier
         __syncthreads();
     }
@@ -199,12 +222,11 @@ __global__ __launch_bounds__(FNT, 2) void window_fwd32_k(WindowArgs a) {
     if (r >= a.n_q) return;
     const bool dead = l == 0.f;
     const float inv = 1.0f / l;
-    float *o = (float *)a.o + row * a.ldo + h * HD + 4 * g;
-#pragma unroll
-    for (int j = 0; j < NU; ++j) {
-        const f32x4 x = dead ? f32x4{0, 0, 0, 0} : ot[j] * inv;
-        store4(o + 16 * j, x[0], x[1], x[2], x[3]);
-    }
+    float *o = (float *)a.o + row * a.ldo + h * HD;
+    acc_cols<NU>(ot, g, [&](int d, f32x4 x) {
+        x = dead ? f32x4{0, 0, 0, 0} : x * inv;
+        store4(o + d, x[0], x[1], x[2], x[3]);
+    });
     if (a.lse && g == 0) a.lse[row * a.n_heads + h] = dead ? -INFINITY : m + logf(l);
 }
 
@@ -218,8 +240,8 @@ __global__ __launch_bounds__(FNT, 2) void window_step32_k(WindowArgs a, int spli
     __shared__ __attribute__((aligned(16))) float tiles[4][2][BN * P];
     __shared__ float ml[4][2][16];
     const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, M = a.n_q * grp, RT = (M + 15) / 16;
-    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
-    const int rt = blockIdx.x / nbk % RT, split = blockIdx.x / nbk / RT;
+    const Pair pr = pair_of(blockIdx.x, gridDim.x, nbk, 4);
+    const int b = pr.bk / a.n_kv_heads, kvh = pr.bk % a.n_kv_heads, rt = pr.y % RT, split = pr.y / RT;
     const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const Span s = span_of(a, b);
@@ -284,20 +306,17 @@ __global__ __launch_bounds__(FNT, 2) void window_step32_k(WindowArgs a, int spli
 #pragma unroll
                     for (int j = 0; j < NU; ++j)
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) acc[j][x] = fmaf(Vl[(4 * g2 + e) * P + 16 * j + 4 * g + x], w, acc[j][x]);
+                        for (int x = 0; x < 4; ++x)
+                            acc[j][x] = fmaf(Vl[(4 * g2 + e) * P + 64 * (j / 4) + 16 * g + 4 * x + j % 4], w, acc[j][x]);
                 }
             continue;
         }
-#pragma unroll
-        for (int j = 0; j < NU; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[j] = mfma16x16x4(Vl[(4 * g + e) * P + 16 * j + c], st[e], acc[j]);
+        add_rows<NU>(acc, Vl + 4 * g * P, P, c, st);
     }
     wave_lds();
     float *res = tiles[wave][0];  // rows of P floats
     const float lt = xsum(l);
-#pragma unroll
-    for (int j = 0; j < NU; ++j) *reinterpret_cast<f32x4 *>(res + c * P + 16 * j + 4 * g) = acc[j];
+    acc_cols<NU>(acc, g, [&](int d, f32x4 x) { *reinterpret_cast<f32x4 *>(res + c * P + d) = x; });
     if (g == 0) ml[wave][0][c] = m, ml[wave][1][c] = lt;
     __syncthreads();
     constexpr int E = HD / 16;
@@ -345,8 +364,8 @@ __global__ __launch_bounds__(FNT, 2) void window_dq32_k(WindowArgs a) {
     constexpr int P = T::P, NU = HD / 16;
     __shared__ __attribute__((aligned(16))) float Ks[2][FT * P], Vs[2][FT * P];
     const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, nqt = (a.n_q + 63) / 64;
-    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
-    const int h = kvh * grp + blockIdx.x / nbk % grp, qt = nqt - 1 - (int)(blockIdx.x / nbk / grp);
+    const Pair pr = pair_of(blockIdx.x, gridDim.x, nbk, 4 * grp);
+    const int b = pr.bk / a.n_kv_heads, kvh = pr.bk % a.n_kv_heads, h = kvh * grp + pr.y % grp, qt = nqt - 1 - pr.y / grp;
     const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const Span s = span_of(a, b);
@@ -416,14 +435,8 @@ __global__ __launch_bounds__(FNT, 2) void window_dq32_k(WindowArgs a) {
             }
         }
 #pragma unroll
-        for (int j = 0; j < NU; ++j)
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                if (!live[ks]) continue;
-                const float *kr = Kl + (16 * ks + 4 * g) * P + 16 * j + c;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) dqt[j] = mfma16x16x4(kr[e * P], da[ks][e], dqt[j]);
-            }
+        for (int ks = 0; ks < 2; ++ks)
+            if (live[ks]) add_rows<NU>(dqt, Kl + (16 * ks + 4 * g) * P, P, c, da[ks]);
         if (it + 1 < kt.n) store(it + 1);
         __syncthreads();
     }
@@ -433,12 +446,11 @@ __global__ __launch_bounds__(FNT, 2) void window_dq32_k(WindowArgs a) {
         return;
     }
     if (r >= a.n_q) return;
-    float *dq = (float *)a.dq + row * a.lddq + h * HD + 4 * g;
-#pragma unroll
-    for (int j = 0; j < NU; ++j) {
-        const f32x4 x = pos >= 0 ? dqt[j] * a.scale : f32x4{0, 0, 0, 0};
-        store4(dq + 16 * j, x[0], x[1], x[2], x[3]);
-    }
+    float *dq = (float *)a.dq + row * a.lddq + h * HD;
+    acc_cols<NU>(dqt, g, [&](int d, f32x4 x) {
+        x = pos >= 0 ? x * a.scale : f32x4{0, 0, 0, 0};
+        store4(dq + d, x[0], x[1], x[2], x[3]);
+    });
 }
 
 // ── backward: dK and dV, block = 64 keys of one KV head ──────────────────
@@ -450,9 +462,10 @@ __global__ __launch_bounds__(FNT, 2) void window_dkv32_k(WindowArgs a, DkvPlan p
     __shared__ __attribute__((aligned(16))) float Qs[2][FT * P], Os[2][FT * P];
     __shared__ float Ls[2][FT], Dl[2][FT];
     const int nbk = a.n_batch * a.n_kv_heads;
-    const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
+    const Pair pr = pair_of(blockIdx.x, gridDim.x, nbk, 4);
+    const int bk = pr.bk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
     int kb, zpart, zparts, slot;
-    dkv_block(plan, blockIdx.x / nbk, kb, zpart, zparts, slot);
+    dkv_block(plan, pr.y, kb, zpart, zparts, slot);
     const int nh = a.n_heads / a.n_kv_heads;
     const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
@@ -537,23 +550,17 @@ __global__ __launch_bounds__(FNT, 2) void window_dkv32_k(WindowArgs a, DkvPlan p
                 da[qs][e] = on ? p * (da[qs][e] - Dl[buf][x]) : 0.f;
             }
         }
-        // dV^T += dO^T P, dK^T += Q^T dS: step (qs, e) is query q0 + 16 qs + 4 g + e
+        // dV^T += dO^T P, dK^T += Q^T dS
 #pragma unroll
-        for (int j = 0; j < NU; ++j)
-#pragma unroll
-            for (int qs = 0; qs < 2; ++qs) {
-                if (!live[qs]) continue;
-                const float *orow = Ol + (16 * qs + 4 * g) * P + 16 * j + c, *qrow = Ql + (16 * qs + 4 * g) * P + 16 * j + c;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    dvt[j] = mfma16x16x4(orow[e * P], sa[qs][e], dvt[j]);
-                    dkt[j] = mfma16x16x4(qrow[e * P], da[qs][e], dkt[j]);
-                }
-            }
+        for (int qs = 0; qs < 2; ++qs) {
+            if (!live[qs]) continue;
+            add_rows<NU>(dvt, Ol + (16 * qs + 4 * g) * P, P, c, sa[qs]);
+            add_rows<NU>(dkt, Ql + (16 * qs + 4 * g) * P, P, c, da[qs]);
+        }
         if (it + 1 < niter) store(it + 1);
         __syncthreads();
     }
-    float *ws = zparts > 1 ? a.ws + ((long)bk * plan.slots() + slot) * (2 * BN * HD) : nullptr;
+    float *ws = slot >= 0 ? a.ws + ((long)bk * plan.slots() + slot) * (2 * BN * HD) : nullptr;
     if (__syncthreads_or(odd)) {
         float *sh = Qs[0] + wave * 2 * HD;
         const Steps st{kvh * nh, qstart, top, nh, false, 1, zpart, zparts};
@@ -564,12 +571,14 @@ __global__ __launch_bounds__(FNT, 2) void window_dkv32_k(WindowArgs a, DkvPlan p
     float *dk = ws ? ws + (16 * wave + c) * HD : (float *)a.dk + krow * a.lddk + kvh * HD;
     float *dv = ws ? ws + (BN + 16 * wave + c) * HD : (float *)a.dv + krow * a.lddv + kvh * HD;
     const bool live = key < s.kl;
-#pragma unroll
-    for (int j = 0; j < NU; ++j) {
-        const f32x4 x = live ? dkt[j] * a.scale : f32x4{0, 0, 0, 0}, y = live ? dvt[j] : f32x4{0, 0, 0, 0};
-        store4(dk + 16 * j + 4 * g, x[0], x[1], x[2], x[3]);
-        store4(dv + 16 * j + 4 * g, y[0], y[1], y[2], y[3]);
-    }
+    acc_cols<NU>(dkt, g, [&](int d, f32x4 x) {
+        x = live ? x * a.scale : f32x4{0, 0, 0, 0};
+        store4(dk + d, x[0], x[1], x[2], x[3]);
+    });
+    acc_cols<NU>(dvt, g, [&](int d, f32x4 x) {
+        x = live ? x : f32x4{0, 0, 0, 0};
+        store4(dv + d, x[0], x[1], x[2], x[3]);
+    });
 }
 
 bool shape_ok(const WindowArgs &a) { return a.dt == DType::F32 && (a.hd == 64 || a.hd == 128) && a.scale > 0.f && a.scale < INFINITY; }
@@ -577,7 +586,7 @@ bool ok(const void *p, long ld) { return aligned_rows(p, ld, 16, 4); }
 bool fwd_ok(const WindowArgs &a) { return shape_ok(a) && ok(a.q, a.ldq) && ok(a.k, a.ldk) && ok(a.v, a.ldv) && ok(a.o, a.ldo); }
 bool few_rows(const WindowArgs &a) { return a.n_q <= kFewRows; }
 int splits32(const WindowArgs &a) { return step_splits(a, 16, 1024); }
-DkvPlan plan32(const WindowArgs &a, bool ws) { return dkv_plan(a, ws, 64, 512, 16, 2); }
+DkvPlan plan32(const WindowArgs &a, bool ws) { return dkv_plan(a, ws, 64, 512, 16, 2, false); }
 
 }  // namespace
 

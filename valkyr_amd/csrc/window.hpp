@@ -1,6 +1,8 @@
 // What the windowed attention's kernel files share.
 #pragma once
 
+#include <math.h>
+
 #include <algorithm>
 
 #include "ops.hpp"
@@ -22,6 +24,18 @@ VKH_DEV Span span_of(const WindowArgs &a, int b) {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr int kAll = 0x7fffffff;  // the window of a sink
+
+// The (sequence, KV head) of block x, and its turn y among that pair's blocks.  Blocks go round the
+// 8 XCDs by their number; runs of up to `run` turns of one pair sit on one XCD and share its L2, and
+// from run to run the pairs move on, so that pairs with little to do (short sequences of a padded
+// batch) do not leave the XCD that would be theirs idle.
+struct Pair {
+    int bk, y;
+};
+VKH_DEV Pair pair_of(int x, int blocks, int pairs, int run) {
+    const int y = x / pairs, r = max(1, min(run, blocks / pairs / pairs));
+    return Pair{(x % pairs + y / r) % pairs, y};
+}
 
 // Whether position t sees key j (t = -1: a row that sees none).
 VKH_DEV bool sees(const WindowArgs &a, int t, int j) {
@@ -228,18 +242,25 @@ struct DkvPlan {
     int key_blocks, sink_blocks;   // per KV head, of `keys` keys; the first sink_blocks hold sinks
     int sink_parts, parts;         // launched blocks per sink block, per other block
     int keys;
+    // pairs of a sink and a row past its window: blocks of their own (0: the key blocks take them) per
+    // slice of 32 sinks, so that no key block has more steps than the others
+    int far_parts, far_slices;
     __host__ __device__ int blocks() const { return sink_blocks * sink_parts + (key_blocks - sink_blocks) * parts; }
-    // slots of partial sums per KV head: a split block's parts
-    __host__ __device__ int slots() const { return (sink_parts > 1 ? sink_blocks * sink_parts : 0) + (parts > 1 ? (key_blocks - sink_blocks) * parts : 0); }
+    // slots of partial sums per KV head: those of the sink blocks, those of the others
+    __host__ __device__ int sink_slots() const { return sink_parts > 1 || far_parts ? sink_blocks * sink_parts : 0; }
+    __host__ __device__ int slots() const { return sink_slots() + (parts > 1 ? (key_blocks - sink_blocks) * parts : 0); }
+    // key blocks whose sums window_dkv_sum_k writes
+    __host__ __device__ int summed() const { return (sink_slots() ? sink_blocks : 0) + (parts > 1 ? key_blocks - sink_blocks : 0); }
 };
+// Key block kb, part z of `parts` and slot (-1: the block writes its results itself) of turn y.
 VKH_DEV void dkv_block(const DkvPlan &p, int y, int &kb, int &z, int &parts, int &slot) {
     const int s = p.sink_blocks * p.sink_parts;
     if (y < s) {
         kb = y / p.sink_parts; z = y % p.sink_parts; parts = p.sink_parts;
-        slot = y;
+        slot = p.sink_slots() ? y : -1;
     } else {
         kb = p.sink_blocks + (y - s) / p.parts; z = (y - s) % p.parts; parts = p.parts;
-        slot = (p.sink_parts > 1 ? s : 0) + y - s;
+        slot = parts > 1 ? p.sink_slots() + y - s : -1;
     }
 }
 
@@ -254,21 +275,29 @@ struct Steps {
         return ((alt ? t / per : t) * nh + (alt ? h - head0 : (h - head0) / per)) % zparts == zpart;
     }
 };
-// dK and dV of the split key blocks: their parts added in order, four values a thread.
+// dK and dV of the split key blocks: their parts and then those of the far pairs ([pair][slice][part] of
+// [dK, dV][32][HD] behind the key blocks' slots) added in order, four values a thread.
 template <int HD, int BN, class TO>
 __global__ __launch_bounds__(256) void window_dkv_sum_k(WindowArgs a, DkvPlan plan) {
     const int nbk = a.n_batch * a.n_kv_heads;
     const int bk = blockIdx.x % nbk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
-    const int kb = blockIdx.x / nbk + (plan.sink_parts > 1 ? 0 : plan.sink_blocks);
+    const int kb = blockIdx.x / nbk + (plan.sink_slots() ? 0 : plan.sink_blocks);
     const bool sink = kb < plan.sink_blocks;
     const int parts = sink ? plan.sink_parts : plan.parts;
-    const int first = sink ? kb * parts : (plan.sink_parts > 1 ? plan.sink_blocks * plan.sink_parts : 0) + (kb - plan.sink_blocks) * parts;
+    const int first = sink ? kb * parts : plan.sink_slots() + (kb - plan.sink_blocks) * parts;
     const float *ws = a.ws + ((long)bk * plan.slots() + first) * (2 * BN * HD);
     const int x = (blockIdx.y * 256 + threadIdx.x) * 4;  // of dK [BN][HD], then dV
-    f32x4 t{0, 0, 0, 0};
-    for (int p = 0; p < parts; ++p) t += *reinterpret_cast<const f32x4 *>(ws + (long)p * 2 * BN * HD + x);
     const bool v = x >= BN * HD;
     const int y = v ? x - BN * HD : x, key = kb * BN + y / HD;
+    f32x4 t{0, 0, 0, 0};
+#pragma unroll 8
+    for (int p = 0; p < parts; ++p) t += *reinterpret_cast<const f32x4 *>(ws + (long)p * 2 * BN * HD + x);
+    if (key / 32 < plan.far_slices) {
+        const float *far = a.ws + (long)nbk * plan.slots() * (2 * BN * HD) +
+                           ((long)bk * plan.far_slices + key / 32) * plan.far_parts * (64 * HD) + (v ? 32 * HD : 0) + y % (32 * HD);
+#pragma unroll 8
+        for (int p = 0; p < plan.far_parts; ++p) t += *reinterpret_cast<const f32x4 *>(far + (long)p * 64 * HD);
+    }
     if (key >= a.n_kv) return;
     const long row = (long)b * a.n_kv + key;
     TO *out = v ? (TO *)a.dv + row * a.lddv : (TO *)a.dk + row * a.lddk;
@@ -329,33 +358,43 @@ __global__ __launch_bounds__(256) void window_join_k(WindowArgs a, int splits) {
 }
 
 // ── host ─────────────────────────────────────────────────────────────────
-// keys: per key block; cu_blocks: that fill the chip; least: steps that a part keeps.  At most 256
-// MiB of partial sums.
-inline DkvPlan dkv_plan(const WindowArgs &a, bool ws, int keys, long cu_blocks, long most_parts, long least) {
+// keys: per key block; cu_blocks: that fill the chip; least: steps that a part keeps; far: whether the
+// far pairs of up to 128 sinks may have blocks of their own.  At most about 256 MiB of partial sums.
+inline DkvPlan dkv_plan(const WindowArgs &a, bool ws, int keys, long cu_blocks, long most_parts, long least, bool far) {
     DkvPlan p;
     p.keys = keys;
     p.key_blocks = (a.n_kv + keys - 1) / keys;
     p.sink_blocks = a.window < a.n_kv ? std::min(p.key_blocks, (a.n_sink + keys - 1) / keys) : 0;
     p.sink_parts = p.parts = 1;
+    p.far_parts = p.far_slices = 0;
     if (!ws) return p;
     const long nbk = (long)a.n_batch * a.n_kv_heads, blocks = nbk * p.key_blocks, hpk = a.n_heads / a.n_kv_heads;
     const long most = hpk * ((a.n_q + 31) / 32), usual = std::min(most, hpk * ((std::min<long>(a.n_kv, a.window) + keys + 31) / 32));
-    p.parts = (int)std::max(1l, std::min({most_parts, cu_blocks / blocks, usual / least}));
-    // a sink block's steps over the usual block's
-    p.sink_parts = (int)std::max<long>(p.parts, std::min<long>(64, (most * p.parts + usual - 1) / usual));
     const long slot = 2l * keys * a.hd * 4;
-    while (p.sink_parts > 1 && p.sink_blocks * nbk * slot * p.sink_parts > (192l << 20)) --p.sink_parts;
+    p.parts = (int)std::max(1l, std::min({most_parts, cu_blocks / blocks, usual / least}));
     while (p.parts > 1 && blocks * slot * p.parts > (64l << 20)) --p.parts;
+    if (far && p.sink_blocks && a.n_sink <= 128) {
+        p.sink_parts = p.parts;
+        p.far_slices = (a.n_sink + 31) / 32;
+        // four waves a CU in all, while each keeps three steps
+        p.far_parts = (int)std::max(1l, std::min(256 / (nbk * p.far_slices), most / 12));
+        return p;
+    }
+    // A sink block's steps over the usual block's; the sink blocks start first, so a part may take as
+    // long as the rounds of the others.
+    const double rounds = std::max(1.0, (double)blocks * p.parts / cu_blocks);
+    p.sink_parts = (int)std::max(1.0, std::min(64.0, ceil((double)most / usual * p.parts / rounds)));
+    while (p.sink_parts > 1 && p.sink_blocks * nbk * slot * p.sink_parts > (192l << 20)) --p.sink_parts;
     return p;
 }
 inline size_t dkv_ws_bytes(const WindowArgs &a, const DkvPlan &p) {
-    return (size_t)a.n_batch * a.n_kv_heads * p.slots() * 2 * p.keys * a.hd * sizeof(float);
+    const size_t nbk = (size_t)a.n_batch * a.n_kv_heads;
+    return nbk * ((size_t)p.slots() * p.keys + (size_t)p.far_slices * p.far_parts * 32) * 2 * a.hd * sizeof(float);
 }
 template <int HD, int BN, class TO>
 void launch_dkv_sum(const WindowArgs &a, const DkvPlan &p, hipStream_t st) {
-    const int split = (p.sink_parts > 1 ? p.sink_blocks : 0) + (p.parts > 1 ? p.key_blocks - p.sink_blocks : 0);
-    if (split)
-        hipLaunchKernelGGL((window_dkv_sum_k<HD, BN, TO>), dim3((unsigned)((long)a.n_batch * a.n_kv_heads * split), BN * HD / 512),
+    if (p.summed())
+        hipLaunchKernelGGL((window_dkv_sum_k<HD, BN, TO>), dim3((unsigned)((long)a.n_batch * a.n_kv_heads * p.summed()), BN * HD / 512),
                            dim3(256), 0, st, a, p);
 }
 
