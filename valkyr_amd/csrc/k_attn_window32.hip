@@ -132,26 +132,25 @@ __device__ __attribute__((noinline)) void dkv_rows32(const WindowArgs &a, const 
 }
 
 // ── forward: block = 64 query rows of one head ───────────────────────────
-template <int HD>
-__global__ __launch_bounds__(FNT, 2) void window_fwd32_k(WindowArgs a) {
-    using T = Tile32<HD, FT, FNT>;
+// KG groups of four waves take every KG-th key tile each (from LDS of their own) and join their results
+// at the end: short sequences leave a CU one block, whose steps then wait for themselves (1001
+// tokens, window 256, 16 / 4 heads of 64: 256 blocks, 33 us with one group).
+template <int HD, int KG>
+__global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_fwd32_k(WindowArgs a) {
+    using T = Tile32<HD, FT, 256>;
     constexpr int P = T::P, NU = HD / 16;
-    __shared__ __attribute__((aligned(16))) float Ks[2][FT * P], Vs[2][FT * P];
+    __shared__ __attribute__((aligned(16))) float tiles[KG][2][2][FT * P];  // [group][K, V][buffer]
     const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, nqt = (a.n_q + 63) / 64;
     const Pair pr = pair_of(blockIdx.x, gridDim.x, nbk, 4 * grp);
     const int b = pr.bk / a.n_kv_heads, kvh = pr.bk % a.n_kv_heads, h = kvh * grp + pr.y % grp, qt = nqt - 1 - pr.y / grp;
-    const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
-    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int tid = threadIdx.x % 256, lane = tid % 64, g = lane / 16, c = lane % 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) % 4, kg = __builtin_amdgcn_readfirstlane(threadIdx.x / 256);
     const Span s = span_of(a, b);
     const int r0 = qt * 64, qw = r0 + 16 * wave, r = qw + c;
     const KeyTiles kt = key_tiles<FT>(a, s, r0, r0 + 64);
     const int wta = max(0, qw + s.off), wtb = min(qw + 16, s.ql) - 1 + s.off;
     const int pos = r < s.ql ? max(-1, r + s.off) : -1;
     const long row = (long)b * a.n_q + r;
-    float4 qf[NU];
-#pragma unroll
-    for (int u = 0; u < NU; ++u)
-        qf[u] = pos >= 0 ? f4((const float *)a.q + row * a.ldq + h * HD + 4 * g + 16 * u) : make_float4(0.f, 0.f, 0.f, 0.f);
     const float *kb = (const float *)a.k + (long)b * a.n_kv * a.ldk + kvh * HD;
     const float *vb = (const float *)a.v + (long)b * a.n_kv * a.ldv + kvh * HD;
     T tk, tv;
@@ -161,25 +160,26 @@ __global__ __launch_bounds__(FNT, 2) void window_fwd32_k(WindowArgs a) {
         tv.load(vb + (long)k0 * a.ldv, a.ldv, tid, s.kl - k0);
     };
     bool odd = false;  // in V of a tile that is not seen in full
-    auto store = [&](int it) {
+    auto store = [&](int it, int buf) {
         const int k0 = kt.tile(it) * FT;
         if (!all_seen(a, kt.ta, kt.tb, k0, k0 + FT - 1)) odd |= tv.odd();
-        tk.store(Ks[it & 1], tid);
-        tv.store(Vs[it & 1], tid);
+        tk.store(tiles[kg][0][buf], tid);
+        tv.store(tiles[kg][1][buf], tid);
     };
-    if (kt.n > 0) {
-        load(0);
-        store(0);
-    }
+    if (kg < kt.n) load(kg);
+    float4 qf[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+        qf[u] = pos >= 0 ? f4((const float *)a.q + row * a.ldq + h * HD + 4 * g + 16 * u) : make_float4(0.f, 0.f, 0.f, 0.f);
+    if (kg < kt.n) store(kg, 0);
     __syncthreads();
     f32x4 ot[NU];  // O^T, columns as acc_cols has them
 #pragma unroll
     for (int j = 0; j < NU; ++j) ot[j] = f32x4{0, 0, 0, 0};
     float m = -INFINITY, l = 0.f;  // running maximum; this lane's share of the sum
-    for (int it = 0; it < kt.n; ++it) {
-        if (it + 1 < kt.n) load(it + 1);
+    auto step = [&](int it, int buf) {
         const int k0 = kt.tile(it) * FT;
-        const float *Kl = Ks[it & 1], *Vl = Vs[it & 1];
+        const float *Kl = tiles[kg][0][buf], *Vl = tiles[kg][1][buf];
         f32x4 st[2];
         bool live[2];
         float tmax = -INFINITY;
@@ -211,14 +211,39 @@ __global__ __launch_bounds__(FNT, 2) void window_fwd32_k(WindowArgs a) {
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
             if (live[ks]) add_rows<NU>(ot, Vl + (16 * ks + 4 * g) * P, P, c, st[ks]);
-        if (it + 1 < kt.n) store(it + 1);  // its buffer was last read before the previous barrier
+    };
+    for (int it = kg, buf = 0; it - kg < kt.n; it += KG, buf ^= 1) {
+        if (it + KG < kt.n) load(it + KG);
+        if (it < kt.n) step(it, buf);
+        if (it + KG < kt.n) store(it + KG, buf ^ 1);  // last read before the previous barrier
         __syncthreads();
     }
     if (__syncthreads_or(odd)) {
-        fwd_rows32(args_again(), b, r0 + wave, min(r0 + 64, a.n_q), h, Ks[0] + wave * HD, lane);
+        if (kg == 0) fwd_rows32(args_again(), b, r0 + wave, min(r0 + 64, a.n_q), h, tiles[0][0][0] + wave * HD, lane);
         return;
     }
     l = xsum(l);
+    if constexpr (KG > 1) {  // the groups' results, joined in order through LDS
+        constexpr int W = (NU + 1) * 4 * 64;  // floats of a wave's result: columns of 64 lanes
+        static_assert(4 * W <= 4 * FT * P, "a group's results fit its tiles");
+        auto column = [&](int k, int j) { return reinterpret_cast<f32x4 *>(tiles[k][0][0] + wave * W + j * 256) + lane; };
+        if (kg) {
+#pragma unroll
+            for (int j = 0; j < NU; ++j) *column(kg, j) = ot[j];
+            *column(kg, NU) = f32x4{m, l, 0, 0};
+        }
+        __syncthreads();
+        if (kg) return;
+#pragma unroll
+        for (int k = 1; k < KG; ++k) {
+            const f32x4 st = *column(k, NU);
+            const float mn = fmaxf(m, st[0]), ms = mn == -INFINITY ? 0.f : mn, f0 = expf(m - ms), f1 = expf(st[0] - ms);
+            m = mn;
+            l = l * f0 + st[1] * f1;
+#pragma unroll
+            for (int j = 0; j < NU; ++j) ot[j] = ot[j] * f0 + *column(k, j) * f1;
+        }
+    }
     if (r >= a.n_q) return;
     const bool dead = l == 0.f;
     const float inv = 1.0f / l;
@@ -358,16 +383,17 @@ __global__ __launch_bounds__(FNT, 2) void window_step32_k(WindowArgs a, int spli
 }
 
 // ── backward: D and dQ, block = 64 query rows of one head ────────────────
-template <int HD>
-__global__ __launch_bounds__(FNT, 2) void window_dq32_k(WindowArgs a) {
-    using T = Tile32<HD, FT, FNT>;
+// Key groups as in the forward.
+template <int HD, int KG>
+__global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_dq32_k(WindowArgs a) {
+    using T = Tile32<HD, FT, 256>;
     constexpr int P = T::P, NU = HD / 16;
-    __shared__ __attribute__((aligned(16))) float Ks[2][FT * P], Vs[2][FT * P];
+    __shared__ __attribute__((aligned(16))) float tiles[KG][2][2][FT * P];  // [group][K, V][buffer]
     const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, nqt = (a.n_q + 63) / 64;
     const Pair pr = pair_of(blockIdx.x, gridDim.x, nbk, 4 * grp);
     const int b = pr.bk / a.n_kv_heads, kvh = pr.bk % a.n_kv_heads, h = kvh * grp + pr.y % grp, qt = nqt - 1 - pr.y / grp;
-    const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
-    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int tid = threadIdx.x % 256, lane = tid % 64, g = lane / 16, c = lane % 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) % 4, kg = __builtin_amdgcn_readfirstlane(threadIdx.x / 256);
     const Span s = span_of(a, b);
     const int r0 = qt * 64, qw = r0 + 16 * wave, r = qw + c;
     const KeyTiles kt = key_tiles<FT>(a, s, r0, r0 + 64);
@@ -375,6 +401,22 @@ __global__ __launch_bounds__(FNT, 2) void window_dq32_k(WindowArgs a) {
     const long row = (long)b * a.n_q + r;
     const float lse = r < s.ql && r + s.off >= 0 ? a.lse[row * a.n_heads + h] : -INFINITY;
     const int pos = lse == -INFINITY ? -1 : r + s.off;
+    const float *kb = (const float *)a.k + (long)b * a.n_kv * a.ldk + kvh * HD;
+    const float *vb = (const float *)a.v + (long)b * a.n_kv * a.ldv + kvh * HD;
+    T tk, tv;
+    auto load = [&](int it) {
+        const int k0 = kt.tile(it) * FT;
+        tk.load(kb + (long)k0 * a.ldk, a.ldk, tid, s.kl - k0);
+        tv.load(vb + (long)k0 * a.ldv, a.ldv, tid, s.kl - k0);
+    };
+    bool odd = false;  // in K of a tile that is not seen in full
+    auto store = [&](int it, int buf) {
+        const int k0 = kt.tile(it) * FT;
+        if (!all_seen(a, kt.ta, kt.tb, k0, k0 + FT - 1)) odd |= tk.odd();
+        tk.store(tiles[kg][0][buf], tid);
+        tv.store(tiles[kg][1][buf], tid);
+    };
+    if (kg < kt.n) load(kg);
     float4 qf[NU], of[NU];
     double acc = 0;
 #pragma unroll
@@ -391,34 +433,15 @@ __global__ __launch_bounds__(FNT, 2) void window_dq32_k(WindowArgs a) {
     acc += __shfl_xor(acc, 16, 64);
     acc += __shfl_xor(acc, 32, 64);
     const float dd = (float)acc;
-    if (r < a.n_q && g == 0) a.d[row * a.n_heads + h] = dd;
-    const float *kb = (const float *)a.k + (long)b * a.n_kv * a.ldk + kvh * HD;
-    const float *vb = (const float *)a.v + (long)b * a.n_kv * a.ldv + kvh * HD;
-    T tk, tv;
-    auto load = [&](int it) {
-        const int k0 = kt.tile(it) * FT;
-        tk.load(kb + (long)k0 * a.ldk, a.ldk, tid, s.kl - k0);
-        tv.load(vb + (long)k0 * a.ldv, a.ldv, tid, s.kl - k0);
-    };
-    bool odd = false;  // in K of a tile that is not seen in full
-    auto store = [&](int it) {
-        const int k0 = kt.tile(it) * FT;
-        if (!all_seen(a, kt.ta, kt.tb, k0, k0 + FT - 1)) odd |= tk.odd();
-        tk.store(Ks[it & 1], tid);
-        tv.store(Vs[it & 1], tid);
-    };
-    if (kt.n > 0) {
-        load(0);
-        store(0);
-    }
+    if (kg == 0 && r < a.n_q && g == 0) a.d[row * a.n_heads + h] = dd;
+    if (kg < kt.n) store(kg, 0);
     __syncthreads();
     f32x4 dqt[NU];
 #pragma unroll
     for (int j = 0; j < NU; ++j) dqt[j] = f32x4{0, 0, 0, 0};
-    for (int it = 0; it < kt.n; ++it) {
-        if (it + 1 < kt.n) load(it + 1);
+    auto step = [&](int it, int buf) {
         const int k0 = kt.tile(it) * FT;
-        const float *Kl = Ks[it & 1], *Vl = Vs[it & 1];
+        const float *Kl = tiles[kg][0][buf], *Vl = tiles[kg][1][buf];
         f32x4 da[2];
         bool live[2];
 #pragma unroll
@@ -437,13 +460,29 @@ __global__ __launch_bounds__(FNT, 2) void window_dq32_k(WindowArgs a) {
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
             if (live[ks]) add_rows<NU>(dqt, Kl + (16 * ks + 4 * g) * P, P, c, da[ks]);
-        if (it + 1 < kt.n) store(it + 1);
+    };
+    for (int it = kg, buf = 0; it - kg < kt.n; it += KG, buf ^= 1) {
+        if (it + KG < kt.n) load(it + KG);
+        if (it < kt.n) step(it, buf);
+        if (it + KG < kt.n) store(it + KG, buf ^ 1);
         __syncthreads();
     }
     if (__syncthreads_or(odd)) {
-        float *sh = Ks[0] + wave * 2 * HD;
-        dq_rows32(args_again(), b, r0 + wave, min(r0 + 64, a.n_q), h, sh, sh + HD, lane);
+        float *sh = tiles[0][0][0] + wave * 2 * HD;
+        if (kg == 0) dq_rows32(args_again(), b, r0 + wave, min(r0 + 64, a.n_q), h, sh, sh + HD, lane);
         return;
+    }
+    if constexpr (KG > 1) {
+        auto column = [&](int k, int j) { return reinterpret_cast<f32x4 *>(tiles[k][0][0] + (wave * NU + j) * 256) + lane; };
+        if (kg)
+#pragma unroll
+            for (int j = 0; j < NU; ++j) *column(kg, j) = dqt[j];
+        __syncthreads();
+        if (kg) return;
+#pragma unroll
+        for (int k = 1; k < KG; ++k)
+#pragma unroll
+            for (int j = 0; j < NU; ++j) dqt[j] += *column(k, j);
     }
     if (r >= a.n_q) return;
     float *dq = (float *)a.dq + row * a.lddq + h * HD;
@@ -454,21 +493,22 @@ __global__ __launch_bounds__(FNT, 2) void window_dq32_k(WindowArgs a) {
 }
 
 // ── backward: dK and dV, block = 64 keys of one KV head ──────────────────
-// Steps and parts as in bf16 (window_dkv16_k), one head a step.
-template <int HD>
-__global__ __launch_bounds__(FNT, 2) void window_dkv32_k(WindowArgs a, DkvPlan plan) {
-    using T = Tile32<HD, FT, FNT>;
+// Steps and parts as in bf16 (window_dkv16_k), one head a step; KG groups of waves take every KG-th of
+// the block's steps each and add their sums at the end.
+template <int HD, int KG>
+__global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_dkv32_k(WindowArgs a, DkvPlan plan) {
+    using T = Tile32<HD, FT, 256>;
     constexpr int P = T::P, NU = HD / 16, BN = 64;
-    __shared__ __attribute__((aligned(16))) float Qs[2][FT * P], Os[2][FT * P];
-    __shared__ float Ls[2][FT], Dl[2][FT];
+    __shared__ __attribute__((aligned(16))) float tiles[KG][2][2][FT * P];  // [group][Q, dO][buffer]
+    __shared__ float Ls[KG][2][FT], Dl[KG][2][FT];
     const int nbk = a.n_batch * a.n_kv_heads;
     const Pair pr = pair_of(blockIdx.x, gridDim.x, nbk, 4);
     const int bk = pr.bk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
     int kb, zpart, zparts, slot;
     dkv_block(plan, pr.y, kb, zpart, zparts, slot);
     const int nh = a.n_heads / a.n_kv_heads;
-    const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
-    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int tid = threadIdx.x % 256, lane = tid % 64, g = lane / 16, c = lane % 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) % 4, kg = __builtin_amdgcn_readfirstlane(threadIdx.x / 256);
     const Span s = span_of(a, b);
     const int k0 = kb * BN, kw = k0 + 16 * wave, key = kw + c;
     const long krow = (long)b * a.n_kv + key, row0 = (long)b * a.n_q;
@@ -506,30 +546,28 @@ __global__ __launch_bounds__(FNT, 2) void window_dkv32_k(WindowArgs a, DkvPlan p
         }
     };
     bool odd = false;  // in Q or dO of a tile whose rows do not all see all keys
-    auto store = [&](int it) {
+    auto store = [&](int it, int buf) {
         int h, q0;
         tile_of(it, h, q0);
         const int ta = q0 + s.off, tb = min(q0 + FT, s.ql) - 1 + s.off;
         if (!all_seen(a, ta, tb, k0, k0 + BN - 1)) odd |= tq.odd() || to.odd();
-        tq.store(Qs[it & 1], tid);
-        to.store(Os[it & 1], tid);
-        if (tid < FT) Ls[it & 1][tid] = stat;
-        else if (tid < 2 * FT) Dl[it & 1][tid - FT] = stat;
+        tq.store(tiles[kg][0][buf], tid);
+        to.store(tiles[kg][1][buf], tid);
+        if (tid < FT) Ls[kg][buf][tid] = stat;
+        else if (tid < 2 * FT) Dl[kg][buf][tid - FT] = stat;
     };
     f32x4 dvt[NU], dkt[NU];
 #pragma unroll
     for (int j = 0; j < NU; ++j) dvt[j] = dkt[j] = f32x4{0, 0, 0, 0};
-    if (niter > 0) {
-        load(0);
-        store(0);
+    if (kg < niter) {
+        load(kg);
+        store(kg, 0);
     }
     __syncthreads();
-    for (int it = 0; it < niter; ++it) {
-        const int buf = it & 1;
-        if (it + 1 < niter) load(it + 1);
+    auto step = [&](int it, int buf) {
         int h, q0;
         tile_of(it, h, q0);
-        const float *Ql = Qs[buf], *Ol = Os[buf];
+        const float *Ql = tiles[kg][0][buf], *Ol = tiles[kg][1][buf];
         f32x4 sa[2], da[2];  // S / dP[q0 + 16 qs + 4 g + e][key]
         bool live[2];
 #pragma unroll
@@ -543,11 +581,11 @@ __global__ __launch_bounds__(FNT, 2) void window_dkv32_k(WindowArgs a, DkvPlan p
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int x = 16 * qs + 4 * g + e;
-                const float l = Ls[buf][x];
+                const float l = Ls[kg][buf][x];
                 const float p = expf(fmaf(sa[qs][e], a.scale, -l));
                 const bool on = l != -INFINITY && sees(a, q0 + x + s.off, key);
                 sa[qs][e] = on ? p : 0.f;
-                da[qs][e] = on ? p * (da[qs][e] - Dl[buf][x]) : 0.f;
+                da[qs][e] = on ? p * (da[qs][e] - Dl[kg][buf][x]) : 0.f;
             }
         }
         // dV^T += dO^T P, dK^T += Q^T dS
@@ -557,15 +595,32 @@ __global__ __launch_bounds__(FNT, 2) void window_dkv32_k(WindowArgs a, DkvPlan p
             add_rows<NU>(dvt, Ol + (16 * qs + 4 * g) * P, P, c, sa[qs]);
             add_rows<NU>(dkt, Ql + (16 * qs + 4 * g) * P, P, c, da[qs]);
         }
-        if (it + 1 < niter) store(it + 1);
+    };
+    for (int it = kg, buf = 0; it - kg < niter; it += KG, buf ^= 1) {
+        if (it + KG < niter) load(it + KG);
+        if (it < niter) step(it, buf);
+        if (it + KG < niter) store(it + KG, buf ^ 1);
         __syncthreads();
     }
     float *ws = slot >= 0 ? a.ws + ((long)bk * plan.slots() + slot) * (2 * BN * HD) : nullptr;
     if (__syncthreads_or(odd)) {
-        float *sh = Qs[0] + wave * 2 * HD;
+        float *sh = tiles[0][0][0] + wave * 2 * HD;
         const Steps st{kvh * nh, qstart, top, nh, false, 1, zpart, zparts};
-        dkv_rows32(args_again(), st, b, kvh, k0, wave, ws, sh, sh + HD, lane);
+        if (kg == 0) dkv_rows32(args_again(), st, b, kvh, k0, wave, ws, sh, sh + HD, lane);
         return;
+    }
+    if constexpr (KG > 1) {
+        static_assert(2 * NU * 4 * 256 <= 4 * FT * P, "a group's sums fit its tiles");
+        auto column = [&](int k, int j) { return reinterpret_cast<f32x4 *>(tiles[k][0][0] + (wave * 2 * NU + j) * 256) + lane; };
+        if (kg)
+#pragma unroll
+            for (int j = 0; j < NU; ++j) *column(kg, j) = dkt[j], *column(kg, NU + j) = dvt[j];
+        __syncthreads();
+        if (kg) return;
+#pragma unroll
+        for (int k = 1; k < KG; ++k)
+#pragma unroll
+            for (int j = 0; j < NU; ++j) dkt[j] += *column(k, j), dvt[j] += *column(k, NU + j);
     }
     if (!ws && key >= a.n_kv) return;
     float *dk = ws ? ws + (16 * wave + c) * HD : (float *)a.dk + krow * a.lddk + kvh * HD;
@@ -586,7 +641,12 @@ bool ok(const void *p, long ld) { return aligned_rows(p, ld, 16, 4); }
 bool fwd_ok(const WindowArgs &a) { return shape_ok(a) && ok(a.q, a.ldq) && ok(a.k, a.ldk) && ok(a.v, a.ldv) && ok(a.o, a.ldo); }
 bool few_rows(const WindowArgs &a) { return a.n_q <= kFewRows; }
 int splits32(const WindowArgs &a) { return step_splits(a, 16, 1024); }
-DkvPlan plan32(const WindowArgs &a, bool ws) { return dkv_plan(a, ws, 64, 512, 16, 2, false); }
+// Two groups of waves a block where the chip has at most two blocks a CU: one or two groups, forward /
+// backward of 1001 tokens, 16 / 8 heads of 128, window 512: 74 / 209 and 63 / 203 us; unlimited: 120 / 307
+// and 97 / 249; 4 x 2048 tokens, window 64 (2048 and 1024 blocks): 123 / 453 and 123 / 502.
+bool grouped(const WindowArgs &a) { return (long)a.n_heads * a.n_batch * ((a.n_q + 63) / 64) <= 512; }
+bool grouped_dkv(const WindowArgs &a) { return (long)a.n_kv_heads * a.n_batch * ((a.n_kv + 63) / 64) <= 512; }
+DkvPlan plan32(const WindowArgs &a, bool ws) { return dkv_plan(a, ws, 64, 512, 16, grouped_dkv(a) ? 4 : 2, false); }
 
 }  // namespace
 
@@ -604,8 +664,13 @@ bool window32_forward(const WindowArgs &a, hipStream_t st) {
         return true;
     }
     const dim3 grid((unsigned)((long)a.n_heads * a.n_batch * ((a.n_q + 63) / 64)));
-    if (a.hd == 128) hipLaunchKernelGGL(window_fwd32_k<128>, grid, dim3(FNT), 0, st, a);
-    else hipLaunchKernelGGL(window_fwd32_k<64>, grid, dim3(FNT), 0, st, a);
+    auto by = [&](auto hd) {
+        constexpr int HD = decltype(hd)::value;
+        if (grouped(a)) hipLaunchKernelGGL((window_fwd32_k<HD, 2>), grid, dim3(512), 0, st, a);
+        else hipLaunchKernelGGL((window_fwd32_k<HD, 1>), grid, dim3(256), 0, st, a);
+    };
+    if (a.hd == 128) by(std::integral_constant<int, 128>{});
+    else by(std::integral_constant<int, 64>{});
     return true;
 }
 
@@ -616,8 +681,10 @@ bool window32_backward(const WindowArgs &a, hipStream_t st) {
     const dim3 gk((unsigned)((long)a.n_batch * a.n_kv_heads * plan.blocks()));
     auto by = [&](auto hd) {
         constexpr int HD = decltype(hd)::value;
-        hipLaunchKernelGGL(window_dq32_k<HD>, gq, dim3(FNT), 0, st, a);
-        hipLaunchKernelGGL(window_dkv32_k<HD>, gk, dim3(FNT), 0, st, a, plan);
+        if (grouped(a)) hipLaunchKernelGGL((window_dq32_k<HD, 2>), gq, dim3(512), 0, st, a);
+        else hipLaunchKernelGGL((window_dq32_k<HD, 1>), gq, dim3(256), 0, st, a);
+        if (grouped_dkv(a)) hipLaunchKernelGGL((window_dkv32_k<HD, 2>), gk, dim3(512), 0, st, a, plan);
+        else hipLaunchKernelGGL((window_dkv32_k<HD, 1>), gk, dim3(256), 0, st, a, plan);
         launch_dkv_sum<HD, 64, float>(a, plan, st);
     };
     if (a.hd == 128) by(std::integral_constant<int, 128>{});
