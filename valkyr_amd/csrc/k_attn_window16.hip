@@ -24,22 +24,31 @@
 namespace vkh {
 namespace {
 
-VKH_DEV bool not_finite(uint4 v) {
-    bool bad = false;
-#pragma unroll
-    for (unsigned w : {v.x, v.y, v.z, v.w})
-        bad |= (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
-    return bad;
-}
-// whether any of the thread's share of `bytes` of LDS holds an infinity or a NaN
+// Whether any of the thread's share of BYTES of LDS holds an infinity or a NaN: exponent bits of all
+// ones, to which one more carries into the sign's place (of either half of a word).
 template <int BYTES, int NT>
 VKH_DEV bool scan(const char *lds, int tid) {
-    bool bad = false;
+    unsigned carry = 0;
 #pragma unroll
     for (int i = 0; i < (BYTES + 16 * NT - 1) / (16 * NT); ++i)
-        if ((i + 1) * 16 * NT <= BYTES || (i * NT + tid) * 16 < BYTES)
-            bad |= not_finite(*reinterpret_cast<const uint4 *>(lds + (i * NT + tid) * 16));
-    return bad;
+        if ((i + 1) * 16 * NT <= BYTES || (i * NT + tid) * 16 < BYTES) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(lds + (i * NT + tid) * 16);
+#pragma unroll
+            for (unsigned w : {v.x, v.y, v.z, v.w}) carry |= (w & 0x7f807f80u) + 0x00800080u;
+        }
+    return carry & 0x80008000u;
+}
+// hide(ks, r) for the keys k0 + 16 ks + 4 g + r, ks < KS, that position t does not see.
+template <int KS, class F>
+VKH_DEV void for_hidden(const WindowArgs &a, int t, int k0, int g, F hide) {
+    const int x = t - k0 - 4 * g;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int d = 16 * ks + r;  // (tiles past the sinks: one comparison)
+            if (k0 >= a.n_sink ? (unsigned)(x - d) >= (unsigned)a.window : !sees(a, t, k0 + 4 * g + d)) hide(ks, r);
+        }
 }
 
 // The resource of rows row0 .. row0 + rows - 1 of one head (rows <= 0: of none).
@@ -83,15 +92,25 @@ __device__ __attribute__((noinline)) void dkv_rows(const WindowArgs &a, const St
     }
 }
 
+template <int N>
+VKH_DEV void wait_vm() {
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4 << 14));
+}
+
 // ── forward ──────────────────────────────────────────────────────────────
-// Block = 64 QS query rows of one head, 4 waves of 16 QS; 64-key tiles, two buffers.  The
-// heaviest (last) rows start first.
+// Block = 64 QS query rows of one head, 4 waves of 16 QS; 32-key tiles, three buffers (two tiles on
+// their way).  The heaviest (last) rows start first.  Matrix cores, vector ALU and LDS each have about
+// as much to do and take turns within a wave, so it is waves that overlap them: 32-key tiles leave
+// registers for three a SIMD.  16384 tokens, window 2048, 32 / 8 heads of 128: 534 us; 64-key tiles, two
+// waves a SIMD: 566; the next tile's scores formed beside this one's exponentials: 710 (two waves).
+// On short grids (64-row blocks) a wave's own chain of steps is the time: heads of 64, whose registers
+// allow it, take 64-key tiles there (2048 tokens, window 2048, 8 / 8 heads: 26 against 32 us).
 template <int HD, int QS, class TO>
-__global__ __launch_bounds__(256, 2) void window_fwd16_k(WindowArgs a) {
+__global__ __launch_bounds__(256, HD == 64 && QS == 2 ? 4 : 3) void window_fwd16_k(WindowArgs a) {
     using R = TileRows<HD>;
-    constexpr int DS = HD / 32, DSUB = HD / 16, BM = 64 * QS, BN = 64, KT = BN * HD * 2;
-    constexpr int RPI = 512 / HD, IPW = 16 / RPI;  // rows per DMA, DMAs per wave and tile
-    __shared__ __attribute__((aligned(16))) char Ks[2][KT], Vs[2][KT];
+    constexpr int DS = HD / 32, DSUB = HD / 16, BM = 64 * QS, BN = HD == 64 && QS == 1 ? 64 : 32, KS = BN / 16, TILE = BN * HD * 2, NBUF = 3;
+    constexpr int RPI = 512 / HD, IPT = BN / RPI, C = 2 * IPT / 4;  // rows per DMA, DMAs per tile and tensor, per wave
+    __shared__ __attribute__((aligned(16))) char Kt[NBUF][TILE], Vt[NBUF][TILE];
     const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, nqt = (a.n_q + BM - 1) / BM;
     const Pair pr = pair_of(blockIdx.x, gridDim.x, nbk, 4 * grp);
     const int b = pr.bk / a.n_kv_heads, kvh = pr.bk % a.n_kv_heads, h = kvh * grp + pr.y % grp, qt = nqt - 1 - pr.y / grp;
@@ -101,6 +120,7 @@ __global__ __launch_bounds__(256, 2) void window_fwd16_k(WindowArgs a) {
     const int r0 = qt * BM, qw0 = r0 + wave * 16 * QS;
     const KeyTiles kt = key_tiles<BN>(a, s, r0, r0 + BM);
     const int wta = max(0, qw0 + s.off), wtb = min(qw0 + 16 * QS, s.ql) - 1 + s.off;
+    const bool whole = qw0 + 16 * QS <= s.ql && qw0 + s.off >= 0;  // every row of the wave is there
     const float c2 = a.scale * LOG2E;
     const long row0 = (long)b * a.n_q, key0 = (long)b * a.n_kv;
 
@@ -114,24 +134,24 @@ __global__ __launch_bounds__(256, 2) void window_fwd16_k(WindowArgs a) {
 #pragma unroll
         for (int ds = 0; ds < DS; ++ds) qf[qs][ds] = pos[qs] >= 0 ? ld_frag(qr + 32 * ds) : bf16x8{};
     }
-    unsigned ko[IPW], vo[IPW];
+    // the wave's DMAs: number q = C wave + i of the 2 IPT of a tile, K's first
+    unsigned off[C];
 #pragma unroll
-    for (int i = 0; i < IPW; ++i) {
-        ko[i] = dma_off<HD>(16 * wave + RPI * i, lane, (int)a.ldk);
-        vo[i] = dma_off<HD>(16 * wave + RPI * i, lane, (int)a.ldv);
+    for (int i = 0; i < C; ++i) {
+        const int q = C * wave + i;
+        off[i] = dma_off<HD>(q % IPT * RPI, lane, (int)(q < IPT ? a.ldk : a.ldv));
     }
     wait_vm0();  // Q fragments are in registers before any DMA is queued
     auto dma = [&](int it, int buf) {
         const int k0 = kt.tile(it) * BN, rows = min(BN, s.kl - k0);
-        const sgpr4 rk = head_rows<HD>(a.k, key0 + k0, a.ldk, kvh * HD, rows);
-        const sgpr4 rv = head_rows<HD>(a.v, key0 + k0, a.ldv, kvh * HD, rows);
+        const bool isk = C * wave < IPT;  // (a wave's DMAs are all K's or all V's)
+        const sgpr4 rs = head_rows<HD>(isk ? a.k : a.v, key0 + k0, isk ? a.ldk : a.ldv, kvh * HD, rows);
+        char *dst = isk ? Kt[buf] + C * wave * 1024 : Vt[buf] + (C * wave - IPT) * 1024;
 #pragma unroll
-        for (int i = 0; i < IPW; ++i) {
-            dma16_async(rk, Ks[buf] + (16 * wave + RPI * i) * HD * 2, ko[i]);
-            dma16_async(rv, Vs[buf] + (16 * wave + RPI * i) * HD * 2, vo[i]);
-        }
+        for (int i = 0; i < C; ++i) dma16_async(rs, dst + i * 1024, off[i]);
     };
-    f32x4 oacc[QS][DSUB];
+    static_assert(IPT % C == 0, "a wave's DMAs are of one tensor");
+    f32x4 oacc[QS][DSUB], st[KS][QS];
     float m[QS], l[QS];  // running maximum in log2 units; this lane's share of the sum
 #pragma unroll
     for (int qs = 0; qs < QS; ++qs) {
@@ -140,85 +160,94 @@ __global__ __launch_bounds__(256, 2) void window_fwd16_k(WindowArgs a) {
 #pragma unroll
         for (int i = 0; i < DSUB; ++i) oacc[qs][i] = f32x4{0, 0, 0, 0};
     }
-    bool odd = false;  // an infinity or a NaN in V of a tile that is not seen in full
-    auto step = [&](const int it, const int buf) {
-        const int k0 = kt.tile(it) * BN;
-        wait_vm0();
-        lds_barrier();  // tile `it` landed; everyone is done with the other buffer
-        if (it + 1 < kt.n) dma(it + 1, buf ^ 1);
-        const char *Kb = Ks[buf], *Vb = Vs[buf];
-        if (!all_seen(a, kt.ta, kt.tb, k0, k0 + BN - 1)) {
-            if (scan<KT, 256>(Vb, tid)) odd = true;
-        }
-        if (none_seen(a, wta, wtb, k0, k0 + BN - 1)) return;
-
-        f32x4 st[4][QS];
+    auto scores = [&](const char *Kb, f32x4 (&x)[KS][QS]) {
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-            for (int qs = 0; qs < QS; ++qs) st[ks][qs] = f32x4{0, 0, 0, 0};
+            for (int qs = 0; qs < QS; ++qs) x[ks][qs] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int ds = 0; ds < DS; ++ds)
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
+            for (int ks = 0; ks < KS; ++ks) {
                 const bf16x8 kf = R::frag_row(Kb, 16 * ks + c16, 32 * ds + 8 * g);
 #pragma unroll
-                for (int qs = 0; qs < QS; ++qs) st[ks][qs] = mfma16x16x32(kf, qf[qs][ds], st[ks][qs]);
+                for (int qs = 0; qs < QS; ++qs) x[ks][qs] = mfma16x16x32(kf, qf[qs][ds], x[ks][qs]);
             }
-        const bool full = all_seen(a, wta, wtb, k0, k0 + BN - 1) && qw0 + 16 * QS <= s.ql && qw0 + s.off >= 0;
-        bf16x8 pf[QS][2];
+    };
+    bool odd = false;  // an infinity or a NaN in V of a tile that is not seen in full
+    if (kt.n > 0) dma(0, 0);
+    if (kt.n > 1) dma(1, 1);
+    auto step = [&](const int it, auto bufc) {
+        constexpr int buf = decltype(bufc)::value;
+        const int k0 = kt.tile(it) * BN;
+        if (it + 1 < kt.n) wait_vm<C>();
+        else wait_vm0();
+        lds_barrier();  // tile it landed; everyone is done with tile it - 1
+        if (it + 2 < kt.n) dma(it + 2, (buf + 2) % NBUF);
+        const char *Kb = Kt[buf], *Vb = Vt[buf];
+        if (!all_seen(a, kt.ta, kt.tb, k0, k0 + BN - 1) && scan<TILE, 256>(Vb, tid)) odd = true;
+        if (none_seen(a, wta, wtb, k0, k0 + BN - 1)) return;
+        scores(Kb, st);
+        if (!whole || !all_seen(a, wta, wtb, k0, k0 + BN - 1)) {
+#pragma unroll
+            for (int qs = 0; qs < QS; ++qs) for_hidden<KS>(a, pos[qs], k0, g, [&](int ks, int r) { st[ks][qs][r] = -INFINITY; });
+        }
+        // The maximum that P is taken against moves only when a row's scores pass it by more than 8 (in
+        // log2 units): P stays under 2^8, where bf16 and fp32 hold it as exactly, and the accumulators
+        // are rescaled in few tiles after the first.  A row's decision is its own.
+        float mt[QS];
+        bool moved = false;
 #pragma unroll
         for (int qs = 0; qs < QS; ++qs) {
-            if (!full) {
+            mt[qs] = -INFINITY;
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks)
+            for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (!sees(a, pos[qs], k0 + 16 * ks + 4 * g + r)) st[ks][qs][r] = -INFINITY;
-            }
-            float mt = -INFINITY;
+                for (int r = 0; r < 4; ++r) mt[qs] = fmaxf(mt[qs], st[ks][qs][r]);
+            moved = moved || mt[qs] * c2 > m[qs] + 8.f;
+        }
+        if (__any(moved)) {
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) mt = fmaxf(mt, st[ks][qs][r]);
-            // The maximum that P is taken against moves only when a row's scores pass it by more
-            // than 8 (in log2 units): P stays under 2^8, where bf16 and fp32 hold it as exactly,
-            // and the accumulators are rescaled in few tiles after the first.  A row's decision
-            // is its own.
-            if (__any(mt * c2 > m[qs] + 8.f)) {
-                const float mn = xrow_max(mt) * c2;
-                const float mo = m[qs];
+            for (int qs = 0; qs < QS; ++qs) {
+                const float mn = xrow_max(mt[qs]) * c2, mo = m[qs];
                 if (mn > mo + 8.f) m[qs] = mn;
                 const float so = m[qs] == mo ? 1.f : __builtin_amdgcn_exp2f(mo - m[qs]);
                 l[qs] *= so;
 #pragma unroll
                 for (int i = 0; i < DSUB; ++i) oacc[qs][i] *= so;
             }
+        }
+        bf16x8 pf[KS / 2][QS];
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs) {
             const float ms = m[qs] == -INFINITY ? 0.f : m[qs];  // no score above -inf yet: P = 0
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
+            for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float p = __builtin_amdgcn_exp2f(fmaf(st[ks][qs][r], c2, -ms));
                     st[ks][qs][r] = p;
                     l[qs] += p;
                 }
-            pf[qs][0] = frag_acc(st[0][qs], st[1][qs]);
-            pf[qs][1] = frag_acc(st[2][qs], st[3][qs]);
+#pragma unroll
+            for (int ks = 0; ks < KS; ks += 2) pf[ks / 2][qs] = frag_acc(st[ks][qs], st[ks + 1][qs]);
         }
 #pragma unroll
-        for (int kst = 0; kst < 2; ++kst)
+        for (int i = 0; i < DSUB; ++i)
 #pragma unroll
-            for (int i = 0; i < DSUB; ++i) {
-                const bf16x8 vf = R::frag_t(Vb, 16 * i, 32 * kst, g, c16);
+            for (int k2 = 0; k2 < KS / 2; ++k2) {
+                const bf16x8 vf = R::frag_t(Vb, 16 * i, 32 * k2, g, c16);
 #pragma unroll
-                for (int qs = 0; qs < QS; ++qs) oacc[qs][i] = mfma16x16x32(vf, pf[qs][kst], oacc[qs][i]);
+                for (int qs = 0; qs < QS; ++qs) oacc[qs][i] = mfma16x16x32(vf, pf[k2][qs], oacc[qs][i]);
             }
     };
-    if (kt.n > 0) dma(0, 0);
-    for (int it = 0; it < kt.n; ++it) step(it, it & 1);
+    for (int it0 = 0; it0 < kt.n; it0 += NBUF) {
+        step(it0, std::integral_constant<int, 0>{});
+        if (it0 + 1 < kt.n) step(it0 + 1, std::integral_constant<int, 1>{});
+        if (it0 + 2 < kt.n) step(it0 + 2, std::integral_constant<int, 2>{});
+    }
     if (__syncthreads_or(odd)) {
-        fwd_rows<TO>(args_again(), b, r0 + wave, min(r0 + BM, a.n_q), 4, h, (float *)Ks + wave * HD, lane);
+        fwd_rows<TO>(args_again(), b, r0 + wave, min(r0 + BM, a.n_q), 4, h, (float *)Kt + wave * HD, lane);
         return;
     }
 #pragma unroll
@@ -246,10 +275,6 @@ __global__ __launch_bounds__(256, 2) void window_fwd16_k(WindowArgs a) {
 // waves), every fourth of the block's, and their results are joined at the end.  `splits` blocks
 // share a KV head's tiles; their results (maximum, sum, O in fp32) go to a.ws and
 // window_join_k joins them in order.
-template <int N>
-VKH_DEV void wait_vm() {
-    __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4 << 14));
-}
 // acc[i][r] += sum over the tile's rows x that `see` names of T[x][16 i + 4 g + r] w[x], where w is
 // held as a B operand: element 4 u + e is row 16 u + 4 g + e.  It goes through `wl`, 1 KB of the
 // wave's own LDS.
@@ -337,13 +362,7 @@ __global__ __launch_bounds__(256, 1) void window_step16_k(WindowArgs a, int spli
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks)
                 st[ks] = mfma16x16x32(R::frag_row(Kb, 16 * ks + c16, 32 * ds + 8 * g), qf[ds], st[ks]);
-        if (!whole) {
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (!sees(a, pos, k0 + 16 * ks + 4 * g + r)) st[ks][r] = -INFINITY;
-        }
+        if (!whole) for_hidden<2>(a, pos, k0, g, [&](int ks, int r) { st[ks][r] = -INFINITY; });
         float mt = -INFINITY;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
@@ -574,13 +593,7 @@ __global__ __launch_bounds__(256, 2) void window_dq16_k(WindowArgs a) {
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) dpt[ks][j][r] = st[ks][j][r] * dpt[ks][j][r];
-            if (!whole) {
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (!sees(a, pos[j], k0 + 16 * ks + 4 * g + r)) dpt[ks][j][r] = 0.f;
-            }
+            if (!whole) for_hidden<KS>(a, pos[j], k0, g, [&](int ks, int r) { dpt[ks][j][r] = 0.f; });
             sb[j] = frag_acc(dpt[0][j], dpt[1][j]);
         }
         // dQ^T += K^T dS^T
@@ -1090,7 +1103,7 @@ bool window16_forward(const WindowArgs &a, hipStream_t st) {
     auto go = [&](auto kernel, int bm) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)(per * ((a.n_q + bm - 1) / bm))), dim3(256), 0, st, a);
     };
-    // grids of 128-row blocks that leave the CUs one block each or fewer take 64 rows, two per CU
+    // grids of 128-row blocks that leave the CUs one block each or fewer take 64 rows
     const bool small = per * ((a.n_q + 127) / 128) <= cu_count();
     auto by = [&](auto to) {
         using TO = decltype(to);
@@ -1106,8 +1119,10 @@ bool window16_backward(const WindowArgs &a, hipStream_t st) {
     const long per = (long)a.n_heads * a.n_batch, nbk = (long)a.n_batch * a.n_kv_heads;
     // 128-row dQ blocks on 4 waves, two a CU (256 rows on 8 waves, one a CU, wait for each other over
     // twice the span of masked tiles: 16384 tokens, window 2048, 996 against 881 us; 4 x 2048, window
-    // 512, 112 against 90); 64 rows where those leave CUs idle
-    const int bq = per * ((a.n_q + 127) / 128) >= 256 ? 128 : 64;
+    // 512, 112 against 90); 64 rows where those leave CUs idle, and on windows whose tiles are masked
+    // in large part (backward of 16384 tokens, window 256, 621 against 596 us; 4 x 2048, window 512,
+    // 224 against 222; window 1024, 294 against 298)
+    const int bq = per * ((a.n_q + 127) / 128) >= 256 && a.window > 512 ? 128 : 64;
     const DkvPlan plan = plan16(a, a.ws != nullptr);
     auto by = [&](auto hd, auto to) {
         constexpr int HD = decltype(hd)::value;
