@@ -105,20 +105,22 @@ VKH_DEV void wait_vm() {
 // waves a SIMD: 566; the next tile's scores formed beside this one's exponentials: 710 (two waves).
 // On short grids (64-row blocks) a wave's own chain of steps is the time: heads of 64, whose registers
 // allow it, take 64-key tiles there (2048 tokens, window 2048, 8 / 8 heads: 26 against 32 us).
-template <int HD, int QS, class TO>
-__global__ __launch_bounds__(256, HD == 64 && QS == 2 ? 4 : 3) void window_fwd16_k(WindowArgs a) {
+template <int HD, int QS, int KG, class TO>
+__global__ __launch_bounds__(256 * KG, KG == 2 ? 2 : HD == 64 && QS == 2 ? 4 : 3) void window_fwd16_k(WindowArgs a) {
     using R = TileRows<HD>;
     constexpr int DS = HD / 32, DSUB = HD / 16, BM = 64 * QS, BN = HD == 64 && QS == 1 ? 64 : 32, KS = BN / 16, TILE = BN * HD * 2, NBUF = 3;
     constexpr int RPI = 512 / HD, IPT = BN / RPI, C = 2 * IPT / 4;  // rows per DMA, DMAs per tile and tensor, per wave
-    __shared__ __attribute__((aligned(16))) char Kt[NBUF][TILE], Vt[NBUF][TILE];
+    __shared__ __attribute__((aligned(16))) char Kts[KG][NBUF][TILE], Vts[KG][NBUF][TILE];
     const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, nqt = (a.n_q + BM - 1) / BM;
     const Pair pr = pair_of(blockIdx.x, gridDim.x, nbk, 4 * grp);
     const int b = pr.bk / a.n_kv_heads, kvh = pr.bk % a.n_kv_heads, h = kvh * grp + pr.y % grp, qt = nqt - 1 - pr.y / grp;
-    const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c16 = lane % 16;
-    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int tid = threadIdx.x % 256, lane = tid % 64, g = lane / 16, c16 = lane % 16;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64), kg = __builtin_amdgcn_readfirstlane(threadIdx.x / 256);
+    char(*Kt)[TILE] = Kts[kg], (*Vt)[TILE] = Vts[kg];
     const Span s = span_of(a, b);
     const int r0 = qt * BM, qw0 = r0 + wave * 16 * QS;
     const KeyTiles kt = key_tiles<BN>(a, s, r0, r0 + BM);
+    const int steps = (kt.n + KG - 1) / KG, n = (kt.n - kg + KG - 1) / KG;  // the block's; the group's
     const int wta = max(0, qw0 + s.off), wtb = min(qw0 + 16 * QS, s.ql) - 1 + s.off;
     const bool whole = qw0 + 16 * QS <= s.ql && qw0 + s.off >= 0;  // every row of the wave is there
     const float c2 = a.scale * LOG2E;
@@ -143,7 +145,7 @@ __global__ __launch_bounds__(256, HD == 64 && QS == 2 ? 4 : 3) void window_fwd16
     }
     wait_vm0();  // Q fragments are in registers before any DMA is queued
     auto dma = [&](int it, int buf) {
-        const int k0 = kt.tile(it) * BN, rows = min(BN, s.kl - k0);
+        const int k0 = kt.tile(KG * it + kg) * BN, rows = min(BN, s.kl - k0);
         const bool isk = C * wave < IPT;  // (a wave's DMAs are all K's or all V's)
         const sgpr4 rs = head_rows<HD>(isk ? a.k : a.v, key0 + k0, isk ? a.ldk : a.ldv, kvh * HD, rows);
         char *dst = isk ? Kt[buf] + C * wave * 1024 : Vt[buf] + (C * wave - IPT) * 1024;
@@ -175,15 +177,16 @@ __global__ __launch_bounds__(256, HD == 64 && QS == 2 ? 4 : 3) void window_fwd16
             }
     };
     bool odd = false;  // an infinity or a NaN in V of a tile that is not seen in full
-    if (kt.n > 0) dma(0, 0);
-    if (kt.n > 1) dma(1, 1);
+    if (n > 0) dma(0, 0);
+    if (n > 1) dma(1, 1);
     auto step = [&](const int it, auto bufc) {
         constexpr int buf = decltype(bufc)::value;
-        const int k0 = kt.tile(it) * BN;
-        if (it + 1 < kt.n) wait_vm<C>();
+        const int k0 = kt.tile(KG * it + kg) * BN;
+        if (it + 1 < n) wait_vm<C>();
         else wait_vm0();
         lds_barrier();  // tile it landed; everyone is done with tile it - 1
-        if (it + 2 < kt.n) dma(it + 2, (buf + 2) % NBUF);
+        if (it + 2 < n) dma(it + 2, (buf + 2) % NBUF);
+        if (KG > 1 && it >= n) return;
         const char *Kb = Kt[buf], *Vb = Vt[buf];
         if (!all_seen(a, kt.ta, kt.tb, k0, k0 + BN - 1) && scan<TILE, 256>(Vb, tid)) odd = true;
         if (none_seen(a, wta, wtb, k0, k0 + BN - 1)) return;
@@ -241,14 +244,33 @@ __global__ __launch_bounds__(256, HD == 64 && QS == 2 ? 4 : 3) void window_fwd16
                 for (int qs = 0; qs < QS; ++qs) oacc[qs][i] = mfma16x16x32(vf, pf[k2][qs], oacc[qs][i]);
             }
     };
-    for (int it0 = 0; it0 < kt.n; it0 += NBUF) {
+    for (int it0 = 0; it0 < steps; it0 += NBUF) {
         step(it0, std::integral_constant<int, 0>{});
-        if (it0 + 1 < kt.n) step(it0 + 1, std::integral_constant<int, 1>{});
-        if (it0 + 2 < kt.n) step(it0 + 2, std::integral_constant<int, 2>{});
+        if (it0 + 1 < steps) step(it0 + 1, std::integral_constant<int, 1>{});
+        if (it0 + 2 < steps) step(it0 + 2, std::integral_constant<int, 2>{});
     }
     if (__syncthreads_or(odd)) {
-        fwd_rows<TO>(args_again(), b, r0 + wave, min(r0 + BM, a.n_q), 4, h, (float *)Kt + wave * HD, lane);
+        if (kg == 0) fwd_rows<TO>(args_again(), b, r0 + wave, min(r0 + BM, a.n_q), 4, h, (float *)Kts + wave * HD, lane);
         return;
+    }
+    if constexpr (KG > 1) {  // the groups' results, joined in order through LDS
+        constexpr int W = (DSUB + 1) * 64 * 16;  // bytes of a wave's result: columns of 64 lanes
+        static_assert(KG == 2 && QS == 1 && 4 * W <= (int)sizeof(Kts), "the results fit the tiles");
+        auto column = [&](int j) { return reinterpret_cast<f32x4 *>((char *)Kts + wave * W + j * 1024) + lane; };
+        if (kg) {
+#pragma unroll
+            for (int i = 0; i < DSUB; ++i) *column(i) = oacc[0][i];
+            *column(DSUB) = f32x4{m[0], l[0], 0, 0};
+        }
+        __syncthreads();
+        if (kg) return;
+        const f32x4 ml = *column(DSUB);
+        const float mn = fmaxf(m[0], ml[0]), ms = mn == -INFINITY ? 0.f : mn;
+        const float f0 = __builtin_amdgcn_exp2f(m[0] - ms), f1 = __builtin_amdgcn_exp2f(ml[0] - ms);
+        m[0] = mn;
+        l[0] = l[0] * f0 + ml[1] * f1;
+#pragma unroll
+        for (int i = 0; i < DSUB; ++i) oacc[0][i] = oacc[0][i] * f0 + *column(i) * f1;
     }
 #pragma unroll
     for (int qs = 0; qs < QS; ++qs) {
@@ -447,23 +469,25 @@ __global__ __launch_bounds__(256, 1) void window_step16_k(WindowArgs a, int spli
 // registers; 32-key tiles of K and V through three buffers (two in flight, the wait counted).
 // D = rowsum(O dO) of the block's rows is formed first (fp64 sums of the bf16 products) and
 // stored for the dK/dV kernel, which runs after this one.
-template <int HD, int BQ, class TO>
-__global__ __launch_bounds__(256, 2) void window_dq16_k(WindowArgs a) {
+template <int HD, int BQ, int KG, class TO>
+__global__ __launch_bounds__(256 * KG, 2) void window_dq16_k(WindowArgs a) {
     using R = TileRows<HD>;
     constexpr int NWV = 4;
     constexpr int QSUB = BQ / 16 / NWV, BN = 32, KS = 2, NBUF = 3, TILE = BN * HD * 2;
     constexpr int DS = HD / 32, DSUB = HD / 16, NF = 2 * DS;
     constexpr int RPI = 512 / HD, IPT = BN / RPI, C = 2 * IPT / NWV;  // DMAs per tile and tensor, per wave
     static_assert(C >= 1 && C * NWV == 2 * IPT, "DMA share");
-    __shared__ __attribute__((aligned(16))) char Kt[NBUF][TILE], Vt[NBUF][TILE];
+    __shared__ __attribute__((aligned(16))) char Kts[KG][NBUF][TILE], Vts[KG][NBUF][TILE];
     const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, nqb = (a.n_q + BQ - 1) / BQ;
     const Pair pr = pair_of(blockIdx.x, gridDim.x, nbk, 4 * grp);
     const int b = pr.bk / a.n_kv_heads, kvh = pr.bk % a.n_kv_heads, h = kvh * grp + pr.y % grp, qb = nqb - 1 - pr.y / grp;
-    const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c16 = lane % 16;
-    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int tid = threadIdx.x % 256, lane = tid % 64, g = lane / 16, c16 = lane % 16;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64), kg = __builtin_amdgcn_readfirstlane(threadIdx.x / 256);
+    char(*Kt)[TILE] = Kts[kg], (*Vt)[TILE] = Vts[kg];
     const Span s = span_of(a, b);
     const int r0 = qb * BQ, qw0 = r0 + wave * 16 * QSUB;
     const KeyTiles kt = key_tiles<BN>(a, s, r0, r0 + BQ);
+    const int steps = (kt.n + KG - 1) / KG, nt = (kt.n - kg + KG - 1) / KG;  // the block's; the group's
     const int wta = max(0, qw0 + s.off), wtb = min(qw0 + 16 * QSUB, s.ql) - 1 + s.off;
     const float c2 = a.scale * LOG2E;
     const long row0 = (long)b * a.n_q, key0 = (long)b * a.n_kv;
@@ -497,7 +521,7 @@ __global__ __launch_bounds__(256, 2) void window_dq16_k(WindowArgs a) {
         acc += __shfl_xor(acc, 16, 64);
         acc += __shfl_xor(acc, 32, 64);
         dd[j] = (float)acc;
-        if (r < a.n_q && g == 0) a.d[t * a.n_heads + h] = dd[j];
+        if (r < a.n_q && g == 0 && kg == 0) a.d[t * a.n_heads + h] = dd[j];
     }
     // the wave's DMAs: number q = C wave + i of the 2 IPT of a tile, K's first
     unsigned off[C];
@@ -508,7 +532,7 @@ __global__ __launch_bounds__(256, 2) void window_dq16_k(WindowArgs a) {
     }
     wait_vm0();
     auto dma = [&](int it, int buf) {
-        const int k0 = kt.tile(it) * BN, rows = min(BN, s.kl - k0);
+        const int k0 = kt.tile(KG * it + kg) * BN, rows = min(BN, s.kl - k0);
         const sgpr4 rk = head_rows<HD>(a.k, key0 + k0, a.ldk, kvh * HD, rows);
         const sgpr4 rv = head_rows<HD>(a.v, key0 + k0, a.ldv, kvh * HD, rows);
 #pragma unroll
@@ -523,17 +547,18 @@ __global__ __launch_bounds__(256, 2) void window_dq16_k(WindowArgs a) {
     for (int j = 0; j < QSUB; ++j)
 #pragma unroll
         for (int i = 0; i < DSUB; ++i) acc[j][i] = f32x4{0, 0, 0, 0};
-    if (kt.n > 0) dma(0, 0);
-    if (kt.n > 1) dma(1, 1);
+    if (nt > 0) dma(0, 0);
+    if (nt > 1) dma(1, 1);
     // unrolled over the three buffers: every LDS address is a lane's base plus a constant
     bool odd = false;  // an infinity or a NaN in K of a tile that is not seen in full
     auto step = [&](const int it, auto bufc) {
         constexpr int buf = decltype(bufc)::value;
-        if (it + 1 < kt.n) __builtin_amdgcn_s_waitcnt(0x0f70 | C);
+        if (it + 1 < nt) wait_vm<C>();
         else wait_vm0();
         lds_barrier();
-        if (it + 2 < kt.n) dma(it + 2, (buf + 2) % NBUF);
-        const int k0 = kt.tile(it) * BN;
+        if (it + 2 < nt) dma(it + 2, (buf + 2) % NBUF);
+        if (KG > 1 && it >= nt) return;
+        const int k0 = kt.tile(KG * it + kg) * BN;
         const char *Kb = Kt[buf], *Vb = Vt[buf];
         if (!all_seen(a, kt.ta, kt.tb, k0, k0 + BN - 1)) {
             if (scan<TILE, NWV * 64>(Kb, tid)) odd = true;
@@ -605,15 +630,28 @@ __global__ __launch_bounds__(256, 2) void window_dq16_k(WindowArgs a) {
             for (int j = 0; j < QSUB; ++j) acc[j][i] = mfma16x16x32(fr[n % RING], sb[j], acc[j][i]);
         }
     };
-    for (int t0 = 0; t0 < kt.n; t0 += NBUF) {
+    for (int t0 = 0; t0 < steps; t0 += NBUF) {
         step(t0, std::integral_constant<int, 0>{});
-        if (t0 + 1 < kt.n) step(t0 + 1, std::integral_constant<int, 1>{});
-        if (t0 + 2 < kt.n) step(t0 + 2, std::integral_constant<int, 2>{});
+        if (t0 + 1 < steps) step(t0 + 1, std::integral_constant<int, 1>{});
+        if (t0 + 2 < steps) step(t0 + 2, std::integral_constant<int, 2>{});
     }
     if (__syncthreads_or(odd)) {
-        float *sh = (float *)Kt + wave * 2 * HD;
+        if (kg) return;
+        float *sh = (float *)Kts + wave * 2 * HD;
         dq_rows<TO>(args_again(), b, r0 + wave, min(r0 + BQ, a.n_q), NWV, h, sh, sh + HD, lane);
         return;
+    }
+    if constexpr (KG > 1) {  // the groups' sums, added through LDS
+        static_assert(KG == 2 && QSUB == 1 && 4 * DSUB * 1024 <= (int)sizeof(Kts), "the sums fit the tiles");
+        auto column = [&](int j) { return reinterpret_cast<f32x4 *>((char *)Kts + (wave * DSUB + j) * 1024) + lane; };
+        if (kg) {
+#pragma unroll
+            for (int i = 0; i < DSUB; ++i) *column(i) = acc[0][i];
+        }
+        __syncthreads();
+        if (kg) return;
+#pragma unroll
+        for (int i = 0; i < DSUB; ++i) acc[0][i] += *column(i);
     }
 #pragma unroll
     for (int j = 0; j < QSUB; ++j) {
@@ -1073,6 +1111,8 @@ int splits16(const WindowArgs &a) { return step_splits(a, 32, 512); }
 // dK/dV: one block per CU, at least four steps of both groups each
 DkvPlan plan16(const WindowArgs &a, bool ws) { return dkv_plan(a, ws, 128, 256, 8, 8, true); }
 
+bool grouped(const WindowArgs &a) { return (long)a.n_heads * a.n_batch * ((a.n_q + 63) / 64) <= cu_count(); }
+
 }  // namespace
 
 size_t window16_fwd_ws_bytes(const WindowArgs &a) { return shape_ok(a) && few_rows(a) ? step_ws_bytes(a, splits16(a)) : 0; }
@@ -1100,17 +1140,23 @@ bool window16_forward(const WindowArgs &a, hipStream_t st) {
         return true;
     }
     const long per = (long)a.n_heads * a.n_batch;
-    auto go = [&](auto kernel, int bm) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(per * ((a.n_q + bm - 1) / bm))), dim3(256), 0, st, a);
-    };
     // grids of 128-row blocks that leave the CUs one block each or fewer take 64 rows
-    const bool small = per * ((a.n_q + 127) / 128) <= cu_count();
-    auto by = [&](auto to) {
-        using TO = decltype(to);
-        if (a.hd == 128) small ? go(window_fwd16_k<128, 1, TO>, 64) : go(window_fwd16_k<128, 2, TO>, 128);
-        else small ? go(window_fwd16_k<64, 1, TO>, 64) : go(window_fwd16_k<64, 2, TO>, 128);
+    const bool small = per * ((a.n_q + 127) / 128) <= cu_count(), pairs = grouped(a);
+    auto go = [&](auto kernel, int bm, int kg) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(per * ((a.n_q + bm - 1) / bm))), dim3(256 * kg), 0, st, a);
     };
-    a.odt == DType::F32 ? by(float{}) : by(bf16{});
+    auto by = [&](auto hd, auto to) {
+        constexpr int HD = decltype(hd)::value;
+        using TO = decltype(to);
+        if (pairs) go(window_fwd16_k<HD, 1, 2, TO>, 64, 2);
+        else if (small) go(window_fwd16_k<HD, 1, 1, TO>, 64, 1);
+        else go(window_fwd16_k<HD, 2, 1, TO>, 128, 1);
+    };
+    auto by_head = [&](auto to) {
+        if (a.hd == 128) by(std::integral_constant<int, 128>{}, to);
+        else by(std::integral_constant<int, 64>{}, to);
+    };
+    a.odt == DType::F32 ? by_head(float{}) : by_head(bf16{});
     return true;
 }
 
@@ -1127,11 +1173,12 @@ bool window16_backward(const WindowArgs &a, hipStream_t st) {
     auto by = [&](auto hd, auto to) {
         constexpr int HD = decltype(hd)::value;
         using TO = decltype(to);
-        auto dq = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3((unsigned)(per * ((a.n_q + bq - 1) / bq))), dim3(256), 0, st, a);
+        auto dq = [&](auto kernel, int kg) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)(per * ((a.n_q + bq - 1) / bq))), dim3(256 * kg), 0, st, a);
         };
-        if (bq == 128) dq(window_dq16_k<HD, 128, TO>);
-        else dq(window_dq16_k<HD, 64, TO>);
+        if (bq == 128) dq(window_dq16_k<HD, 128, 1, TO>, 1);
+        else if (grouped(a)) dq(window_dq16_k<HD, 64, 2, TO>, 2);
+        else dq(window_dq16_k<HD, 64, 1, TO>, 1);
         WindowArgs near = a;
         if (plan.far_parts) {
             near.n_sink = 0;
