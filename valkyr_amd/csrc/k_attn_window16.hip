@@ -41,14 +41,22 @@ VKH_DEV bool scan(const char *lds, int tid) {
 // hide(ks, r) for the keys k0 + 16 ks + 4 g + r, ks < KS, that position t does not see.
 template <int KS, class F>
 VKH_DEV void for_hidden(const WindowArgs &a, int t, int k0, int g, F hide) {
-    const int x = t - k0 - 4 * g;
+    int x = t - k0 - 4 * g;
+    if (k0 < a.n_sink && k0 + 16 * KS > a.n_sink) {  // sinks and others: the others outside the window
+        const int ns = a.n_sink - k0 - 4 * g;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (16 * ks + r >= ns && x - 16 * ks - r >= a.window) hide(ks, r);
+    }
+    asm("" : "+v"(x));  // (the differences below are not kept from those above)
+    const unsigned reach = k0 < a.n_sink ? kAll : a.window;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int d = 16 * ks + r;  // (tiles past the sinks: one comparison)
-            if (k0 >= a.n_sink ? (unsigned)(x - d) >= (unsigned)a.window : !sees(a, t, k0 + 4 * g + d)) hide(ks, r);
-        }
+        for (int r = 0; r < 4; ++r)
+            if ((unsigned)(x - 16 * ks - r) >= reach) hide(ks, r);
 }
 
 // The resource of rows row0 .. row0 + rows - 1 of one head (rows <= 0: of none).
@@ -61,6 +69,14 @@ template <int HD>
 VKH_DEV unsigned dma_off(int r0, int lane, int ld) {
     const int r = r0 + lane / (HD / 8), c = (lane % (HD / 8)) ^ TileRows<HD>::swz(r);
     return (unsigned)((r * ld + 8 * c) * 2);
+}
+
+// The DMA to a wave-uniform LDS address that the caller keeps as a number.
+VKH_DEV unsigned lds_addr(const char *p) {
+    return __builtin_amdgcn_readfirstlane((int)(unsigned)(unsigned long)(const __attribute__((address_space(3))) char *)p);
+}
+VKH_DEV void dma16_at(const sgpr4 &rs, unsigned lds, unsigned voff) {
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(voff), "s"(rs) : "memory");
 }
 
 // A block's rows one at a time, for blocks that met an infinity or a NaN in a tile which some of
@@ -122,7 +138,9 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 2 : HD == 64 && QS == 2 ? 4 : 3
     const KeyTiles kt = key_tiles<BN>(a, s, r0, r0 + BM);
     const int steps = (kt.n + KG - 1) / KG, n = (kt.n - kg + KG - 1) / KG;  // the block's; the group's
     const int wta = max(0, qw0 + s.off), wtb = min(qw0 + 16 * QS, s.ql) - 1 + s.off;
-    const bool whole = qw0 + 16 * QS <= s.ql && qw0 + s.off >= 0;  // every row of the wave is there
+    Reach mine = reach<BN>(a, kt, wta, wtb);
+    if (qw0 + 16 * QS > s.ql || qw0 + s.off < 0) mine.n_all = mine.n_sink_all = 0;  // rows that are not there
+    const Reach block = reach<BN>(a, kt, kt.ta, kt.tb);
     const float c2 = a.scale * LOG2E;
     const long row0 = (long)b * a.n_q, key0 = (long)b * a.n_kv;
 
@@ -137,20 +155,19 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 2 : HD == 64 && QS == 2 ? 4 : 3
         for (int ds = 0; ds < DS; ++ds) qf[qs][ds] = pos[qs] >= 0 ? ld_frag(qr + 32 * ds) : bf16x8{};
     }
     // the wave's DMAs: number q = C wave + i of the 2 IPT of a tile, K's first
+    const bool isk = C * wave < IPT;  // (a wave's DMAs are all K's or all V's)
+    const int ld = (int)(isk ? a.ldk : a.ldv), row = C * wave - (isk ? 0 : IPT);
+    const bf16 *src = (const bf16 *)(isk ? a.k : a.v) + key0 * ld + kvh * HD;
+    const unsigned dst = lds_addr(isk ? Kt[0] : Vt[0]) + row * 1024;
     unsigned off[C];
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-        const int q = C * wave + i;
-        off[i] = dma_off<HD>(q % IPT * RPI, lane, (int)(q < IPT ? a.ldk : a.ldv));
-    }
+    for (int i = 0; i < C; ++i) off[i] = dma_off<HD>((row + i) * RPI, lane, ld);
     wait_vm0();  // Q fragments are in registers before any DMA is queued
     auto dma = [&](int it, int buf) {
-        const int k0 = kt.tile(KG * it + kg) * BN, rows = min(BN, s.kl - k0);
-        const bool isk = C * wave < IPT;  // (a wave's DMAs are all K's or all V's)
-        const sgpr4 rs = head_rows<HD>(isk ? a.k : a.v, key0 + k0, isk ? a.ldk : a.ldv, kvh * HD, rows);
-        char *dst = isk ? Kt[buf] + C * wave * 1024 : Vt[buf] + (C * wave - IPT) * 1024;
+        const int k0 = kt.tile(KG * it + kg) * BN;
+        const sgpr4 rs = rsrc4(src + (long)k0 * ld, (unsigned)(((min(BN, s.kl - k0) - 1) * ld + HD) * 2));
 #pragma unroll
-        for (int i = 0; i < C; ++i) dma16_async(rs, dst + i * 1024, off[i]);
+        for (int i = 0; i < C; ++i) dma16_at(rs, dst + buf * TILE + i * 1024, off[i]);
     };
     static_assert(IPT % C == 0, "a wave's DMAs are of one tensor");
     f32x4 oacc[QS][DSUB], st[KS][QS];
@@ -188,10 +205,10 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 2 : HD == 64 && QS == 2 ? 4 : 3
         if (it + 2 < n) dma(it + 2, (buf + 2) % NBUF);
         if (KG > 1 && it >= n) return;
         const char *Kb = Kt[buf], *Vb = Vt[buf];
-        if (!all_seen(a, kt.ta, kt.tb, k0, k0 + BN - 1) && scan<TILE, 256>(Vb, tid)) odd = true;
-        if (none_seen(a, wta, wtb, k0, k0 + BN - 1)) return;
+        if (!block.whole(KG * it + kg) && scan<TILE, 256>(Vb, tid)) odd = true;
+        if (mine.none(KG * it + kg)) return;
         scores(Kb, st);
-        if (!whole || !all_seen(a, wta, wtb, k0, k0 + BN - 1)) {
+        if (!mine.whole(KG * it + kg)) {
 #pragma unroll
             for (int qs = 0; qs < QS; ++qs) for_hidden<KS>(a, pos[qs], k0, g, [&](int ks, int r) { st[ks][qs][r] = -INFINITY; });
         }
@@ -489,6 +506,8 @@ __global__ __launch_bounds__(256 * KG, 2) void window_dq16_k(WindowArgs a) {
     const KeyTiles kt = key_tiles<BN>(a, s, r0, r0 + BQ);
     const int steps = (kt.n + KG - 1) / KG, nt = (kt.n - kg + KG - 1) / KG;  // the block's; the group's
     const int wta = max(0, qw0 + s.off), wtb = min(qw0 + 16 * QSUB, s.ql) - 1 + s.off;
+    Reach mine = reach<BN>(a, kt, wta, wtb);
+    const Reach block = reach<BN>(a, kt, kt.ta, kt.tb);
     const float c2 = a.scale * LOG2E;
     const long row0 = (long)b * a.n_q, key0 = (long)b * a.n_kv;
 
@@ -523,25 +542,26 @@ __global__ __launch_bounds__(256 * KG, 2) void window_dq16_k(WindowArgs a) {
         dd[j] = (float)acc;
         if (r < a.n_q && g == 0 && kg == 0) a.d[t * a.n_heads + h] = dd[j];
     }
+    bool live = true;
+#pragma unroll
+    for (int j = 0; j < QSUB; ++j) live = live && pos[j] >= 0;
+    if (!__all(live)) mine.n_all = mine.n_sink_all = 0;  // rows of no gradient
     // the wave's DMAs: number q = C wave + i of the 2 IPT of a tile, K's first
+    const bool isk = C * wave < IPT;  // (a wave's DMAs are all K's or all V's)
+    const int ld = (int)(isk ? a.ldk : a.ldv), row = C * wave - (isk ? 0 : IPT);
+    const bf16 *src = (const bf16 *)(isk ? a.k : a.v) + key0 * ld + kvh * HD;
+    const unsigned dst = lds_addr(isk ? Kt[0] : Vt[0]) + row * 1024;
     unsigned off[C];
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-        const int q = C * wave + i;
-        off[i] = dma_off<HD>(q % IPT * RPI, lane, (int)(q < IPT ? a.ldk : a.ldv));
-    }
+    for (int i = 0; i < C; ++i) off[i] = dma_off<HD>((row + i) * RPI, lane, ld);
     wait_vm0();
     auto dma = [&](int it, int buf) {
-        const int k0 = kt.tile(KG * it + kg) * BN, rows = min(BN, s.kl - k0);
-        const sgpr4 rk = head_rows<HD>(a.k, key0 + k0, a.ldk, kvh * HD, rows);
-        const sgpr4 rv = head_rows<HD>(a.v, key0 + k0, a.ldv, kvh * HD, rows);
+        const int k0 = kt.tile(KG * it + kg) * BN;
+        const sgpr4 rs = rsrc4(src + (long)k0 * ld, (unsigned)(((min(BN, s.kl - k0) - 1) * ld + HD) * 2));
 #pragma unroll
-        for (int i = 0; i < C; ++i) {
-            const int q = C * wave + i;
-            if (q < IPT) dma16_async(rk, Kt[buf] + q * 1024, off[i]);
-            else dma16_async(rv, Vt[buf] + (q - IPT) * 1024, off[i]);
-        }
+        for (int i = 0; i < C; ++i) dma16_at(rs, dst + buf * TILE + i * 1024, off[i]);
     };
+    static_assert(IPT % C == 0, "a wave's DMAs are of one tensor");
     f32x4 acc[QSUB][DSUB];
 #pragma unroll
     for (int j = 0; j < QSUB; ++j)
@@ -560,10 +580,8 @@ __global__ __launch_bounds__(256 * KG, 2) void window_dq16_k(WindowArgs a) {
         if (KG > 1 && it >= nt) return;
         const int k0 = kt.tile(KG * it + kg) * BN;
         const char *Kb = Kt[buf], *Vb = Vt[buf];
-        if (!all_seen(a, kt.ta, kt.tb, k0, k0 + BN - 1)) {
-            if (scan<TILE, NWV * 64>(Kb, tid)) odd = true;
-        }
-        if (none_seen(a, wta, wtb, k0, k0 + BN - 1)) return;
+        if (!block.whole(KG * it + kg) && scan<TILE, NWV * 64>(Kb, tid)) odd = true;
+        if (mine.none(KG * it + kg)) return;
         // the dP^T accumulators start at -D (one query per lane), so they end as dP^T - D
         f32x4 st[KS][QSUB], dpt[KS][QSUB];
 #pragma unroll
@@ -606,11 +624,7 @@ __global__ __launch_bounds__(256 * KG, 2) void window_dq16_k(WindowArgs a) {
                     st[ks2][j2][r] = __builtin_amdgcn_exp2f(fmaf(st[ks2][j2][r], c2, -lq[j2]));
             }
         }
-        bool whole = all_seen(a, wta, wtb, k0, k0 + BN - 1);
-        bool live = true;
-#pragma unroll
-        for (int j = 0; j < QSUB; ++j) live = live && pos[j] >= 0;
-        whole = whole && __all(live);
+        const bool whole = mine.whole(KG * it + kg);
         bf16x8 sb[QSUB];
 #pragma unroll
         for (int j = 0; j < QSUB; ++j) {

@@ -76,6 +76,27 @@ VKH_DEV KeyTiles key_tiles(const WindowArgs &a, const Span &s, int r0, int r1) {
     return k;
 }
 
+// Which of those tiles some, and which all, of the positions ta .. tb among the block's see.  (Tiles of
+// sinks that all see without being of sinks only are taken as not whole: they are masked.)
+struct Reach {
+    int n_sink, some0, some1, all0, n_all, n_sink_all;
+    VKH_DEV bool none(int it) const { return it >= some1 || (it < some0 && it >= n_sink); }
+    VKH_DEV bool whole(int it) const { return (unsigned)(it - all0) < (unsigned)n_all || it < n_sink_all; }
+};
+template <int BN>
+VKH_DEV Reach reach(const WindowArgs &a, const KeyTiles &k, int ta, int tb) {
+    const int to_it = k.n_sink - k.w0, last = (ta + 1) / BN;
+    const bool dead = tb < ta;
+    Reach r;
+    r.n_sink = k.n_sink;
+    r.some0 = a.n_sink > k.w0 * BN ? 0 : max(0, ta - a.window + 1) / BN + to_it;
+    r.some1 = dead ? 0 : tb / BN + 1 + to_it;
+    r.all0 = (int)((max(0, tb - a.window + 1) + (unsigned)BN - 1) / BN) + to_it;
+    r.n_all = dead ? 0 : max(0, last + to_it - r.all0);
+    r.n_sink_all = dead ? 0 : min(k.n_sink, a.n_sink / BN);
+    return r;
+}
+
 // A kernel's first argument, read anew from where the launch put it (the kernel arguments begin
 // with it): its values need not stay in registers for the calls below.
 VKH_DEV const WindowArgs &args_again() {
