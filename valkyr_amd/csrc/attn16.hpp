@@ -1,4 +1,4 @@
-// Pieces of the windowed bf16 attention kernels: LDS tiles of head rows and their MFMA fragments.
+// Pieces of the windowed attention's tile kernels: LDS tiles of head rows and their MFMA fragments.
 #pragma once
 
 #include "gemm16.hpp"
@@ -34,6 +34,19 @@ VKH_DEV float xrow_sum(float v) {
     lane_halves<16>(v, a, b);
     lane_halves<32>(a + b, a, b);
     return a + b;
+}
+
+// The DMA to a wave-uniform LDS address that the caller keeps as a number.
+VKH_DEV unsigned lds_addr(const char *p) {
+    return __builtin_amdgcn_readfirstlane((int)(unsigned)(unsigned long)(const __attribute__((address_space(3))) char *)p);
+}
+VKH_DEV void dma16_at(const sgpr4 &rs, unsigned lds, unsigned voff) {
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(voff), "s"(rs) : "memory");
+}
+
+template <int N>
+VKH_DEV void wait_vm() {
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4 << 14));
 }
 
 // LDS tiles of bf16 head rows of HD values, as the DMA writes them: 16-byte chunk c of row r at

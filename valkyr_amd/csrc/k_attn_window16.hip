@@ -38,26 +38,6 @@ VKH_DEV bool scan(const char *lds, int tid) {
         }
     return carry & 0x80008000u;
 }
-// hide(ks, r) for the keys k0 + 16 ks + 4 g + r, ks < KS, that position t does not see.
-template <int KS, class F>
-VKH_DEV void for_hidden(const WindowArgs &a, int t, int k0, int g, F hide) {
-    int x = t - k0 - 4 * g;
-    if (k0 < a.n_sink && k0 + 16 * KS > a.n_sink) {  // sinks and others: the others outside the window
-        const int ns = a.n_sink - k0 - 4 * g;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (16 * ks + r >= ns && x - 16 * ks - r >= a.window) hide(ks, r);
-    }
-    asm("" : "+v"(x));  // (the differences below are not kept from those above)
-    const unsigned reach = k0 < a.n_sink ? kAll : a.window;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if ((unsigned)(x - 16 * ks - r) >= reach) hide(ks, r);
-}
 
 // The resource of rows row0 .. row0 + rows - 1 of one head (rows <= 0: of none).
 template <int HD>
@@ -69,14 +49,6 @@ template <int HD>
 VKH_DEV unsigned dma_off(int r0, int lane, int ld) {
     const int r = r0 + lane / (HD / 8), c = (lane % (HD / 8)) ^ TileRows<HD>::swz(r);
     return (unsigned)((r * ld + 8 * c) * 2);
-}
-
-// The DMA to a wave-uniform LDS address that the caller keeps as a number.
-VKH_DEV unsigned lds_addr(const char *p) {
-    return __builtin_amdgcn_readfirstlane((int)(unsigned)(unsigned long)(const __attribute__((address_space(3))) char *)p);
-}
-VKH_DEV void dma16_at(const sgpr4 &rs, unsigned lds, unsigned voff) {
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(voff), "s"(rs) : "memory");
 }
 
 // A block's rows one at a time, for blocks that met an infinity or a NaN in a tile which some of
@@ -106,11 +78,6 @@ __device__ __attribute__((noinline)) void dkv_rows(const WindowArgs &a, const St
         else window_dkv_row<bf16>(a, b, k0 + x, kvh, k, v, (TO *)a.dk + row * a.lddk + kvh * HD,
                                   (TO *)a.dv + row * a.lddv + kvh * HD, lane, mine);
     }
-}
-
-template <int N>
-VKH_DEV void wait_vm() {
-    __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4 << 14));
 }
 
 // ── forward ──────────────────────────────────────────────────────────────

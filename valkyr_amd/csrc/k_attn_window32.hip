@@ -31,36 +31,66 @@ VKH_DEV f32x4 mfma4(const float4 &a, const float4 &b, f32x4 c) {
     c = mfma16x16x4(a.z, b.z, c);
     return mfma16x16x4(a.w, b.w, c);
 }
-VKH_DEV float xmax(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
-}
-VKH_DEV float xsum(float v) {
-    v += __shfl_xor(v, 16, 64);
-    return v + __shfl_xor(v, 32, 64);
+// LDS tiles of FT head rows as the DMA writes them: 16-byte chunk n of row r at chunk n ^ (r & 15), so
+// that the 16 rows of a fragment read lie in 16 different chunk columns of LDS's 256 bytes a cycle.
+template <int HD>
+struct Rows32 {
+    static constexpr int TILE = FT * HD, RPI = 256 / HD, IPT = FT / RPI;  // floats; rows a DMA of 1 KB; DMAs
+    int row[4], col[4];  // a lane's offsets: of values 16 u + 4 g .. of row c (u % 4), of values 4 c .. of row 4 g + e
+    VKH_DEV Rows32(int g, int c) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            row[x] = c * HD + 4 * ((4 * x + g) ^ c);
+            col[x] = (4 * g + x) * HD + 4 * (c ^ (4 * g + x));
+        }
+    }
+    // a lane's byte offset in a tile's DMA number q
+    static VKH_DEV unsigned dma(int q, int lane, int ld) {
+        const int r = q * RPI + lane / (HD / 4), n = (lane % (HD / 4)) ^ (r & 15);
+        return (unsigned)((r * ld + 4 * n) * 4);
+    }
+    static VKH_DEV unsigned bytes(int rows, int ld) { return rows > 0 ? (unsigned)(((min(rows, FT) - 1) * ld + HD) * 4) : 0u; }
+};
+// Whether a group of 256 threads' tile holds an infinity or a NaN (exponent bits of all ones, to which
+// one more carries into the sign's place): each thread's share.
+template <int HD>
+VKH_DEV bool scan32(const float *tile, int tid) {
+    unsigned carry = 0;
+#pragma unroll
+    for (int i = 0; i < FT * HD / 1024; ++i) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(tile + (i * 256 + tid) * 4);
+        carry |= ((v.x & 0x7f800000u) + 0x00800000u) | ((v.y & 0x7f800000u) + 0x00800000u);
+        carry |= ((v.z & 0x7f800000u) + 0x00800000u) | ((v.w & 0x7f800000u) + 0x00800000u);
+    }
+    return carry & 0x80000000u;
 }
 template <int NU>
-VKH_DEV f32x4 head_dot(const float *row, const float4 (&f)[NU]) {
-    f32x4 a[NU] = {};
-#pragma unroll
-    for (int u = 0; u < NU; ++u) a[u] = mfma4(f4(row + 16 * u), f[u], a[u]);
+VKH_DEV f32x4 chains(f32x4 (&a)[NU]) {
 #pragma unroll
     for (int w = NU / 2; w; w /= 2)
 #pragma unroll
         for (int u = 0; u < w; ++u) a[u] += a[u + w];
     return a[0];
 }
-
-// acc += T^T w over 16 rows of an LDS tile: element e of w is row 4 g + e (row0 points at the lane's row
-// 4 g).  Matrix row i of acc[4 J + j] is column 64 J + 4 i + j of the tile, so that one 16-byte read
-// feeds four products (a 4-byte read for each left them waiting on LDS: see acc_cols for the way back).
-template <int NU>
-VKH_DEV void add_rows(f32x4 (&acc)[NU], const float *row0, int P, int c, const f32x4 &w) {
+// the lane's element of 16 tile rows' products with its column of f
+template <int HD>
+VKH_DEV f32x4 head_dot(const float *tile, const Rows32<HD> &t, const float4 (&f)[HD / 16]) {
+    constexpr int NU = HD / 16;
+    f32x4 a[NU] = {};
+#pragma unroll
+    for (int u = 0; u < NU; ++u) a[u] = mfma4(f4(tile + t.row[u % 4] + 64 * (u / 4)), f[u], a[u]);
+    return chains(a);
+}
+// acc += T^T w over 16 rows of an LDS tile: element e of w is row 4 g + e.  Matrix row i of acc[4 J + j]
+// is column 64 J + 4 i + j of the tile, so that one 16-byte read feeds four products (a 4-byte read for
+// each left them waiting on LDS: see acc_cols for the way back).  `at(e)` is values 4 c .. of row 4 g + e.
+template <int NU, class At>
+VKH_DEV void add_rows_at(f32x4 (&acc)[NU], At at, const f32x4 &w) {
 #pragma unroll
     for (int J = 0; J < NU / 4; ++J) {
         float4 t[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) t[e] = f4(row0 + e * P + 64 * J + 4 * c);
+        for (int e = 0; e < 4; ++e) t[e] = f4(at(e) + 64 * J);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             acc[4 * J] = mfma16x16x4(t[e].x, w[e], acc[4 * J]);
@@ -70,6 +100,13 @@ VKH_DEV void add_rows(f32x4 (&acc)[NU], const float *row0, int P, int c, const f
         }
     }
 }
+template <int HD>
+VKH_DEV void add_rows(f32x4 (&acc)[HD / 16], const float *tile, const Rows32<HD> &t, const f32x4 &w) {
+    add_rows_at(acc, [&](int e) { return tile + t.col[e]; }, w);
+}
+// e^x with one rounding more than the instruction's: that of x log2(e), relative to x
+VKH_DEV float exp_(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
+
 // Four columns of the lane's item: f(first column, their values) for columns 64 J + 16 g + 4 r.
 template <int NU, class F>
 VKH_DEV void acc_cols(const f32x4 (&acc)[NU], int g, F f) {
@@ -137,9 +174,9 @@ __device__ __attribute__((noinline)) void dkv_rows32(const WindowArgs &a, const 
 // tokens, window 256, 16 / 4 heads of 64: 256 blocks, 33 us with one group).
 template <int HD, int KG>
 __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_fwd32_k(WindowArgs a) {
-    using T = Tile32<HD, FT, 256>;
-    constexpr int P = T::P, NU = HD / 16;
-    __shared__ __attribute__((aligned(16))) float tiles[KG][2][2][FT * P];  // [group][K, V][buffer]
+    using T = Rows32<HD>;
+    constexpr int NU = HD / 16, TILE = T::TILE, C = T::IPT / 2;  // DMAs per wave and step
+    __shared__ __attribute__((aligned(16))) float tiles[KG][2][2][TILE];  // [group][buffer][K, V]
     const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, nqt = (a.n_q + 63) / 64;
     const Pair pr = pair_of(blockIdx.x, gridDim.x, nbk, 4 * grp);
     const int b = pr.bk / a.n_kv_heads, kvh = pr.bk % a.n_kv_heads, h = kvh * grp + pr.y % grp, qt = nqt - 1 - pr.y / grp;
@@ -151,81 +188,101 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_fwd32_k(Wind
     const int wta = max(0, qw + s.off), wtb = min(qw + 16, s.ql) - 1 + s.off;
     const int pos = r < s.ql ? max(-1, r + s.off) : -1;
     const long row = (long)b * a.n_q + r;
-    const float *kb = (const float *)a.k + (long)b * a.n_kv * a.ldk + kvh * HD;
-    const float *vb = (const float *)a.v + (long)b * a.n_kv * a.ldv + kvh * HD;
-    T tk, tv;
-    auto load = [&](int it) {
-        const int k0 = kt.tile(it) * FT;
-        tk.load(kb + (long)k0 * a.ldk, a.ldk, tid, s.kl - k0);
-        tv.load(vb + (long)k0 * a.ldv, a.ldv, tid, s.kl - k0);
-    };
-    bool odd = false;  // in V of a tile that is not seen in full
-    auto store = [&](int it, int buf) {
-        const int k0 = kt.tile(it) * FT;
-        if (!all_seen(a, kt.ta, kt.tb, k0, k0 + FT - 1)) odd |= tv.odd();
-        tk.store(tiles[kg][0][buf], tid);
-        tv.store(tiles[kg][1][buf], tid);
-    };
-    if (kg < kt.n) load(kg);
+    Reach mine = reach<FT>(a, kt, wta, wtb);
+    if (qw + 16 > s.ql || qw + s.off < 0) mine.n_all = mine.n_sink_all = 0;  // rows that are not there
+    const Reach block = reach<FT>(a, kt, kt.ta, kt.tb);
+    const int steps = (kt.n + KG - 1) / KG, n = (kt.n - kg + KG - 1) / KG;  // the block's; the group's
     float4 qf[NU];
 #pragma unroll
     for (int u = 0; u < NU; ++u)
         qf[u] = pos >= 0 ? f4((const float *)a.q + row * a.ldq + h * HD + 4 * g + 16 * u) : make_float4(0.f, 0.f, 0.f, 0.f);
-    if (kg < kt.n) store(kg, 0);
-    __syncthreads();
+    // waves 0 and 1 move K, 2 and 3 V
+    const int ld = (int)(wave < 2 ? a.ldk : a.ldv);
+    const float *src = (const float *)(wave < 2 ? a.k : a.v) + (long)b * a.n_kv * ld + kvh * HD;
+    const unsigned dst = lds_addr((const char *)tiles[kg][0][wave / 2]) + wave % 2 * C * 1024;
+    unsigned off[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) off[i] = T::dma(wave % 2 * C + i, lane, ld);
+    wait_vm0();  // Q is in registers before any DMA is queued
+    auto dma = [&](int it, int buf) {
+        const int k0 = kt.tile(KG * it + kg) * FT;
+        const sgpr4 rs = rsrc4(src + (long)k0 * ld, T::bytes(s.kl - k0, ld));
+#pragma unroll
+        for (int i = 0; i < C; ++i) dma16_at(rs, dst + buf * 2 * TILE * 4 + i * 1024, off[i]);
+    };
+    const T t(g, c);
+    const float c2 = a.scale * LOG2E;
     f32x4 ot[NU];  // O^T, columns as acc_cols has them
 #pragma unroll
     for (int j = 0; j < NU; ++j) ot[j] = f32x4{0, 0, 0, 0};
-    float m = -INFINITY, l = 0.f;  // running maximum; this lane's share of the sum
-    auto step = [&](int it, int buf) {
-        const int k0 = kt.tile(it) * FT;
-        const float *Kl = tiles[kg][0][buf], *Vl = tiles[kg][1][buf];
+    float m = -INFINITY, l = 0.f;  // running maximum of q k; this lane's share of the sum
+    bool odd = false;              // in V of a tile that is not seen in full
+    if (n > 0) dma(0, 0);
+    auto step = [&](const int it, auto bufc) {
+        constexpr int buf = decltype(bufc)::value;
+        wait_vm0();
+        lds_barrier();  // tile it landed; everyone is done with tile it - 1
+        if (it + 1 < n) dma(it + 1, buf ^ 1);
+        if (KG > 1 && it >= n) return;
+        const float *Kl = tiles[kg][buf][0], *Vl = tiles[kg][buf][1];
+        const int tile = KG * it + kg;
+        if (!block.whole(tile) && scan32<HD>(Vl, tid)) odd = true;
+        if (mine.none(tile)) return;
+        const int k0 = kt.tile(tile) * FT;
         f32x4 st[2];
-        bool live[2];
-        float tmax = -INFINITY;
+        bool live[2] = {true, true};
+        if (mine.whole(tile)) {
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            live[ks] = !none_seen(a, wta, wtb, k0 + 16 * ks, k0 + 16 * ks + 15);  // wave-uniform
-            st[ks] = f32x4{0, 0, 0, 0};
-            if (live[ks]) st[ks] = head_dot<NU>(Kl + (16 * ks + c) * P + 4 * g, qf) * a.scale;
+            for (int ks = 0; ks < 2; ++ks) st[ks] = head_dot<HD>(Kl + 16 * ks * HD, t, qf);
+        } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (!sees(a, pos, k0 + 16 * ks + 4 * g + e)) st[ks][e] = -INFINITY;
-                tmax = fmaxf(tmax, st[ks][e]);
+            for (int ks = 0; ks < 2; ++ks) {
+                live[ks] = !none_seen(a, wta, wtb, k0 + 16 * ks, k0 + 16 * ks + 15);  // wave-uniform
+                st[ks] = f32x4{0, 0, 0, 0};
+                if (live[ks]) st[ks] = head_dot<HD>(Kl + 16 * ks * HD, t, qf);
             }
+            for_hidden<2>(a, pos, k0, g, [&](int ks, int r) { st[ks][r] = -INFINITY; });
         }
-        const float mn = fmaxf(m, xmax(tmax)), ms = mn == -INFINITY ? 0.f : mn;
-        const float alpha = expf(m - ms);
-        l *= alpha;
+        // The maximum moves only when a row's scores pass it by more than 8 (in log2 units): P stays
+        // under 2^8, which fp32 holds as exactly.
+        float mt = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < NU; ++j) ot[j] *= alpha;
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mt = fmaxf(mt, st[ks][e]);
+        if (__any(m == -INFINITY ? mt > m : (mt - m) * c2 > 8.f)) {
+            const float mn = xrow_max(mt), mo = m;
+            if (mo == -INFINITY || (mn - mo) * c2 > 8.f) m = mn;
+            const float alpha = m == mo ? 1.f : __builtin_amdgcn_exp2f((mo - m) * c2);
+            l *= alpha;
+#pragma unroll
+            for (int j = 0; j < NU; ++j) ot[j] *= alpha;
+        }
+        const float ms = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                st[ks][e] = expf(st[ks][e] - ms);
+                st[ks][e] = __builtin_amdgcn_exp2f((st[ks][e] - ms) * c2);
                 l += st[ks][e];
             }
-        m = mn;
         // O^T += V^T P^T
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
-            if (live[ks]) add_rows<NU>(ot, Vl + (16 * ks + 4 * g) * P, P, c, st[ks]);
+            if (live[ks]) add_rows<HD>(ot, Vl + 16 * ks * HD, t, st[ks]);
     };
-    for (int it = kg, buf = 0; it - kg < kt.n; it += KG, buf ^= 1) {
-        if (it + KG < kt.n) load(it + KG);
-        if (it < kt.n) step(it, buf);
-        if (it + KG < kt.n) store(it + KG, buf ^ 1);  // last read before the previous barrier
-        __syncthreads();
+    for (int it0 = 0; it0 < steps; it0 += 2) {
+        step(it0, std::integral_constant<int, 0>{});
+        if (it0 + 1 < steps) step(it0 + 1, std::integral_constant<int, 1>{});
     }
     if (__syncthreads_or(odd)) {
         if (kg == 0) fwd_rows32(args_again(), b, r0 + wave, min(r0 + 64, a.n_q), h, tiles[0][0][0] + wave * HD, lane);
         return;
     }
-    l = xsum(l);
+    l = xrow_sum(l);
     if constexpr (KG > 1) {  // the groups' results, joined in order through LDS
         constexpr int W = (NU + 1) * 4 * 64;  // floats of a wave's result: columns of 64 lanes
-        static_assert(4 * W <= 4 * FT * P, "a group's results fit its tiles");
+        static_assert(4 * W <= 4 * TILE, "a group's results fit its tiles");
         auto column = [&](int k, int j) { return reinterpret_cast<f32x4 *>(tiles[k][0][0] + wave * W + j * 256) + lane; };
         if (kg) {
 #pragma unroll
@@ -237,7 +294,8 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_fwd32_k(Wind
 #pragma unroll
         for (int k = 1; k < KG; ++k) {
             const f32x4 st = *column(k, NU);
-            const float mn = fmaxf(m, st[0]), ms = mn == -INFINITY ? 0.f : mn, f0 = expf(m - ms), f1 = expf(st[0] - ms);
+            const float mn = fmaxf(m, st[0]), ms = mn == -INFINITY ? 0.f : mn;
+            const float f0 = __builtin_amdgcn_exp2f((m - ms) * c2), f1 = __builtin_amdgcn_exp2f((st[0] - ms) * c2);
             m = mn;
             l = l * f0 + st[1] * f1;
 #pragma unroll
@@ -252,7 +310,7 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_fwd32_k(Wind
         x = dead ? f32x4{0, 0, 0, 0} : x * inv;
         store4(o + d, x[0], x[1], x[2], x[3]);
     });
-    if (a.lse && g == 0) a.lse[row * a.n_heads + h] = dead ? -INFINITY : m + logf(l);
+    if (a.lse && g == 0) a.lse[row * a.n_heads + h] = dead ? -INFINITY : fmaf(m, a.scale, logf(l));
 }
 
 // ── forward of a few rows ────────────────────────────────────────────────
@@ -303,14 +361,17 @@ __global__ __launch_bounds__(FNT, 2) void window_step32_k(WindowArgs a, int spli
         tv.store(Vl, lane);
         if (it + 4 < last) load(it + 4);
         wave_lds();
-        f32x4 st = head_dot<NU>(Kl + c * P + 4 * g, qf) * c2;
+        f32x4 a0[NU] = {};
+#pragma unroll
+        for (int u = 0; u < NU; ++u) a0[u] = mfma4(f4(Kl + c * P + 4 * g + 16 * u), qf[u], a0[u]);
+        f32x4 st = chains(a0) * c2;
         float mt = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (!sees(a, pos, k0 + 4 * g + e)) st[e] = -INFINITY;
             mt = fmaxf(mt, st[e]);
         }
-        const float mn = fmaxf(m, xmax(mt)), ms = mn == -INFINITY ? 0.f : mn;
+        const float mn = fmaxf(m, xrow_max(mt)), ms = mn == -INFINITY ? 0.f : mn;
         const float so = __builtin_amdgcn_exp2f(m - ms);
         m = mn;
         l *= so;
@@ -336,11 +397,11 @@ __global__ __launch_bounds__(FNT, 2) void window_step32_k(WindowArgs a, int spli
                 }
             continue;
         }
-        add_rows<NU>(acc, Vl + 4 * g * P, P, c, st);
+        add_rows_at(acc, [&](int e) { return Vl + (4 * g + e) * P + 4 * c; }, st);
     }
     wave_lds();
     float *res = tiles[wave][0];  // rows of P floats
-    const float lt = xsum(l);
+    const float lt = xrow_sum(l);
     acc_cols<NU>(acc, g, [&](int d, f32x4 x) { *reinterpret_cast<f32x4 *>(res + c * P + d) = x; });
     if (g == 0) ml[wave][0][c] = m, ml[wave][1][c] = lt;
     __syncthreads();
@@ -386,9 +447,9 @@ __global__ __launch_bounds__(FNT, 2) void window_step32_k(WindowArgs a, int spli
 // Key groups as in the forward.
 template <int HD, int KG>
 __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_dq32_k(WindowArgs a) {
-    using T = Tile32<HD, FT, 256>;
-    constexpr int P = T::P, NU = HD / 16;
-    __shared__ __attribute__((aligned(16))) float tiles[KG][2][2][FT * P];  // [group][K, V][buffer]
+    using T = Rows32<HD>;
+    constexpr int NU = HD / 16, TILE = T::TILE, C = T::IPT / 2;
+    __shared__ __attribute__((aligned(16))) float tiles[KG][2][2][TILE];  // [group][buffer][K, V]
     const int nbk = a.n_batch * a.n_kv_heads, grp = a.n_heads / a.n_kv_heads, nqt = (a.n_q + 63) / 64;
     const Pair pr = pair_of(blockIdx.x, gridDim.x, nbk, 4 * grp);
     const int b = pr.bk / a.n_kv_heads, kvh = pr.bk % a.n_kv_heads, h = kvh * grp + pr.y % grp, qt = nqt - 1 - pr.y / grp;
@@ -401,22 +462,6 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_dq32_k(Windo
     const long row = (long)b * a.n_q + r;
     const float lse = r < s.ql && r + s.off >= 0 ? a.lse[row * a.n_heads + h] : -INFINITY;
     const int pos = lse == -INFINITY ? -1 : r + s.off;
-    const float *kb = (const float *)a.k + (long)b * a.n_kv * a.ldk + kvh * HD;
-    const float *vb = (const float *)a.v + (long)b * a.n_kv * a.ldv + kvh * HD;
-    T tk, tv;
-    auto load = [&](int it) {
-        const int k0 = kt.tile(it) * FT;
-        tk.load(kb + (long)k0 * a.ldk, a.ldk, tid, s.kl - k0);
-        tv.load(vb + (long)k0 * a.ldv, a.ldv, tid, s.kl - k0);
-    };
-    bool odd = false;  // in K of a tile that is not seen in full
-    auto store = [&](int it, int buf) {
-        const int k0 = kt.tile(it) * FT;
-        if (!all_seen(a, kt.ta, kt.tb, k0, k0 + FT - 1)) odd |= tk.odd();
-        tk.store(tiles[kg][0][buf], tid);
-        tv.store(tiles[kg][1][buf], tid);
-    };
-    if (kg < kt.n) load(kg);
     float4 qf[NU], of[NU];
     double acc = 0;
 #pragma unroll
@@ -434,38 +479,61 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_dq32_k(Windo
     acc += __shfl_xor(acc, 32, 64);
     const float dd = (float)acc;
     if (kg == 0 && r < a.n_q && g == 0) a.d[row * a.n_heads + h] = dd;
-    if (kg < kt.n) store(kg, 0);
-    __syncthreads();
+    Reach mine = reach<FT>(a, kt, wta, wtb);
+    if (!__all(pos >= 0)) mine.n_all = mine.n_sink_all = 0;  // rows of no gradient
+    const Reach block = reach<FT>(a, kt, kt.ta, kt.tb);
+    const int steps = (kt.n + KG - 1) / KG, n = (kt.n - kg + KG - 1) / KG;
+    const int ld = (int)(wave < 2 ? a.ldk : a.ldv);
+    const float *src = (const float *)(wave < 2 ? a.k : a.v) + (long)b * a.n_kv * ld + kvh * HD;
+    const unsigned dst = lds_addr((const char *)tiles[kg][0][wave / 2]) + wave % 2 * C * 1024;
+    unsigned off[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) off[i] = T::dma(wave % 2 * C + i, lane, ld);
+    wait_vm0();
+    auto dma = [&](int it, int buf) {
+        const int k0 = kt.tile(KG * it + kg) * FT;
+        const sgpr4 rs = rsrc4(src + (long)k0 * ld, T::bytes(s.kl - k0, ld));
+#pragma unroll
+        for (int i = 0; i < C; ++i) dma16_at(rs, dst + buf * 2 * TILE * 4 + i * 1024, off[i]);
+    };
+    const T t(g, c);
     f32x4 dqt[NU];
 #pragma unroll
     for (int j = 0; j < NU; ++j) dqt[j] = f32x4{0, 0, 0, 0};
-    auto step = [&](int it, int buf) {
-        const int k0 = kt.tile(it) * FT;
-        const float *Kl = tiles[kg][0][buf], *Vl = tiles[kg][1][buf];
+    bool odd = false;  // in K of a tile that is not seen in full
+    if (n > 0) dma(0, 0);
+    auto step = [&](const int it, auto bufc) {
+        constexpr int buf = decltype(bufc)::value;
+        wait_vm0();
+        lds_barrier();
+        if (it + 1 < n) dma(it + 1, buf ^ 1);
+        if (KG > 1 && it >= n) return;
+        const float *Kl = tiles[kg][buf][0], *Vl = tiles[kg][buf][1];
+        const int tile = KG * it + kg;
+        if (!block.whole(tile) && scan32<HD>(Kl, tid)) odd = true;
+        if (mine.none(tile)) return;
+        const int k0 = kt.tile(tile) * FT;
+        const bool whole = mine.whole(tile);
         f32x4 da[2];
         bool live[2];
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-            live[ks] = !none_seen(a, wta, wtb, k0 + 16 * ks, k0 + 16 * ks + 15);  // wave-uniform
+            live[ks] = whole || !none_seen(a, wta, wtb, k0 + 16 * ks, k0 + 16 * ks + 15);  // wave-uniform
             da[ks] = f32x4{0, 0, 0, 0};
             if (!live[ks]) continue;
-            const f32x4 sa = head_dot<NU>(Kl + (16 * ks + c) * P + 4 * g, qf);
-            da[ks] = head_dot<NU>(Vl + (16 * ks + c) * P + 4 * g, of);
+            const f32x4 sa = head_dot<HD>(Kl + 16 * ks * HD, t, qf);
+            da[ks] = head_dot<HD>(Vl + 16 * ks * HD, t, of);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float p = expf(fmaf(sa[e], a.scale, -lse));
-                da[ks][e] = sees(a, pos, k0 + 16 * ks + 4 * g + e) ? p * (da[ks][e] - dd) : 0.f;
-            }
+            for (int e = 0; e < 4; ++e) da[ks][e] = exp_(fmaf(sa[e], a.scale, -lse)) * (da[ks][e] - dd);
         }
+        if (!whole) for_hidden<2>(a, pos, k0, g, [&](int ks, int r) { da[ks][r] = 0.f; });
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
-            if (live[ks]) add_rows<NU>(dqt, Kl + (16 * ks + 4 * g) * P, P, c, da[ks]);
+            if (live[ks]) add_rows<HD>(dqt, Kl + 16 * ks * HD, t, da[ks]);
     };
-    for (int it = kg, buf = 0; it - kg < kt.n; it += KG, buf ^= 1) {
-        if (it + KG < kt.n) load(it + KG);
-        if (it < kt.n) step(it, buf);
-        if (it + KG < kt.n) store(it + KG, buf ^ 1);
-        __syncthreads();
+    for (int it0 = 0; it0 < steps; it0 += 2) {
+        step(it0, std::integral_constant<int, 0>{});
+        if (it0 + 1 < steps) step(it0 + 1, std::integral_constant<int, 1>{});
     }
     if (__syncthreads_or(odd)) {
         float *sh = tiles[0][0][0] + wave * 2 * HD;
@@ -497,10 +565,10 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_dq32_k(Windo
 // the block's steps each and add their sums at the end.
 template <int HD, int KG>
 __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_dkv32_k(WindowArgs a, DkvPlan plan) {
-    using T = Tile32<HD, FT, 256>;
-    constexpr int P = T::P, NU = HD / 16, BN = 64;
-    __shared__ __attribute__((aligned(16))) float tiles[KG][2][2][FT * P];  // [group][Q, dO][buffer]
-    __shared__ float Ls[KG][2][FT], Dl[KG][2][FT];
+    using T = Rows32<HD>;
+    constexpr int NU = HD / 16, BN = 64, TILE = T::TILE, C = T::IPT / 2;
+    __shared__ __attribute__((aligned(16))) float tiles[KG][2][2][TILE];  // [group][buffer][Q, dO]
+    __shared__ __attribute__((aligned(16))) float stat[KG][2][2][64];     // [group][buffer][LSE, D]
     const int nbk = a.n_batch * a.n_kv_heads;
     const Pair pr = pair_of(blockIdx.x, gridDim.x, nbk, 4);
     const int bk = pr.bk, b = bk / a.n_kv_heads, kvh = bk % a.n_kv_heads;
@@ -527,80 +595,96 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_dkv32_k(Wind
     const int qend = k0 < a.n_sink ? s.ql : (int)min((long)s.ql, (long)k1 + a.window - s.off);
     const int nqt = k1 >= k0 && qend > qstart ? (qend - qstart + FT - 1) / FT : 0;
     const int niter = max(0, (nh * nqt - zpart + zparts - 1) / zparts), top = nqt - 1;
-    auto tile_of = [&](int it, int &h, int &q0) {
-        it = it * zparts + zpart;
-        h = kvh * nh + it % nh;
-        q0 = qstart + (top - it / nh) * FT;
+    // The group's steps kg, kg + KG, ... of the block's zpart, zpart + zparts, ... of (query tile, head),
+    // heads inner: head and tile of one, moved on by steps of `stride`.
+    const int stride = KG * zparts, dh = stride % nh, dt = stride / nh;
+    struct Cursor {
+        int head, tile;
     };
-    T tq, to;
-    float stat = 0.f;  // LSE (threads 0..31) or D (32..63) of one tile row
-    auto load = [&](int it) {
-        int h, q0;
-        tile_of(it, h, q0);
-        const int rows = s.ql - q0;
-        tq.load((const float *)a.q + (row0 + q0) * a.ldq + h * HD, a.ldq, tid, rows);
-        to.load((const float *)a.dout + (row0 + q0) * a.lddo + h * HD, a.lddo, tid, rows);
-        if (tid < 2 * FT) {  // rows past the end: of no gradient, as rows of LSE = -inf
-            stat = tid < FT ? -INFINITY : 0.f;
-            if (tid % FT < rows) stat = (tid < FT ? a.lse : a.d)[(row0 + q0 + tid % FT) * a.n_heads + h];
+    auto advance = [&](Cursor &x) {
+        x.head += dh;
+        x.tile += dt;
+        if (x.head >= nh) x.head -= nh, ++x.tile;
+    };
+    const int x0 = kg * zparts + zpart;
+    Cursor ahead{x0 % nh, x0 / nh}, now = ahead;
+    const int steps = (niter + KG - 1) / KG, n = (niter - kg + KG - 1) / KG;  // the block's; the group's
+    // waves 0 and 1 move Q, 2 and 3 dO; 0 the rows' LSE too, 2 their D
+    const int ld = (int)(wave < 2 ? a.ldq : a.lddo);
+    const float *src = (const float *)(wave < 2 ? a.q : a.dout) + row0 * ld + kvh * nh * HD;
+    const float *stat_src = (wave < 2 ? a.lse : a.d) + row0 * a.n_heads + kvh * nh;
+    const unsigned dst = lds_addr((const char *)tiles[kg][0][wave / 2]) + wave % 2 * C * 1024;
+    const unsigned off_stat = lane < FT ? (unsigned)(lane * a.n_heads * 4) : kOOB;
+    unsigned off[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) off[i] = T::dma(wave % 2 * C + i, lane, ld);
+    wait_vm0();  // K and V are in registers before any DMA is queued
+    auto dma = [&](int buf) {
+        const int h = ahead.head, q0 = qstart + (top - ahead.tile) * FT, rows = s.ql - q0;
+        advance(ahead);
+        const sgpr4 rs = rsrc4(src + (long)q0 * ld + h * HD, T::bytes(rows, ld));
+#pragma unroll
+        for (int i = 0; i < C; ++i) dma16_at(rs, dst + buf * 2 * TILE * 4 + i * 1024, off[i]);
+        if (wave % 2 == 0) {
+            const sgpr4 r1 = rsrc4(stat_src + (long)q0 * a.n_heads + h, (unsigned)(((min(rows, FT) - 1) * a.n_heads + 1) * 4));
+            dma4_async(r1, stat[kg][buf][wave / 2], off_stat);
         }
     };
+    const T t(g, c);
     bool odd = false;  // in Q or dO of a tile whose rows do not all see all keys
-    auto store = [&](int it, int buf) {
-        int h, q0;
-        tile_of(it, h, q0);
-        const int ta = q0 + s.off, tb = min(q0 + FT, s.ql) - 1 + s.off;
-        if (!all_seen(a, ta, tb, k0, k0 + BN - 1)) odd |= tq.odd() || to.odd();
-        tq.store(tiles[kg][0][buf], tid);
-        to.store(tiles[kg][1][buf], tid);
-        if (tid < FT) Ls[kg][buf][tid] = stat;
-        else if (tid < 2 * FT) Dl[kg][buf][tid - FT] = stat;
-    };
     f32x4 dvt[NU], dkt[NU];
 #pragma unroll
     for (int j = 0; j < NU; ++j) dvt[j] = dkt[j] = f32x4{0, 0, 0, 0};
-    if (kg < niter) {
-        load(kg);
-        store(kg, 0);
-    }
-    __syncthreads();
-    auto step = [&](int it, int buf) {
-        int h, q0;
-        tile_of(it, h, q0);
-        const float *Ql = tiles[kg][0][buf], *Ol = tiles[kg][1][buf];
+    if (n > 0) dma(0);
+    auto step = [&](const int it, auto bufc) {
+        constexpr int buf = decltype(bufc)::value;
+        wait_vm0();
+        lds_barrier();
+        if (it + 1 < n) dma(buf ^ 1);
+        if (KG > 1 && it >= n) return;
+        const int q0 = qstart + (top - now.tile) * FT, ta = q0 + s.off, tb = min(q0 + FT, s.ql) - 1 + s.off;
+        advance(now);
+        const float *Ql = tiles[kg][buf][0], *Ol = tiles[kg][buf][1], *Ll = stat[kg][buf][0] + 4 * g, *Dl = stat[kg][buf][1] + 4 * g;
+        if (!all_seen(a, ta, tb, k0, k0 + BN - 1) && (scan32<HD>(Ql, tid) || scan32<HD>(Ol, tid))) odd = true;
+        if (none_seen(a, ta, tb, kw, kw + 15)) return;
+        const bool whole = q0 + FT <= s.ql && all_seen(a, ta, tb, kw, kw + 15);
         f32x4 sa[2], da[2];  // S / dP[q0 + 16 qs + 4 g + e][key]
         bool live[2];
 #pragma unroll
         for (int qs = 0; qs < 2; ++qs) {
-            const int ta = q0 + 16 * qs + s.off, tb = min(q0 + 16 * qs + 16, s.ql) - 1 + s.off;
             sa[qs] = da[qs] = f32x4{0, 0, 0, 0};
-            live[qs] = !none_seen(a, ta, tb, kw, kw + 15);  // wave-uniform
+            live[qs] = whole || !none_seen(a, ta + 16 * qs, min(ta + 16 * qs + 15, s.kl - 1), kw, kw + 15);  // wave-uniform
             if (!live[qs]) continue;
-            sa[qs] = head_dot<NU>(Ql + (16 * qs + c) * P + 4 * g, kf);
-            da[qs] = head_dot<NU>(Ol + (16 * qs + c) * P + 4 * g, vf);
+            sa[qs] = head_dot<HD>(Ql + 16 * qs * HD, t, kf);
+            da[qs] = head_dot<HD>(Ol + 16 * qs * HD, t, vf);
+            const f32x4 l = *reinterpret_cast<const f32x4 *>(Ll + 16 * qs), d = *reinterpret_cast<const f32x4 *>(Dl + 16 * qs);
+            // (a row of no gradient has an LSE of -inf: P = 0 for it and, behind the last row, below)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int x = 16 * qs + 4 * g + e;
-                const float l = Ls[kg][buf][x];
-                const float p = expf(fmaf(sa[qs][e], a.scale, -l));
-                const bool on = l != -INFINITY && sees(a, q0 + x + s.off, key);
-                sa[qs][e] = on ? p : 0.f;
-                da[qs][e] = on ? p * (da[qs][e] - Dl[kg][buf][x]) : 0.f;
+                sa[qs][e] = l[e] == -INFINITY ? 0.f : exp_(fmaf(sa[qs][e], a.scale, -l[e]));
+                da[qs][e] = l[e] == -INFINITY ? 0.f : sa[qs][e] * (da[qs][e] - d[e]);
             }
+        }
+        if (!whole) {
+#pragma unroll
+            for (int qs = 0; qs < 2; ++qs)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int x = q0 + 16 * qs + 4 * g + e;
+                    if (x >= s.ql || !sees(a, x + s.off, key)) sa[qs][e] = da[qs][e] = 0.f;
+                }
         }
         // dV^T += dO^T P, dK^T += Q^T dS
 #pragma unroll
         for (int qs = 0; qs < 2; ++qs) {
             if (!live[qs]) continue;
-            add_rows<NU>(dvt, Ol + (16 * qs + 4 * g) * P, P, c, sa[qs]);
-            add_rows<NU>(dkt, Ql + (16 * qs + 4 * g) * P, P, c, da[qs]);
+            add_rows<HD>(dvt, Ol + 16 * qs * HD, t, sa[qs]);
+            add_rows<HD>(dkt, Ql + 16 * qs * HD, t, da[qs]);
         }
     };
-    for (int it = kg, buf = 0; it - kg < niter; it += KG, buf ^= 1) {
-        if (it + KG < niter) load(it + KG);
-        if (it < niter) step(it, buf);
-        if (it + KG < niter) store(it + KG, buf ^ 1);
-        __syncthreads();
+    for (int it0 = 0; it0 < steps; it0 += 2) {
+        step(it0, std::integral_constant<int, 0>{});
+        if (it0 + 1 < steps) step(it0 + 1, std::integral_constant<int, 1>{});
     }
     float *ws = slot >= 0 ? a.ws + ((long)bk * plan.slots() + slot) * (2 * BN * HD) : nullptr;
     if (__syncthreads_or(odd)) {
@@ -610,7 +694,7 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_dkv32_k(Wind
         return;
     }
     if constexpr (KG > 1) {
-        static_assert(2 * NU * 4 * 256 <= 4 * FT * P, "a group's sums fit its tiles");
+        static_assert(2 * NU * 4 * 256 <= 4 * TILE, "a group's sums fit its tiles");
         auto column = [&](int k, int j) { return reinterpret_cast<f32x4 *>(tiles[k][0][0] + (wave * 2 * NU + j) * 256) + lane; };
         if (kg)
 #pragma unroll
@@ -636,8 +720,8 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_dkv32_k(Wind
     });
 }
 
-bool shape_ok(const WindowArgs &a) { return a.dt == DType::F32 && (a.hd == 64 || a.hd == 128) && a.scale > 0.f && a.scale < INFINITY; }
-bool ok(const void *p, long ld) { return aligned_rows(p, ld, 16, 4); }
+bool shape_ok(const WindowArgs &a) { return a.dt == DType::F32 && (a.hd == 64 || a.hd == 128) && a.scale > 0.f && a.scale < INFINITY && a.n_heads < (1 << 16); }
+bool ok(const void *p, long ld) { return aligned_rows(p, ld, 16, 4) && ld < (1l << 23); }
 bool fwd_ok(const WindowArgs &a) { return shape_ok(a) && ok(a.q, a.ldq) && ok(a.k, a.ldk) && ok(a.v, a.ldv) && ok(a.o, a.ldo); }
 bool few_rows(const WindowArgs &a) { return a.n_q <= kFewRows; }
 int splits32(const WindowArgs &a) { return step_splits(a, 16, 1024); }

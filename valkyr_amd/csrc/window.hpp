@@ -49,6 +49,27 @@ VKH_DEV bool none_seen(const WindowArgs &a, int ta, int tb, int j0, int j1) {
     return tb < ta || j0 > tb || (j1 <= ta - a.window && j0 >= a.n_sink);
 }
 
+// hide(ks, r) for the keys k0 + 16 ks + 4 g + r, ks < KS, that position t does not see.
+template <int KS, class F>
+VKH_DEV void for_hidden(const WindowArgs &a, int t, int k0, int g, F hide) {
+    int x = t - k0 - 4 * g;
+    if (k0 < a.n_sink && k0 + 16 * KS > a.n_sink) {  // sinks and others: the others outside the window
+        const int ns = a.n_sink - k0 - 4 * g;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (16 * ks + r >= ns && x - 16 * ks - r >= a.window) hide(ks, r);
+    }
+    asm("" : "+v"(x));  // (the differences below are not kept from those above)
+    const unsigned reach = k0 < a.n_sink ? kAll : a.window;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if ((unsigned)(x - 16 * ks - r) >= reach) hide(ks, r);
+}
+
 VKH_DEV void store4(float *p, float x, float y, float z, float w) {
     *reinterpret_cast<float4 *>(p) = make_float4(x, y, z, w);
 }
