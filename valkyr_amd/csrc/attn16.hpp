@@ -44,6 +44,10 @@ VKH_DEV void dma16_at(const sgpr4 &rs, unsigned lds, unsigned voff) {
     asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(voff), "s"(rs) : "memory");
 }
 
+VKH_DEV void dma4_at(const sgpr4 &rs, unsigned lds, unsigned voff) {
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds" : : "s"(lds), "v"(voff), "s"(rs) : "memory");
+}
+
 template <int N>
 VKH_DEV void wait_vm() {
     __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4 << 14));

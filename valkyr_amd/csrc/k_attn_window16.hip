@@ -715,62 +715,62 @@ __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan p
     const int nsteps = nh * (alt ? (nqt + 1) / 2 : nqt);
     const int niter = max(0, (nsteps - zpart + zparts - 1) / zparts);
     char *strm = smem + hg * STREAM;
-    const void *tp = tdo ? a.dout : a.q;
-    const long ldt = tdo ? a.lddo : a.ldq;
-    const float *sp = tdo ? a.d : a.lse;
     // A cursor runs over the block's steps zpart, zpart + zparts, ... of (query tile, head), heads
-    // inner; the group's tile and head of a step.
+    // inner: the group's first row and head (of the KV head's) of a step.
     struct Cursor {
-        int head, tile;
+        int h, q0;
     };
-    const int dh = zparts % nh, dt = zparts / nh;
+    const int span = alt ? 2 * BM : BM, dh = zparts % nh * (alt ? 1 : 2), dq = zparts / nh * span;
     auto advance = [&](Cursor &c) {
-        c.head += dh;
-        c.tile += dt;
-        if (c.head >= nh) c.head -= nh, ++c.tile;
+        c.h += dh;
+        c.q0 -= dq;
+        if (c.h >= hpk) c.h -= hpk, c.q0 -= span;
     };
     const int top = alt ? (nqt + 1) / 2 * 2 - 1 : nqt - 1;  // the last tile (alt: of a pair)
-    auto head_of = [&](const Cursor &c) { return kvh * hpk + (alt ? c.head : hg + 2 * c.head); };
-    auto row_of = [&](const Cursor &c) { return qstart + (top - (alt ? 2 * c.tile + hg : c.tile)) * BM; };
-    Cursor ahead{zpart % nh, zpart / nh}, now = ahead;
-    // C DMAs per wave and tile, and one more for the waves that move LSE or D
-    // (the lane id is laundered so that the offsets are recomputed here rather than held in
-    // registers across the loop: spilled, their reloads would wait for the DMA in flight)
+    Cursor ahead{zpart % nh * (alt ? 1 : 2) + (alt ? 0 : hg), qstart + (top - (alt ? hg : 0)) * BM - zpart / nh * span};
+    Cursor now = ahead;
+    // C DMAs per wave and tile, and one more for the waves that move LSE or D.  (The lane id is
+    // laundered so that the offsets are formed here rather than held in registers across the loop:
+    // spilled, their reloads would wait for the DMA in flight.)
+    const int ldt = (int)(tdo ? a.lddo : a.ldq);
+    const bf16 *tp = (const bf16 *)(tdo ? a.dout : a.q) + (row0 + 16 * part) * ldt + kvh * hpk * HD;
+    const float *sp = (tdo ? a.d : a.lse) + row0 * a.n_heads + kvh * hpk;
+    const unsigned dst = lds_addr(strm) + (tdo ? TILE : 0) + part * 16 * HD * 2;
+    const unsigned dst_stat = lds_addr((const char *)(tdo ? Dd[hg][0] : Ls[hg][0]));
     auto dma = [&](int buf) {
-        const int h = head_of(ahead), q0 = row_of(ahead), rows = min(BM, s.ql - q0);
-        advance(ahead);
-        const sgpr4 rt = head_rows<HD>(tp, row0 + q0, ldt, h * HD, rows);
-        char *dst = strm + buf * 2 * TILE + (tdo ? TILE : 0) + part * 16 * HD * 2;
+        const int rows = s.ql - ahead.q0 - 16 * part;
+        const sgpr4 rt = rsrc4(tp + (long)ahead.q0 * ldt + ahead.h * HD, rows > 0 ? (unsigned)(((min(rows, 16) - 1) * ldt + HD) * 2) : 0u);
         int ln = lane;
         asm volatile("" : "+v"(ln));
+        // row r = RPI i + ln / (HD / 8) of the 16, chunk ln % (HD / 8) ^ swz(r): the part of i is 4 i
+        const unsigned x = (unsigned)(ln % (HD / 8) ^ ln / 16) * 16, ro = __umul24(ln / (HD / 8), 2 * ldt);
 #pragma unroll
-        for (int i = 0; i < C; ++i) dma16_async(rt, dst + i * 1024, dma_off<HD>(16 * part + RPI * i, ln, (int)ldt));
+        for (int i = 0; i < C; ++i) dma16_at(rt, dst + buf * 2 * TILE + i * 1024, (x ^ 64 * i) + (ro + i * RPI * 2 * ldt));
         if (part == 0) {
-            const sgpr4 rs = rsrc4(sp + (row0 + q0) * a.n_heads + h, rows > 0 ? (unsigned)(((rows - 1) * a.n_heads + 1) * 4) : 0u);
-            const unsigned so = ln < BM ? (unsigned)(ln * a.n_heads * 4) : kOOB;
-            if (tdo) dma4_async(rs, Dd[hg][buf], so);
-            else dma4_async(rs, Ls[hg][buf], so);
+            const sgpr4 rs = rsrc4(sp + (long)ahead.q0 * a.n_heads + ahead.h, rows > 0 ? (unsigned)(((min(rows, BM) - 1) * a.n_heads + 1) * 4) : 0u);
+            dma4_at(rs, dst_stat + buf * 256, ln < BM ? (unsigned)__umul24(ln, a.n_heads * 4) : kOOB);
         }
+        advance(ahead);
     };
+    const RowReach block = row_reach<BM>(a, s, k0, k0 + BN - 1), mine = row_reach<BM>(a, s, kw0, kw0 + KW - 1);
     if (niter > 0) dma(0);
     if (niter > 1) dma(1);
     bool odd = false;  // an infinity or a NaN in Q or dO of a tile whose rows do not all see all keys
     auto step = [&](const int it, auto bufc) {
         constexpr int buf = decltype(bufc)::value;
         if (it + 1 < niter) {
-            if (part == 0) __builtin_amdgcn_s_waitcnt(0x0f70 | (C + 1));
-            else __builtin_amdgcn_s_waitcnt(0x0f70 | C);
+            if (part == 0) wait_vm<C + 1>();
+            else wait_vm<C>();
         } else {
             wait_vm0();
         }
         lds_barrier();
         if (it + 2 < niter) dma((buf + 2) % NBUF);
-        const int q0 = row_of(now);
+        const int q0 = now.q0;
         advance(now);
         const char *Qb = strm + buf * 2 * TILE, *Ob = Qb + TILE;
-        const int ta = q0 + s.off, tb = min(q0 + BM, s.ql) - 1 + s.off;  // the tile's live positions
-        if (!all_seen(a, ta, tb, k0, k0 + BN - 1)) odd |= scan<2 * TILE, 256>(Qb, tid % 256);
-        if (none_seen(a, ta, tb, kw0, kw0 + KW - 1)) return;
+        if (!block.whole(q0)) odd |= scan<2 * TILE, 256>(Qb, tid % 256);
+        if (!mine.some(q0)) return;
         auto dval = [&](int qs, int r) { return Dd[hg][buf][16 * qs + 4 * g + r]; };
         auto prob = [&](float x, int qs, int r) {
             return __builtin_amdgcn_exp2f(fmaf(x, c2, -(Ls[hg][buf][16 * qs + 4 * g + r] * LOG2E)));
@@ -816,7 +816,7 @@ __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan p
             }
         }
         const bool dead = __any(lane < BM && Ls[hg][buf][lane % BM] == -INFINITY);  // a row of no gradient
-        if (dead || q0 + BM > s.ql || !all_seen(a, ta, tb, kw0, kw0 + KW - 1)) {
+        if (dead || !mine.whole(q0)) {
 #pragma unroll
             for (int qs = 0; qs < QS; ++qs)
 #pragma unroll

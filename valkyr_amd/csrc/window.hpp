@@ -118,6 +118,24 @@ VKH_DEV Reach reach(const WindowArgs &a, const KeyTiles &k, int ta, int tb) {
     return r;
 }
 
+// The same for the keys j0 .. j1 and tiles of BM query rows, by their first row q0.  (Tiles beside the
+// reach of which no row sees a key may count as some.)
+struct RowReach {
+    int some0, n_some, all0, n_all;
+    VKH_DEV bool some(int q0) const { return (unsigned)(q0 - some0) < (unsigned)n_some; }
+    VKH_DEV bool whole(int q0) const { return (unsigned)(q0 - all0) < (unsigned)n_all; }
+};
+template <int BM>
+VKH_DEV RowReach row_reach(const WindowArgs &a, const Span &s, int j0, int j1) {
+    RowReach r;
+    r.some0 = j0 - s.off - BM + 1;
+    r.n_some = max(0, (j0 < a.n_sink ? s.ql : (int)min((long)s.ql, (long)j1 + a.window - s.off)) - r.some0);
+    r.all0 = j1 - s.off;
+    const int last = s.ql - BM + 1;
+    r.n_all = max(0, (j1 < a.n_sink ? last : (int)min((long)last, (long)j0 + a.window - BM + 1 - s.off)) - r.all0);
+    return r;
+}
+
 // A kernel's first argument, read anew from where the launch put it (the kernel arguments begin
 // with it): its values need not stay in registers for the calls below.
 VKH_DEV const WindowArgs &args_again() {
