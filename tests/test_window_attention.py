@@ -265,6 +265,73 @@ def test_lengths_and_strides(nq, nk, window, sinks, ql, kl, hd, pad, form):
     c.check(c.read(), c.want())
 
 
+# grids of more blocks than the chip has CUs (by 64 and by 128 rows), more than one group's steps, and
+# longer calls whose few rows' tiles see many keys
+LARGER = [
+    (1, 700, 700, 32, 8, 64, 130, 3),
+    (1, 1100, 1100, 32, 8, 128, 600, 70),
+    (1, 1100, 1100, 32, 32, 64, 90, 1),
+    (1, 90, 2000, 4, 2, 128, 1900, 70),
+    (2, 200, 1700, 3, 1, 64, 0, 0),
+    (1, 40, 700, 8, 4, 64, 300, 5),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ragged", [False, True], ids=["whole", "ragged"])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("shape", LARGER, ids=lambda s: "-".join(str(x) for x in s))
+def test_larger_calls(shape, form, ragged):
+    note(f"larger window attention {shape} {form} {ragged}")
+    b, nq, nk = shape[:3]
+    ql, kl = [nq - 45 * i - 7 for i in range(b)], [nk - 77 * i - 30 for i in range(b)]
+
+    def spoil(v):
+        for i in range(b if ragged else 0):
+            v["k"][i, kl[i]:] = v["v"][i, kl[i]:] = np.nan
+            v["q"][i, ql[i]:] = v["do"][i, ql[i]:] = np.inf
+
+    c = Call(*shape, form, lens=(ql, kl) if ragged else None, spoil=spoil)
+    c.forward()
+    c.backward()
+    c.check(c.read(), c.want())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [np.nan, -np.inf])
+@pytest.mark.parametrize("form", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 1100, 1100, 32, 8, 64, 600, 3), (1, 700, 700, 32, 32, 128, 48, 2), (1, 90, 2000, 4, 2, 128, 1600, 3),
+                                   (1, 40, 700, 4, 2, 64, 250, 1)], ids=lambda s: "-".join(str(x) for x in s))
+def test_what_is_not_seen_reaches_nothing_in_larger_calls(shape, form, bad):
+    """As below, on the larger calls' kernels: one key's and one query's rows hold infinities or NaN."""
+    b, nq, nk, H, Hkv, hd, window, sinks = shape
+    note(f"larger window attention unseen {shape} {form} {bad}")
+    jbad, rbad = nk - nq + nq // 3, nq // 2
+
+    def spoil(v):
+        v["k"][:, jbad], v["v"][:, jbad] = bad, bad
+        v["q"][:, rbad], v["do"][:, rbad] = bad, bad
+
+    c, clean = Call(*shape, form, spoil=spoil), Call(*shape, form)
+    for x in (c, clean):
+        x.forward()
+        x.backward()
+    got, want = c.read(), clean.want()
+    see = visible(nq, nk, nq, nk, window, sinks)
+    rows = ~see[:, jbad]
+    rows[rbad] = False
+    keys = ~see[rbad]
+    keys[jbad] = False
+    keys &= ~see[see[:, jbad]].any(0)
+    assert rows.any()
+    for n in ("o", "lse", "dq"):
+        want[n], got[n] = want[n][:, rows], got[n][:, rows]
+    want["size"], want["edq"], want["edk"] = want["size"][:, rows], want["edq"][:, rows], want["edk"][:, keys]
+    for n in ("dk", "dv"):
+        want[n], got[n] = want[n][:, keys], got[n][:, keys]
+    c.check(got, want, [n for n in ("o", "lse", "dq", "dk", "dv") if want[n].size])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("form", FORMS)
@@ -409,7 +476,8 @@ def test_same_bits_every_time_with_any_workspace(form, shape):
 @pytest.mark.gpu
 @pytest.mark.parametrize("own_ws", [False, True], ids=["no-workspace", "workspace"])
 @pytest.mark.parametrize("form,shape", [("bf16", (2, 1, 2000, 8, 2, 128, 900, 4)), ("bf16", (1, 333, 333, 4, 2, 64, 60, 1)),
-                                        ("fp32", (1, 200, 200, 4, 1, 128, 60, 1))])
+                                        ("fp32", (1, 200, 200, 4, 1, 128, 60, 1)), ("bf16", (1, 50, 2000, 4, 2, 64, 1700, 1)),
+                                        ("fp32", (2, 40, 600, 4, 2, 64, 500, 2))])
 def test_on_a_captured_stream_with_lengths_that_grow(form, shape, own_ws):
     """A step recorded once is replayed while the lengths on the device change."""
     from test_gpu_kernels import _replays

@@ -1085,8 +1085,10 @@ bool bwd_ok(const WindowArgs &a) {
            aligned_rows(a.dk, a.lddk, 4 * es, es) && aligned_rows(a.dv, a.lddv, 4 * es, es);
 }
 
-// Few rows: the tile kernel would give a KV head's keys to one block per head.
-bool few_rows(const WindowArgs &a) { return a.n_q <= kFewRows; }
+// Against the tile kernel, us: 64 / 24 rows, window 4096, 16 / 8 heads of 128: 22 against 48, 17.5
+// against 52; 200 rows, 2000 keys, 8 / 8 heads of 64 (104 tiles) 12.5 against 19; 500 tokens, 4 / 1 heads
+// (125 tiles) 14.3 against 11.1; 8 x 16 rows, window 2048, 32 / 4 heads of 64 (256 tiles) 28.5 against 25.5.
+bool few_rows(const WindowArgs &a) { return few_rows_of(a, 192, 1536); }
 // two rounds of one block per CU
 int splits16(const WindowArgs &a) { return step_splits(a, 32, 512); }
 // dK/dV: one block per CU, at least four steps of both groups each
@@ -1104,7 +1106,7 @@ size_t window16_bwd_ws_bytes(const WindowArgs &a) {
 
 bool window16_forward(const WindowArgs &a, hipStream_t st) {
     if (!fwd_ok(a)) return false;
-    if (few_rows(a)) {
+    if (few_rows(a) && (a.n_q <= kFewRows || a.ws)) {
         const int grp = a.n_heads / a.n_kv_heads, rt = (a.n_q * grp + 15) / 16, splits = a.ws ? splits16(a) : 1;
         const long blocks = (long)a.n_batch * a.n_kv_heads * rt * splits;
         auto by = [&](auto hd, auto to) {

@@ -723,11 +723,14 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_dkv32_k(Wind
 bool shape_ok(const WindowArgs &a) { return a.dt == DType::F32 && (a.hd == 64 || a.hd == 128) && a.scale > 0.f && a.scale < INFINITY && a.n_heads < (1 << 16); }
 bool ok(const void *p, long ld) { return aligned_rows(p, ld, 16, 4) && ld < (1l << 23); }
 bool fwd_ok(const WindowArgs &a) { return shape_ok(a) && ok(a.q, a.ldq) && ok(a.k, a.ldk) && ok(a.v, a.ldv) && ok(a.o, a.ldo); }
-bool few_rows(const WindowArgs &a) { return a.n_q <= kFewRows; }
+// Against the tile kernel, us: 64 rows, window 4096, 16 / 8 heads of 128: 45 against 294; 500 tokens, 4 / 1
+// heads (125 tiles) 23 against 43; 300 tokens, 8 / 4 heads of 64: 12 against 17; 8 x 32 rows, window 2048,
+// 32 / 4 heads (512 tiles) 80 against 83; 1000 tokens, window 64 (252 tiles) 13.5 against 11.8.
+bool few_rows(const WindowArgs &a) { return few_rows_of(a, 512, 192); }
 int splits32(const WindowArgs &a) { return step_splits(a, 16, 1024); }
-// Two groups of waves a block where the chip has at most two blocks a CU: one or two groups, forward /
-// backward of 1001 tokens, 16 / 8 heads of 128, window 512: 74 / 209 and 63 / 203 us; unlimited: 120 / 307
-// and 97 / 249; 4 x 2048 tokens, window 64 (2048 and 1024 blocks): 123 / 453 and 123 / 502.
+// Two groups of waves a block where the chip has at most two blocks a CU.  One or two groups, forward /
+// backward in us: 2 x 1024 tokens, 16 / 16 heads of 128, window 1024 (512 blocks): 111 / 387 and 94 / 315; heads
+// of 64: 60 / 211 and 57 / 179; 4 x 1024 tokens, 16 / 8 heads of 64, window 256 (1024 blocks): 51 / 212 and 55 / 215.
 bool grouped(const WindowArgs &a) { return (long)a.n_heads * a.n_batch * ((a.n_q + 63) / 64) <= 512; }
 bool grouped_dkv(const WindowArgs &a) { return (long)a.n_kv_heads * a.n_batch * ((a.n_kv + 63) / 64) <= 512; }
 DkvPlan plan32(const WindowArgs &a, bool ws) { return dkv_plan(a, ws, 64, 512, 16, grouped_dkv(a) ? 4 : 2, false); }
@@ -739,7 +742,7 @@ size_t window32_bwd_ws_bytes(const WindowArgs &a) { return shape_ok(a) ? dkv_ws_
 
 bool window32_forward(const WindowArgs &a, hipStream_t st) {
     if (!fwd_ok(a)) return false;
-    if (few_rows(a)) {
+    if (few_rows(a) && (a.n_q <= kFewRows || a.ws)) {
         const int grp = a.n_heads / a.n_kv_heads, splits = a.ws ? splits32(a) : 1;
         const dim3 grid((unsigned)((long)a.n_batch * a.n_kv_heads * ((a.n_q * grp + 15) / 16) * splits));
         if (a.hd == 128) hipLaunchKernelGGL(window_step32_k<128>, grid, dim3(FNT), 0, st, a, splits);

@@ -458,11 +458,21 @@ void launch_dkv_sum(const WindowArgs &a, const DkvPlan &p, hipStream_t st) {
                            dim3(256), 0, st, a, p);
 }
 
-// Blocks that share a KV head's keys where few rows see them (n_q query rows at most kFewRows):
-// towards `fill` blocks, while each of a block's four waves keeps a tile of `keys` keys.
+// The kernels of few rows: 16 rows of a KV head's query heads a block, whose keys several blocks share.
+// Calls of at most kFewRows query rows take them; of longer calls those whose 16-row tiles are few
+// (`max_tiles`) and see many keys (`min_span`), for which the tile kernels leave CUs without a block
+// and each block a long chain of steps.
 constexpr int kFewRows = 16;
+inline long row_tiles(const WindowArgs &a) {
+    return (long)a.n_batch * a.n_kv_heads * (((long)a.n_q * (a.n_heads / a.n_kv_heads) + 15) / 16);
+}
+inline bool few_rows_of(const WindowArgs &a, long max_tiles, int min_span) {
+    return a.n_q <= kFewRows || (row_tiles(a) <= max_tiles && std::min<long>(a.n_kv, (long)a.window + 64) >= min_span);
+}
+// Blocks that share a KV head's keys: towards `fill` blocks, while each of a block's four waves keeps a
+// tile of `keys` keys.
 inline int step_splits(const WindowArgs &a, int keys, long fill) {
-    const long base = (long)a.n_batch * a.n_kv_heads * ((a.n_q * (a.n_heads / a.n_kv_heads) + 15) / 16);
+    const long base = row_tiles(a);
     const long tiles = (std::min<long>(a.n_kv, (long)a.window + a.n_q) + a.n_sink + 2 * keys - 1) / keys;
     return (int)std::max(1l, std::min({64l, fill / base, (tiles + 3) / 4}));
 }
