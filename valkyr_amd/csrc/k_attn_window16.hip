@@ -84,8 +84,9 @@ __device__ __attribute__((noinline)) void dkv_rows(const WindowArgs &a, const St
 // Block = 64 QS query rows of one head, 4 waves of 16 QS; 32-key tiles, three buffers (two tiles on
 // their way).  The heaviest (last) rows start first.  Matrix cores, vector ALU and LDS each have about
 // as much to do and take turns within a wave, so it is waves that overlap them: 32-key tiles leave
-// registers for three a SIMD.  16384 tokens, window 2048, 32 / 8 heads of 128: 534 us; 64-key tiles, two
-// waves a SIMD: 566; the next tile's scores formed beside this one's exponentials: 710 (two waves).
+// registers for three a SIMD.  16384 tokens, window 2048, 32 / 8 heads of 128: 513 to 536 us, 1.0 PFLOP/s;
+// as first measured 534, 64-key tiles on two waves a SIMD 566, the next tile's scores formed beside this
+// one's exponentials (two waves) 710.
 // On short grids (64-row blocks) a wave's own chain of steps is the time: heads of 64, whose registers
 // allow it, take 64-key tiles there (2048 tokens, window 2048, 8 / 8 heads: 26 against 32 us).
 template <int HD, int QS, int KG, class TO>
@@ -280,7 +281,9 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 2 : HD == 64 && QS == 2 ? 4 : 3
 // time; each of the 4 waves streams 32-key tiles of its own (two in LDS, no barrier between the
 // waves), every fourth of the block's, and their results are joined at the end.  `splits` blocks
 // share a KV head's tiles; their results (maximum, sum, O in fp32) go to a.ws and
-// window_join_k joins them in order.
+// window_join_k joins them in order.  32 sequences of up to 32768 tokens, window 4096, 32 / 8 heads of
+// 128 (0.52 GB of K and V): 92 to 98 us, 5.3 to 5.6 TB/s, and 4 to join; one sequence, window 1024: 6 and 3,
+// two launches' latency.
 // acc[i][r] += sum over the tile's rows x that `see` names of T[x][16 i + 4 g + r] w[x], where w is
 // held as a B operand: element 4 u + e is row 16 u + 4 g + e.  It goes through `wl`, 1 KB of the
 // wave's own LDS.
@@ -452,7 +455,11 @@ __global__ __launch_bounds__(256, 1) void window_step16_k(WindowArgs a, int spli
 // Block = BQ query rows of one head on 4 waves of 16 QSUB rows, whose Q and dO fragments stay in
 // registers; 32-key tiles of K and V through three buffers (two in flight, the wait counted).
 // D = rowsum(O dO) of the block's rows is formed first (fp64 sums of the bf16 products) and
-// stored for the dK/dV kernel, which runs after this one.
+// stored for the dK/dV kernel, which runs after this one.  As the forward, it is bound by what a wave
+// does between its products (softmax, rounding, LDS reads) and by masked tiles: 16384 tokens, window
+// 2048, 32 / 8 heads of 128: 780 us, 0.99 PFLOP/s; 4 x 2048, window 512, 16 / 8 heads: 78 us, 0.58 PFLOP/s.  KG = 2 (short
+// grids: one block a CU): two groups of waves take every other tile; 2048 tokens, window 2048, 8 / 8
+// heads of 64, forward / backward: 24.8 / 73 us without, 19.3 / 63 with.
 template <int HD, int BQ, int KG, class TO>
 __global__ __launch_bounds__(256 * KG, 2) void window_dq16_k(WindowArgs a) {
     using R = TileRows<HD>;
@@ -656,7 +663,10 @@ __global__ __launch_bounds__(256 * KG, 2) void window_dq16_k(WindowArgs a) {
 // its window, or to the last row of all where the block holds sinks; such a block has a share of
 // work as many times the others' as the sequence is longer than the window, and is split between
 // `parts` blocks, as all blocks are where they are too few for the chip.  Parts write fp32 sums
-// to their slots of a.ws, which window_dkv_sum_k adds in order.
+// to their slots of a.ws, which window_dkv_sum_k adds in order.  Bound by the one block a CU that
+// the dK and dV accumulators (2 x 32 x HD a wave) and their registers leave: eight waves, half of whose
+// time goes to waiting for each other and for LDS.  16384 tokens, window 2048, 32 / 8 heads of 128: 1160
+// us, 0.89 PFLOP/s; 4 x 2048, window 512, 16 / 8 heads: 112 us, 0.54 PFLOP/s.
 template <int HD, class TO>
 __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan plan) {
     using R = TileRows<HD>;
@@ -1094,6 +1104,8 @@ int splits16(const WindowArgs &a) { return step_splits(a, 32, 512); }
 // dK/dV: one block per CU, at least four steps of both groups each
 DkvPlan plan16(const WindowArgs &a, bool ws) { return dkv_plan(a, ws, 128, 256, 8, 8, true); }
 
+// Two groups of waves a block where the chip has at most one block a CU (up to two: 1 x 4096 tokens, window
+// 512, 8 / 8 heads of 128, 512 blocks: forward 30 us with two groups, 24 with one).
 bool grouped(const WindowArgs &a) { return (long)a.n_heads * a.n_batch * ((a.n_q + 63) / 64) <= cu_count(); }
 
 }  // namespace
@@ -1123,7 +1135,8 @@ bool window16_forward(const WindowArgs &a, hipStream_t st) {
         return true;
     }
     const long per = (long)a.n_heads * a.n_batch;
-    // grids of 128-row blocks that leave the CUs one block each or fewer take 64 rows
+    // grids of 128-row blocks that leave the CUs one block each or fewer take 64 rows (2 x 1001 tokens,
+    // window 256, 16 / 4 heads, 256 blocks: 25.8 us with 128 rows, 16.8 with 64)
     const bool small = per * ((a.n_q + 127) / 128) <= cu_count(), pairs = grouped(a);
     auto go = [&](auto kernel, int bm, int kg) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)(per * ((a.n_q + bm - 1) / bm))), dim3(256 * kg), 0, st, a);
