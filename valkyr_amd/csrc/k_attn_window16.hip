@@ -346,9 +346,9 @@ __global__ __launch_bounds__(256, 1) void window_step16_k(WindowArgs a, int spli
         const sgpr4 rk = head_rows<HD>(a.k, key0 + k0, a.ldk, kvh * HD, rows);
         const sgpr4 rv = head_rows<HD>(a.v, key0 + k0, a.ldv, kvh * HD, rows);
 #pragma unroll
-        for (int i = 0; i < IPT; ++i) dma16_async(rk, Kt + buf * TILE + i * 1024, ko[i]);
+        for (int i = 0; i < IPT; ++i) dma16_at(rk, lds_addr(Kt + buf * TILE + i * 1024), ko[i]);
 #pragma unroll
-        for (int i = 0; i < IPT; ++i) dma16_async(rv, Vt + buf * TILE + i * 1024, vo[i]);
+        for (int i = 0; i < IPT; ++i) dma16_at(rv, lds_addr(Vt + buf * TILE + i * 1024), vo[i]);
     };
     f32x4 acc[DSUB];
 #pragma unroll
@@ -708,7 +708,7 @@ __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan p
     if (hg == 0) {
         const sgpr4 rv = head_rows<HD>(a.v, key0 + kw0, a.ldv, kvh * HD, min(KW, s.kl - kw0));
 #pragma unroll
-        for (int i = 0; i < KW / RPI; ++i) dma16_async(rv, vsl + i * 1024, dma_off<HD>(RPI * i, lane, (int)a.ldv));
+        for (int i = 0; i < KW / RPI; ++i) dma16_at(rv, lds_addr(vsl + i * 1024), dma_off<HD>(RPI * i, lane, (int)a.ldv));
     }
     wait_vm0();
     __syncthreads();
@@ -746,7 +746,7 @@ __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan p
     const bf16 *tp = (const bf16 *)(tdo ? a.dout : a.q) + (row0 + 16 * part) * ldt + kvh * hpk * HD;
     const float *sp = (tdo ? a.d : a.lse) + row0 * a.n_heads + kvh * hpk;
     const unsigned dst = lds_addr(strm) + (tdo ? TILE : 0) + part * 16 * HD * 2;
-    const unsigned dst_stat = lds_addr((const char *)(tdo ? Dd[hg][0] : Ls[hg][0]));
+    const unsigned dst_stat = lds_addr(tdo ? Dd[hg][0] : Ls[hg][0]);
     auto dma = [&](int buf) {
         const int rows = s.ql - ahead.q0 - 16 * part;
         const sgpr4 rt = rsrc4(tp + (long)ahead.q0 * ldt + ahead.h * HD, rows > 0 ? (unsigned)(((min(rows, 16) - 1) * ldt + HD) * 2) : 0u);
@@ -972,11 +972,11 @@ __global__ __launch_bounds__(256, 1) void window_far16_k(WindowArgs a, DkvPlan p
         const long at = (row0 + q0) * a.n_heads + h;
         const unsigned bytes = (unsigned)(((rows - 1) * a.n_heads + 1) * 4);
 #pragma unroll
-        for (int i = 0; i < C; ++i) dma16_async(rq, tiles[wave][buf] + i * 1024, qo[i]);
+        for (int i = 0; i < C; ++i) dma16_at(rq, lds_addr(tiles[wave][buf] + i * 1024), qo[i]);
 #pragma unroll
-        for (int i = 0; i < C; ++i) dma16_async(rg, tiles[wave][buf] + TILE + i * 1024, go[i]);
-        dma4_async(rsrc4(a.lse + at, bytes), stat[wave][buf][0], so);
-        dma4_async(rsrc4(a.d + at, bytes), stat[wave][buf][1], so);
+        for (int i = 0; i < C; ++i) dma16_at(rg, lds_addr(tiles[wave][buf] + TILE + i * 1024), go[i]);
+        dma4_at(rsrc4(a.lse + at, bytes), lds_addr(stat[wave][buf][0]), so);
+        dma4_at(rsrc4(a.d + at, bytes), lds_addr(stat[wave][buf][1]), so);
     };
     const int it0 = 4 * part + wave;
     if (it0 < n) dma(it0, 0);

@@ -199,7 +199,7 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_fwd32_k(Wind
     // waves 0 and 1 move K, 2 and 3 V
     const int ld = (int)(wave < 2 ? a.ldk : a.ldv);
     const float *src = (const float *)(wave < 2 ? a.k : a.v) + (long)b * a.n_kv * ld + kvh * HD;
-    const unsigned dst = lds_addr((const char *)tiles[kg][0][wave / 2]) + wave % 2 * C * 1024;
+    const unsigned dst = lds_addr(tiles[kg][0][wave / 2]) + wave % 2 * C * 1024;
     unsigned off[C];
 #pragma unroll
     for (int i = 0; i < C; ++i) off[i] = T::dma(wave % 2 * C + i, lane, ld);
@@ -486,7 +486,7 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_dq32_k(Windo
     const int steps = (kt.n + KG - 1) / KG, n = (kt.n - kg + KG - 1) / KG;
     const int ld = (int)(wave < 2 ? a.ldk : a.ldv);
     const float *src = (const float *)(wave < 2 ? a.k : a.v) + (long)b * a.n_kv * ld + kvh * HD;
-    const unsigned dst = lds_addr((const char *)tiles[kg][0][wave / 2]) + wave % 2 * C * 1024;
+    const unsigned dst = lds_addr(tiles[kg][0][wave / 2]) + wave % 2 * C * 1024;
     unsigned off[C];
 #pragma unroll
     for (int i = 0; i < C; ++i) off[i] = T::dma(wave % 2 * C + i, lane, ld);
@@ -614,7 +614,7 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_dkv32_k(Wind
     const int ld = (int)(wave < 2 ? a.ldq : a.lddo);
     const float *src = (const float *)(wave < 2 ? a.q : a.dout) + row0 * ld + kvh * nh * HD;
     const float *stat_src = (wave < 2 ? a.lse : a.d) + row0 * a.n_heads + kvh * nh;
-    const unsigned dst = lds_addr((const char *)tiles[kg][0][wave / 2]) + wave % 2 * C * 1024;
+    const unsigned dst = lds_addr(tiles[kg][0][wave / 2]) + wave % 2 * C * 1024;
     const unsigned off_stat = lane < FT ? (unsigned)(lane * a.n_heads * 4) : kOOB;
     unsigned off[C];
 #pragma unroll
@@ -628,7 +628,7 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_dkv32_k(Wind
         for (int i = 0; i < C; ++i) dma16_at(rs, dst + buf * 2 * TILE * 4 + i * 1024, off[i]);
         if (wave % 2 == 0) {
             const sgpr4 r1 = rsrc4(stat_src + (long)q0 * a.n_heads + h, (unsigned)(((min(rows, FT) - 1) * a.n_heads + 1) * 4));
-            dma4_async(r1, stat[kg][buf][wave / 2], off_stat);
+            dma4_at(r1, lds_addr(stat[kg][buf][wave / 2]), off_stat);
         }
     };
     const T t(g, c);
