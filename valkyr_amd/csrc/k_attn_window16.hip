@@ -917,16 +917,18 @@ __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan p
 }
 
 // ── backward: dK and dV of the sinks from rows past their window ─────────
-// A wave holds 32 sinks' K and V in registers and streams 32-query tiles of its own (Q and dO, two
+// A wave holds 16 or 32 sinks' K and V in registers and streams 32-query tiles of its own (Q and dO, two
 // tiles in LDS, no barrier between the waves) from the first row past a sink's window to the last,
 // over the query heads of the KV head; the block's four waves and then the blocks' parts are added in
 // order.  The key blocks leave these pairs out: with them, the sink blocks' steps past the window, for
 // which three waves of four had nothing to do, took 1442 us of dK/dV to 1177 without (16384 tokens,
-// window 2048, 4 sinks, 32 / 8 heads of 128).
-template <int HD>
+// window 2048, 4 sinks, 32 / 8 heads of 128).  Bound by reading Q and dO
+// once more (51 us there, 5 TB/s); on shorter sequences by the chain of loads, steps and join (4 x 2048
+// tokens, window 512, 16 / 8 heads: 17 us; with 32 sinks a wave, 4 of them there, 20).
+template <int HD, int KS>
 __global__ __launch_bounds__(256, 1) void window_far16_k(WindowArgs a, DkvPlan plan) {
     using R = TileRows<HD>;
-    constexpr int KS = 2, QS = 2, BM = 32, TILE = BM * HD * 2, DS = HD / 32, DSUB = HD / 16, RPI = 512 / HD, C = BM / RPI;
+    constexpr int NK = 16 * KS, QS = 2, BM = 32, TILE = BM * HD * 2, DS = HD / 32, DSUB = HD / 16, RPI = 512 / HD, C = BM / RPI;
     __shared__ __attribute__((aligned(16))) char tiles[4][2][2 * TILE];
     __shared__ __attribute__((aligned(16))) float stat[4][2][2][64];  // LSE and D of a tile's rows
     __shared__ bf16x8 wl[4][64];
@@ -936,19 +938,9 @@ __global__ __launch_bounds__(256, 1) void window_far16_k(WindowArgs a, DkvPlan p
     const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c16 = lane % 16;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const Span s = span_of(a, b);
-    const int k0 = 32 * slice, nk = min(min(a.n_sink, s.kl) - k0, 32);  // this slice's sinks
+    const int k0 = NK * slice, nk = min(min(a.n_sink, s.kl) - k0, NK);  // this slice's sinks
     const float c2 = a.scale * LOG2E;
     const long row0 = (long)b * a.n_q, key0 = (long)b * a.n_kv;
-    bf16x8 kr[KS][DS], vr[KS][DS];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-        const long row = key0 + min(k0 + 16 * ks + c16, a.n_kv - 1);
-#pragma unroll
-        for (int ds = 0; ds < DS; ++ds) {
-            kr[ks][ds] = ld_frag((const bf16 *)a.k + row * a.ldk + kvh * HD + 8 * g + 32 * ds);
-            vr[ks][ds] = ld_frag((const bf16 *)a.v + row * a.ldv + kvh * HD + 8 * g + 32 * ds);
-        }
-    }
     unsigned qo[C], go[C];
 #pragma unroll
     for (int i = 0; i < C; ++i) {
@@ -981,6 +973,16 @@ __global__ __launch_bounds__(256, 1) void window_far16_k(WindowArgs a, DkvPlan p
     const int it0 = 4 * part + wave;
     if (it0 < n) dma(it0, 0);
     if (it0 + step < n) dma(it0 + step, 1);
+    bf16x8 kr[KS][DS], vr[KS][DS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        const long row = key0 + min(k0 + 16 * ks + c16, a.n_kv - 1);
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds) {
+            kr[ks][ds] = ld_frag((const bf16 *)a.k + row * a.ldk + kvh * HD + 8 * g + 32 * ds);
+            vr[ks][ds] = ld_frag((const bf16 *)a.v + row * a.ldv + kvh * HD + 8 * g + 32 * ds);
+        }
+    }
     for (int it = it0, buf = 0; it < n; it += step, buf ^= 1) {
         const int q0 = qstart + it / hpk * BM;
         const char *Qb = tiles[wave][buf], *Ob = Qb + TILE;
@@ -988,11 +990,9 @@ __global__ __launch_bounds__(256, 1) void window_far16_k(WindowArgs a, DkvPlan p
         if (it + step < n) wait_vm<2 * C + 2>();
         else wait_vm0();
         asm volatile("" ::: "memory");
-        // whether row q0 + x is past the window of key (ks, c16) and has a gradient
-        auto far = [&](int x, int ks) {
-            const int key = 16 * ks + c16;
-            return key < nk && q0 + x < s.ql && q0 + x + s.off - k0 - key >= a.window && L[x] != -INFINITY;
-        };
+        // whether row q0 + x is past the window of key (ks, c16); all rows' past all keys'
+        auto far = [&](int x, int ks) { return q0 + x < s.ql && q0 + x + s.off - k0 - 16 * ks - c16 >= a.window; };
+        const bool whole = q0 + BM <= s.ql && q0 + s.off - k0 - NK + 1 >= a.window;
         f32x4 sc[QS][KS], dp[QS][KS];
 #pragma unroll
         for (int qs = 0; qs < QS; ++qs)
@@ -1017,14 +1017,14 @@ __global__ __launch_bounds__(256, 1) void window_far16_k(WindowArgs a, DkvPlan p
                 const float l2 = L[x] * LOG2E, d = D[x];
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    const bool on = far(x, ks);
+                    const bool on = L[x] != -INFINITY && (whole || far(x, ks));  // (-inf: no gradient)
                     const float p = __builtin_amdgcn_exp2f(fmaf(sc[qs][ks][r], c2, -l2));
                     sc[qs][ks][r] = on ? p : 0.f;
                     dp[qs][ks][r] = on ? p * (dp[qs][ks][r] - d) : 0.f;
                 }
             }
         // the first tiles hold rows that are past some sinks' windows only
-        const bool odd = q0 + s.off < k0 + 31 + a.window && __any(scan<2 * TILE, 64>(Qb, lane));
+        const bool odd = !whole && __any(scan<2 * TILE, 64>(Qb, lane));
         bf16x8 pb[KS], sb[KS];
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -1034,9 +1034,9 @@ __global__ __launch_bounds__(256, 1) void window_far16_k(WindowArgs a, DkvPlan p
         if (odd) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                add_pairs<HD>(dvt[ks], Ob, pb[ks], wl[wave], lane, [&](int x) { return far(x, ks); });
+                add_pairs<HD>(dvt[ks], Ob, pb[ks], wl[wave], lane, [&](int x) { return L[x] != -INFINITY && far(x, ks); });
                 wave_lds();
-                add_pairs<HD>(dkt[ks], Qb, sb[ks], wl[wave], lane, [&](int x) { return far(x, ks); });
+                add_pairs<HD>(dkt[ks], Qb, sb[ks], wl[wave], lane, [&](int x) { return L[x] != -INFINITY && far(x, ks); });
                 wave_lds();
             }
         } else {
@@ -1055,26 +1055,26 @@ __global__ __launch_bounds__(256, 1) void window_far16_k(WindowArgs a, DkvPlan p
             dma(it + 2 * step, buf);
         }
     }
-    // the four waves' sums, each [dK, dV][32][HD] floats over its own tiles
+    // the four waves' sums, each [dK, dV][NK][HD] floats over its own tiles
     wave_lds();
-    static_assert(64 * HD * 4 <= (int)sizeof(tiles[0]), "a wave's sums fit its tiles");
+    static_assert(2 * NK * HD * 4 <= (int)sizeof(tiles[0]), "a wave's sums fit its tiles");
     float *mine = reinterpret_cast<float *>(tiles[wave]);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int i = 0; i < DSUB; ++i) {
             *reinterpret_cast<f32x4 *>(mine + (16 * ks + c16) * HD + 16 * i + 4 * g) = dkt[ks][i] * a.scale;
-            *reinterpret_cast<f32x4 *>(mine + (32 + 16 * ks + c16) * HD + 16 * i + 4 * g) = dvt[ks][i];
+            *reinterpret_cast<f32x4 *>(mine + (NK + 16 * ks + c16) * HD + 16 * i + 4 * g) = dvt[ks][i];
         }
     __syncthreads();
-    float *ws = a.ws + (long)nbk * plan.slots() * (2 * 128 * HD) + (((long)bk * plan.far_slices + slice) * plan.far_parts + part) * (64 * HD);
+    float *ws = a.ws + (long)nbk * plan.slots() * (2 * 128 * HD) + (((long)bk * plan.far_slices + slice) * plan.far_parts + part) * (2 * NK * HD);
 #pragma unroll
-    for (int i = 0; i < 64 * HD / 1024; ++i) {
+    for (int i = 0; i < 2 * NK * HD / 1024; ++i) {
         const int x = (i * 256 + tid) * 4;
         f32x4 t{0, 0, 0, 0};
 #pragma unroll
         for (int w = 0; w < 4; ++w) t += *reinterpret_cast<const f32x4 *>(reinterpret_cast<const float *>(tiles[w]) + x);
-        if (x / HD % 32 >= nk) t = f32x4{0, 0, 0, 0};
+        if (x / HD % NK >= nk) t = f32x4{0, 0, 0, 0};
         *reinterpret_cast<f32x4 *>(ws + x) = t;
     }
 }
@@ -1178,7 +1178,9 @@ bool window16_backward(const WindowArgs &a, hipStream_t st) {
         WindowArgs near = a;
         if (plan.far_parts) {
             near.n_sink = 0;
-            hipLaunchKernelGGL((window_far16_k<HD>), dim3((unsigned)(nbk * plan.far_slices * plan.far_parts)), dim3(256), 0, st, a, plan);
+            const dim3 grid((unsigned)(nbk * plan.far_slices * plan.far_parts));
+            if (plan.far_keys == 16) hipLaunchKernelGGL((window_far16_k<HD, 1>), grid, dim3(256), 0, st, a, plan);
+            else hipLaunchKernelGGL((window_far16_k<HD, 2>), grid, dim3(256), 0, st, a, plan);
         }
         hipLaunchKernelGGL((window_dkv16_k<HD, TO>), dim3((unsigned)(nbk * plan.blocks())), dim3(512), 0, st, near, plan);
         launch_dkv_sum<HD, 128, TO>(a, plan, st);

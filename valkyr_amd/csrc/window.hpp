@@ -303,8 +303,8 @@ struct DkvPlan {
     int sink_parts, parts;         // launched blocks per sink block, per other block
     int keys;
     // pairs of a sink and a row past its window: blocks of their own (0: the key blocks take them) per
-    // slice of 32 sinks, so that no key block has more steps than the others
-    int far_parts, far_slices;
+    // slice of far_keys sinks, so that no key block has more steps than the others
+    int far_parts, far_slices, far_keys;
     __host__ __device__ int blocks() const { return sink_blocks * sink_parts + (key_blocks - sink_blocks) * parts; }
     // slots of partial sums per KV head: those of the sink blocks, those of the others
     __host__ __device__ int sink_slots() const { return sink_parts > 1 || far_parts ? sink_blocks * sink_parts : 0; }
@@ -336,7 +336,7 @@ struct Steps {
     }
 };
 // dK and dV of the split key blocks: their parts and then those of the far pairs ([pair][slice][part] of
-// [dK, dV][32][HD] behind the key blocks' slots) added in order, four values a thread.
+// [dK, dV][far_keys][HD] behind the key blocks' slots) added in order, four values a thread.
 template <int HD, int BN, class TO>
 __global__ __launch_bounds__(256) void window_dkv_sum_k(WindowArgs a, DkvPlan plan) {
     const int nbk = a.n_batch * a.n_kv_heads;
@@ -352,11 +352,12 @@ __global__ __launch_bounds__(256) void window_dkv_sum_k(WindowArgs a, DkvPlan pl
     f32x4 t{0, 0, 0, 0};
 #pragma unroll 8
     for (int p = 0; p < parts; ++p) t += *reinterpret_cast<const f32x4 *>(ws + (long)p * 2 * BN * HD + x);
-    if (key / 32 < plan.far_slices) {
+    if (plan.far_parts && key / plan.far_keys < plan.far_slices) {
+        const int fk = plan.far_keys;
         const float *far = a.ws + (long)nbk * plan.slots() * (2 * BN * HD) +
-                           ((long)bk * plan.far_slices + key / 32) * plan.far_parts * (64 * HD) + (v ? 32 * HD : 0) + y % (32 * HD);
+                           ((long)bk * plan.far_slices + key / fk) * plan.far_parts * (2 * fk * HD) + (v ? fk * HD : 0) + key % fk * HD + y % HD;
 #pragma unroll 8
-        for (int p = 0; p < plan.far_parts; ++p) t += *reinterpret_cast<const f32x4 *>(far + (long)p * 64 * HD);
+        for (int p = 0; p < plan.far_parts; ++p) t += *reinterpret_cast<const f32x4 *>(far + (long)p * 2 * fk * HD);
     }
     if (key >= a.n_kv) return;
     const long row = (long)b * a.n_kv + key;
@@ -426,7 +427,7 @@ inline DkvPlan dkv_plan(const WindowArgs &a, bool ws, int keys, long cu_blocks, 
     p.key_blocks = (a.n_kv + keys - 1) / keys;
     p.sink_blocks = a.window < a.n_kv ? std::min(p.key_blocks, (a.n_sink + keys - 1) / keys) : 0;
     p.sink_parts = p.parts = 1;
-    p.far_parts = p.far_slices = 0;
+    p.far_parts = p.far_slices = p.far_keys = 0;
     if (!ws) return p;
     const long nbk = (long)a.n_batch * a.n_kv_heads, blocks = nbk * p.key_blocks, hpk = a.n_heads / a.n_kv_heads;
     const long most = hpk * ((a.n_q + 31) / 32), usual = std::min(most, hpk * ((std::min<long>(a.n_kv, a.window) + keys + 31) / 32));
@@ -435,7 +436,8 @@ inline DkvPlan dkv_plan(const WindowArgs &a, bool ws, int keys, long cu_blocks, 
     while (p.parts > 1 && blocks * slot * p.parts > (64l << 20)) --p.parts;
     if (far && p.sink_blocks && a.n_sink <= 128) {
         p.sink_parts = p.parts;
-        p.far_slices = (a.n_sink + 31) / 32;
+        p.far_keys = a.n_sink > 16 ? 32 : 16;
+        p.far_slices = (a.n_sink + p.far_keys - 1) / p.far_keys;
         // four waves a CU in all, while each keeps three steps
         p.far_parts = (int)std::max(1l, std::min(256 / (nbk * p.far_slices), most / 12));
         return p;
@@ -449,7 +451,7 @@ inline DkvPlan dkv_plan(const WindowArgs &a, bool ws, int keys, long cu_blocks, 
 }
 inline size_t dkv_ws_bytes(const WindowArgs &a, const DkvPlan &p) {
     const size_t nbk = (size_t)a.n_batch * a.n_kv_heads;
-    return nbk * ((size_t)p.slots() * p.keys + (size_t)p.far_slices * p.far_parts * 32) * 2 * a.hd * sizeof(float);
+    return nbk * ((size_t)p.slots() * p.keys + (size_t)p.far_slices * p.far_parts * p.far_keys) * 2 * a.hd * sizeof(float);
 }
 template <int HD, int BN, class TO>
 void launch_dkv_sum(const WindowArgs &a, const DkvPlan &p, hipStream_t st) {
