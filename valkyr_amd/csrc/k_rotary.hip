@@ -58,13 +58,16 @@ VKH_DEV void store_v(float *p, const float (&o)[V]) {
     for (int i = 0; i < V; i += 4)
         *reinterpret_cast<float4 *>(p + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
 }
+// Past the caches: what is written is read by another kernel, and each store covers whole lines over its
+// lanes (16384 rows, 32 / 8 heads of 128: norm and rotation 69 us through the caches, 62 past them, their backward
+// 112 and 102; fp32 stores of 8 values a lane, in two halves, go through them).
 template <int V>
 VKH_DEV void store_v(bf16 *p, const float (&o)[V]) {
     typedef bf16 vec __attribute__((ext_vector_type(V)));
     vec f;
 #pragma unroll
     for (int i = 0; i < V; ++i) f[i] = (bf16)o[i];
-    *reinterpret_cast<vec *>(p) = f;
+    __builtin_nontemporal_store(f, reinterpret_cast<vec *>(p));
 }
 
 // gains (any alignment)
@@ -109,12 +112,12 @@ VKH_DEV float row_sum(float v, int LP) {
     return v;
 }
 
-// Lane t of a head row: its two chunks start at values e0 and e1.
+// Lane t of a head row: its two chunks start at values e0 and e1, of the turned part's halves or of the
+// rest's: what a load or store of one chunk touches is contiguous over the lanes of either part.
 VKH_DEV void chunks(const RotaryArgs &a, int t, int V, int &e0, int &e1) {
-    const bool turned = 2 * t * V < a.rot;
-    e0 = 2 * t * V;
-    e1 = e0 + V;
-    if (!a.interleaved && turned) e0 = t * V, e1 = a.rot / 2 + t * V;
+    const int lo = 2 * t * V < a.rot ? 0 : a.rot, n = lo ? a.hd - a.rot : a.rot;
+    e0 = lo + t * V - lo / 2;
+    e1 = e0 + n / 2;
 }
 
 // The cosines and sines of a row for the V pairs of each lane: a wave computes one pair a lane and
@@ -125,8 +128,10 @@ VKH_DEV void row_angles(const RotaryArgs &a, unsigned pos, float2 *sh, int lane,
     for (int j = lane; j < a.rot / 2; j += 64) sh[j] = cos_sin(a, pos, j);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (2 * t * V < a.rot) {
+        // half layout: pairs t V ..; neighbours: half of them in either chunk
+        const int p0 = a.interleaved ? t * V / 2 : t * V, p1 = a.interleaved ? a.rot / 4 + p0 : p0 + V / 2;
 #pragma unroll
-        for (int i = 0; i < V; ++i) cs[i] = sh[t * V + i];
+        for (int i = 0; i < V / 2; ++i) cs[i] = sh[p0 + i], cs[V / 2 + i] = sh[p1 + i];
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) cs[i] = make_float2(1.f, 0.f);
@@ -136,8 +141,9 @@ VKH_DEV void row_angles(const RotaryArgs &a, unsigned pos, float2 *sh, int lane,
 // Forward of both operators, and the rotary backward (a.sign = -1, dy in, dx out).  HS waves share
 // a row (4 where rows are few: one token's latency; 1 where they fill the chip), 64 / LP heads at a
 // time; the next heads' values are on their way while the present ones are turned.
-// 16384 rows, 32 / 8 heads of 128, bf16 (0.34 GB): 71 us a rotation (4.7 TB/s), 68 with the norm; a
-// block per 4 rows over a flat list of heads took 73 and 105.
+// 16384 rows, 32 / 8 heads of 128, bf16 (0.34 GB): 68 us a rotation of 64 neighbouring pairs' values (4.9
+// TB/s; 71 with both chunks of a lane side by side), 62 with the norm (5.4 TB/s); a block per 4 rows over a
+// flat list of heads took 73 and 105.
 template <class TX, class TY, int V, bool NORM>
 __global__ __launch_bounds__(RNT) void rotary_fwd_k(RotaryArgs a, int HS, int LP) {
     __shared__ float2 sh[RNT / 64][128];
@@ -208,7 +214,7 @@ __global__ __launch_bounds__(RNT) void rotary_fwd_k(RotaryArgs a, int HS, int LP
 // head row), and registers for more waves.  A wave walks rows, 64 / LP heads at a time; the next
 // heads' values, also the next row's, are on their way while the present ones are worked on.  A
 // block's sums go to its row of `partial` ([blocks][hd]), which rotary_dw_k adds in block order.
-// 16384 rows, 32 / 8 heads of 128, bf16 (0.5 GB): 117 us, 4.3 TB/s; rotary_dw_k 6.
+// 16384 rows, 32 / 8 heads of 128, bf16 (0.5 GB): 102 us, 4.9 TB/s; rotary_dw_k 6.
 template <class TX, class TG, class TD, int V>
 __global__ __launch_bounds__(RNT) void rotary_norm_bwd_k(RotaryArgs a, int LP, RotaryParts parts, float *partial) {
     __shared__ float2 sh[RNT / 64][128];
@@ -477,8 +483,8 @@ void by_type(DType d, F f) {
 }  // namespace
 
 // Blocks of each side: five a CU in all (as many as fit at 4-value chunks), shared by the sides'
-// heads, at most one a wave's row.  16384 rows, 32 / 8 heads of 128, bf16: 114 us; 8-value chunks fill
-// the registers with three a CU and take 123; 2048 rows, 16 / 8 heads, fp32 to bf16: 14 against 18.
+// heads, at most one a wave's row.  16384 rows, 32 / 8 heads of 128, bf16, as first measured: 114 us; 8-value
+// chunks fill the registers with three a CU and take 123; 2048 rows, 16 / 8 heads, fp32 to bf16: 14 against 18.
 RotaryParts rotary_parts(const RotaryArgs &a) {
     const long H = a.nh[0] + a.nh[1], rows = (a.n_rows + RNT / 64 - 1) / (RNT / 64);
     auto of = [&](int nh) { return nh ? (int)std::max(1l, std::min(rows, 1280 * nh / H)) : 0; };
