@@ -444,3 +444,47 @@ def test_qk_norm_rotary_on_a_captured_stream():
     graph = C.c_void_p()
     assert lib().hipStreamEndCapture(st.handle, C.byref(graph)) == 0 and lib().hipGraphDestroy(graph) == 0
     assert name == "InvalidArgument"
+
+
+@pytest.mark.gpu
+def test_rows_past_two_to_the_31_bytes():
+    """The last rows of bf16 matrices of 2.2e9 bytes: norm and rotation in place, and their backward in place
+    of the gradient; the rows before them are zeros and stay so."""
+    from valkyr_amd import kernels as K
+    from valkyr_amd._lib import check, lib
+    from valkyr_amd.device import DeviceBuffer, bf16_bits_to_f32, f32_to_bf16_bits
+
+    rows, n, nh, hd, pos0 = 270_000, 16, 32, 128, 77
+    rng, row = np.random.default_rng(8), nh * hd * 2
+    note("rotary on 2.2e9 bytes")
+
+    def make():
+        buf, bits = DeviceBuffer.zeros(rows * row), f32_to_bf16_bits(rng.standard_normal((n, nh * hd)).astype(np.float32))
+        check(lib().vkh_memcpy_h2d(buf.offset((rows - n) * row), bits.ctypes.data, bits.nbytes))
+        return buf, bf16_bits_to_f32(bits).astype(np.float64).reshape(n, nh, hd)
+
+    def last(buf):
+        got = np.empty((n, nh * hd), np.uint16)
+        check(lib().vkh_memcpy_d2h(got.ctypes.data, buf.offset((rows - n) * row), got.nbytes))
+        return bf16_bits_to_f32(got).astype(np.float64).reshape(n, nh, hd)
+
+    (x, vx), (dy, vdy) = make(), make()
+    w = rng.uniform(0.5, 1.5, hd).astype(np.float32)
+    p = K.rotary_params(rows, nh, 0, hd, pos0=pos0, x_dtype=1, y_dtype=1, dy_dtype=1, dx_dtype=1)
+    plan, (f, a), dw = plan_of(hd), frequencies(hd, 1e4), dev(np.zeros(hd, np.float32))
+    pos = pos0 + np.arange(rows - n, rows)
+    xh, r, g = norm64(vx, w.astype(np.float64), 1e-6, False)
+    K.qk_norm_rotary_backward(p, plan, dev(w), None, x, None, dy, None, dy, None, dw)
+    t = turn(vdy, pos, f, a, 0, True)
+    ref = r * (t * g - xh * (t * g * xh).mean(-1, keepdims=True))
+    assert np.linalg.norm(last(dy) - ref) <= (U16 + 100 * U) * np.linalg.norm(ref)
+    dref = (t * xh).sum((0, 1))
+    assert np.linalg.norm(host(dw) - dref) <= 1e-5 * np.linalg.norm(dref)
+    K.qk_norm_rotary_forward(p, plan, dev(w), None, x, x)
+    ref = turn(xh * g, pos, f, a, 0)
+    assert np.linalg.norm(last(x) - ref) <= (U16 + 100 * U) * np.linalg.norm(ref)
+    for buf in (x, dy):
+        some = np.ones((64, nh * hd), np.uint16)
+        for at in (0, rows // 2, rows - n - 64):
+            check(lib().vkh_memcpy_d2h(some.ctypes.data, buf.offset(at * row), some.nbytes))
+            assert not (some & 0x7fff).any()

@@ -545,6 +545,80 @@ def test_a_cache_past_two_to_the_31_bytes():
 
 
 @pytest.mark.gpu
+def test_rows_at_the_end_of_a_cache_past_two_to_the_31_bytes():
+    """The last 100 rows of a bf16 sequence of 2^20 + 5 keys, forward and backward: offsets of K, V and their
+    gradients pass 31 bits, and keys that no row sees get gradients of zero."""
+    from valkyr_amd import kernels as K
+    from valkyr_amd._lib import check, lib
+    from valkyr_amd.device import DeviceBuffer, f32_to_bf16_bits
+
+    nq, nk, H, Hkv, hd, window, sinks = 100, (1 << 20) + 5, 16, 8, 128, 300, 3
+    rng, row = np.random.default_rng(3), Hkv * hd * 2
+    note("window attention at the end of 2 GiB")
+    at = np.concatenate([np.arange(sinks), np.arange(nk - window - nq, nk)])  # the keys that count
+    cache, vals = [DeviceBuffer.zeros(nk * row) for _ in range(2)], []
+    for buf in cache:
+        bits = f32_to_bf16_bits(rng.standard_normal((len(at), Hkv * hd)).astype(np.float32))
+        for lo, part in ((0, bits[:sinks]), (nk - window - nq, bits[sinks:])):
+            part = np.ascontiguousarray(part)
+            check(lib().vkh_memcpy_h2d(buf.offset(lo * row), part.ctypes.data, part.nbytes))
+        vals.append((bits.astype(np.uint32) << 16).view(np.float32).astype(np.float64).reshape(-1, Hkv, hd))
+    (bq, q), (bdo, do) = (bf16_dev(rng.standard_normal((nq, H * hd))) for _ in range(2))
+    q, do = (np.asarray(x, np.float64).reshape(nq, H, hd) for x in (q, do))
+    f32 = lambda n: dev(np.zeros(n, np.float32))  # noqa: E731
+    o, dq, lse, d = f32(nq * H * hd), f32(nq * H * hd), f32(nq * H), f32(nq * H)
+    grads = [DeviceBuffer.zeros(nk * row * 2) for _ in range(2)]  # fp32: past 2^32 bytes
+    unseen, sevens = (sinks, 1 << 18, nk // 2, nk - window - nq - 64), np.full((64, Hkv * hd), 7.0, np.float32)
+    for buf in grads:
+        for lo in unseen:
+            check(lib().vkh_memcpy_h2d(buf.offset(lo * row * 2), sevens.ctypes.data, sevens.nbytes))
+    p = K.window_params(nq, nk, H, Hkv, hd, window, sinks, dtype=K.BF16, out_dtype=K.F32)
+    K.fa_window_forward(p, bq, *cache, o, lse)
+    K.fa_window_backward(p, bq, *cache, o, bdo, lse, d, dq, *grads)
+    t = np.arange(nk - nq, nk)[:, None]
+    see = (at <= t) & ((at > t - window) | (at < sinks))
+    ref = attention64(q, *vals, do, see, 1 / math.sqrt(hd))
+    assert rel_l2(ref["o"], host(o)) <= U16
+    assert rel_l2(ref["dq"], host(dq)) <= 2 * U16
+    for n, buf in zip(("dk", "dv"), grads):
+        for lo, part in ((0, ref[n][:sinks]), (nk - window - nq, ref[n][sinks:])):
+            got = np.empty(part.shape, np.float32)
+            check(lib().vkh_memcpy_d2h(got.ctypes.data, buf.offset(lo * row * 2), got.nbytes))
+            assert rel_l2(part, got) <= 2 * U16, n
+        for lo in unseen:
+            got = np.ones((64, Hkv * hd), np.float32)
+            check(lib().vkh_memcpy_d2h(got.ctypes.data, buf.offset(lo * row * 2), got.nbytes))
+            assert not got.any(), (n, lo)
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once():
+    """Calls of few rows and a training pass that both split their work, queued on two streams without
+    workspaces: the results of the same calls alone."""
+    from valkyr_amd.device import Stream, synchronize
+
+    calls = [Call(2, 1, 3000, 8, 2, 128, 1500, 4, "bf16"), Call(1, 300, 300, 4, 2, 64, 90, 2, "bf16", seed=1)]
+    alone = []
+    for c in calls:
+        c.forward()
+        c.backward()
+        alone.append(c.read())
+    streams = [Stream(), Stream()]
+    for c in calls:
+        c.out = {n: c.empty(n) for n in c.out}
+    synchronize()
+    for _ in range(5):
+        for c, st in zip(calls, streams):
+            c.forward(stream=st)
+            c.backward(stream=st)
+    synchronize()
+    for c, want in zip(calls, alone):
+        got = c.read()
+        for n in want:
+            assert np.array_equal(got[n], want[n]), n
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("form", ["fp32", "bf16"])
 def test_the_operators_as_a_layer_runs_them(form):
     """q|k|v rows of a projection -> norm and rotation -> windowed attention, and backward to the rows and
