@@ -1101,8 +1101,9 @@ bool bwd_ok(const WindowArgs &a) {
 bool few_rows(const WindowArgs &a) { return few_rows_of(a, 192, 1536); }
 // two rounds of one block per CU
 int splits16(const WindowArgs &a) { return step_splits(a, 32, 512); }
-// dK/dV: one block per CU, at least four steps of both groups each
-DkvPlan plan16(const WindowArgs &a, bool ws) { return dkv_plan(a, ws, 128, 256, 8, 8, true); }
+// dK/dV: one block per CU, at least two steps of both groups each (of four / of two, backward in us: 2 x 2989
+// tokens, window 9, 3 / 1 heads: 64 / 55; 300 tokens, 8 / 4 heads of 64: 25 / 23; 4 x 430, 4 / 4 heads: 37 / 38)
+DkvPlan plan16(const WindowArgs &a, bool ws) { return dkv_plan(a, ws, 128, 256, 8, 4, true); }
 
 // Two groups of waves a block where the chip has at most one block a CU (up to two: 1 x 4096 tokens, window
 // 512, 8 / 8 heads of 128, 512 blocks: forward 30 us with two groups, 24 with one).

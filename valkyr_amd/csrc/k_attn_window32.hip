@@ -734,7 +734,10 @@ int splits32(const WindowArgs &a) { return step_splits(a, 16, 1024); }
 // of 64: 60 / 211 and 57 / 179; 4 x 1024 tokens, 16 / 8 heads of 64, window 256 (1024 blocks): 51 / 212 and 55 / 215.
 bool grouped(const WindowArgs &a) { return (long)a.n_heads * a.n_batch * ((a.n_q + 63) / 64) <= 512; }
 bool grouped_dkv(const WindowArgs &a) { return (long)a.n_kv_heads * a.n_batch * ((a.n_kv + 63) / 64) <= 512; }
-DkvPlan plan32(const WindowArgs &a, bool ws) { return dkv_plan(a, ws, 64, 512, 16, grouped_dkv(a) ? 4 : 2, false); }
+// Parts of two steps (backward in us, parts of four / of two: 50 tokens, 4 / 2 heads of 128: 41 / 33; 2 x 92, 16 / 8
+// heads: 55 / 42), as many as the CUs take at once: two blocks each, one of two groups of 128-wide heads (2 x 473
+// tokens, window 18, 16 / 8 heads, one sink: 70 us, with parts for two a CU 90).
+DkvPlan plan32(const WindowArgs &a, bool ws) { return dkv_plan(a, ws, 64, grouped_dkv(a) && a.hd == 128 ? 256 : 512, 16, 2, false); }
 
 }  // namespace
 

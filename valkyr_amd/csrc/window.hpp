@@ -443,9 +443,12 @@ inline DkvPlan dkv_plan(const WindowArgs &a, bool ws, int keys, long cu_blocks, 
         return p;
     }
     // A sink block's steps over the usual block's; the sink blocks start first, so a part may take as
-    // long as the rounds of the others.
-    const double rounds = std::max(1.0, (double)blocks * p.parts / cu_blocks);
-    p.sink_parts = (int)std::max(1.0, std::min(64.0, ceil((double)most / usual * p.parts / rounds)));
+    // long as the rounds of the others.  Fewer parts where they would not all start at once.
+    for (;; --p.parts) {
+        const double rounds = std::max(1.0, (double)blocks * p.parts / cu_blocks);
+        p.sink_parts = p.sink_blocks ? (int)std::max(1.0, std::min(64.0, ceil((double)most / usual * p.parts / rounds))) : 1;
+        if (p.parts == 1 || nbk * p.blocks() <= cu_blocks) break;
+    }
     while (p.sink_parts > 1 && p.sink_blocks * nbk * slot * p.sink_parts > (192l << 20)) --p.sink_parts;
     return p;
 }
