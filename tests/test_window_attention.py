@@ -271,6 +271,8 @@ LARGER = [
     (1, 700, 700, 32, 8, 64, 130, 3),
     (1, 1100, 1100, 32, 8, 128, 600, 70),
     (1, 1100, 1100, 32, 32, 64, 90, 1),
+    (2, 520, 520, 32, 32, 64, 40, 40),
+    (1, 1030, 1030, 32, 32, 128, 200, 100),
     (1, 90, 2000, 4, 2, 128, 1900, 70),
     (2, 200, 1700, 3, 1, 64, 0, 0),
     (1, 40, 700, 8, 4, 64, 300, 5),
@@ -300,7 +302,8 @@ def test_larger_calls(shape, form, ragged):
 @pytest.mark.gpu
 @pytest.mark.parametrize("bad", [np.nan, -np.inf])
 @pytest.mark.parametrize("form", ["fp32", "bf16"])
-@pytest.mark.parametrize("shape", [(1, 1100, 1100, 32, 8, 64, 600, 3), (1, 700, 700, 32, 32, 128, 48, 2), (1, 90, 2000, 4, 2, 128, 1600, 3),
+@pytest.mark.parametrize("shape", [(1, 1100, 1100, 32, 8, 64, 600, 3), (1, 700, 700, 32, 32, 128, 48, 2), (1, 1100, 1100, 32, 32, 64, 90, 40),
+                                   (1, 90, 2000, 4, 2, 128, 1600, 3),
                                    (1, 40, 700, 4, 2, 64, 250, 1)], ids=lambda s: "-".join(str(x) for x in s))
 def test_what_is_not_seen_reaches_nothing_in_larger_calls(shape, form, bad):
     """As below, on the larger calls' kernels: one key's and one query's rows hold infinities or NaN."""

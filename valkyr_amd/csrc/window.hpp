@@ -434,20 +434,26 @@ inline DkvPlan dkv_plan(const WindowArgs &a, bool ws, int keys, long cu_blocks, 
     const long slot = 2l * keys * a.hd * 4;
     p.parts = (int)std::max(1l, std::min({most_parts, cu_blocks / blocks, usual / least}));
     while (p.parts > 1 && blocks * slot * p.parts > (64l << 20)) --p.parts;
-    if (far && p.sink_blocks && a.n_sink <= 128) {
-        p.sink_parts = p.parts;
+    // A sink block's steps over the usual block's; the sink blocks start first, so a part may take as
+    // long as the rounds of the others.  Fewer parts where they would not all start at once.
+    const int parts = p.parts;
+    for (;; --p.parts) {
+        const double rounds = std::max(1.0, (double)blocks * p.parts / cu_blocks);
+        p.sink_parts = p.sink_blocks ? (int)std::max(1.0, std::min(64.0, ceil((double)most / usual * p.parts / rounds))) : 1;
+        if (p.parts == 1 || nbk * p.blocks() <= cu_blocks) break;
+    }
+    // Far pairs apart (two launches, 15 to 20 us) where the sink blocks' parts do not all start at once or take
+    // many steps from the others.  Backward in us, with the sink blocks / apart: 3 x 21 tokens, window 13: 16 / 27;
+    // 2 x 1001, window 256, 16 / 4 heads of 128: 59 / 67; 2048, window 16, 16 / 8 heads: 44 / 58; 4 x 1001, window
+    // 256, 16 / 8 heads: 103 / 95; 4 x 2048, window 16: 130 / 119; 4000, window 1024, 100 sinks: 213 / 180.
+    if (far && p.sink_blocks && a.n_sink <= 128 &&
+        (nbk * p.blocks() > cu_blocks || usual * (1.0 / p.parts - 1.0 / parts) > 24)) {
+        p.sink_parts = p.parts = parts;
         p.far_keys = a.n_sink > 16 ? 32 : 16;
         p.far_slices = (a.n_sink + p.far_keys - 1) / p.far_keys;
         // four waves a CU in all, while each keeps three steps
         p.far_parts = (int)std::max(1l, std::min(256 / (nbk * p.far_slices), most / 12));
         return p;
-    }
-    // A sink block's steps over the usual block's; the sink blocks start first, so a part may take as
-    // long as the rounds of the others.  Fewer parts where they would not all start at once.
-    for (;; --p.parts) {
-        const double rounds = std::max(1.0, (double)blocks * p.parts / cu_blocks);
-        p.sink_parts = p.sink_blocks ? (int)std::max(1.0, std::min(64.0, ceil((double)most / usual * p.parts / rounds))) : 1;
-        if (p.parts == 1 || nbk * p.blocks() <= cu_blocks) break;
     }
     while (p.sink_parts > 1 && p.sink_blocks * nbk * slot * p.sink_parts > (192l << 20)) --p.sink_parts;
     return p;
