@@ -270,6 +270,8 @@ def test_lengths_and_strides(nq, nk, window, sinks, ql, kl, hd, pad, form):
 LARGER = [
     (1, 700, 700, 32, 8, 64, 130, 3),
     (1, 1100, 1100, 32, 8, 128, 600, 70),
+    (1, 1100, 1100, 64, 8, 128, 600, 70),
+    (1, 1100, 1100, 64, 16, 64, 700, 3),
     (1, 1100, 1100, 32, 32, 64, 90, 1),
     (2, 520, 520, 32, 32, 64, 40, 40),
     (1, 1030, 1030, 32, 32, 128, 200, 100),
@@ -302,7 +304,7 @@ def test_larger_calls(shape, form, ragged):
 @pytest.mark.gpu
 @pytest.mark.parametrize("bad", [np.nan, -np.inf])
 @pytest.mark.parametrize("form", ["fp32", "bf16"])
-@pytest.mark.parametrize("shape", [(1, 1100, 1100, 32, 8, 64, 600, 3), (1, 700, 700, 32, 32, 128, 48, 2), (1, 1100, 1100, 32, 32, 64, 90, 40),
+@pytest.mark.parametrize("shape", [(1, 1100, 1100, 32, 8, 64, 600, 3), (1, 1100, 1100, 64, 8, 128, 600, 3), (1, 700, 700, 32, 32, 128, 48, 2), (1, 1100, 1100, 32, 32, 64, 90, 40),
                                    (1, 90, 2000, 4, 2, 128, 1600, 3),
                                    (1, 40, 700, 4, 2, 64, 250, 1)], ids=lambda s: "-".join(str(x) for x in s))
 def test_what_is_not_seen_reaches_nothing_in_larger_calls(shape, form, bad):

@@ -1136,9 +1136,12 @@ bool window16_forward(const WindowArgs &a, hipStream_t st) {
         return true;
     }
     const long per = (long)a.n_heads * a.n_batch;
-    // grids of 128-row blocks that leave the CUs one block each or fewer take 64 rows (2 x 1001 tokens,
-    // window 256, 16 / 4 heads, 256 blocks: 25.8 us with 128 rows, 16.8 with 64)
-    const bool small = per * ((a.n_q + 127) / 128) <= cu_count(), pairs = grouped(a);
+    // 64-row blocks where 128-row ones would be two a CU or fewer, with small windows (more of whose tiles are
+    // masked in part) four of 128-wide heads.  With 128 / 64 rows, us: 5000 tokens, window 256, 8 / 8 heads of 64 (320
+    // blocks of 128): 16 / 12; 3377, window 2000, 16 / 8 heads of 128 (432): 67 / 60; 4 x 2048 (1024), windows 64, 256,
+    // 512, 2048: 35.5 / 32.5, 47 / 43, 61 / 59, 94 / 100, heads of 64, window 512: 33 / 37; 16384, window 256: 173 / 196.
+    const long blocks = per * ((a.n_q + 127) / 128);
+    const bool small = blocks <= 2l * cu_count() || (a.hd == 128 && a.window <= 512 && blocks <= 4l * cu_count()), pairs = grouped(a);
     auto go = [&](auto kernel, int bm, int kg) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)(per * ((a.n_q + bm - 1) / bm))), dim3(256 * kg), 0, st, a);
     };
@@ -1162,10 +1165,11 @@ bool window16_backward(const WindowArgs &a, hipStream_t st) {
     const long per = (long)a.n_heads * a.n_batch, nbk = (long)a.n_batch * a.n_kv_heads;
     // 128-row dQ blocks on 4 waves, two a CU (256 rows on 8 waves, one a CU, wait for each other over
     // twice the span of masked tiles: 16384 tokens, window 2048, 996 against 881 us; 4 x 2048, window
-    // 512, 112 against 90); 64 rows where those leave CUs idle, and on windows whose tiles are masked
-    // in large part (backward of 16384 tokens, window 256, 621 against 596 us; 4 x 2048, window 512,
-    // 224 against 222; window 1024, 294 against 298)
-    const int bq = per * ((a.n_q + 127) / 128) >= 256 && a.window > 512 ? 128 : 64;
+    // 512, 112 against 90); 64 rows where those would be less than two a CU (backward of 3377 tokens, window
+    // 2000, 16 / 8 heads: 227 us with 128, 219 with 64; of 2 x 4096, window 800, 8 / 4 heads, 512 blocks of
+    // 128: 140 and 146), and on windows whose tiles are masked in large part (16384 tokens, window 256, 621
+    // and 596; 4 x 2048, window 512, 224 and 222; window 1024, 294 and 298)
+    const int bq = per * ((a.n_q + 127) / 128) >= 2l * cu_count() && a.window > 512 ? 128 : 64;
     const DkvPlan plan = plan16(a, a.ws != nullptr);
     auto by = [&](auto hd, auto to) {
         constexpr int HD = decltype(hd)::value;
