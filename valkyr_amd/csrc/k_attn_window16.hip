@@ -457,7 +457,7 @@ __global__ __launch_bounds__(256, 1) void window_step16_k(WindowArgs a, int spli
 // D = rowsum(O dO) of the block's rows is formed first (fp64 sums of the bf16 products) and
 // stored for the dK/dV kernel, which runs after this one.  As the forward, it is bound by what a wave
 // does between its products (softmax, rounding, LDS reads) and by masked tiles: 16384 tokens, window
-// 2048, 32 / 8 heads of 128: 780 us, 0.99 PFLOP/s; 4 x 2048, window 512, 16 / 8 heads: 78 us, 0.58 PFLOP/s.  KG = 2 (short
+// 2048, 32 / 8 heads of 128: 760 us, 1.02 PFLOP/s; 4 x 2048, window 512, 16 / 8 heads: 77 us, 0.59 PFLOP/s.  KG = 2 (short
 // grids: one block a CU): two groups of waves take every other tile; 2048 tokens, window 2048, 8 / 8
 // heads of 64, forward / backward: 24.8 / 73 us without, 19.3 / 63 with.
 template <int HD, int BQ, int KG, class TO>
@@ -660,13 +660,14 @@ __global__ __launch_bounds__(256 * KG, 2) void window_dq16_k(WindowArgs a) {
 // share the KV head: group 0 every other head, group 1 the rest, or for an odd number of heads
 // alternate query tiles of every head.  Each group streams its Q and dO tiles through three
 // buffers.  Query tiles run from the first row that sees the block's first key to the last in
-// its window, or to the last row of all where the block holds sinks; such a block has a share of
-// work as many times the others' as the sequence is longer than the window, and is split between
-// `parts` blocks, as all blocks are where they are too few for the chip.  Parts write fp32 sums
+// its window, or to the last row of all where the block holds sinks (unless window_far16_k takes
+// the rows past their window); such a block has a share of work as many times the others' as the
+// sequence is longer than the window, and is split between `sink_parts` blocks, as the others are between
+// `parts` where they are too few for the chip.  Parts write fp32 sums
 // to their slots of a.ws, which window_dkv_sum_k adds in order.  Bound by the one block a CU that
 // the dK and dV accumulators (2 x 32 x HD a wave) and their registers leave: eight waves, half of whose
-// time goes to waiting for each other and for LDS.  16384 tokens, window 2048, 32 / 8 heads of 128: 1160
-// us, 0.89 PFLOP/s; 4 x 2048, window 512, 16 / 8 heads: 112 us, 0.54 PFLOP/s.
+// time goes to waiting for each other and for LDS.  16384 tokens, window 2048, 32 / 8 heads of 128: 1140
+// us, 0.91 PFLOP/s; 4 x 2048, window 512, 16 / 8 heads: 112 us, 0.54 PFLOP/s.
 template <int HD, class TO>
 __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan plan) {
     using R = TileRows<HD>;

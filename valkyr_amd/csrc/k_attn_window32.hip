@@ -11,7 +11,7 @@
 // coarsely, and each product would wait for the one before).  Bound by the fp32 matrix cores, and on
 // short sequences by the few steps that each block has: 4 x 2048 tokens, window 2048, 16 / 8 heads of 128,
 // forward / backward 563 / 2091 us, 122 / 82 TFLOP/s; 2 x 1001 tokens, window 256, 16 / 4 heads of 64, half of them
-// padding: 23.5 + 33 (dQ) + 47 us (dK/dV), about 40 TFLOP/s each.
+// padding: 23.5 + 33 (dQ) + 44 us (dK/dV), about 40 TFLOP/s each.
 //
 // As in the bf16 kernels, a block that meets an infinity or a NaN in a tile that its rows do not see
 // in full forms its rows anew one at a time.
