@@ -488,3 +488,29 @@ def test_rows_past_two_to_the_31_bytes():
         for at in (0, rows // 2, rows - n - 64):
             check(lib().vkh_memcpy_d2h(some.ctypes.data, buf.offset(at * row), some.nbytes))
             assert not (some & 0x7fff).any()
+
+
+# nothing turned, on chunks of 8 and of 4 values a lane
+UNTURNED = [
+    (5, 4, 2, 64, 0, 0, "none", False, False, 0),
+    (5, 4, 2, 64, 0, 1, "none", True, True, 0),
+    (33, 3, 1, 128, 0, 0, "none", True, True, 16),
+    (7, 2, 1, 256, 0, 0, "none", False, True, 0),
+    (9, 3, 2, 72, 0, 0, "none", False, False, 0),
+    (9, 3, 2, 72, 0, 1, "none", True, True, 0),
+    (1030, 2, 1, 64, 0, 0, "none", True, False, 0),
+    (2050, 1, 0, 128, 0, 0, "none", False, False, 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("back", [False, True], ids=["forward", "backward"])
+@pytest.mark.parametrize("case", UNTURNED, ids=lambda c: "-".join(str(x) for x in c))
+def test_rotary_that_turns_nothing(case, back):
+    test_rotary_matches_the_formula(case, back)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", UNTURNED, ids=lambda c: "-".join(str(x) for x in c))
+def test_qk_norm_that_turns_nothing(case):
+    test_qk_norm_rotary_matches_the_formula(case, False)

@@ -113,9 +113,11 @@ VKH_DEV float row_sum(float v, int LP) {
 }
 
 // Lane t of a head row: its two chunks start at values e0 and e1, of the turned part's halves or of the
-// rest's: what a load or store of one chunk touches is contiguous over the lanes of either part.
+// rest's (all of the row where nothing is turned): what a load or store of one chunk touches is contiguous
+// over the lanes of either part.
 VKH_DEV void chunks(const RotaryArgs &a, int t, int V, int &e0, int &e1) {
-    const int lo = 2 * t * V < a.rot ? 0 : a.rot, n = lo ? a.hd - a.rot : a.rot;
+    const bool turned = 2 * t * V < a.rot;
+    const int lo = turned ? 0 : a.rot, n = turned ? a.rot : a.hd - a.rot;
     e0 = lo + t * V - lo / 2;
     e1 = e0 + n / 2;
 }
