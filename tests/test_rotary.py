@@ -514,3 +514,64 @@ def test_rotary_that_turns_nothing(case, back):
 @pytest.mark.parametrize("case", UNTURNED, ids=lambda c: "-".join(str(x) for x in c))
 def test_qk_norm_that_turns_nothing(case):
     test_qk_norm_rotary_matches_the_formula(case, False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("back", [False, True], ids=["forward", "backward"])
+@pytest.mark.parametrize("bf16", [False, True], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("hd,r,layout", [(128, 64, 0), (128, 32, 1), (72, 24, 0), (72, 24, 1), (64, 0, 0), (33, 14, 0)])
+def test_values_behind_the_turned_ones_keep_their_bits(hd, r, layout, bf16, back):
+    """Infinities, NaN and zeros of both signs among the values that are not turned stay where they are, and
+    reach no other value."""
+    from valkyr_amd import kernels as K
+
+    note(f"rotary rest {hd} {r} {layout} {bf16} {back}")
+    rows, nq, nk = 6, 3, 2
+    plan, (f, a), rng = plan_of(r, layout=layout), frequencies(r, 1e4), np.random.default_rng(11)
+    pos = rng.integers(0, 5000, rows).astype(np.uint32)
+    odd, ins, vals, outs = [np.nan, np.inf, -np.inf, -0.0, 0.0, 1.5], [], [], []
+    for n in (nq, nk):
+        x = rng.standard_normal((rows, n, hd))
+        for e in range(r, hd):
+            x[:, :, e] = np.where(rng.random((rows, n)) < 0.5, x[:, :, e], odd[e % 6])
+        b, w = up(x.reshape(rows, -1), bf16)
+        ins.append(b)
+        vals.append(w.reshape(rows, n, hd))
+        outs.append(filled(rows, n * hd, bf16))
+    d = int(bf16)
+    p = K.rotary_params(rows, nq, nk, hd, x_dtype=d, y_dtype=d, dy_dtype=d, dx_dtype=d)
+    (K.rotary_backward if back else K.rotary_forward)(p, plan, ins[0], outs[0], ins[1], outs[1], positions=dev(pos))
+    for x, o, n in zip(vals, outs, (nq, nk)):
+        got = down(o, x.shape, bf16)
+        rest, want = got[..., r:], x[..., r:]
+        assert np.array_equal(np.isnan(rest), np.isnan(want))
+        nan = np.isnan(want)
+        assert np.array_equal(rest[~nan], want[~nan]) and np.array_equal(np.signbit(rest[~nan]), np.signbit(want[~nan]))
+        ref = turn(x[..., :r], pos, f, a, layout, back)
+        tol = 12 * U * pair_size(x[..., :r], r, layout, a) + (U16 * np.abs(ref) if bf16 else 0) + 1e-30
+        assert np.all(np.abs(got[..., :r] - ref) <= tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("hd,r", [(128, 64), (72, 24), (64, 0), (33, 14)])
+def test_an_infinite_gradient_behind_the_turned_values_reaches_its_own_gain_only(hd, r, bf16):
+    from valkyr_amd import kernels as K
+
+    note(f"qk norm infinite gradient {hd} {r} {bf16}")
+    rows, n, rng, d = 9, 3, np.random.default_rng(14), int(bf16)
+    (f, a), pos, w, at = frequencies(r, 1e4), np.arange(9), rng.uniform(0.5, 1.5, hd).astype(np.float32), hd - 3
+    x, X = up(rng.standard_normal((rows, n * hd)), bf16)
+    g = rng.standard_normal((rows, n * hd))
+    g[4, hd + at] = np.inf  # of the middle head
+    g, G = up(g, bf16)
+    p = K.rotary_params(rows, n, 0, hd, x_dtype=d, y_dtype=d, dy_dtype=d, dx_dtype=d)
+    dw = filled(1, hd, False)
+    K.qk_norm_rotary_backward(p, plan_of(r), dev(w), None, x, None, g, None, filled(rows, n * hd, bf16), None, dw)
+    xh, _, _ = norm64(X.reshape(rows, n, hd), w.astype(np.float64), 1e-6, False)
+    G = np.delete(G.reshape(rows, n, hd), at, -1)
+    xh = np.delete(xh, at, -1)
+    want, size = (turn(G, pos, f, a, 0, True) * xh).sum((0, 1)), (pair_size(G, r, 0, a) * np.abs(xh)).sum((0, 1))
+    got = host(dw)
+    assert not np.isfinite(got[at])
+    assert np.all(np.abs(np.delete(got, at) - want) <= (33 + 64 + 32 + 32 + 16) * U * size + 1e-30)

@@ -78,26 +78,29 @@ VKH_DEV void load_gain(const float *p, float (&o)[V], float quirk) {
 }
 
 // The V pairs that a lane holds as two chunks, turned.  Half layout: pair i is (a[i], b[i]);
-// interleaved: neighbours within a, then within b.
-template <int V>
-VKH_DEV void turn_pairs(float (&a)[V], float (&b)[V], const float2 (&cs)[V], bool interleaved) {
+// interleaved: neighbours within a, then within b.  SELECT: lanes that are not `turned` (their cs is (1, 0))
+// may call it too; what their sines multiply is taken as 0, since 0 times an infinity or a NaN is NaN (the
+// norm's backward, which a branch around the call would take 140 in place of 100 us: registers).
+template <bool SELECT, int V>
+VKH_DEV void turn_pairs(float (&a)[V], float (&b)[V], const float2 (&cs)[V], bool interleaved, bool turned = true) {
+    auto part = [&](float x) { return !SELECT || turned ? x : 0.f; };
     if (interleaved) {
 #pragma unroll
         for (int i = 0; i < V / 2; ++i) {
             const float2 u = cs[i], w = cs[V / 2 + i];
             const float a0 = a[2 * i], a1 = a[2 * i + 1], b0 = b[2 * i], b1 = b[2 * i + 1];
-            a[2 * i] = a0 * u.x - a1 * u.y;
-            a[2 * i + 1] = a1 * u.x + a0 * u.y;
-            b[2 * i] = b0 * w.x - b1 * w.y;
-            b[2 * i + 1] = b1 * w.x + b0 * w.y;
+            a[2 * i] = a0 * u.x - part(a1) * u.y;
+            a[2 * i + 1] = a1 * u.x + part(a0) * u.y;
+            b[2 * i] = b0 * w.x - part(b1) * w.y;
+            b[2 * i + 1] = b1 * w.x + part(b0) * w.y;
         }
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const float2 u = cs[i];
             const float a0 = a[i], b0 = b[i];
-            a[i] = a0 * u.x - b0 * u.y;
-            b[i] = b0 * u.x + a0 * u.y;
+            a[i] = a0 * u.x - part(b0) * u.y;
+            b[i] = b0 * u.x + part(a0) * u.y;
         }
     }
 }
@@ -123,13 +126,14 @@ VKH_DEV void chunks(const RotaryArgs &a, int t, int V, int &e0, int &e1) {
 }
 
 // The cosines and sines of a row for the V pairs of each lane: a wave computes one pair a lane and
-// hands them round through its own LDS (128 pairs).
+// hands them round through its own LDS (128 pairs); whether the lane's values are turned at all.
 template <int V>
-VKH_DEV void row_angles(const RotaryArgs &a, unsigned pos, float2 *sh, int lane, int t, float2 (&cs)[V]) {
+VKH_DEV bool row_angles(const RotaryArgs &a, unsigned pos, float2 *sh, int lane, int t, float2 (&cs)[V]) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last row's are read
     for (int j = lane; j < a.rot / 2; j += 64) sh[j] = cos_sin(a, pos, j);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (2 * t * V < a.rot) {
+    const bool turned = 2 * t * V < a.rot;
+    if (turned) {
         // half layout: pairs t V ..; neighbours: half of them in either chunk
         const int p0 = a.interleaved ? t * V / 2 : t * V, p1 = a.interleaved ? a.rot / 4 + p0 : p0 + V / 2;
 #pragma unroll
@@ -138,6 +142,7 @@ VKH_DEV void row_angles(const RotaryArgs &a, unsigned pos, float2 *sh, int lane,
 #pragma unroll
         for (int i = 0; i < V; ++i) cs[i] = make_float2(1.f, 0.f);
     }
+    return turned;
 }
 
 // Forward of both operators, and the rotary backward (a.sign = -1, dy in, dx out).  HS waves share
@@ -159,7 +164,7 @@ __global__ __launch_bounds__(RNT) void rotary_fwd_k(RotaryArgs a, int HS, int LP
     chunks(a, t, V, e0, e1);
     const float inv_hd = 1.0f / (float)hd;
     float2 cs[V];
-    bool angles = false;
+    bool angles = false, turned = false;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const RotarySide &s = a.s[k];
@@ -184,7 +189,7 @@ __global__ __launch_bounds__(RNT) void rotary_fwd_k(RotaryArgs a, int HS, int LP
                 load_gain<V>(s.w + e1, w1, a.quirk);
             }
         }
-        if (!angles) row_angles<V>(a, position(a, row), sh[wave], lane, t, cs);
+        if (!angles) turned = row_angles<V>(a, position(a, row), sh[wave], lane, t, cs);
         angles = true;
         for (int h0 = first; h0 < H; h0 += step) {
             float nu[V], nv[V];
@@ -200,7 +205,7 @@ __global__ __launch_bounds__(RNT) void rotary_fwd_k(RotaryArgs a, int HS, int LP
                     v[i] = v[i] * r * w1[i];
                 }
             }
-            turn_pairs<V>(u, v, cs, a.interleaved);
+            if (turned) turn_pairs<false>(u, v, cs, a.interleaved);
             if (h0 + grp < H && act) {
                 store_v<V>(y + (h0 + grp) * hd + e0, u);
                 store_v<V>(y + (h0 + grp) * hd + e1, v);
@@ -217,8 +222,9 @@ __global__ __launch_bounds__(RNT) void rotary_fwd_k(RotaryArgs a, int HS, int LP
 // heads' values, also the next row's, are on their way while the present ones are worked on.  A
 // block's sums go to its row of `partial` ([blocks][hd]), which rotary_dw_k adds in block order.
 // 16384 rows, 32 / 8 heads of 128, bf16 (0.5 GB): 102 us, 4.9 TB/s; rotary_dw_k 6.
-template <class TX, class TG, class TD, int V>
-__global__ __launch_bounds__(RNT) void rotary_norm_bwd_k(RotaryArgs a, int LP, RotaryParts parts, float *partial) {
+// REST: some values of a head are not turned (five waves a SIMD asked for: without, 99 registers leave four).
+template <class TX, class TG, class TD, int V, bool REST>
+__global__ __launch_bounds__(RNT, REST ? 5 : 1) void rotary_norm_bwd_k(RotaryArgs a, int LP, RotaryParts parts, float *partial) {
     __shared__ float2 sh[RNT / 64][128];
     extern __shared__ float sums[];  // 256 / LP head rows of hd gain sums
     const bool isk = (int)blockIdx.x >= parts.q;
@@ -257,7 +263,7 @@ __global__ __launch_bounds__(RNT) void rotary_norm_bwd_k(RotaryArgs a, int LP, R
     while (row < a.n_rows) {
         const long next = row + stride;
         const unsigned npos = next < a.n_rows ? position(a, next) : 0;
-        row_angles<V>(a, pos, sh[wave], lane, t, cs);
+        const bool turned = row_angles<V>(a, pos, sh[wave], lane, t, cs);
         for (int h0 = 0; h0 < H; h0 += NG) {
             float nx0[V], nx1[V], ng0[V], ng1[V];
             const bool same = h0 + NG < H;
@@ -265,7 +271,7 @@ __global__ __launch_bounds__(RNT) void rotary_norm_bwd_k(RotaryArgs a, int LP, R
             float ss = 0.f, dot = 0.f;
 #pragma unroll
             for (int i = 0; i < V; ++i) ss = fmaf(x0[i], x0[i], fmaf(x1[i], x1[i], ss));
-            turn_pairs<V>(g0, g1, cs, a.interleaved);
+            turn_pairs<REST>(g0, g1, cs, a.interleaved, turned);
             const float r = rsqrtf(fmaf(row_sum(ss, LP), inv_hd, a.eps));
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -539,7 +545,8 @@ hipError_t rotary_norm_backward(const RotaryArgs &a, DType xt, DType gt, DType d
                     return;
                 }
                 const int LP = lanes(a.hd, 4);
-                hipLaunchKernelGGL((rotary_norm_bwd_k<X, G, D, 4>), grid, dim3(RNT), RNT / LP * a.hd * sizeof(float), st, a, LP, parts, partial);
+                auto k = a.rot < a.hd ? rotary_norm_bwd_k<X, G, D, 4, true> : rotary_norm_bwd_k<X, G, D, 4, false>;
+                hipLaunchKernelGGL(k, grid, dim3(RNT), RNT / LP * a.hd * sizeof(float), st, a, LP, parts, partial);
             });
         });
     });
