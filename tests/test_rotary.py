@@ -575,3 +575,27 @@ def test_an_infinite_gradient_behind_the_turned_values_reaches_its_own_gain_only
     got = host(dw)
     assert not np.isfinite(got[at])
     assert np.all(np.abs(np.delete(got, at) - want) <= (33 + 64 + 32 + 32 + 16) * U * size + 1e-30)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("nq,nk,hd,r", [(3, 1, 64, 64), (5, 2, 128, 64), (1, 1, 256, 0), (9, 3, 32, 32), (3, 2, 33, 14)])
+def test_gain_gradients_without_an_eps(nq, nk, hd, r, bf16):
+    """eps = 0, and fewer heads than the rows' lanes hold at a time: lanes without a head add nothing."""
+    from valkyr_amd import kernels as K
+
+    note(f"qk norm without eps {nq} {nk} {hd} {r} {bf16}")
+    rows, rng = 19, np.random.default_rng(12)
+    plan, (f, a), pos = plan_of(r), frequencies(r, 1e4), np.arange(19)
+    p = K.rotary_params(rows, nq, nk, hd, eps=0.0, x_dtype=int(bf16), y_dtype=int(bf16), dy_dtype=int(bf16), dx_dtype=int(bf16))
+    w = [rng.uniform(0.5, 1.5, hd).astype(np.float32) for _ in range(2)]
+    (x, X), (g, G) = (tuple(zip(*(up(rng.standard_normal((rows, n * hd)), bf16) for n in (nq, nk)))) for _ in range(2))
+    dx, dw = [filled(rows, n * hd, bf16) for n in (nq, nk)], [filled(1, hd, False) for _ in range(2)]
+    K.qk_norm_rotary_backward(p, plan, dev(w[0]), dev(w[1]), *x, *g, *dx, *dw)
+    for i, n in enumerate((nq, nk)):
+        xh, _, _ = norm64(X[i].reshape(rows, n, hd), w[i].astype(np.float64), 0.0, False)
+        gi = G[i].reshape(rows, n, hd)
+        want = (turn(gi, pos, f, a, 0, True) * xh).sum((0, 1))
+        size = (pair_size(gi, r, 0, a) * np.abs(xh)).sum((0, 1))
+        # as in the test of the formula above: 33 u a term, and the sums' own steps
+        assert np.all(np.abs(host(dw[i]) - want) <= (33 + 64 + 32 + 32 + 16) * U * size + 1e-30)

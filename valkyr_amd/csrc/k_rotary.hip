@@ -272,7 +272,8 @@ __global__ __launch_bounds__(RNT, REST ? 5 : 1) void rotary_norm_bwd_k(RotaryArg
 #pragma unroll
             for (int i = 0; i < V; ++i) ss = fmaf(x0[i], x0[i], fmaf(x1[i], x1[i], ss));
             turn_pairs<REST>(g0, g1, cs, a.interleaved, turned);
-            const float r = rsqrtf(fmaf(row_sum(ss, LP), inv_hd, a.eps));
+            // lanes without a head add nothing to the gains' sums (0 times the root of eps = 0 would be NaN)
+            const float root = rsqrtf(fmaf(row_sum(ss, LP), inv_hd, a.eps)), r = h0 + grp < H ? root : 0.f;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 x0[i] *= r;
