@@ -781,7 +781,8 @@ vkh_status vkh_rotary_plan_init(const vkh_rotary_spec *spec, vkh_rotary_plan *ou
 /* Query and key head rows of one call, x -> y forward, dy -> dx backward.  Row strides are in
  * elements, 0 for dense rows.  y may be x, and dx may be dy or x, where type and stride are the
  * same.  n_q_heads or n_kv_heads may be 0, its pointers NULL.  head_dim up to 256; rows and
- * pointers aligned to 16 bytes with head_dim and rotary_dim multiples of 16 are the fast form. */
+ * pointers aligned to 16 bytes with head_dim and rotary_dim multiples of 16 are the fast form.
+ * Under 2^31 rows, 2^16 heads a side and 2^39 head rows. */
 typedef struct vkh_rotary_params {
     uint32_t n_rows, n_q_heads, n_kv_heads, head_dim;
     uint32_t seq_len, pos0; /* without positions: row r is at pos0 + r % seq_len (0: n_rows) */

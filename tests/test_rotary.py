@@ -599,3 +599,51 @@ def test_gain_gradients_without_an_eps(nq, nk, hd, r, bf16):
         size = (pair_size(gi, r, 0, a) * np.abs(xh)).sum((0, 1))
         # as in the test of the formula above: 33 u a term, and the sums' own steps
         assert np.all(np.abs(host(dw[i]) - want) <= (33 + 64 + 32 + 32 + 16) * U * size + 1e-30)
+
+
+def test_more_head_rows_than_a_launch_takes_are_refused():
+    from valkyr_amd import kernels as K
+
+    p, plan = K.rotary_params(1 << 30, 1 << 9, 1, 64), plan_of(64)
+    assert refused(K.rotary_forward, p, plan, 256, 256, 256, 256) == "Unsupported"
+    assert refused(K.rotary_backward, p, plan, 256, 256, 256, 256) == "Unsupported"
+    assert refused(K.qk_norm_rotary_backward, p, plan, *([256] * 8)) == "Unsupported"
+    assert K.qk_norm_rotary_workspace_bytes(p) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nh,hd,rows", [(1, 8, (1 << 26) + 37), (2, 6, (1 << 25) + 40)], ids=["chunks", "values"])
+def test_more_rows_than_one_axis_of_a_launch_holds(nh, hd, rows):
+    """2^26 head rows and a few: more than 2^32 lanes.  Rows at both ends and about the axis' end hold
+    numbers, the others zeros, which stay zeros."""
+    from valkyr_amd import kernels as K
+    from valkyr_amd._lib import check, lib
+    from valkyr_amd.device import DeviceBuffer, bf16_bits_to_f32, f32_to_bf16_bits
+
+    note(f"rotary and norm on {rows} rows of {nh} x {hd}")
+    rng, n, row = np.random.default_rng(15), 16, nh * hd * 2
+    starts = (0, (1 << 24) - 8, rows // 2, (1 << 26) // nh - 8, rows - n)
+    pos0, (f, a), w = 5, frequencies(hd, 1e4), rng.uniform(0.5, 1.5, hd).astype(np.float32)
+    x, y, vals = DeviceBuffer.zeros(rows * row), DeviceBuffer.zeros(rows * row), []
+    for at in starts:
+        bits = f32_to_bf16_bits(rng.standard_normal((n, nh * hd)).astype(np.float32))
+        check(lib().vkh_memcpy_h2d(x.offset(at * row), bits.ctypes.data, bits.nbytes))
+        vals.append(bf16_bits_to_f32(bits).astype(np.float64).reshape(n, nh, hd))
+    p = K.rotary_params(rows, nh, 0, hd, seq_len=1000003, pos0=pos0, x_dtype=1, y_dtype=1, dy_dtype=1, dx_dtype=1)
+
+    def rows_at(at, count=n):
+        got = np.empty((count, nh * hd), np.uint16)
+        check(lib().vkh_memcpy_d2h(got.ctypes.data, y.offset(at * row), got.nbytes))
+        return bf16_bits_to_f32(got).astype(np.float64).reshape(count, nh, hd)
+
+    for op in ("forward", "backward", "norm"):
+        if op == "norm":
+            K.qk_norm_rotary_forward(p, plan_of(hd), dev(w), None, x, y)
+        else:
+            (K.rotary_forward if op == "forward" else K.rotary_backward)(p, plan_of(hd), x, y)
+        for at, v in zip(starts, vals):
+            pos = pos0 + (at + np.arange(n)) % 1000003
+            z = norm64(v, w.astype(np.float64), 1e-6, False)[0] * w if op == "norm" else v
+            ref = turn(z, pos, f, a, 0, op == "backward")
+            assert np.all(np.abs(rows_at(at) - ref) <= 32 * U * pair_size(z, hd, 0, a) + U16 * np.abs(ref) + 1e-30), (op, at)
+        assert not rows_at(rows // 3, 64).any() and not rows_at((1 << 24) + 64, 64).any()

@@ -1181,6 +1181,7 @@ static vkh_status rotary_args(const vkh_rotary_params *p, const vkh_rotary_plan 
     if (p->head_dim > 256) return fail(VKH_ERR_UNSUPPORTED, "head_dim > 256");
     if (p->n_rows >= (1u << 31) || p->n_q_heads >= (1u << 16) || p->n_kv_heads >= (1u << 16))
         return fail(VKH_ERR_UNSUPPORTED, "2^31 rows or 2^16 heads");
+    if ((uint64_t)p->n_rows * (p->n_q_heads + p->n_kv_heads) >= 1ull << 39) return fail(VKH_ERR_UNSUPPORTED, "2^39 head rows");
     a = RotaryArgs{};
     const uint32_t lds[2][4] = {{p->ld_xq, p->ld_yq, p->ld_dyq, p->ld_dxq}, {p->ld_xk, p->ld_yk, p->ld_dyk, p->ld_dxk}};
     for (int k = 0; k < 2; ++k) {

@@ -156,7 +156,7 @@ __global__ __launch_bounds__(RNT) void rotary_fwd_k(RotaryArgs a, int HS, int LP
     __shared__ float2 sh[RNT / 64][128];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int t = lane % LP, grp = lane / LP, NG = 64 / LP, hd = a.hd;
-    const long row = (long)blockIdx.x * (RNT / 64 / HS) + wave / HS;
+    const long row = block_number() * (RNT / 64 / HS) + wave / HS;
     if (row >= a.n_rows) return;
     const bool act = 2 * t * V < hd;
     const int step = NG * HS, first = wave % HS * NG;
@@ -330,7 +330,7 @@ VKH_DEV RotItem rot_item(const RotaryArgs &a, int i) {
 template <class TX, class TY, bool NORM>
 __global__ __launch_bounds__(RNT) void rotary_fwd_any_k(RotaryArgs a) {
     const int lane = threadIdx.x % 64, H = a.nh[0] + a.nh[1];
-    const long it = (long)blockIdx.x * (RNT / 64) + threadIdx.x / 64;
+    const long it = block_number() * (RNT / 64) + threadIdx.x / 64;
     if (it >= a.n_rows * H) return;
     const long row = it / H;
     const int hh = (int)(it % H);
@@ -505,18 +505,17 @@ hipError_t rotary_forward(const RotaryArgs &a, bool norm, DType xt, DType yt, hi
     if (a.n_rows <= 0 || !H) return hipSuccess;
     const int V = chunk_width(a, {{xt, 0}, {yt, 1}});
     if (!V) {
-        const long blocks = (a.n_rows * H + RNT / 64 - 1) / (RNT / 64);
-        if (blocks >= (1L << 31)) return hipErrorInvalidValue;
+        const dim3 grid = long_grid((a.n_rows * H + RNT / 64 - 1) / (RNT / 64));
         by_type(xt, [&](auto x) {
             by_type(yt, [&](auto y) {
                 auto k = norm ? rotary_fwd_any_k<decltype(x), decltype(y), true> : rotary_fwd_any_k<decltype(x), decltype(y), false>;
-                hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(RNT), 0, st, a);
+                hipLaunchKernelGGL(k, grid, dim3(RNT), 0, st, a);
             });
         });
         return hipGetLastError();
     }
     const int LP = lanes(a.hd, V), HS = a.n_rows >= 2048 ? 1 : a.n_rows >= 1024 ? 2 : 4, per = RNT / 64 / HS;
-    const dim3 grid((unsigned)((a.n_rows + per - 1) / per));
+    const dim3 grid = long_grid((a.n_rows + per - 1) / per);
     by_type(xt, [&](auto x) {
         by_type(yt, [&](auto y) {
             using X = decltype(x);
