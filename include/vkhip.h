@@ -563,8 +563,8 @@ vkh_status vkh_fa_backward_from_o(const vkh_attn_params *p, const void *q, const
  * keys from kv_len[b] on get gradients of 0. */
 typedef struct vkh_window_params {
     uint32_t n_batch;    /* 0 means 1 */
-    uint32_t n_q, n_kv;  /* rows per sequence, n_q <= n_kv */
-    uint32_t n_heads, n_kv_heads, head_dim; /* head_dim up to 256; 64 and 128 on aligned rows are the fast form */
+    uint32_t n_q, n_kv;  /* rows per sequence, n_q <= n_kv < 2^30; under 2^31 head rows of q and of k in all */
+    uint32_t n_heads, n_kv_heads, head_dim; /* under 2^16 heads; head_dim up to 256; 64 and 128 on aligned rows are the fast form */
     uint32_t window;     /* keys up to and with the query's own; 0: no limit */
     uint32_t n_sink;
     float inv_sqrt_dim;

@@ -683,3 +683,76 @@ def test_the_operators_as_a_layer_runs_them(form):
         want = r * (gw - xh * (gw * xh).mean(-1, keepdims=True))
         assert rel_l2(want.reshape(T, -1), got_dx[:, lo:lo + z.shape[1] * hd]) <= tol
         assert rel_l2((gr * xh).sum((0, 1)), host(dw[side])) <= tol
+
+
+class Long:
+    """A call of `b` sequences of n tokens, whose operands are zeros but for some sequences' rows."""
+
+    def __init__(self, b, n, H, Hkv, hd, window, sinks, bf, some, seed=0):
+        from valkyr_amd import kernels as K
+        from valkyr_amd._lib import check, lib
+        from valkyr_amd.device import DeviceBuffer
+
+        self.n, self.H, self.Hkv, self.hd, self.es, self.some = n, H, Hkv, hd, 2 if bf else 4, some
+        rng = np.random.default_rng(seed)
+        self.p = K.window_params(n, n, H, Hkv, hd, window, sinks, n_batch=b, dtype=int(bf))
+        self.heads = dict(q=H, k=Hkv, v=Hkv, do=H, o=H, dq=H, dk=Hkv, dv=Hkv)
+        self.buf = {name: DeviceBuffer.zeros(b * n * h * hd * self.es) for name, h in self.heads.items()}
+        self.lse, self.d = (DeviceBuffer.zeros(b * n * H * 4) for _ in range(2))
+        self.vals = []
+        for i in some:
+            v = {}
+            for name in ("q", "k", "v", "do"):
+                x = rng.standard_normal((n, self.heads[name], hd))
+                up, w = bf16_dev(x) if bf else (dev(x.astype(np.float32)), x.astype(np.float32))
+                raw = host(up, dtype=np.uint16 if bf else np.float32)
+                check(lib().vkh_memcpy_h2d(self.at(name, i), raw.ctypes.data, raw.nbytes))
+                v[name] = np.asarray(w, np.float64).reshape(x.shape)
+            self.vals.append(v)
+        u = self.buf
+        K.fa_window_forward(self.p, u["q"], u["k"], u["v"], u["o"], self.lse)
+        K.fa_window_backward(self.p, u["q"], u["k"], u["v"], u["o"], u["do"], self.lse, self.d, u["dq"], u["dk"], u["dv"])
+
+    def at(self, name, i):
+        return self.buf[name].offset(i * self.n * self.heads[name] * self.hd * self.es)
+
+    def rows(self, name, i):
+        from valkyr_amd._lib import check, lib
+        from valkyr_amd.device import bf16_bits_to_f32
+
+        x = np.empty((self.n, self.heads[name], self.hd), np.uint16 if self.es == 2 else np.float32)
+        check(lib().vkh_memcpy_d2h(x.ctypes.data, self.at(name, i), x.nbytes))
+        return (bf16_bits_to_f32(x) if self.es == 2 else x).astype(np.float64)
+
+    def log_sums(self, i):
+        from valkyr_amd._lib import check, lib
+
+        x = np.empty((self.n, self.H), np.float32)
+        check(lib().vkh_memcpy_d2h(x.ctypes.data, self.lse.offset(i * self.n * self.H * 4), x.nbytes))
+        return x.astype(np.float64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b,n,H,Hkv,hd,window,sinks,bf", [
+    ((1 << 16) + 3, 1024, 1, 1, 4, 3, 1, False),  # 2^26 rows and more, a wave each
+    ((1 << 13) + 1, 4096, 2, 1, 6, 2, 0, True),
+    ((1 << 24) + 5, 1, 1, 1, 64, 1, 0, True),     # more tiles than a launch takes
+    ((1 << 24) + 5, 1, 1, 1, 64, 0, 0, False),
+    ((1 << 23) + 3, 1, 1, 1, 64, 1, 0, True),     # forward and dQ would fit, dK/dV would not
+], ids=lambda x: str(x))
+def test_more_rows_than_one_axis_of_a_launch_holds(b, n, H, Hkv, hd, window, sinks, bf):
+    note(f"window attention {b} x {n}, {H} / {Hkv} heads of {hd}")
+    some = (0, (1 << 24) // n if n > 1 else 1 << 22, b // 2 + 1, b - 1)
+    c = Long(b, n, H, Hkv, hd, window, sinks, bf, some)
+    see = visible(n, n, n, n, window, sinks)
+    for i, v in zip(some, c.vals):
+        want = attention64(v["q"], v["k"], v["v"], v["do"], see, 1 / math.sqrt(hd))
+        off = np.abs(c.log_sums(i) - want["lse"])
+        assert np.all(off <= (hd / 16 + 8) * U * want["size"] + 8 * U * (1 + np.abs(want["lse"])))
+        for name in ("o", "dq", "dk", "dv"):
+            bar = 1e-5 if not bf else (2 if name == "o" else 3) * U16
+            slack = np.linalg.norm(want["e" + name]) if "e" + name in want else 0.0
+            assert np.linalg.norm(c.rows(name, i) - want[name]) <= bar * np.linalg.norm(want[name]) + slack, (i, name)
+    for i in (1, b // 3, b - 2):  # sequences of zeros
+        assert np.abs(c.log_sums(i)[:, 0] - np.log(see.sum(1))).max() <= 8 * U * (1 + np.log(n))
+        assert not any(c.rows(name, i).any() for name in ("o", "dq", "dk", "dv")), i

@@ -23,7 +23,7 @@ template <class T, class TO>
 __global__ __launch_bounds__(WNT) void window_fwd_any_k(WindowArgs a) {
     __shared__ float qs[WPB][256];
     const int lane = threadIdx.x % 64, w = threadIdx.x / 64;
-    const long it = (long)blockIdx.x * WPB + w, row = it / a.n_heads;
+    const long it = block_number() * WPB + w, row = it / a.n_heads;
     if (row >= (long)a.n_batch * a.n_q) return;
     window_fwd_row<T, TO>(a, (int)(row / a.n_q), (int)(row % a.n_q), (int)(it % a.n_heads), qs[w], lane);
 }
@@ -31,7 +31,7 @@ template <class T, class TO>
 __global__ __launch_bounds__(WNT) void window_dq_any_k(WindowArgs a) {
     __shared__ float qs[WPB][256], gs[WPB][256];
     const int lane = threadIdx.x % 64, w = threadIdx.x / 64;
-    const long it = (long)blockIdx.x * WPB + w, row = it / a.n_heads;
+    const long it = block_number() * WPB + w, row = it / a.n_heads;
     if (row >= (long)a.n_batch * a.n_q) return;
     window_dq_row<T, TO>(a, (int)(row / a.n_q), (int)(row % a.n_q), (int)(it % a.n_heads), qs[w], gs[w], lane);
 }
@@ -39,7 +39,7 @@ template <class T, class TO>
 __global__ __launch_bounds__(WNT) void window_dkv_any_k(WindowArgs a) {
     __shared__ float ks[WPB][256], vs[WPB][256];
     const int lane = threadIdx.x % 64, w = threadIdx.x / 64;
-    const long it = (long)blockIdx.x * WPB + w, row = it / a.n_kv_heads;
+    const long it = block_number() * WPB + w, row = it / a.n_kv_heads;
     if (row >= (long)a.n_batch * a.n_kv) return;
     const int kh = (int)(it % a.n_kv_heads);
     window_dkv_row<T>(a, (int)(row / a.n_kv), (int)(row % a.n_kv), kh, ks[w], vs[w],
@@ -54,7 +54,7 @@ void by_types(const WindowArgs &a, F f) {
     else if (a.odt == DType::F32) f(bf16{}, float{});
     else f(bf16{}, bf16{});
 }
-unsigned row_blocks(long rows) { return (unsigned)((rows + WPB - 1) / WPB); }
+dim3 row_blocks(long rows) { return long_grid((rows + WPB - 1) / WPB); }
 
 }  // namespace
 
@@ -65,7 +65,7 @@ hipError_t window_forward(const WindowArgs &a, hipStream_t st) {
     if (window16_forward(a, st) || window32_forward(a, st)) return hipGetLastError();
     by_types(a, [&](auto t, auto o) {
         hipLaunchKernelGGL((window_fwd_any_k<decltype(t), decltype(o)>),
-                           dim3(row_blocks((long)a.n_batch * a.n_q * a.n_heads)), dim3(WNT), 0, st, a);
+                           row_blocks((long)a.n_batch * a.n_q * a.n_heads), dim3(WNT), 0, st, a);
     });
     return hipGetLastError();
 }
@@ -74,9 +74,10 @@ hipError_t window_backward(const WindowArgs &a, hipStream_t st) {
     if (window16_backward(a, st) || window32_backward(a, st)) return hipGetLastError();
     by_types(a, [&](auto t, auto o) {
         hipLaunchKernelGGL((window_dq_any_k<decltype(t), decltype(o)>),
-                           dim3(row_blocks((long)a.n_batch * a.n_q * a.n_heads)), dim3(WNT), 0, st, a);
+                           row_blocks((long)a.n_batch * a.n_q * a.n_heads), dim3(WNT), 0, st, a);
+        if (hipPeekAtLastError() != hipSuccess) return;  // (D is not there)
         hipLaunchKernelGGL((window_dkv_any_k<decltype(t), decltype(o)>),
-                           dim3(row_blocks((long)a.n_batch * a.n_kv * a.n_kv_heads)), dim3(WNT), 0, st, a);
+                           row_blocks((long)a.n_batch * a.n_kv * a.n_kv_heads), dim3(WNT), 0, st, a);
     });
     return hipGetLastError();
 }

@@ -1123,6 +1123,7 @@ bool window16_forward(const WindowArgs &a, hipStream_t st) {
     if (few_rows(a) && (a.n_q <= kFewRows || a.ws)) {
         const int grp = a.n_heads / a.n_kv_heads, rt = (a.n_q * grp + 15) / 16, splits = a.ws ? splits16(a) : 1;
         const long blocks = (long)a.n_batch * a.n_kv_heads * rt * splits;
+        if (!launchable(blocks, 256)) return false;
         auto by = [&](auto hd, auto to) {
             constexpr int HD = decltype(hd)::value;
             using TO = decltype(to);
@@ -1143,6 +1144,7 @@ bool window16_forward(const WindowArgs &a, hipStream_t st) {
     // 512, 2048: 35.5 / 32.5, 47 / 43, 61 / 59, 94 / 100, heads of 64, window 512: 33 / 37; 16384, window 256: 173 / 196.
     const long blocks = per * ((a.n_q + 127) / 128);
     const bool small = blocks <= 2l * cu_count() || (a.hd == 128 && a.window <= 512 && blocks <= 4l * cu_count()), pairs = grouped(a);
+    if (!launchable(small ? per * ((a.n_q + 63) / 64) : blocks, 256)) return false;
     auto go = [&](auto kernel, int bm, int kg) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)(per * ((a.n_q + bm - 1) / bm))), dim3(256 * kg), 0, st, a);
     };
@@ -1172,6 +1174,7 @@ bool window16_backward(const WindowArgs &a, hipStream_t st) {
     // and 596; 4 x 2048, window 512, 224 and 222; window 1024, 294 and 298)
     const int bq = per * ((a.n_q + 127) / 128) >= 2l * cu_count() && a.window > 512 ? 128 : 64;
     const DkvPlan plan = plan16(a, a.ws != nullptr);
+    if (!launchable(a, plan, per * ((a.n_q + bq - 1) / bq), 256)) return false;
     auto by = [&](auto hd, auto to) {
         constexpr int HD = decltype(hd)::value;
         using TO = decltype(to);
@@ -1181,6 +1184,7 @@ bool window16_backward(const WindowArgs &a, hipStream_t st) {
         if (bq == 128) dq(window_dq16_k<HD, 128, 1, TO>, 1);
         else if (grouped(a)) dq(window_dq16_k<HD, 64, 2, TO>, 2);
         else dq(window_dq16_k<HD, 64, 1, TO>, 1);
+        if (hipPeekAtLastError() != hipSuccess) return;  // (D is not there)
         WindowArgs near = a;
         if (plan.far_parts) {
             near.n_sink = 0;

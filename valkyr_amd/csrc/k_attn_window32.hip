@@ -748,13 +748,17 @@ bool window32_forward(const WindowArgs &a, hipStream_t st) {
     if (!fwd_ok(a)) return false;
     if (few_rows(a) && (a.n_q <= kFewRows || a.ws)) {
         const int grp = a.n_heads / a.n_kv_heads, splits = a.ws ? splits32(a) : 1;
-        const dim3 grid((unsigned)((long)a.n_batch * a.n_kv_heads * ((a.n_q * grp + 15) / 16) * splits));
+        const long blocks = (long)a.n_batch * a.n_kv_heads * ((a.n_q * grp + 15) / 16) * splits;
+        if (!launchable(blocks, FNT)) return false;
+        const dim3 grid((unsigned)blocks);
         if (a.hd == 128) hipLaunchKernelGGL(window_step32_k<128>, grid, dim3(FNT), 0, st, a, splits);
         else hipLaunchKernelGGL(window_step32_k<64>, grid, dim3(FNT), 0, st, a, splits);
         if (splits > 1) a.hd == 128 ? launch_join<128, float>(a, splits, st) : launch_join<64, float>(a, splits, st);
         return true;
     }
-    const dim3 grid((unsigned)((long)a.n_heads * a.n_batch * ((a.n_q + 63) / 64)));
+    const long blocks = (long)a.n_heads * a.n_batch * ((a.n_q + 63) / 64);
+    if (!launchable(blocks, 256)) return false;
+    const dim3 grid((unsigned)blocks);
     auto by = [&](auto hd) {
         constexpr int HD = decltype(hd)::value;
         if (grouped(a)) hipLaunchKernelGGL((window_fwd32_k<HD, 2>), grid, dim3(512), 0, st, a);
@@ -768,12 +772,15 @@ bool window32_forward(const WindowArgs &a, hipStream_t st) {
 bool window32_backward(const WindowArgs &a, hipStream_t st) {
     if (!fwd_ok(a) || !ok(a.dout, a.lddo) || !ok(a.dq, a.lddq) || !ok(a.dk, a.lddk) || !ok(a.dv, a.lddv)) return false;
     const DkvPlan plan = plan32(a, a.ws != nullptr);
-    const dim3 gq((unsigned)((long)a.n_heads * a.n_batch * ((a.n_q + 63) / 64)));
+    const long blocks = (long)a.n_heads * a.n_batch * ((a.n_q + 63) / 64);
+    if (!launchable(a, plan, blocks, 256)) return false;
+    const dim3 gq((unsigned)blocks);
     const dim3 gk((unsigned)((long)a.n_batch * a.n_kv_heads * plan.blocks()));
     auto by = [&](auto hd) {
         constexpr int HD = decltype(hd)::value;
         if (grouped(a)) hipLaunchKernelGGL((window_dq32_k<HD, 2>), gq, dim3(512), 0, st, a);
         else hipLaunchKernelGGL((window_dq32_k<HD, 1>), gq, dim3(256), 0, st, a);
+        if (hipPeekAtLastError() != hipSuccess) return;  // (D is not there)
         if (grouped_dkv(a)) hipLaunchKernelGGL((window_dkv32_k<HD, 2>), gk, dim3(512), 0, st, a, plan);
         else hipLaunchKernelGGL((window_dkv32_k<HD, 1>), gk, dim3(256), 0, st, a, plan);
         launch_dkv_sum<HD, 64, float>(a, plan, st);

@@ -495,6 +495,14 @@ void launch_join(const WindowArgs &a, int splits, hipStream_t st) {
     const long rows = (long)a.n_batch * a.n_q * a.n_heads;
     hipLaunchKernelGGL((window_join_k<HD, TO>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a, splits);
 }
+// A launch takes fewer than 2^32 threads along x.  Calls of more tiles go row by row (k_attn_window.hip).
+inline bool launchable(long blocks, int threads) { return blocks < (1l << 32) / threads; }
+// the launches of a backward pass: dQ's blocks, dK/dV's with its sums and far pairs
+inline bool launchable(const WindowArgs &a, const DkvPlan &p, long dq_blocks, int threads) {
+    const long nbk = (long)a.n_batch * a.n_kv_heads;
+    return launchable(dq_blocks, threads) && launchable(nbk * p.blocks(), 512) && launchable(nbk * p.summed(), 256) &&
+           launchable(nbk * p.far_slices * p.far_parts, 256);
+}
 inline bool aligned_rows(const void *x, long ld, int align, int es) { return (uintptr_t)x % align == 0 && ld * es % align == 0; }
 
 // The tile kernels on bf16 (k_attn_window16.hip) and fp32 operands (k_attn_window32.hip): false,
