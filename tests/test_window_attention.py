@@ -756,3 +756,19 @@ def test_more_rows_than_one_axis_of_a_launch_holds(b, n, H, Hkv, hd, window, sin
     for i in (1, b // 3, b - 2):  # sequences of zeros
         assert np.abs(c.log_sums(i)[:, 0] - np.log(see.sum(1))).max() <= 8 * U * (1 + np.log(n))
         assert not any(c.rows(name, i).any() for name in ("o", "dq", "dk", "dv")), i
+
+
+def test_the_backward_asks_for_a_bounded_workspace():
+    """Partial sums of at most 256 MiB, whatever the batch; many sequences need none."""
+    from valkyr_amd import kernels as K
+
+    for dtype in (K.F32, K.BF16):
+        for hd in (64, 128):
+            for b in (1, 3, 16, 64, 256, 512, 4096, 1 << 15):
+                for n in (1, 100, 256, 1024, 5000):
+                    for heads, kv in ((1, 1), (16, 8), (48, 16)):
+                        for window, sinks in ((64, 4), (256, 100), (900, 300), (0, 0)):
+                            p = K.window_params(n, n, heads, kv, hd, window, sinks, n_batch=b, dtype=dtype)
+                            assert K.fa_window_backward_workspace_bytes(p) <= 256 << 20, (dtype, hd, b, n, heads, kv, window)
+    for b, n, window in ((512, 256, 64), (4096, 256, 64), (512, 512, 256)):
+        assert K.fa_window_backward_workspace_bytes(K.window_params(n, n, 16, 8, 128, window, 4, n_batch=b, dtype=K.BF16)) == 0

@@ -419,8 +419,12 @@ __global__ __launch_bounds__(256) void window_join_k(WindowArgs a, int splits) {
 }
 
 // ── host ─────────────────────────────────────────────────────────────────
+inline size_t dkv_ws_bytes(const WindowArgs &a, const DkvPlan &p) {
+    const size_t nbk = (size_t)a.n_batch * a.n_kv_heads;
+    return nbk * ((size_t)p.slots() * p.keys + (size_t)p.far_slices * p.far_parts * p.far_keys) * 2 * a.hd * sizeof(float);
+}
 // keys: per key block; cu_blocks: that fill the chip; least: steps that a part keeps; far: whether the
-// far pairs of up to 128 sinks may have blocks of their own.  At most about 256 MiB of partial sums.
+// far pairs of up to 128 sinks may have blocks of their own.  At most 256 MiB of partial sums.
 inline DkvPlan dkv_plan(const WindowArgs &a, bool ws, int keys, long cu_blocks, long most_parts, long least, bool far) {
     DkvPlan p;
     p.keys = keys;
@@ -446,21 +450,21 @@ inline DkvPlan dkv_plan(const WindowArgs &a, bool ws, int keys, long cu_blocks, 
     // many steps from the others.  Backward in us, with the sink blocks / apart: 3 x 21 tokens, window 13: 16 / 27;
     // 2 x 1001, window 256, 16 / 4 heads of 128: 59 / 67; 2048, window 16, 16 / 8 heads: 44 / 58; 4 x 1001, window
     // 256, 16 / 8 heads: 103 / 95; 4 x 2048, window 16: 130 / 119; 4000, window 1024, 100 sinks: 213 / 180.
+    // They make every sink block's sums go through a slot: not where the slots of a large batch pass the bound
+    // (forward and backward in ms, with the sink blocks / apart: 512 x 256 tokens, window 64, 16 / 8 heads of 128,
+    // 576 MiB of slots: 2.31 / 2.62; 256 x 1024, window 256, 288 MiB: 6.61 / 6.69).
     if (far && p.sink_blocks && a.n_sink <= 128 &&
         (nbk * p.blocks() > cu_blocks || usual * (1.0 / p.parts - 1.0 / parts) > 24)) {
-        p.sink_parts = p.parts = parts;
-        p.far_keys = a.n_sink > 16 ? 32 : 16;
-        p.far_slices = (a.n_sink + p.far_keys - 1) / p.far_keys;
+        DkvPlan f = p;
+        f.sink_parts = f.parts = parts;
+        f.far_keys = a.n_sink > 16 ? 32 : 16;
+        f.far_slices = (a.n_sink + f.far_keys - 1) / f.far_keys;
         // four waves a CU in all, while each keeps three steps
-        p.far_parts = (int)std::max(1l, std::min(256 / (nbk * p.far_slices), most / 12));
-        return p;
+        f.far_parts = (int)std::max(1l, std::min(256 / (nbk * f.far_slices), most / 12));
+        if (dkv_ws_bytes(a, f) <= (256u << 20)) return f;
     }
     while (p.sink_parts > 1 && p.sink_blocks * nbk * slot * p.sink_parts > (192l << 20)) --p.sink_parts;
     return p;
-}
-inline size_t dkv_ws_bytes(const WindowArgs &a, const DkvPlan &p) {
-    const size_t nbk = (size_t)a.n_batch * a.n_kv_heads;
-    return nbk * ((size_t)p.slots() * p.keys + (size_t)p.far_slices * p.far_parts * p.far_keys) * 2 * a.hd * sizeof(float);
 }
 template <int HD, int BN, class TO>
 void launch_dkv_sum(const WindowArgs &a, const DkvPlan &p, hipStream_t st) {
