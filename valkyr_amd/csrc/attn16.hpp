@@ -36,18 +36,6 @@ VKH_DEV float xrow_sum(float v) {
     return a + b;
 }
 
-// The DMA to a wave-uniform LDS address that the caller may keep as a number (s_nop: the one wait state that
-// a load to LDS needs after a scalar write of M0).
-VKH_DEV unsigned lds_addr(const void *p) {
-    return __builtin_amdgcn_readfirstlane((int)(unsigned)(unsigned long)(const __attribute__((address_space(3))) char *)p);
-}
-VKH_DEV void dma16_at(const sgpr4 &rs, unsigned lds, unsigned voff) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(voff), "s"(rs) : "memory");
-}
-VKH_DEV void dma4_at(const sgpr4 &rs, unsigned lds, unsigned voff) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" : : "s"(lds), "v"(voff), "s"(rs) : "memory");
-}
-
 template <int N>
 VKH_DEV void wait_vm() {
     __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4 << 14));

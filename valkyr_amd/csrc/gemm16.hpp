@@ -116,22 +116,19 @@ VKH_DEV int mn_swz(int k) {
 // aliases of the in-flight slab (it would wait for the DMA before reading the
 // current one); the slab loops wait for their DMA explicitly (vmcnt) before
 // the barrier that publishes a slab.
-VKH_DEV void dma16_async(const sgpr4 &rs, const void *lds, unsigned voff) {
-    const unsigned m0 = __builtin_amdgcn_readfirstlane(
-        (int)(unsigned)(unsigned long)(const __attribute__((address_space(3))) char *)lds);
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                 :
-                 : "s"(m0), "v"(voff), "s"(rs)
-                 : "memory");
+// (s_nop: the wait state that a load to LDS needs after a scalar write of M0, which nothing inserts into inline
+// assembly.)  _at: to a wave-uniform LDS address that the caller may keep as a number.
+VKH_DEV unsigned lds_addr(const void *p) {
+    return __builtin_amdgcn_readfirstlane((int)(unsigned)(unsigned long)(const __attribute__((address_space(3))) char *)p);
 }
-VKH_DEV void dma4_async(const sgpr4 &rs, const void *lds, unsigned voff) {
-    const unsigned m0 = __builtin_amdgcn_readfirstlane(
-        (int)(unsigned)(unsigned long)(const __attribute__((address_space(3))) char *)lds);
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-                 :
-                 : "s"(m0), "v"(voff), "s"(rs)
-                 : "memory");
+VKH_DEV void dma16_at(const sgpr4 &rs, unsigned lds, unsigned voff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(voff), "s"(rs) : "memory");
 }
+VKH_DEV void dma4_at(const sgpr4 &rs, unsigned lds, unsigned voff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" : : "s"(lds), "v"(voff), "s"(rs) : "memory");
+}
+VKH_DEV void dma16_async(const sgpr4 &rs, const void *lds, unsigned voff) { dma16_at(rs, lds_addr(lds), voff); }
+VKH_DEV void dma4_async(const sgpr4 &rs, const void *lds, unsigned voff) { dma4_at(rs, lds_addr(lds), voff); }
 
 // Block barrier for LDS hand-offs: this wave's LDS operations complete, then
 // s_barrier (no wait on outstanding global operations, unlike __syncthreads'
