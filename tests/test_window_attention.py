@@ -772,3 +772,28 @@ def test_the_backward_asks_for_a_bounded_workspace():
                             assert K.fa_window_backward_workspace_bytes(p) <= 256 << 20, (dtype, hd, b, n, heads, kv, window)
     for b, n, window in ((512, 256, 64), (4096, 256, 64), (512, 512, 256)):
         assert K.fa_window_backward_workspace_bytes(K.window_params(n, n, 16, 8, 128, window, 4, n_batch=b, dtype=K.BF16)) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("shape", [(1, 400, 400, 4, 2, 128, 0, 0), (1, 400, 400, 3, 1, 64, 300, 2), (8, 300, 300, 32, 16, 64, 40, 3),
+                                   (1, 90, 120, 2, 1, 40, 0, 0)], ids=lambda s: "-".join(str(x) for x in s))
+def test_queries_of_minus_infinity_have_no_gradient(shape, form):
+    """A query of -inf against keys over 0: all of its scores are -inf, so O = 0, LSE = -inf, and neither it nor
+    any key has a gradient from it, also where all rows beside it see the same keys."""
+    b, nq, nk, H, Hkv, hd, window, sinks = shape
+    rbad = nq * 3 // 4
+    note(f"window attention -inf query {shape} {form}")
+
+    def spoil(v):
+        v["k"][:] = np.abs(v["k"]) + 0.01
+        v["q"][:, rbad] = -np.inf
+
+    c = Call(*shape, form, spoil=spoil)
+    c.forward()
+    c.backward()
+    got = c.read()
+    see = visible(nq, nk, nq, nk, window, sinks)
+    see[rbad] = False
+    each = [attention64(*(c.vals[n][i] for n in ("q", "k", "v", "do")), see, c.scale) for i in range(b)]
+    c.check(got, {n: np.stack([e[n] for e in each]) for n in each[0]})

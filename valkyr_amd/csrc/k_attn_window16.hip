@@ -766,7 +766,7 @@ __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan p
     const RowReach block = row_reach<BM>(a, s, k0, k0 + BN - 1), mine = row_reach<BM>(a, s, kw0, kw0 + KW - 1);
     if (niter > 0) dma(0);
     if (niter > 1) dma(1);
-    bool odd = false;  // an infinity or a NaN in Q or dO of a tile whose rows do not all see all keys
+    bool odd = false;  // an infinity or a NaN in Q or dO of a tile whose rows do not all see all keys, or have no gradient
     auto step = [&](const int it, auto bufc) {
         constexpr int buf = decltype(bufc)::value;
         if (it + 1 < niter) {
@@ -828,6 +828,7 @@ __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan p
         }
         const bool dead = __any(lane < BM && Ls[hg][buf][lane % BM] == -INFINITY);  // a row of no gradient
         if (dead || !mine.whole(q0)) {
+            if (block.whole(q0)) odd |= scan<2 * TILE, 256>(Qb, tid % 256);  // (every wave of the group is here)
 #pragma unroll
             for (int qs = 0; qs < QS; ++qs)
 #pragma unroll
@@ -995,6 +996,7 @@ __global__ __launch_bounds__(256, 1) void window_far16_k(WindowArgs a, DkvPlan p
         auto far = [&](int x, int ks) { return q0 + x < s.ql && q0 + x + s.off - k0 - 16 * ks - c16 >= a.window; };
         const bool whole = q0 + BM <= s.ql && q0 + s.off - k0 - NK + 1 >= a.window;
         f32x4 sc[QS][KS], dp[QS][KS];
+        bool dead = false;
 #pragma unroll
         for (int qs = 0; qs < QS; ++qs)
 #pragma unroll
@@ -1016,6 +1018,7 @@ __global__ __launch_bounds__(256, 1) void window_far16_k(WindowArgs a, DkvPlan p
             for (int r = 0; r < 4; ++r) {
                 const int x = 16 * qs + 4 * g + r;
                 const float l2 = L[x] * LOG2E, d = D[x];
+                dead = dead || L[x] == -INFINITY;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     const bool on = L[x] != -INFINITY && (whole || far(x, ks));  // (-inf: no gradient)
@@ -1024,8 +1027,8 @@ __global__ __launch_bounds__(256, 1) void window_far16_k(WindowArgs a, DkvPlan p
                     dp[qs][ks][r] = on ? p * (dp[qs][ks][r] - d) : 0.f;
                 }
             }
-        // the first tiles hold rows that are past some sinks' windows only
-        const bool odd = !whole && __any(scan<2 * TILE, 64>(Qb, lane));
+        // the first tiles hold rows that are past some sinks' windows only; any tile may hold rows of no gradient
+        const bool odd = (!whole || __any(dead)) && __any(scan<2 * TILE, 64>(Qb, lane));
         bf16x8 pb[KS], sb[KS];
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {

@@ -632,7 +632,7 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_dkv32_k(Wind
         }
     };
     const T t(g, c);
-    bool odd = false;  // in Q or dO of a tile whose rows do not all see all keys
+    bool odd = false;  // in Q or dO of a tile whose rows do not all see all keys, or have no gradient
     f32x4 dvt[NU], dkt[NU];
 #pragma unroll
     for (int j = 0; j < NU; ++j) dvt[j] = dkt[j] = f32x4{0, 0, 0, 0};
@@ -646,11 +646,12 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_dkv32_k(Wind
         const int q0 = qstart + (top - now.tile) * FT, ta = q0 + s.off, tb = min(q0 + FT, s.ql) - 1 + s.off;
         advance(now);
         const float *Ql = tiles[kg][buf][0], *Ol = tiles[kg][buf][1], *Ll = stat[kg][buf][0] + 4 * g, *Dl = stat[kg][buf][1] + 4 * g;
-        if (!all_seen(a, ta, tb, k0, k0 + BN - 1) && (scan32<HD>(Ql, tid) || scan32<HD>(Ol, tid))) odd = true;
+        const bool all = all_seen(a, ta, tb, k0, k0 + BN - 1);
+        if (!all && (scan32<HD>(Ql, tid) || scan32<HD>(Ol, tid))) odd = true;
         if (none_seen(a, ta, tb, kw, kw + 15)) return;
         const bool whole = q0 + FT <= s.ql && all_seen(a, ta, tb, kw, kw + 15);
         f32x4 sa[2], da[2];  // S / dP[q0 + 16 qs + 4 g + e][key]
-        bool live[2];
+        bool live[2], dead = false;
 #pragma unroll
         for (int qs = 0; qs < 2; ++qs) {
             sa[qs] = da[qs] = f32x4{0, 0, 0, 0};
@@ -664,8 +665,10 @@ __global__ __launch_bounds__(256 * KG, KG == 1 ? 2 : 1) void window_dkv32_k(Wind
             for (int e = 0; e < 4; ++e) {
                 sa[qs][e] = l[e] == -INFINITY ? 0.f : exp_(fmaf(sa[qs][e], a.scale, -l[e]));
                 da[qs][e] = l[e] == -INFINITY ? 0.f : sa[qs][e] * (da[qs][e] - d[e]);
+                dead = dead || l[e] == -INFINITY;
             }
         }
+        if (all && __any(dead) && (scan32<HD>(Ql, tid) || scan32<HD>(Ol, tid))) odd = true;  // (every wave's rows here)
         if (!whole) {
 #pragma unroll
             for (int qs = 0; qs < 2; ++qs)
