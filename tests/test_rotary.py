@@ -647,3 +647,26 @@ def test_more_rows_than_one_axis_of_a_launch_holds(nh, hd, rows):
             ref = turn(z, pos, f, a, 0, op == "backward")
             assert np.all(np.abs(rows_at(at) - ref) <= 32 * U * pair_size(z, hd, 0, a) + U16 * np.abs(ref) + 1e-30), (op, at)
         assert not rows_at(rows // 3, 64).any() and not rows_at((1 << 24) + 64, 64).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("rows,nq,nk,hd,r", [(3000, 16, 4, 128, 64), (700, 5, 3, 96, 96), (11, 3, 2, 33, 14)])
+def test_qk_norm_rotary_backward_in_place_of_x(rows, nq, nk, hd, r, bf16):
+    """dx over x, or over dy: the bits of a call with rows of its own."""
+    from valkyr_amd import kernels as K
+
+    note(f"qk norm backward over x {rows} {nq} {nk} {hd} {r} {bf16}")
+    rng, d = np.random.default_rng(13), int(bf16)
+    plan, p = plan_of(r), K.rotary_params(rows, nq, nk, hd, x_dtype=d, y_dtype=d, dy_dtype=d, dx_dtype=d)
+    X, G = ([rng.standard_normal((rows, n * hd)) for n in (nq, nk)] for _ in range(2))
+    w = [dev(rng.uniform(0.5, 1.5, hd).astype(np.float32)) for _ in range(2)]
+    seen = []
+    for over in (None, "x", "dy"):
+        x, g = ([up(z, bf16)[0] for z in zs] for zs in (X, G))
+        dx = {None: [filled(rows, n * hd, bf16) for n in (nq, nk)], "x": x, "dy": g}[over]
+        dw = [filled(1, hd, False) for _ in range(2)]
+        K.qk_norm_rotary_backward(p, plan, *w, *x, *g, *dx, *dw)
+        seen.append([down(b, (rows, n * hd), bf16) for b, n in zip(dx, (nq, nk))] + [host(b) for b in dw])
+    for s in seen[1:]:
+        assert all(np.array_equal(a, b) for a, b in zip(seen[0], s))

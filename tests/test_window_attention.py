@@ -797,3 +797,105 @@ def test_queries_of_minus_infinity_have_no_gradient(shape, form):
     see[rbad] = False
     each = [attention64(*(c.vals[n][i] for n in ("q", "k", "v", "do")), see, c.scale) for i in range(b)]
     c.check(got, {n: np.stack([e[n] for e in each]) for n in each[0]})
+
+
+# ── each row by itself ───────────────────────────────────────────────────
+
+def row_bounds(c, want):
+    """How far each head row of a bf16 call's O, dQ, dK and dV may be off, as 2-norms.  P (dS) is rounded
+    once for its products, u = 2^-8 of itself at most: a sum of n such terms T_j x_j is off by sum u |T_j|
+    |x_j| at the very most, and roundings that do not conspire stay within 8 u sqrt(sum T_j^2 |x_j|^2) (a mean
+    of at most one such root, and bounded differences leave 7 more a chance of e^-24).  O's own error, bf16 or
+    not, moves D, and with it dQ along P K, and dK by that share of each row.  bf16 results are rounded once
+    more; 1e-5 of the terms covers the sums and the exponentials in 32 bits (of scores under 64)."""
+    b, nq, nk, H, Hkv, hd, window, sinks = c.shape
+    out = {n: np.zeros(want[n].shape[:3]) for n in ("o", "dq", "dk", "dv")}
+    g, f32 = H // Hkv, 1e-5
+    norm = lambda x: np.linalg.norm(x, axis=-1)  # noqa: E731
+    sure = lambda t, x, ax: np.minimum(8 * U16 * np.sqrt((t * t) @ (x * x)) if ax else 8 * U16 * np.sqrt((t * t).T @ (x * x)),  # noqa: E731
+                                       (U16 * np.abs(t) @ x) if ax else (U16 * np.abs(t).T @ x))
+    for i in range(b):
+        see = visible(nq, nk, c.ql[i], c.kl[i], window, sinks)
+        k, v = (np.where(see.any(0)[:, None, None], c.vals[n][i], 0) for n in ("k", "v"))
+        q, do = (np.where(see.any(1)[:, None, None], c.vals[n][i], 0) for n in ("q", "do"))
+        live = see.any(1)
+        for h in range(H):
+            kh, vh, qh, gh = k[:, h // g], v[:, h // g], q[:, h], do[:, h]
+            s = np.where(see, qh @ kh.T * c.scale, -np.inf)
+            p = np.where(live[:, None], np.exp(s - np.where(live, want["lse"][i][:, h], 0)[:, None]), 0)
+            dd = (gh * want["o"][i][:, h]).sum(-1)
+            ds = p * (gh @ vh.T - dd[:, None]) * c.scale
+            eo = sure(p, norm(vh), True) + f32 * (p @ norm(vh)) + (U16 * norm(want["o"][i][:, h]) if c.obf else 0)
+            out["o"][i][:, h] = eo
+            ed = norm(gh) * eo
+            out["dq"][i][:, h] = (sure(ds, norm(kh), True) + f32 * (np.abs(ds) @ norm(kh)) + ed * norm(p @ kh) * c.scale +
+                                  norm(want["edq"][i][:, h]) + (U16 * norm(want["dq"][i][:, h]) if c.obf else 0))
+            t = p * (ed * norm(qh))[:, None] * c.scale
+            out["dk"][i][:, h // g] += (sure(ds, norm(qh), False) + f32 * (np.abs(ds).T @ norm(qh)) +
+                                        np.minimum(8 * np.sqrt((t * t).sum(0)), t.sum(0)))
+            out["dv"][i][:, h // g] += sure(p, norm(gh), False) + f32 * (p.T @ norm(gh))
+    out["dk"] += norm(want["edk"])
+    if c.obf:
+        for n in ("dk", "dv"):
+            out[n] += U16 * norm(want[n])
+    return out
+
+
+def check_rows(c):
+    got, want = c.read(), c.want()
+    c.check(got, want)
+    for n, most in row_bounds(c, want).items():
+        off = np.linalg.norm(got[n] - want[n], axis=-1)
+        worst = np.unravel_index(np.argmax(off - most), off.shape)
+        assert np.all(off <= most), (n, worst, off[worst], most[worst], int((off > most).sum()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["bf16", "bf16-fp32"])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "-".join(str(x) for x in s))
+def test_each_row_of_bf16_calls(shape, form):
+    note(f"window attention rows {shape} {form}")
+    c = Call(*shape, form, seed=7)
+    c.forward()
+    c.backward()
+    check_rows(c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", LARGER, ids=lambda s: "-".join(str(x) for x in s))
+def test_each_row_of_larger_bf16_calls(shape):
+    note(f"larger window attention rows {shape}")
+    c = Call(*shape, "bf16", seed=7)
+    c.forward()
+    c.backward()
+    check_rows(c)
+
+
+# more key blocks than CUs, few sinks: the pairs of a sink and a row past its window have blocks of their own,
+# here with several query heads on a KV head, an odd number of them, and slices of 16 and of 32 sinks
+FAR = [
+    (8, 300, 300, 32, 16, 64, 40, 3),
+    (8, 300, 300, 48, 16, 128, 60, 40),
+    (6, 420, 420, 64, 16, 64, 30, 100),
+    (8, 290, 290, 32, 16, 128, 50, 17),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ragged", [False, True], ids=["whole", "ragged"])
+@pytest.mark.parametrize("form", ["bf16", "bf16-fp32"])
+@pytest.mark.parametrize("shape", FAR, ids=lambda s: "-".join(str(x) for x in s))
+def test_sinks_of_several_heads_apart(shape, form, ragged):
+    note(f"window attention far pairs {shape} {form} {ragged}")
+    b, n = shape[:2]
+    lens = ([n - 31 * i for i in range(b)],) * 2 if ragged else None
+
+    def spoil(v):
+        for i in range(b if ragged else 0):
+            v["k"][i, lens[1][i]:] = v["v"][i, lens[1][i]:] = np.nan
+            v["q"][i, lens[0][i]:] = v["do"][i, lens[0][i]:] = np.inf
+
+    c = Call(*shape, form, lens=lens, seed=8, spoil=spoil)
+    c.forward()
+    c.backward()
+    check_rows(c)
