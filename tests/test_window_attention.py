@@ -899,3 +899,17 @@ def test_sinks_of_several_heads_apart(shape, form, ragged):
     c.forward()
     c.backward()
     check_rows(c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(2, 1, 300, 4, 2, 128, 64, 4), (3, 1, 3000, 8, 2, 128, 1500, 4), (1, 4, 900, 6, 2, 64, 0, 0),
+                                   (1, 13, 1200, 8, 1, 64, 500, 2), (1, 50, 2000, 4, 2, 64, 1700, 1)],
+                         ids=lambda s: "-".join(str(x) for x in s))
+def test_few_rows_of_bf16_operands_lose_nothing_to_p(shape):
+    """O in fp32 of a few rows: P is held as two bf16 terms, off by 2^-16 of itself at most, beside the fp32
+    bar for the sums."""
+    note(f"window attention few rows {shape}")
+    c = Call(*shape, "bf16-fp32", seed=9)
+    c.forward()
+    got, want = c.read(), c.want()
+    assert np.linalg.norm(got["o"] - want["o"]) <= (2.0 ** -16 + 1e-5) * np.linalg.norm(want["o"])
