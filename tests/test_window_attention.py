@@ -913,3 +913,12 @@ def test_few_rows_of_bf16_operands_lose_nothing_to_p(shape):
     c.forward()
     got, want = c.read(), c.want()
     assert np.linalg.norm(got["o"] - want["o"]) <= (2.0 ** -16 + 1e-5) * np.linalg.norm(want["o"])
+
+
+def test_lengths_that_are_not_aligned_are_refused():
+    from valkyr_amd import kernels as K
+
+    p, args = K.window_params(4, 4, 2, 1, 64, 2, 1), [256] * 10
+    for kw in (dict(q_len=258), dict(kv_len=257), dict(q_len=256, kv_len=254)):
+        assert refused(K.fa_window_forward, p, *args[:4], **kw) == "InvalidArgument"
+        assert refused(K.fa_window_backward, p, *args, **kw) == "InvalidArgument"

@@ -520,6 +520,8 @@ static vkh_status window_args(const vkh_window_params *p, WindowArgs &a) {
     return VKH_OK;
 }
 static bool aligned_to(const void *x, DType t) { return (uintptr_t)x % (t == DType::F32 ? 4 : 2) == 0; }
+// (scalar loads take a length from the word that its address lies in)
+static bool lens_aligned(const uint32_t *q_len, const uint32_t *kv_len) { return ((uintptr_t)q_len | (uintptr_t)kv_len) % 4 == 0; }
 
 // The caller's workspace, else the stream's scratch; none (ws = null) under capture or where
 // there is no memory for it.
@@ -549,7 +551,7 @@ vkh_status vkh_fa_window_forward(const vkh_window_params *p, const void *q, cons
     VKH_TRY(window_args(p, a));
     CHECK_ARG(q && k && v && o, "null pointer");
     CHECK_ARG(aligned_to(q, a.dt) && aligned_to(k, a.dt) && aligned_to(v, a.dt) && aligned_to(o, a.odt) &&
-                  aligned_to(lse, DType::F32),
+                  aligned_to(lse, DType::F32) && lens_aligned(q_len, kv_len),
               "a pointer is not aligned to its type");
     a.q = q; a.k = k; a.v = v; a.o = o; a.lse = lse; a.q_len = q_len; a.kv_len = kv_len;
     ScratchLease lease;
@@ -572,7 +574,7 @@ vkh_status vkh_fa_window_backward(const vkh_window_params *p, const void *q, con
     CHECK_ARG(q && k && v && o && dout && lse && d && dq && dk && dv, "null pointer");
     CHECK_ARG(aligned_to(q, a.dt) && aligned_to(k, a.dt) && aligned_to(v, a.dt) && aligned_to(dout, a.dt) &&
                   aligned_to(o, a.odt) && aligned_to(dq, a.odt) && aligned_to(dk, a.odt) && aligned_to(dv, a.odt) &&
-                  aligned_to(lse, DType::F32) && aligned_to(d, DType::F32),
+                  aligned_to(lse, DType::F32) && aligned_to(d, DType::F32) && lens_aligned(q_len, kv_len),
               "a pointer is not aligned to its type");
     a.q = q; a.k = k; a.v = v; a.o = (void *)o; a.dout = dout; a.lse = (float *)lse; a.d = d;
     a.dq = dq; a.dk = dk; a.dv = dv; a.q_len = q_len; a.kv_len = kv_len;
