@@ -42,8 +42,10 @@ VKH_DEV void wait_vm() {
 }
 
 // LDS tiles of bf16 head rows of HD values, as the DMA writes them: 16-byte chunk c of row r at
-// chunk c ^ swz(r), so the 16 rows of a fragment read land in 16 different chunk columns of
-// LDS's 256 bytes a cycle (rows of 128 bytes: two of them side by side).
+// chunk c ^ swz(r), so the 16 rows of a fragment read (frag_row) land in 16 different chunk columns of
+// LDS's 256 bytes a cycle (rows of 128 bytes: two of them side by side).  A transposing read (tr4) takes
+// two neighbouring chunks of each row, which rows r and r ^ 1 hold in the same two columns: half of the
+// banks twice, two cycles more a read (a quarter to a third of the cycles that the kernels' LDS is active).
 template <int HD>
 struct TileRows {
     static_assert(HD == 64 || HD == 128, "head width");

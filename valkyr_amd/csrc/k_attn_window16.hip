@@ -473,7 +473,7 @@ __global__ __launch_bounds__(256, 1) void window_step16_k(WindowArgs a, int spli
 // D = rowsum(O dO) of the block's rows is formed first (fp64 sums of the bf16 products) and
 // stored for the dK/dV kernel, which runs after this one.  As the forward, it is bound by what a wave
 // does between its products (softmax, rounding, LDS reads) and by masked tiles: 16384 tokens, window
-// 2048, 32 / 8 heads of 128: 760 us, 1.02 PFLOP/s; 4 x 2048, window 512, 16 / 8 heads: 77 us, 0.59 PFLOP/s.  KG = 2 (short
+// 2048, 32 / 8 heads of 128: 760 to 773 us, 1.0 PFLOP/s; 4 x 2048, window 512, 16 / 8 heads: 77 us, 0.59 PFLOP/s.  KG = 2 (short
 // grids: one block a CU): two groups of waves take every other tile; 2048 tokens, window 2048, 8 / 8
 // heads of 64, forward / backward: 24.8 / 73 us without, 19.3 / 63 with.
 template <int HD, int BQ, int KG, class TO>
@@ -941,8 +941,8 @@ __global__ __launch_bounds__(512, 1) void window_dkv16_k(WindowArgs a, DkvPlan p
 // order.  The key blocks leave these pairs out: with them, the sink blocks' steps past the window, for
 // which three waves of four had nothing to do, took 1442 us of dK/dV to 1177 without (16384 tokens,
 // window 2048, 4 sinks, 32 / 8 heads of 128).  Bound by reading Q and dO
-// once more (51 us there, 5 TB/s); on shorter sequences by the chain of loads, steps and join (4 x 2048
-// tokens, window 512, 16 / 8 heads: 17 us; with 32 sinks a wave, 4 of them there, 20).
+// once more (51 to 56 us there, 5 TB/s); on shorter sequences by the chain of loads, steps and join (4 x 2048
+// tokens, window 512, 16 / 8 heads: 18 us; with 32 sinks a wave, 4 of them there, 20).
 template <int HD, int KS>
 __global__ __launch_bounds__(256, 1) void window_far16_k(WindowArgs a, DkvPlan plan) {
     using R = TileRows<HD>;
