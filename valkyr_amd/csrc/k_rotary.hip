@@ -79,8 +79,8 @@ VKH_DEV void load_gain(const float *p, float (&o)[V], float quirk) {
 
 // The V pairs that a lane holds as two chunks, turned.  Half layout: pair i is (a[i], b[i]);
 // interleaved: neighbours within a, then within b.  SELECT: lanes that are not `turned` (their cs is (1, 0))
-// may call it too; what their sines multiply is taken as 0, since 0 times an infinity or a NaN is NaN (the
-// norm's backward, which a branch around the call would take 140 in place of 100 us: registers).
+// may call it too; what their sines multiply is taken as 0, since 0 times an infinity or a NaN is NaN.  (For the
+// norm's backward: with a branch around the call it has four waves a SIMD in place of five, 140 us for 100.)
 template <bool SELECT, int V>
 VKH_DEV void turn_pairs(float (&a)[V], float (&b)[V], const float2 (&cs)[V], bool interleaved, bool turned = true) {
     auto part = [&](float x) { return !SELECT || turned ? x : 0.f; };
@@ -126,7 +126,7 @@ VKH_DEV void chunks(const RotaryArgs &a, int t, int V, int &e0, int &e1) {
 }
 
 // The cosines and sines of a row for the V pairs of each lane: a wave computes one pair a lane and
-// hands them round through its own LDS (128 pairs); whether the lane's values are turned at all.
+// hands them round through its own LDS (128 pairs).  True where the lane's values are turned.
 template <int V>
 VKH_DEV bool row_angles(const RotaryArgs &a, unsigned pos, float2 *sh, int lane, int t, float2 (&cs)[V]) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last row's are read
