@@ -718,6 +718,68 @@ vkh_status vkh_rmsnorm_backward_noalloc(const float *dy, const float *x, const f
  * entry points use), so a test can check that an entry point allocates
  * nothing. */
 uint64_t vkh_allocation_count(void);
+/* Layer norm of rows: y = (x - mean) rstd w + b with rstd = 1 / sqrt(variance + eps) (the reference's
+ * layernorm.comp, layernorm_backward.comp, in its inference half; fp32 and dense rows there).  Any
+ * dim, any row strides (in elements, 0 for dense rows) and pointers aligned to their types alone;
+ * y may be x, and dx may be dy, x or the residual, where type and stride are the same.  Under 2^31
+ * rows, dim under 2^24. */
+typedef struct vkh_layernorm_params {
+    uint32_t n_rows, dim;
+    float eps;
+    uint32_t x_dtype, y_dtype, dy_dtype, dx_dtype; /* vkh_dtype */
+    uint32_t ld_x, ld_y, ld_dy, ld_dx;
+} vkh_layernorm_params;
+/* w, b [dim] fp32; NULL: ones, zeros. */
+vkh_status vkh_layernorm_forward(const vkh_layernorm_params *p, const void *x, const float *w,
+                                 const float *b, void *y, vkh_stream stream);
+/* dx (plus `residual`, rows of dx's type and stride, if non-NULL), and the gradients dw, db [dim] fp32
+ * (overwrite, summed in a fixed order; either may be NULL), from the forward's x: the statistics
+ * are formed again.  `workspace` (16-byte aligned) holds vkh_layernorm_backward_workspace_bytes(p)
+ * bytes; NULL takes the library's per-stream scratch, which a call with dw or db on a stream under
+ * capture may not (VKH_ERR_INVALID_ARGUMENT). */
+size_t vkh_layernorm_backward_workspace_bytes(const vkh_layernorm_params *p);
+vkh_status vkh_layernorm_backward(const vkh_layernorm_params *p, const void *dy, const void *x,
+                                  const float *w, void *dx, const void *residual, float *dw,
+                                  float *db, void *workspace, vkh_stream stream);
+/* A gated linear recurrence over each sequence's rows, every channel on its own:
+ *   h_t = a_t h_{t-1} + u_t,   h_{-1} = h0 (NULL: zeros)
+ *   a_t = sigmoid(g_t) (VKH_SCAN_SIGMOID) or g_t itself, at most 1 in size (VKH_SCAN_DECAY)
+ *   u_t = x_t, or (coupled) (1 - a_t) x_t
+ * Sequence b is rows b n_pos .. of every matrix [n_batch n_pos, dim] and has length[b] of them (uint32
+ * [n_batch] on the device, values beyond n_pos taken as n_pos; NULL: all).  Rows from length[b] on take no
+ * part, whatever they hold: their h and gradients are 0.  States and their sums are fp32
+ * throughout.  The reference has the single-token step of a gated delta rule only
+ * (gated_delta_step.comp).  Values that are not finite reach the rest of their channel's sequence,
+ * and no other channel. */
+typedef enum vkh_scan_gate { VKH_SCAN_SIGMOID = 0, VKH_SCAN_DECAY = 1 } vkh_scan_gate;
+typedef struct vkh_scan_params {
+    uint32_t n_batch;    /* 0 means 1; under 2^16 */
+    uint32_t n_pos, dim; /* rows of a sequence (under 2^30), channels (under 2^24) */
+    uint32_t gate;       /* vkh_scan_gate */
+    uint32_t coupled;
+    uint32_t dtype;      /* vkh_dtype of x, g, dh */
+    uint32_t out_dtype;  /* of h, dx, dg */
+    uint32_t ld_x, ld_g, ld_h, ld_dh, ld_dx, ld_dg; /* row strides in elements; 0: dense */
+} vkh_scan_params;
+/* h, and (each if non-NULL) h_last [n_batch, dim] fp32, the state behind the last row (h0 where there is none;
+ * may be h0: a decode loop's state), and `states`, vkh_gated_scan_states_floats(p) floats that the
+ * backward starts from.  h may be x or g where type and stride are the same.  `workspace` (16-byte
+ * aligned, may be NULL) holds vkh_gated_scan_workspace_bytes(p) bytes, with which long sequences of
+ * few channels are split over time.  Without it the call takes the library's per-stream scratch, and
+ * where that is not to be had (a stream under capture) runs unsplit.  One call or captured graph at a
+ * time uses a workspace. */
+size_t vkh_gated_scan_states_floats(const vkh_scan_params *p);
+size_t vkh_gated_scan_workspace_bytes(const vkh_scan_params *p);
+vkh_status vkh_gated_scan_forward(const vkh_scan_params *p, const void *x, const void *g,
+                                  const float *h0, void *h, float *h_last, float *states,
+                                  const uint32_t *length, void *workspace, vkh_stream stream);
+/* dx, dg (overwrite) and, if non-NULL, dh0 [n_batch, dim] fp32, from the forward's x, g and `states`
+ * and the gradients dh of h and dh_last [n_batch, dim] fp32 of h_last (NULL: zeros; may be dh0).
+ * dx and dg may be dh, x or g (not the same one) where type and stride are the same. */
+vkh_status vkh_gated_scan_backward(const vkh_scan_params *p, const void *x, const void *g,
+                                   const float *states, const void *dh, const float *dh_last,
+                                   void *dx, void *dg, float *dh0, const uint32_t *length,
+                                   void *workspace, vkh_stream stream);
 /* shaders/swiglu_forward.comp / swiglu_backward.comp (SwigluPush {n}) */
 vkh_status vkh_swiglu_forward(const float *pre_gate, const float *up, float *gated, size_t n,
                               vkh_stream stream);
@@ -844,6 +906,25 @@ vkh_status vkh_embedding_backward(const float *dy, const uint32_t *ids, float *d
 vkh_status vkh_adam_step(float *param, const float *grad, float *m, float *v, size_t n, float lr,
                          float beta1, float beta2, float eps, uint32_t t, float weight_decay,
                          vkh_stream stream);
+/* Gradients of many tensors at once, ahead of Adam.  The reference has no clipping. */
+typedef struct vkh_grad {
+    const void *grad;
+    size_t n;       /* values; 0: left out */
+    uint32_t dtype; /* vkh_dtype */
+    void *out;      /* vkh_grad_clip: where the clipped gradient goes; NULL: in place */
+} vkh_grad;
+/* norm[0] (fp32) = the root of the sum of all squares, summed in 64 bits in a fixed order.  `grads`
+ * is a host array, read before the call returns.  `workspace` (16-byte aligned) holds
+ * vkh_grad_clip_workspace_bytes(n_grads) bytes; NULL takes the library's per-stream scratch, which
+ * a call on a stream under capture may not (VKH_ERR_INVALID_ARGUMENT). */
+size_t vkh_grad_clip_workspace_bytes(size_t n_grads);
+vkh_status vkh_grad_norm(const vkh_grad *grads, size_t n_grads, float *norm, void *workspace,
+                         vkh_stream stream);
+/* The same norm (norm may be NULL), and every gradient times max_norm / norm where the norm is over
+ * max_norm (at least 0) and finite; elsewhere they stay as they are, so a caller finds a step that overflowed in
+ * its norm.  No output may overlap another tensor of the list (VKH_ERR_INVALID_ARGUMENT). */
+vkh_status vkh_grad_clip(const vkh_grad *grads, size_t n_grads, float max_norm, float *norm,
+                         void *workspace, vkh_stream stream);
 /* shaders/add_in_place.comp, vec_add.comp, scale.comp */
 vkh_status vkh_add_in_place(float *dst, const float *src, size_t n, vkh_stream stream);
 vkh_status vkh_vec_add(const float *a, const float *b, float *c, size_t n, vkh_stream stream);

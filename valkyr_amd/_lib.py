@@ -134,6 +134,21 @@ class WindowParams(C.Structure):
                                            "ld_do", "ld_dq", "ld_dk", "ld_dv")]
 
 
+class LayernormParams(C.Structure):
+    _fields_ = [("n_rows", C.c_uint32), ("dim", C.c_uint32), ("eps", C.c_float)]
+    _fields_ += [(n, C.c_uint32) for n in ("x_dtype", "y_dtype", "dy_dtype", "dx_dtype", "ld_x", "ld_y",
+                                           "ld_dy", "ld_dx")]
+
+
+class ScanParams(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("n_batch", "n_pos", "dim", "gate", "coupled", "dtype", "out_dtype",
+                                          "ld_x", "ld_g", "ld_h", "ld_dh", "ld_dx", "ld_dg")]
+
+
+class Grad(C.Structure):
+    _fields_ = [("grad", C.c_void_p), ("n", C.c_size_t), ("dtype", C.c_uint32), ("out", C.c_void_p)]
+
+
 class TrainBudget(C.Structure):
     _fields_ = [("mode", C.c_uint32), ("steps", C.c_uint32), ("microseconds", C.c_uint64)]
 
@@ -264,6 +279,16 @@ SIGNATURES = [
     ("vkh_rmsnorm_backward", ST, [P, P, P, P, P, P, U32, U32, F, U32, P]),
     ("vkh_rmsnorm_backward_noalloc", ST, [P, P, P, P, P, P, U32, U32, F, U32, P]),
     ("vkh_allocation_count", C.c_uint64, []),
+    ("vkh_layernorm_forward", ST, [C.POINTER(LayernormParams), P, P, P, P, P]),
+    ("vkh_layernorm_backward_workspace_bytes", SZ, [C.POINTER(LayernormParams)]),
+    ("vkh_layernorm_backward", ST, [C.POINTER(LayernormParams), P, P, P, P, P, P, P, P, P]),
+    ("vkh_gated_scan_states_floats", SZ, [C.POINTER(ScanParams)]),
+    ("vkh_gated_scan_workspace_bytes", SZ, [C.POINTER(ScanParams)]),
+    ("vkh_gated_scan_forward", ST, [C.POINTER(ScanParams), P, P, P, P, P, P, P, P, P]),
+    ("vkh_gated_scan_backward", ST, [C.POINTER(ScanParams), P, P, P, P, P, P, P, P, P, P, P]),
+    ("vkh_grad_clip_workspace_bytes", SZ, [SZ]),
+    ("vkh_grad_norm", ST, [C.POINTER(Grad), SZ, P, P, P]),
+    ("vkh_grad_clip", ST, [C.POINTER(Grad), SZ, F, P, P, P]),
     ("vkh_swiglu_forward", ST, [P, P, P, SZ, P]),
     ("vkh_swiglu_backward", ST, [P, P, P, P, P, SZ, P]),
     ("vkh_qk_rope_forward", ST, [C.POINTER(RopeParams), P, P, P, P, P]),

@@ -13,6 +13,7 @@
 #include <map>
 #include <memory>
 #include <mutex>
+#include <new>
 #include <tuple>
 #include <utility>
 #include <vector>
@@ -1086,6 +1087,140 @@ vkh_status vkh_rmsnorm_backward_noalloc(const float *dy, const float *x, const f
 
 uint64_t vkh_allocation_count(void) { return g_allocations.load(std::memory_order_relaxed); }
 
+// ── layer norm ─────────────────────────────────────────────────────────
+
+static inline DType DT(uint32_t d) { return d == VKH_BF16 ? DType::BF16 : DType::F32; }
+
+static vkh_status layernorm_args(const vkh_layernorm_params *p, LayernormArgs &a) {
+    CHECK_ARG(p, "null params");
+    CHECK_ARG(p->dim, "zero dimension");
+    CHECK_ARG(p->x_dtype <= VKH_BF16 && p->y_dtype <= VKH_BF16 && p->dy_dtype <= VKH_BF16 && p->dx_dtype <= VKH_BF16, "dtype");
+    if (p->n_rows >= (1u << 31) || p->dim >= (1u << 24)) return fail(VKH_ERR_UNSUPPORTED, "2^31 rows or 2^24 values of one");
+    for (uint32_t ld : {p->ld_x, p->ld_y, p->ld_dy, p->ld_dx}) CHECK_ARG(!ld || ld >= p->dim, "a row stride is less than the row");
+    auto ld = [&](uint32_t l) { return (long)(l ? l : p->dim); };
+    a.ldx = ld(p->ld_x); a.ldy = ld(p->ld_y); a.lddy = ld(p->ld_dy); a.lddx = ld(p->ld_dx);
+    a.n_rows = p->n_rows; a.dim = (int)p->dim; a.eps = p->eps;
+    return VKH_OK;
+}
+
+vkh_status vkh_layernorm_forward(const vkh_layernorm_params *p, const void *x, const float *w, const float *b,
+                                 void *y, vkh_stream stream) {
+    LayernormArgs a;
+    VKH_TRY(layernorm_args(p, a));
+    if (!a.n_rows) return VKH_OK;
+    const DType xt = DT(p->x_dtype), yt = DT(p->y_dtype);
+    CHECK_ARG(x && y, "null pointer");
+    CHECK_ARG(aligned_to(x, xt) && aligned_to(y, yt) && aligned_to(w, DType::F32) && aligned_to(b, DType::F32),
+              "a pointer is not aligned to its type");
+    a.x = x; a.y = y; a.w = w; a.b = b;
+    VKH_HIP(layernorm_forward(a, xt, yt, S(stream)));
+    return VKH_OK;
+}
+
+size_t vkh_layernorm_backward_workspace_bytes(const vkh_layernorm_params *p) {
+    LayernormArgs a;
+    return layernorm_args(p, a) == VKH_OK ? layernorm_partial_floats(a) * sizeof(float) : 0;
+}
+
+// A workspace that the call cannot do without: the caller's, else the stream's scratch.
+static vkh_status needed_ws(void *workspace, size_t bytes, ScratchLease &lease, hipStream_t st, void **ws) {
+    CHECK_ARG((uintptr_t)workspace % 16 == 0, "the workspace is not 16-byte aligned");
+    CHECK_ARG(workspace || !capturing(st), "this call on a stream under capture needs a workspace");
+    *ws = workspace;
+    if (!workspace) VKH_TRY(lease.acquire(bytes, st, ws));
+    return VKH_OK;
+}
+
+vkh_status vkh_layernorm_backward(const vkh_layernorm_params *p, const void *dy, const void *x, const float *w,
+                                  void *dx, const void *residual, float *dw, float *db, void *workspace,
+                                  vkh_stream stream) {
+    LayernormArgs a;
+    VKH_TRY(layernorm_args(p, a));
+    const DType xt = DT(p->x_dtype), gt = DT(p->dy_dtype), dt = DT(p->dx_dtype);
+    hipStream_t st = S(stream);
+    CHECK_ARG(aligned_to(dw, DType::F32) && aligned_to(db, DType::F32), "a pointer is not aligned to its type");
+    if (!a.n_rows) {  // empty sums
+        if (dw) VKH_HIP(fill_f32(dw, a.dim, 0.f, st));
+        if (db) VKH_HIP(fill_f32(db, a.dim, 0.f, st));
+        return VKH_OK;
+    }
+    CHECK_ARG(dy && x && dx, "null pointer");
+    CHECK_ARG(aligned_to(x, xt) && aligned_to(dy, gt) && aligned_to(dx, dt) && aligned_to(residual, dt) && aligned_to(w, DType::F32),
+              "a pointer is not aligned to its type");
+    a.x = x; a.dy = dy; a.dx = dx; a.res = residual; a.w = w; a.dw = dw; a.db = db;
+    ScratchLease lease;
+    if (dw || db) {
+        void *ws = nullptr;
+        VKH_TRY(needed_ws(workspace, layernorm_partial_floats(a) * sizeof(float), lease, st, &ws));
+        a.partial = (float *)ws;
+    }
+    VKH_HIP(layernorm_backward(a, xt, gt, dt, st));
+    return VKH_OK;
+}
+
+// ── gated linear recurrence ────────────────────────────────────────────
+
+static vkh_status scan_args(const vkh_scan_params *p, ScanArgs &a) {
+    CHECK_ARG(p, "null params");
+    CHECK_ARG(p->dim, "zero dimension");
+    CHECK_ARG(p->gate <= VKH_SCAN_DECAY, "gate");
+    CHECK_ARG(p->dtype <= VKH_BF16 && p->out_dtype <= VKH_BF16, "dtype");
+    if (p->n_batch >= (1u << 16) || p->n_pos >= (1u << 30) || p->dim >= (1u << 24))
+        return fail(VKH_ERR_UNSUPPORTED, "2^16 sequences, 2^30 rows of one or 2^24 channels");
+    for (uint32_t ld : {p->ld_x, p->ld_g, p->ld_h, p->ld_dh, p->ld_dx, p->ld_dg})
+        CHECK_ARG(!ld || ld >= p->dim, "a row stride is less than the row");
+    auto ld = [&](uint32_t l) { return (long)(l ? l : p->dim); };
+    a.ldx = ld(p->ld_x); a.ldg = ld(p->ld_g); a.ldh = ld(p->ld_h);
+    a.lddh = ld(p->ld_dh); a.lddx = ld(p->ld_dx); a.lddg = ld(p->ld_dg);
+    a.n_batch = p->n_batch ? (int)p->n_batch : 1; a.n_pos = (int)p->n_pos; a.dim = (int)p->dim;
+    a.sigmoid = p->gate == VKH_SCAN_SIGMOID; a.coupled = p->coupled != 0;
+    a.dt = DT(p->dtype); a.odt = DT(p->out_dtype);
+    return VKH_OK;
+}
+
+size_t vkh_gated_scan_states_floats(const vkh_scan_params *p) {
+    ScanArgs a;
+    return scan_args(p, a) == VKH_OK ? scan_states_floats(a) : 0;
+}
+size_t vkh_gated_scan_workspace_bytes(const vkh_scan_params *p) {
+    ScanArgs a;
+    return scan_args(p, a) == VKH_OK ? scan_ws_bytes(a) : 0;
+}
+
+vkh_status vkh_gated_scan_forward(const vkh_scan_params *p, const void *x, const void *g, const float *h0, void *h,
+                                  float *h_last, float *states, const uint32_t *length, void *workspace,
+                                  vkh_stream stream) {
+    ScanArgs a;
+    VKH_TRY(scan_args(p, a));
+    CHECK_ARG(!a.n_pos || (x && g && h), "null pointer");
+    CHECK_ARG(aligned_to(x, a.dt) && aligned_to(g, a.dt) && aligned_to(h, a.odt) && aligned_to(h0, DType::F32) &&
+                  aligned_to(h_last, DType::F32) && aligned_to(states, DType::F32) && (uintptr_t)length % 4 == 0,
+              "a pointer is not aligned to its type");
+    a.x = x; a.g = g; a.h0 = h0; a.h = h; a.h_last = h_last; a.states = states; a.len = length;
+    ScratchLease lease;
+    VKH_TRY(optional_ws(workspace, scan_ws_bytes(a), lease, S(stream), (float **)&a.ws));
+    VKH_HIP(scan_forward(a, S(stream)));
+    return VKH_OK;
+}
+
+vkh_status vkh_gated_scan_backward(const vkh_scan_params *p, const void *x, const void *g, const float *states,
+                                   const void *dh, const float *dh_last, void *dx, void *dg, float *dh0,
+                                   const uint32_t *length, void *workspace, vkh_stream stream) {
+    ScanArgs a;
+    VKH_TRY(scan_args(p, a));
+    CHECK_ARG(!a.n_pos || (x && g && states && dh && dx && dg), "null pointer");
+    CHECK_ARG(aligned_to(x, a.dt) && aligned_to(g, a.dt) && aligned_to(dh, a.dt) && aligned_to(dx, a.odt) &&
+                  aligned_to(dg, a.odt) && aligned_to(states, DType::F32) && aligned_to(dh_last, DType::F32) &&
+                  aligned_to(dh0, DType::F32) && (uintptr_t)length % 4 == 0,
+              "a pointer is not aligned to its type");
+    CHECK_ARG(!a.n_pos || dx != dg, "dx and dg are the same rows");
+    a.x = x; a.g = g; a.states = (float *)states; a.dh = dh; a.dh_last = dh_last; a.dx = dx; a.dg = dg; a.dh0 = dh0; a.len = length;
+    ScratchLease lease;
+    VKH_TRY(optional_ws(workspace, scan_ws_bytes(a), lease, S(stream), (float **)&a.ws));
+    VKH_HIP(scan_backward(a, S(stream)));
+    return VKH_OK;
+}
+
 vkh_status vkh_swiglu_forward(const float *pg, const float *up, float *g, size_t n,
                               vkh_stream stream) {
     CHECK_ARG(pg && up && g, "null pointer");
@@ -1172,8 +1307,6 @@ vkh_status vkh_rotary_plan_init(const vkh_rotary_spec *sp, vkh_rotary_plan *out)
     *out = pl;
     return VKH_OK;
 }
-
-static inline DType DT(uint32_t d) { return d == VKH_BF16 ? DType::BF16 : DType::F32; }
 
 static vkh_status rotary_args(const vkh_rotary_params *p, const vkh_rotary_plan *pl, const uint32_t *positions,
                               RotaryArgs &a) {
@@ -1380,6 +1513,77 @@ vkh_status vkh_adam_step(float *param, const float *grad, float *m, float *v, si
     VKH_HIP(adam_step(param, grad, m, v, n, lr, beta1, beta2, eps, 1.0f - powf(beta1, tf),
                       1.0f - powf(beta2, tf), wd, nullptr, S(stream)));
     return VKH_OK;
+}
+
+// ── norm and clipping of a list of gradients ───────────────────────────
+
+// Whether an output shares memory with another tensor of the list (or, shifted, with its own).
+static bool grads_overlap(const std::vector<GradTensor> &t) {
+    struct Span { uintptr_t lo, hi; };
+    std::vector<Span> reads, writes;
+    for (const GradTensor &x : t) {
+        const uintptr_t g = (uintptr_t)x.g, o = (uintptr_t)x.out, n = x.n * (x.dt == DType::F32 ? 4 : 2);
+        if (g != o) reads.push_back({g, g + n});
+        writes.push_back({o, o + n});
+    }
+    auto before = [](const Span &x, const Span &y) { return x.lo < y.lo; };
+    for (auto *v : {&reads, &writes})
+        if (!std::is_sorted(v->begin(), v->end(), before)) std::sort(v->begin(), v->end(), before);
+    uintptr_t wrote = 0, read = 0;  // the furthest ends of what starts before
+    for (size_t r = 0, w = 0; r < reads.size() || w < writes.size();) {
+        if (w == writes.size() || (r < reads.size() && reads[r].lo < writes[w].lo)) {
+            if (reads[r].lo < wrote) return true;
+            read = std::max(read, reads[r++].hi);
+        } else {
+            if (writes[w].lo < wrote || writes[w].lo < read) return true;
+            wrote = std::max(wrote, writes[w++].hi);
+        }
+    }
+    return false;
+}
+
+static vkh_status grad_call(const vkh_grad *grads, size_t n, bool clip, float max_norm, float *norm, void *workspace,
+                            vkh_stream stream) {
+    CHECK_ARG(grads || !n, "null list");
+    CHECK_ARG(aligned_to(norm, DType::F32), "a pointer is not aligned to its type");
+    if (n >= (1u << 24)) return fail(VKH_ERR_UNSUPPORTED, "2^24 tensors");
+    try {
+        std::vector<GradTensor> t;
+        t.reserve(n);
+        size_t total = 0;
+        for (size_t i = 0; i < n; ++i) {
+            const vkh_grad &g = grads[i];
+            if (!g.n) continue;
+            CHECK_ARG(g.dtype <= VKH_BF16, "dtype");
+            CHECK_ARG(g.grad, "null gradient");
+            const GradTensor x{g.grad, g.out ? g.out : (void *)g.grad, g.n, DT(g.dtype)};
+            CHECK_ARG(aligned_to(x.g, x.dt) && aligned_to(x.out, x.dt), "a pointer is not aligned to its type");
+            if (g.n >= 1ull << 40 || (total += g.n) >= 1ull << 42) return fail(VKH_ERR_UNSUPPORTED, "2^40 values of a tensor, or 2^42 in all");
+            t.push_back(x);
+        }
+        CHECK_ARG(!clip || !grads_overlap(t), "an output overlaps another tensor of the list");
+        hipStream_t st = S(stream);
+        ScratchLease lease;
+        void *ws = nullptr;
+        if (total) VKH_TRY(needed_ws(workspace, grad_ws_bytes(n), lease, st, &ws));
+        VKH_HIP(grad_clip(t.data(), t.size(), clip, max_norm, norm, ws, st));
+        return VKH_OK;
+    } catch (const std::bad_alloc &) {
+        return fail(VKH_ERR_OUT_OF_MEMORY, "the list of gradients");
+    }
+}
+
+size_t vkh_grad_clip_workspace_bytes(size_t n_grads) { return n_grads < (1u << 24) ? grad_ws_bytes(n_grads) : 0; }
+
+vkh_status vkh_grad_norm(const vkh_grad *grads, size_t n_grads, float *norm, void *workspace, vkh_stream stream) {
+    CHECK_ARG(norm, "null pointer");
+    return grad_call(grads, n_grads, false, 0.f, norm, workspace, stream);
+}
+
+vkh_status vkh_grad_clip(const vkh_grad *grads, size_t n_grads, float max_norm, float *norm, void *workspace,
+                         vkh_stream stream) {
+    CHECK_ARG(max_norm >= 0.f, "max_norm is negative or not a number");
+    return grad_call(grads, n_grads, true, max_norm, norm, workspace, stream);
 }
 
 vkh_status vkh_add_in_place(float *dst, const float *src, size_t n, vkh_stream stream) {

@@ -239,6 +239,52 @@ int rmsnorm_partial_rows(int rows);
 hipError_t column_sums(const float *partial, int nparts, long stride, int dim, float *out,
                        hipStream_t st);
 
+// ── layer norm (k_layernorm.hip) ──────────────────────────────────────
+// Rows of dim values, strides in elements; any of w (ones), b (zeros), res, dw and db may be null.
+struct LayernormArgs {
+    const void *x = nullptr, *dy = nullptr, *res = nullptr;
+    void *y = nullptr, *dx = nullptr;
+    long ldx = 0, ldy = 0, lddy = 0, lddx = 0;
+    const float *w = nullptr, *b = nullptr;
+    float *dw = nullptr, *db = nullptr, *partial = nullptr;
+    long n_rows = 0;
+    int dim = 0;
+    float eps = 0.f;
+};
+hipError_t layernorm_forward(const LayernormArgs &a, DType xt, DType yt, hipStream_t st);
+// `partial` (layernorm_partial_floats(a)) only with dw or db
+hipError_t layernorm_backward(const LayernormArgs &a, DType xt, DType gt, DType dt, hipStream_t st);
+size_t layernorm_partial_floats(const LayernormArgs &a);
+
+// ── gated linear recurrence (k_scan.hip) ──────────────────────────────
+struct ScanArgs {
+    const void *x = nullptr, *g = nullptr, *dh = nullptr;
+    void *h = nullptr, *dx = nullptr, *dg = nullptr;
+    long ldx = 0, ldg = 0, ldh = 0, lddh = 0, lddx = 0, lddg = 0;
+    const float *h0 = nullptr, *dh_last = nullptr;
+    float *h_last = nullptr, *dh0 = nullptr, *states = nullptr;
+    const uint32_t *len = nullptr;
+    void *ws = nullptr;  // scan_ws_bytes(a), or null: unsplit
+    int n_batch = 0, n_pos = 0, dim = 0, sigmoid = 0, coupled = 0;
+    DType dt = DType::F32, odt = DType::F32;
+};
+constexpr int kScanTile = 128;  // rows between two states
+size_t scan_states_floats(const ScanArgs &a);
+size_t scan_ws_bytes(const ScanArgs &a);
+hipError_t scan_forward(const ScanArgs &a, hipStream_t st);
+hipError_t scan_backward(const ScanArgs &a, hipStream_t st);
+
+// ── norm and clipping of a list of gradients (k_grads.hip) ────────────
+struct GradTensor {
+    const void *g;
+    void *out;
+    size_t n;
+    DType dt;
+};
+size_t grad_ws_bytes(size_t n);
+// norm (if non-null) = the root of the sum of squares; with `clip` the outputs too.  ws: grad_ws_bytes(n).
+hipError_t grad_clip(const GradTensor *t, size_t n, bool clip, float max_norm, float *norm, void *ws, hipStream_t st);
+
 // RoPE cos/sin table [seq_len][rotary_dim/2] as float2, built on the host
 // with the fp32 formula of qk_rope_partial_batched.comp:76-81.
 void rope_table_host(float2 *tab, int seq_len, int rotary_dim, float theta);

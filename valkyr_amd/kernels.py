@@ -10,13 +10,14 @@ from __future__ import annotations
 import ctypes as C
 import math
 
-from ._lib import (AttnParams, CceParams, LoraAdapter, RopeParams, RotaryParams, RotaryPlan,
-                   RotarySpec, WindowParams, check, lib)
+from ._lib import (AttnParams, CceParams, Grad, LayernormParams, LoraAdapter, RopeParams, RotaryParams,
+                   RotaryPlan, RotarySpec, ScanParams, WindowParams, check, lib)
 
 F32, BF16 = 0, 1
 ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
 ROTARY_UNSCALED, ROTARY_LINEAR, ROTARY_NTK, ROTARY_YARN, ROTARY_BANDS = range(5)
 PRECISION_FP32, PRECISION_BF16 = 0, 1
+SCAN_SIGMOID, SCAN_DECAY = 0, 1
 
 
 def _p(x):
@@ -241,6 +242,82 @@ def rmsnorm_backward_noalloc(dy, x, w, dx, dw=None, n_rows=0, dim=0, eps=1e-6,
     per-device array: no allocation; calls on one GPU must not overlap."""
     check(lib().vkh_rmsnorm_backward_noalloc(_p(dy), _p(x), _p(w), _p(dx), _p(residual), _p(dw),
                                              n_rows, dim, eps, int(gemma_quirk), _s(stream)))
+
+
+def layernorm_params(n_rows, dim, eps=1e-5, x_dtype=F32, y_dtype=F32, dy_dtype=F32, dx_dtype=F32, ld_x=0,
+                     ld_y=0, ld_dy=0, ld_dx=0):
+    return LayernormParams(n_rows, dim, eps, x_dtype, y_dtype, dy_dtype, dx_dtype, ld_x, ld_y, ld_dy, ld_dx)
+
+
+def layernorm_forward(p, x, w, b, y, stream=None):
+    """y = (x - mean) rstd w + b of each row (w, b may be None: ones, zeros)."""
+    check(lib().vkh_layernorm_forward(C.byref(p), _p(x), _p(w), _p(b), _p(y), _s(stream)))
+
+
+def layernorm_backward_workspace_bytes(p):
+    return lib().vkh_layernorm_backward_workspace_bytes(C.byref(p))
+
+
+def layernorm_backward(p, dy, x, w, dx, residual=None, dw=None, db=None, workspace=None, stream=None):
+    """dx (+ residual), and the gain's and bias's gradients, of layernorm_forward."""
+    check(lib().vkh_layernorm_backward(C.byref(p), _p(dy), _p(x), _p(w), _p(dx), _p(residual), _p(dw), _p(db),
+                                       _p(workspace), _s(stream)))
+
+
+def scan_params(n_pos, dim, n_batch=1, gate=SCAN_SIGMOID, coupled=False, dtype=F32, out_dtype=None, ld_x=0,
+                ld_g=0, ld_h=0, ld_dh=0, ld_dx=0, ld_dg=0):
+    """h_t = a_t h_{t-1} + u_t over n_batch sequences of n_pos rows: a = sigmoid(g) or g, u = x or
+    (1 - a) x; h and gradients are stored as out_dtype (None: dtype)."""
+    return ScanParams(n_batch, n_pos, dim, gate, 1 if coupled else 0, dtype,
+                      dtype if out_dtype is None else out_dtype, ld_x, ld_g, ld_h, ld_dh, ld_dx, ld_dg)
+
+
+def gated_scan_states_floats(p):
+    return lib().vkh_gated_scan_states_floats(C.byref(p))
+
+
+def gated_scan_workspace_bytes(p):
+    return lib().vkh_gated_scan_workspace_bytes(C.byref(p))
+
+
+def gated_scan_forward(p, x, g, h, h0=None, h_last=None, states=None, length=None, workspace=None, stream=None):
+    """h of every row, the state behind each sequence (h_last) and, for the backward, states;
+    length: each sequence's rows (uint32 [n_batch] on the device), None for all."""
+    check(lib().vkh_gated_scan_forward(C.byref(p), _p(x), _p(g), _p(h0), _p(h), _p(h_last), _p(states), _p(length),
+                                       _p(workspace), _s(stream)))
+
+
+def gated_scan_backward(p, x, g, states, dh, dx, dg, dh_last=None, dh0=None, length=None, workspace=None,
+                        stream=None):
+    """dx, dg and dh0 from the gradients of h and of h_last."""
+    check(lib().vkh_gated_scan_backward(C.byref(p), _p(x), _p(g), _p(states), _p(dh), _p(dh_last), _p(dx), _p(dg),
+                                        _p(dh0), _p(length), _p(workspace), _s(stream)))
+
+
+def grad_list(tensors):
+    """ctypes array of vkh_grad from (gradient, values, dtype) or (gradient, values, dtype, out)."""
+    def addr(x):
+        p = _p(x)
+        return None if p is None else p.value
+
+    arr = (Grad * len(tensors))()
+    for i, (g, n, dtype, *out) in enumerate(tensors):
+        arr[i] = Grad(addr(g), n, dtype, addr(out[0]) if out else None)
+    return arr
+
+
+def grad_clip_workspace_bytes(grads):
+    return lib().vkh_grad_clip_workspace_bytes(len(grads))
+
+
+def grad_norm(grads, norm, workspace=None, stream=None):
+    """The norm of all tensors of a grad_list together, into norm (fp32 on the device)."""
+    check(lib().vkh_grad_norm(grads, len(grads), _p(norm), _p(workspace), _s(stream)))
+
+
+def grad_clip(grads, max_norm, norm=None, workspace=None, stream=None):
+    """Every gradient scaled by max_norm / norm where the norm of all is over max_norm and finite."""
+    check(lib().vkh_grad_clip(grads, len(grads), max_norm, _p(norm), _p(workspace), _s(stream)))
 
 
 def swiglu_forward(pre_gate, up, gated, n, stream=None):
