@@ -14,19 +14,18 @@ namespace vkh {
 namespace {
 
 constexpr int GNT = 256;
-constexpr int kChunk = 4096;    // values: a block's unit of work, of one tensor
-constexpr int kTensors = 112;   // of one launch: its table is an argument of the kernel
+constexpr int kChunk = 8192;    // values: a block's unit of work, of one tensor
+constexpr int kTensors = 180;   // of one launch: its table is an argument of the kernel
 constexpr int kParts = 2048;    // partial sums of all launches, but for one more a launch
 
-// Tensor i takes chunks first[i] .. first[i + 1].
+// Tensor i takes chunks first[i] .. first[i + 1], the last of them of (tail & 0x7fff) + 1 values.
 struct Table {
     int n;
     unsigned chunks;
     unsigned first[kTensors + 1];
-    uint8_t bf16s[kTensors];
+    uint16_t tail[kTensors];  // bit 15: bf16
     const void *g[kTensors];
     void *out[kTensors];
-    size_t len[kTensors];
 };
 static_assert(sizeof(Table) + 64 < 4096, "kernel arguments");
 
@@ -59,21 +58,70 @@ VKH_DEV double block_sum64(double v, double *sh) {
     return t;
 }
 
+// 16 bytes of a tensor, which may start at any of its values: two neighbouring lines at most take a lane's load, and
+// the lanes of a wave whole lines but for the first and last.
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef bf16 bf16x8u __attribute__((ext_vector_type(8), aligned(2)));
+template <class T> struct Vec;
+template <> struct Vec<float> { typedef f32x4u type; };
+template <> struct Vec<bf16> { typedef bf16x8u type; };
+
+// f(vector of U at i) over the chunk's n values, 16 bytes a lane and 32 KiB under way, and f1(value) behind the last
+// whole vector.
+template <class T, class F, class F1>
+VKH_DEV void over_chunk(const T *g, int n, F f, F1 f1) {
+    typedef typename Vec<T>::type V;
+    constexpr int W = 16 / sizeof(T), U = kChunk / W / GNT;
+    if (n == kChunk) {
+        V v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const V *>(g + (u * GNT + threadIdx.x) * W);
+#pragma unroll
+        for (int u = 0; u < U; ++u) f((u * GNT + threadIdx.x) * W, v[u]);
+        return;
+    }
+    for (int i = threadIdx.x * W; i + W <= n; i += GNT * W) f(i, *reinterpret_cast<const V *>(g + i));
+    const int i = n / W * W + threadIdx.x;
+    if (i < n) f1(i, g[i]);
+}
+
+// The chunk c of tensor t: its values from `at` on, and how many.
+VKH_DEV size_t chunk_at(const Table &T, int t, unsigned c, int &n) {
+    n = c + 1 == T.first[t + 1] ? (T.tail[t] & 0x7fff) + 1 : kChunk;
+    return (size_t)(c - T.first[t]) * kChunk;
+}
+
+template <class T>
+VKH_DEV void squares_of(const T *g, int n, double (&s)[4]) {
+    constexpr int W = 16 / sizeof(T);
+    over_chunk(
+        g, n,
+        [&](int, typename Vec<T>::type v) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const double d = (float)v[i];
+                s[i % 4] = fma(d, d, s[i % 4]);
+            }
+        },
+        [&](int, T v) {
+            const double d = (float)v;
+            s[0] = fma(d, d, s[0]);
+        });
+}
+
 __global__ __launch_bounds__(GNT) void grad_squares_k(Table T, double *part) {
     __shared__ double sh[GNT / 64];
-    double s = 0.0;
+    double s[4] = {};
     Share w = share(T);
     for (; w.c < w.end; ++w.c) {
         while (w.c >= T.first[w.t + 1]) ++w.t;
-        const size_t at = (size_t)(w.c - T.first[w.t]) * kChunk;
-        const size_t n = T.len[w.t] - at < kChunk ? T.len[w.t] - at : kChunk;
-        for (size_t i = threadIdx.x; i < n; i += GNT) {
-            const double v = T.bf16s[w.t] ? (float)((const bf16 *)T.g[w.t])[at + i] : ((const float *)T.g[w.t])[at + i];
-            s = fma(v, v, s);
-        }
+        int n;
+        const size_t at = chunk_at(T, w.t, w.c, n);
+        if (T.tail[w.t] >> 15) squares_of((const bf16 *)T.g[w.t] + at, n, s);
+        else squares_of((const float *)T.g[w.t] + at, n, s);
     }
-    s = block_sum64(s, sh);
-    if (threadIdx.x == 0) part[blockIdx.x] = s;
+    const double sum = block_sum64((s[0] + s[1]) + (s[2] + s[3]), sh);
+    if (threadIdx.x == 0) part[blockIdx.x] = sum;
 }
 
 VKH_DEV double norm_of(const double *part, int n_part, double *sh) {
@@ -88,6 +136,21 @@ __global__ __launch_bounds__(GNT) void grad_norm_k(const double *part, int n_par
     if (threadIdx.x == 0) norm[0] = (float)n;
 }
 
+// (scaled = false: the bits as they are)
+template <class T>
+VKH_DEV void scale_of(const T *g, T *out, int n, bool scaled, double c) {
+    typedef typename Vec<T>::type V;
+    auto one = [&](T v) { return scaled ? (T)(float)((double)(float)v * c) : v; };
+    over_chunk(
+        g, n,
+        [&](int i, V v) {
+#pragma unroll
+            for (int k = 0; k < (int)(16 / sizeof(T)); ++k) v[k] = one(v[k]);
+            *reinterpret_cast<V *>(out + i) = v;
+        },
+        [&](int i, T v) { out[i] = one(v); });
+}
+
 __global__ __launch_bounds__(GNT) void grad_scale_k(Table T, const double *part, int n_part, float max_norm, float *norm) {
     __shared__ double sh[GNT / 64];
     const double n = norm_of(part, n_part, sh);
@@ -98,17 +161,10 @@ __global__ __launch_bounds__(GNT) void grad_scale_k(Table T, const double *part,
     for (; w.c < w.end; ++w.c) {
         while (w.c >= T.first[w.t + 1]) ++w.t;
         if (!scaled && T.g[w.t] == T.out[w.t]) continue;
-        const size_t at = (size_t)(w.c - T.first[w.t]) * kChunk;
-        const size_t n = T.len[w.t] - at < kChunk ? T.len[w.t] - at : kChunk;
-        for (size_t i = threadIdx.x; i < n; i += GNT) {
-            if (T.bf16s[w.t]) {
-                const bf16 v = ((const bf16 *)T.g[w.t])[at + i];
-                ((bf16 *)T.out[w.t])[at + i] = scaled ? (bf16)(float)((double)(float)v * c) : v;
-            } else {
-                const float v = ((const float *)T.g[w.t])[at + i];
-                ((float *)T.out[w.t])[at + i] = scaled ? (float)((double)v * c) : v;
-            }
-        }
+        int n;
+        const size_t at = chunk_at(T, w.t, w.c, n);
+        if (T.tail[w.t] >> 15) scale_of((const bf16 *)T.g[w.t] + at, (bf16 *)T.out[w.t] + at, n, scaled, c);
+        else scale_of((const float *)T.g[w.t] + at, (float *)T.out[w.t] + at, n, scaled, c);
     }
 }
 
@@ -132,10 +188,9 @@ hipError_t grad_clip(const GradTensor *t, size_t n, bool clip, float max_norm, f
             for (; i < n && T.n < kTensors; ++i) {
                 if (!t[i].n) continue;
                 T.first[T.n] = T.chunks;
-                T.bf16s[T.n] = t[i].dt == DType::BF16;
+                T.tail[T.n] = (uint16_t)((t[i].n - 1) % kChunk | (t[i].dt == DType::BF16 ? 0x8000 : 0));
                 T.g[T.n] = t[i].g;
-                T.out[T.n] = t[i].out;
-                T.len[T.n++] = t[i].n;
+                T.out[T.n++] = t[i].out;
                 T.chunks += chunks_of(t[i]);
             }
             if (!T.n) break;
