@@ -334,8 +334,10 @@ __global__ __launch_bounds__(1024) void layernorm_dw_k(const float *partial, int
     const int l = threadIdx.x % 64, part = threadIdx.x / 64;
     const long c = (long)blockIdx.x * 64 + l;
     float s = 0.f;
-    if (c < 2l * dim)
+    if (c < 2l * dim) {
+#pragma unroll 8
         for (int b = part; b < n; b += 16) s += partial[(long)b * 2 * dim + c];
+    }
     sh[part][l] = s;
     __syncthreads();
     float *out = c < dim ? dw : db;
