@@ -754,7 +754,7 @@ vkh_status vkh_layernorm_backward(const vkh_layernorm_params *p, const void *dy,
 typedef enum vkh_scan_gate { VKH_SCAN_SIGMOID = 0, VKH_SCAN_DECAY = 1 } vkh_scan_gate;
 typedef struct vkh_scan_params {
     uint32_t n_batch;    /* 0 means 1; under 2^16 */
-    uint32_t n_pos, dim; /* rows of a sequence (under 2^30), channels (under 2^24) */
+    uint32_t n_pos, dim; /* rows of a sequence (under 2^30), channels (under 2^24; 2^37 of all sequences) */
     uint32_t gate;       /* vkh_scan_gate */
     uint32_t coupled;
     uint32_t dtype;      /* vkh_dtype of x, g, dh */

@@ -1167,6 +1167,7 @@ static vkh_status scan_args(const vkh_scan_params *p, ScanArgs &a) {
     CHECK_ARG(p->dtype <= VKH_BF16 && p->out_dtype <= VKH_BF16, "dtype");
     if (p->n_batch >= (1u << 16) || p->n_pos >= (1u << 30) || p->dim >= (1u << 24))
         return fail(VKH_ERR_UNSUPPORTED, "2^16 sequences, 2^30 rows of one or 2^24 channels");
+    if ((uint64_t)p->n_batch * ((p->dim + 63) / 64) >= 1ull << 31) return fail(VKH_ERR_UNSUPPORTED, "2^37 channels in all");
     for (uint32_t ld : {p->ld_x, p->ld_g, p->ld_h, p->ld_dh, p->ld_dx, p->ld_dg})
         CHECK_ARG(!ld || ld >= p->dim, "a row stride is less than the row");
     auto ld = [&](uint32_t l) { return (long)(l ? l : p->dim); };

@@ -8,7 +8,7 @@
 //   dg = da, or da a (1 - a),  dh0 = R_0
 //
 // A stretch of rows maps the state before it to the one behind it as h -> A h + B (A the product of its a, B what
-// the stretch makes of h = 0), and the same A carries R the other way: R -> A R + Q.  A block takes 64 V
+// the stretch makes of h = 0), and the same A carries R the other way: R -> A R + Q.  A block takes 64
 // channels and tiles of a few rows for each of its waves: a wave holds its rows of all these channels in
 // registers, forms A and B of them, and joins the others' before it through LDS; then it runs its rows again from
 // the state that they start from.  Each value is read and written once: bound by HBM.  The forward keeps the state
@@ -17,8 +17,8 @@
 // Where channels are few, the tiles of a sequence go to blocks of their own.  A tile's block publishes its A and B
 // as soon as it has them, looks for the nearest tile before it whose state behind it is known, applies the A and B
 // of the tiles between in their order, and publishes its own state.  That is the same arithmetic whichever tile it
-// starts from, so results do not depend on timing, nor on whether a sequence is split.  Blocks take their tiles
-// by a ticket, in order of time: a tile waits only for tiles that running blocks hold already, and the first of
+// starts from, so results do not depend on timing, nor on whether a sequence is split.  Blocks take a sequence's
+// tiles by tickets, in order of time: a tile waits only for tiles that running blocks hold already, and the first of
 // those waits for none.  Published words are single atomic stores past the XCDs' own caches, valid once they differ
 // from kUnset, so nothing has to be ordered.
 #include <algorithm>
@@ -32,10 +32,11 @@ namespace {
 constexpr int kFwdWaves = 8, kBwdWaves = 16;
 constexpr int kFwdRows = 16, kBwdRows = 8;  // a wave's
 constexpr int kFwdTile = kFwdWaves * kFwdRows, kBwdTile = kBwdWaves * kBwdRows;
-static_assert(kScanTile % kFwdRows == 0 && kFwdTile % kScanTile == 0 && kBwdTile == kScanTile, "states");
+static_assert(kFwdTile == kScanTile && kBwdTile == kScanTile, "states");
 constexpr int kFew = 16;  // rows of a short sequence
 constexpr int kPerSimd = 4;  // waves: registers for 16 a CU
 constexpr int kLook = 4;  // tiles looked back over at a time
+constexpr size_t kMostChannels = 80l << 20;  // of a split call's words (12 bytes each)
 constexpr uint32_t kUnset = 0xffffffffu;
 
 template <class F>
@@ -66,10 +67,8 @@ struct Walk {
         asm volatile("" : "+v"(bytes));
         return (Row)p + bytes;
     }
-    template <int V>
-    VKH_DEV Raw<T, V> load(unsigned bytes) const { return *(__attribute__((address_space(1))) Raw<T, V> *)at(bytes); }
-    template <int V>
-    VKH_DEV void store(unsigned bytes, const float (&o)[V]) const;
+    VKH_DEV T load(unsigned bytes) const { return *(__attribute__((address_space(1))) T *)at(bytes); }
+    VKH_DEV void store(unsigned bytes, float v) const { *(__attribute__((address_space(1))) T *)at(bytes) = (T)v; }
     VKH_DEV void next(bool more = true) { p += more ? step : 0; }
     VKH_DEV void back() { p -= step; }
 };
@@ -97,12 +96,6 @@ VKH_DEV Raw<T, V> raw_of(const float (&o)[V]) {
 }
 template <class T, int V>
 VKH_DEV void store_v(T *p, const float (&o)[V]) { *reinterpret_cast<Raw<T, V> *>(p) = raw_of<T, V>(o); }
-template <class T>
-template <int V>
-VKH_DEV void Walk<T>::store(unsigned bytes, const float (&o)[V]) const {
-    *(__attribute__((address_space(1))) Raw<T, V> *)at(bytes) = raw_of<T, V>(o);
-}
-
 // a and 1 - a of a gate, each to its own last digits: e = exp(-|g|) from a product in two parts (one alone is
 // off by |g| steps), 1 / (1 + e) and e / (1 + e).
 template <bool SIG>
@@ -128,23 +121,25 @@ VKH_DEV int rows_of(const ScanArgs &a, int b) {
     return n < (unsigned)a.n_pos ? (int)n : a.n_pos;
 }
 
-// The workspace of a split call: a ticket, then each tile's A and B (a 64-bit word a channel) and the state behind it.
+// The workspace of a split call: a counter for each sequence and channel group, in lines of their own, then each
+// tile's A and B (a 64-bit word a channel) and the state behind it.
+constexpr int kTicketBytes = 128;
 struct Words {
-    unsigned *ticket;
+    char *tickets;
     uint64_t *ab;
     uint32_t *h;
 };
-__host__ __device__ inline Words words_of(void *ws, size_t channels) {
+__host__ __device__ inline Words words_of(void *ws, size_t lines, size_t channels) {
     Words w;
-    w.ticket = (unsigned *)ws;
-    w.ab = (uint64_t *)((char *)ws + 64);
+    w.tickets = (char *)ws;
+    w.ab = (uint64_t *)((char *)ws + lines * kTicketBytes);
     w.h = (uint32_t *)(w.ab + channels);
     return w;
 }
-__global__ __launch_bounds__(256) void scan_clear_k(uint4 *ws, size_t n) {
+__global__ __launch_bounds__(256) void scan_clear_k(uint4 *ws, size_t zeros, size_t n) {
     const size_t step = (size_t)gridDim.x * 256;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step)
-        ws[i] = i ? make_uint4(kUnset, kUnset, kUnset, kUnset) : make_uint4(0, 0, 0, 0);
+        ws[i] = i < zeros ? make_uint4(0, 0, 0, 0) : make_uint4(kUnset, kUnset, kUnset, kUnset);
 }
 
 VKH_DEV uint32_t bits_of(float x) {
@@ -165,322 +160,290 @@ VKH_DEV void publish(void *at, unsigned bytes, T v) {
     const Walk<T> w(at, 0, 0);
     __hip_atomic_store((__attribute__((address_space(1))) T *)w.at(bytes), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-template <int V>
-using States = std::conditional_t<V == 1, uint32_t, uint64_t>;
 
-// By one wave, for the 64 V channels at `base` of the words (tile s of the sequence at s 64 V after it): publishes
-// this tile's A and B, sets H (given for the first tile) to the state before tile s, and publishes the one behind it.
-// A tile's states of a lane are one word.
-template <int V>
-VKH_DEV void look_back(const Words &W, size_t base, int s, unsigned lane, const float (&A)[V], const float (&B)[V], float (&H)[V]) {
-    const unsigned lab = lane * V * 8, lh = lane * V * 4;
-    auto ab = [&](int k) { return W.ab + base + (size_t)k * 64 * V; };
-    auto hs = [&](int k) { return W.h + base + (size_t)k * 64 * V; };
-    if (s) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) publish(ab(s), lab + v * 8, word_of(A[v], B[v]));
-    }
+// By one wave, for the 64 channels at `base` of the words (tile s of the sequence at 64 s after it): publishes this
+// tile's A and B, sets H (given for the first tile) to the state before tile s, and publishes the one behind it.
+VKH_DEV void look_back(const Words &W, size_t base, int s, unsigned lane, float A, float B, float &H) {
+    auto ab = [&](int k) { return W.ab + base + (size_t)k * 64; };
+    auto hs = [&](int k) { return W.h + base + (size_t)k * 64; };
+    if (s) publish(ab(s), lane * 8, word_of(A, B));
     for (bool found = s == 0; !found;) {
-        uint64_t w[kLook][V];
-        States<V> h[kLook];
+        uint64_t w[kLook];
+        uint32_t h[kLook];
 #pragma unroll
         for (int d = 0; d < kLook; ++d) {  // tile s - 1 - d
             const int k = max(s - 1 - d, 0);
-            h[d] = peek<States<V>>(hs(k), lh);
-#pragma unroll
-            for (int v = 0; v < V; ++v) w[d][v] = peek<uint64_t>(ab(k), lab + v * 8);
+            h[d] = peek<uint32_t>(hs(k), lane * 4);
+            w[d] = peek<uint64_t>(ab(k), lane * 8);
         }
         int n = 0;  // tiles between the nearest known state and this tile
         bool going = true;
 #pragma unroll
         for (int d = 0; d < kLook; ++d) {
-            const bool known = (uint32_t)h[d] != kUnset && (V == 1 || (uint32_t)((uint64_t)h[d] >> 32) != kUnset);
-            if (going && __ballot(!known) == 0) {
+            if (going && __ballot(h[d] == kUnset) == 0) {
                 going = false;
                 found = true;
                 n = d;
-#pragma unroll
-                for (int v = 0; v < V; ++v) H[v] = __builtin_bit_cast(float, (uint32_t)((uint64_t)h[d] >> 32 * v));
+                H = __builtin_bit_cast(float, h[d]);
             }
-            bool there = s - 1 - d > 0;  // (the first tile publishes its state alone)
-#pragma unroll
-            for (int v = 0; v < V; ++v) there = there && (uint32_t)(w[d][v] >> 32) != kUnset;
-            going = going && __ballot(!there) == 0;
+            // (the first tile publishes its state alone)
+            going = going && s - 1 - d > 0 && __ballot((uint32_t)(w[d] >> 32) == kUnset) == 0;
         }
         if (found) {
 #pragma unroll
             for (int d = kLook - 2; d >= 0; --d)
-                if (d < n)
-#pragma unroll
-                    for (int v = 0; v < V; ++v) H[v] = fmaf(low_of(w[d][v]), H[v], high_of(w[d][v]));
+                if (d < n) H = fmaf(low_of(w[d]), H, high_of(w[d]));
         } else {
             __builtin_amdgcn_s_sleep(1);
         }
     }
-    uint64_t out = 0;
-#pragma unroll
-    for (int v = 0; v < V; ++v) out |= (uint64_t)bits_of(fmaf(A[v], H[v], B[v])) << 32 * v;
-    publish(hs(s), lh, (States<V>)out);
+    publish(hs(s), lane * 4, bits_of(fmaf(A, H, B)));
 }
 
-// The tiles of a block: of a split call those that its tickets name, in order of time from the side that the scan
-// starts from (s: the how manieth), each ticket fetched while the tile before it is worked on; else all tiles of a
-// sequence and channel group.
+// The tiles of a block, all of one sequence and channel group.  In a split call several blocks share them, each
+// taking the tiles that its tickets name: a ticket is handed round at a barrier of the tile before, and the next one
+// fetched from there on, while that tile is worked on.  (One counter for all of them took 15 ns a tile: atomics on one
+// address wait for each other.)
 template <bool SPLIT>
 struct Tiles {
-    int b, grp, s = -1, groups, n_batch, tiles;
-    unsigned *sh, next;
-    VKH_DEV Tiles(const Words &W, int groups_, int n_batch_, int tiles_, unsigned *sh_)
-        : b(blockIdx.y), grp(blockIdx.x), groups(groups_), n_batch(n_batch_), tiles(tiles_), sh(sh_) {
-        if (SPLIT && threadIdx.x == 0) next = atomicAdd(W.ticket, 1u);
+    unsigned *ticket, *sh, next = 0;
+    VKH_DEV void fetch() {
+        if (SPLIT && threadIdx.x == 0) next = atomicAdd(ticket, 1u);
     }
-    VKH_DEV bool take(const Words &W) {
-        if (!SPLIT) return ++s < tiles;
-        if (threadIdx.x == 0) *sh = next;
-        __syncthreads();  // (also behind the last tile's reads of LDS)
-        const unsigned t = __builtin_amdgcn_readfirstlane(*sh), per = groups * n_batch, at = t % per;
-        s = t / per, b = at / groups, grp = at % groups;
-        if (s >= tiles) return false;
-        if (threadIdx.x == 0) next = atomicAdd(W.ticket, 1u);
-        return true;
+    VKH_DEV void hand_round() {  // ahead of a barrier
+        if (SPLIT && threadIdx.x == 0) *sh = next;
+    }
+    VKH_DEV int take(int now) {  // behind it
+        if (!SPLIT) return now + 1;
+        const int t = __builtin_amdgcn_readfirstlane(*sh);
+        fetch();
+        return t;
+    }
+    VKH_DEV int first() {
+        if (!SPLIT) return 0;
+        fetch();
+        hand_round();
+        __syncthreads();
+        return take(0);
     }
 };
 
-template <class TI, class TO, int V, bool SIG, bool COUP, bool SPLIT>
+template <class TI, class TO, bool SIG, bool COUP, bool SPLIT>
 __global__ __launch_bounds__(kFwdWaves * 64, kPerSimd) void scan_fwd_k(ScanArgs s, int groups) {
     constexpr int R = kFwdRows;
-    __shared__ float shA[2][kFwdWaves][64 * V], shB[2][kFwdWaves][64 * V], shH[64 * V];
+    __shared__ float shA[2][kFwdWaves][64], shB[2][kFwdWaves][64], shH[64];
     __shared__ unsigned ticket;
     const int lane = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int tiles = (s.n_pos + kFwdTile - 1) / kFwdTile, marks = (s.n_pos + kScanTile - 1) / kScanTile;
-    const Words W = words_of(s.ws, (size_t)s.n_batch * groups * tiles * 64 * V);
-    Tiles<SPLIT> at(W, groups, s.n_batch, tiles, &ticket);
-    float H[V];
-    while (at.take(W)) {
-        const int k = at.s, b = at.b, c = (at.grp * 64 + lane) * V, len = rows_of(s, b);
-        const bool act = c < s.dim;
-        const unsigned in_bytes = (act ? c : s.dim - V) * sizeof(TI), out_bytes = c * sizeof(TO);  // (lanes past the channels read the last ones)
-        if (SPLIT || k == 0) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) H[v] = 0.f;
-            if (k == 0 && act && s.h0) load_v<float, V>(s.h0 + (long)b * s.dim + c, H);
-        }
+    const int tiles = (s.n_pos + kFwdTile - 1) / kFwdTile;
+    const long blk = SPLIT ? blockIdx.x % (groups * s.n_batch) : block_number();
+    if (blk >= groups * s.n_batch) return;
+    const int line = __builtin_amdgcn_readfirstlane((int)blk), b = __builtin_amdgcn_readfirstlane(line / groups);
+    const int c = (line - b * groups) * 64 + lane, len = __builtin_amdgcn_readfirstlane(rows_of(s, b));
+    const bool act = c < s.dim;
+    const unsigned in_bytes = min(c, s.dim - 1) * sizeof(TI);  // (lanes past the channels: the last one)
+    const Words W = words_of(s.ws, (size_t)s.n_batch * groups, (size_t)s.n_batch * groups * tiles * 64);
+    Tiles<SPLIT> order{(unsigned *)(W.tickets + (size_t)line * kTicketBytes), &ticket};
+    TI xr[R], gr[R];
+    auto load = [&](int k) {
         const int t0 = k * kFwdTile + w * R;
+        if (t0 >= len) return;
         const long row0 = (long)b * s.n_pos + t0;
-        Raw<TI, V> xr[R], gr[R];
-        if (t0 < len) {  // (rows behind the end: the last one again)
-            Walk<TI> g(s.g, row0, s.ldg), x(s.x, row0, s.ldx);
+        Walk<TI> g(s.g, row0, s.ldg), x(s.x, row0, s.ldx);
 #pragma unroll
-            for (int i = 0; i < R; ++i) {
-                gr[i] = g.template load<V>(in_bytes);
-                xr[i] = x.template load<V>(in_bytes);
-                g.next(t0 + i + 1 < len);
-                x.next(t0 + i + 1 < len);
-            }
+        for (int i = 0; i < R; ++i) {  // (rows behind the end: the last one again)
+            gr[i] = g.load(in_bytes);
+            xr[i] = x.load(in_bytes);
+            g.next(t0 + i + 1 < len);
+            x.next(t0 + i + 1 < len);
         }
-        float a[R][V], u[R][V], p[V], q[V];
+    };
+    float H = 0.f;
+    int at = order.first();
+    if (at >= tiles) return;
+    for (int turn = 0;; turn ^= 1) {
+        load(at);
+        const int k = at, t0 = k * kFwdTile + w * R;
+        if (k == 0) {
+            H = act && s.h0 ? s.h0[(long)b * s.dim + c] : 0.f;
+            asm volatile("" : "+v"(H));  // (it has been read when the block meets at its barrier: h_last may be h0)
+        }
+        float a[R], u[R], p = 1.f, q = 0.f;
 #pragma unroll
-        for (int i = 0; i < R; ++i)
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                float rest;
-                gate<SIG>(part<TI, V>(gr[i], v), a[i][v], rest);
-                u[i][v] = part<TI, V>(xr[i], v);
-                if (COUP) u[i][v] *= rest;
-            }
+        for (int i = 0; i < R; ++i) {
+            float rest;
+            gate<SIG>((float)gr[i], a[i], rest);
+            u[i] = COUP ? rest * (float)xr[i] : (float)xr[i];
+        }
         if (t0 + R > len) {  // rows behind the end leave the state alone
 #pragma unroll
             for (int i = 0; i < R; ++i)
-#pragma unroll
-                for (int v = 0; v < V; ++v)
-                    if (t0 + i >= len) a[i][v] = 1.f, u[i][v] = 0.f;
+                if (t0 + i >= len) a[i] = 1.f, u[i] = 0.f;
         }
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            p[v] = 1.f, q[v] = 0.f;
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                p[v] *= a[i][v];
-                q[v] = fmaf(a[i][v], q[v], u[i][v]);
-            }
+        for (int i = 0; i < R; ++i) {
+            p *= a[i];
+            q = fmaf(a[i], q, u[i]);
         }
-        float (&A)[kFwdWaves][64 * V] = shA[k & 1], (&B)[kFwdWaves][64 * V] = shB[k & 1];
-#pragma unroll
-        for (int v = 0; v < V; ++v) A[w][lane * V + v] = p[v], B[w][lane * V + v] = q[v];
+        float (&A)[kFwdWaves][64] = shA[turn], (&B)[kFwdWaves][64] = shB[turn];
+        A[w][lane] = p;
+        B[w][lane] = q;
+        order.hand_round();
         __syncthreads();
+        const int then = order.take(at);
+        const bool more = then < tiles;
         // of the waves before this one, and of the tile
-        float pa[V], pb[V], ta[V], tb[V], h[V];
+        float pa = 1.f, pb = 0.f, ta = 1.f, tb = 0.f;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            ta[v] = 1.f, tb[v] = 0.f;
-#pragma unroll
-            for (int j = 0; j < kFwdWaves; ++j) {
-                if (j == w) pa[v] = ta[v], pb[v] = tb[v];
-                ta[v] *= A[j][lane * V + v];
-                tb[v] = fmaf(A[j][lane * V + v], tb[v], B[j][lane * V + v]);
-            }
+        for (int j = 0; j < kFwdWaves; ++j) {
+            if (j == w) pa = ta, pb = tb;
+            ta *= A[j][lane];
+            tb = fmaf(A[j][lane], tb, B[j][lane]);
         }
         if (SPLIT) {
             if (w == 0) {
-                look_back<V>(W, ((size_t)b * groups + at.grp) * tiles * 64 * V, k, lane, ta, tb, H);
-#pragma unroll
-                for (int v = 0; v < V; ++v) shH[lane * V + v] = H[v];
+                look_back(W, (size_t)line * tiles * 64, at, lane, ta, tb, H);
+                shH[lane] = H;
             }
             __syncthreads();
-#pragma unroll
-            for (int v = 0; v < V; ++v) H[v] = shH[lane * V + v];
+            H = shH[lane];
         }
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            h[v] = fmaf(pa[v], H[v], pb[v]);
-            H[v] = fmaf(ta[v], H[v], tb[v]);
-        }
-        if (s.states && w * R % kScanTile == 0 && t0 < s.n_pos && act)
-            store_v<float, V>(s.states + ((long)b * marks + t0 / kScanTile) * s.dim + c, h);
+        float h = fmaf(pa, H, pb);
+        H = fmaf(ta, H, tb);
         if (act) {
+            if (s.states && w == 0) s.states[((long)b * tiles + k) * s.dim + c] = h;
+            const long row0 = (long)b * s.n_pos + t0;
             Walk<TO> out(s.h, row0, s.ldh);
 #pragma unroll
             for (int i = 0; i < R; ++i) {
-                float o[V];
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    h[v] = fmaf(a[i][v], h[v], u[i][v]);
-                    o[v] = t0 + i < len ? h[v] : 0.f;
-                }
-                if (t0 + i < s.n_pos) out.store(out_bytes, o);
+                h = fmaf(a[i], h, u[i]);
+                if (t0 + i < s.n_pos) out.store(c * sizeof(TO), t0 + i < len ? h : 0.f);
                 out.next();
             }
+            if (k + 1 == tiles && s.h_last && w == 0) s.h_last[(long)b * s.dim + c] = H;
         }
-        if (k + 1 == tiles && s.h_last && w == 0 && act) store_v<float, V>(s.h_last + (long)b * s.dim + c, H);
+        if (!more) return;
+        at = then;
     }
 }
 
-template <class TI, class TO, int V, bool SIG, bool COUP, bool SPLIT>
+template <class TI, class TO, bool SIG, bool COUP, bool SPLIT>
 __global__ __launch_bounds__(kBwdWaves * 64, kPerSimd) void scan_bwd_k(ScanArgs s, int groups) {
     constexpr int N = kBwdRows;
-    __shared__ float shA[2][kBwdWaves][64 * V], shB[2][kBwdWaves][64 * V], shQ[2][kBwdWaves][64 * V], shR[64 * V];
+    __shared__ float shA[2][kBwdWaves][64], shB[2][kBwdWaves][64], shQ[2][kBwdWaves][64], shR[64];
     __shared__ unsigned ticket;
     const int lane = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int tiles = (s.n_pos + kBwdTile - 1) / kBwdTile;
-    const Words W = words_of(s.ws, (size_t)s.n_batch * groups * tiles * 64 * V);
-    Tiles<SPLIT> at(W, groups, s.n_batch, tiles, &ticket);
-    float R[V];
-    while (at.take(W)) {
-        const int k = tiles - 1 - at.s, b = at.b, c = (at.grp * 64 + lane) * V, len = rows_of(s, b);
-        const bool act = c < s.dim;
-        const unsigned in_bytes = (act ? c : s.dim - V) * sizeof(TI), out_bytes = c * sizeof(TO);  // (lanes past the channels read the last ones)
-        if (SPLIT || at.s == 0) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) R[v] = 0.f;
-            if (at.s == 0 && act && s.dh_last) load_v<float, V>(s.dh_last + (long)b * s.dim + c, R);
-        }
-        const int t0 = k * kBwdTile + w * N;
+    const long blk = SPLIT ? blockIdx.x % (groups * s.n_batch) : block_number();
+    if (blk >= groups * s.n_batch) return;
+    const int line = __builtin_amdgcn_readfirstlane((int)blk), b = __builtin_amdgcn_readfirstlane(line / groups);
+    const int c = (line - b * groups) * 64 + lane, len = __builtin_amdgcn_readfirstlane(rows_of(s, b));
+    const bool act = c < s.dim;
+    const unsigned in_bytes = min(c, s.dim - 1) * sizeof(TI);  // (lanes past the channels: the last one)
+    const Words W = words_of(s.ws, (size_t)s.n_batch * groups, (size_t)s.n_batch * groups * tiles * 64);
+    Tiles<SPLIT> order{(unsigned *)(W.tickets + (size_t)line * kTicketBytes), &ticket};
+    TI xr[N], gr[N], dr[N];
+    float hr = 0.f;  // the state before the tile (one behind the sequence's end has none, and needs none)
+    auto load = [&](int at) {
+        const int k = tiles - 1 - at, t0 = k * kBwdTile + w * N;
+        hr = act && k * kBwdTile < len ? s.states[((long)b * tiles + k) * s.dim + c] : 0.f;
+        if (t0 >= len) return;
         const long row0 = (long)b * s.n_pos + t0;
-        Raw<TI, V> xr[N], gr[N], dr[N];
-        float h[V] = {};
-        if (t0 < len) {  // (rows behind the end: the last one again)
-            Walk<TI> g(s.g, row0, s.ldg), d(s.dh, row0, s.lddh), x(s.x, row0, s.ldx);
+        Walk<TI> g(s.g, row0, s.ldg), d(s.dh, row0, s.lddh), x(s.x, row0, s.ldx);
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                gr[i] = g.template load<V>(in_bytes);
-                dr[i] = d.template load<V>(in_bytes);
-                xr[i] = x.template load<V>(in_bytes);
-                g.next(t0 + i + 1 < len);
-                d.next(t0 + i + 1 < len);
-                x.next(t0 + i + 1 < len);
-            }
+        for (int i = 0; i < N; ++i) {  // (rows behind the end: the last one again)
+            gr[i] = g.load(in_bytes);
+            dr[i] = d.load(in_bytes);
+            xr[i] = x.load(in_bytes);
+            g.next(t0 + i + 1 < len);
+            d.next(t0 + i + 1 < len);
+            x.next(t0 + i + 1 < len);
         }
-        // (a tile behind the sequence's end has no state, and needs none)
-        if (act && k * kBwdTile < len) load_v<float, V>(s.states + ((long)b * tiles + k) * s.dim + c, h);
-        float a[N][V], rest[N][V], x[N][V], d[N][V];
+    };
+    float R = 0.f;
+    int at = order.first();
+    if (at >= tiles) return;
+    for (int turn = 0;; turn ^= 1) {
+        load(at);
+        const int k = tiles - 1 - at, t0 = k * kBwdTile + w * N;
+        if (at == 0) {
+            R = act && s.dh_last ? s.dh_last[(long)b * s.dim + c] : 0.f;
+            asm volatile("" : "+v"(R));  // (as in the forward: dh0 may be dh_last)
+        }
+        float a[N], rest[N], x[N], d[N], h = hr;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                gate<SIG>(part<TI, V>(gr[i], v), a[i][v], rest[i][v]);
-                x[i][v] = part<TI, V>(xr[i], v);
-                d[i][v] = part<TI, V>(dr[i], v);
-            }
+        for (int i = 0; i < N; ++i) {
+            gate<SIG>((float)gr[i], a[i], rest[i]);
+            x[i] = (float)xr[i];
+            d[i] = (float)dr[i];
+        }
         if (t0 + N > len) {  // rows behind the end leave state and gradient alone
 #pragma unroll
             for (int i = 0; i < N; ++i)
-#pragma unroll
-                for (int v = 0; v < V; ++v)
-                    if (t0 + i >= len) a[i][v] = 1.f, rest[i][v] = x[i][v] = d[i][v] = 0.f;
+                if (t0 + i >= len) a[i] = 1.f, rest[i] = x[i] = d[i] = 0.f;
         }
-        auto u = [&](int i, int v) { return COUP ? rest[i][v] * x[i][v] : x[i][v]; };
-        float (&A)[kBwdWaves][64 * V] = shA[k & 1], (&B)[kBwdWaves][64 * V] = shB[k & 1], (&Q)[kBwdWaves][64 * V] = shQ[k & 1];
+        auto u = [&](int i) { return COUP ? rest[i] * x[i] : x[i]; };
+        float p = 1.f, q = 0.f, z = 0.f;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            float p = 1.f, q = 0.f, z = 0.f;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                p *= a[i][v];
-                q = fmaf(a[i][v], q, u(i, v));
-            }
-#pragma unroll
-            for (int i = N - 1; i >= 0; --i) z = a[i][v] * (d[i][v] + z);
-            A[w][lane * V + v] = p;
-            B[w][lane * V + v] = q;
-            Q[w][lane * V + v] = z;
+        for (int i = 0; i < N; ++i) {
+            p *= a[i];
+            q = fmaf(a[i], q, u(i));
         }
+#pragma unroll
+        for (int i = N - 1; i >= 0; --i) z = a[i] * (d[i] + z);
+        float (&A)[kBwdWaves][64] = shA[turn], (&B)[kBwdWaves][64] = shB[turn], (&Q)[kBwdWaves][64] = shQ[turn];
+        A[w][lane] = p;
+        B[w][lane] = q;
+        Q[w][lane] = z;
+        order.hand_round();
         __syncthreads();
+        const int then = order.take(at);
+        const bool more = then < tiles;
         // of the waves behind this one, and of the tile; and the state before this wave's rows
-        float pa[V], pb[V], ta[V], tb[V], e[V];
+        float pa = 1.f, pb = 0.f, ta = 1.f, tb = 0.f;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            ta[v] = 1.f, tb[v] = 0.f;
-#pragma unroll
-            for (int j = kBwdWaves - 1; j >= 0; --j) {
-                if (j == w) pa[v] = ta[v], pb[v] = tb[v];
-                ta[v] *= A[j][lane * V + v];
-                tb[v] = fmaf(A[j][lane * V + v], tb[v], Q[j][lane * V + v]);
-            }
-#pragma unroll
-            for (int j = 0; j < w; ++j) h[v] = fmaf(A[j][lane * V + v], h[v], B[j][lane * V + v]);
+        for (int j = kBwdWaves - 1; j >= 0; --j) {
+            if (j == w) pa = ta, pb = tb;
+            ta *= A[j][lane];
+            tb = fmaf(A[j][lane], tb, Q[j][lane]);
         }
+#pragma unroll
+        for (int j = 0; j < kBwdWaves; ++j)
+            if (j < w) h = fmaf(A[j][lane], h, B[j][lane]);
         if (SPLIT) {
             if (w == 0) {
-                look_back<V>(W, ((size_t)b * groups + at.grp) * tiles * 64 * V, at.s, lane, ta, tb, R);
-#pragma unroll
-                for (int v = 0; v < V; ++v) shR[lane * V + v] = R[v];
+                look_back(W, (size_t)line * tiles * 64, at, lane, ta, tb, R);
+                shR[lane] = R;
             }
             __syncthreads();
-#pragma unroll
-            for (int v = 0; v < V; ++v) R[v] = shR[lane * V + v];
+            R = shR[lane];
         }
-        float hp[N][V];
+        float hp[N], e = fmaf(pa, R, pb);
+        R = fmaf(ta, R, tb);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            e[v] = fmaf(pa[v], R[v], pb[v]);
-            R[v] = fmaf(ta[v], R[v], tb[v]);
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                hp[i][v] = h[v];
-                h[v] = fmaf(a[i][v], h[v], u(i, v));
-            }
+        for (int i = 0; i < N; ++i) {
+            hp[i] = h;
+            h = fmaf(a[i], h, u(i));
         }
-        Walk<TO> ox(s.dx, row0 + N - 1, s.lddx), og(s.dg, row0 + N - 1, s.lddg);
+        if (act) {
+            const long row0 = (long)b * s.n_pos + t0;
+            Walk<TO> ox(s.dx, row0 + N - 1, s.lddx), og(s.dg, row0 + N - 1, s.lddg);
 #pragma unroll
-        for (int i = N - 1; i >= 0; --i) {
-            float dx[V], dg[V];
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float G = d[i][v] + e[v];
-                e[v] = a[i][v] * G;
-                dx[v] = COUP ? rest[i][v] * G : G;
-                dg[v] = COUP ? G * (hp[i][v] - x[i][v]) : G * hp[i][v];
-                if (SIG) dg[v] *= a[i][v] * rest[i][v];
-                if (t0 + i >= len) dx[v] = dg[v] = 0.f;
+            for (int i = N - 1; i >= 0; --i) {
+                const float G = d[i] + e;
+                e = a[i] * G;
+                float dx = COUP ? rest[i] * G : G, dg = COUP ? G * (hp[i] - x[i]) : G * hp[i];
+                if (SIG) dg *= a[i] * rest[i];
+                if (t0 + i < s.n_pos) {
+                    ox.store(c * sizeof(TO), t0 + i < len ? dx : 0.f);
+                    og.store(c * sizeof(TO), t0 + i < len ? dg : 0.f);
+                }
+                ox.back();
+                og.back();
             }
-            if (act && t0 + i < s.n_pos) {
-                ox.store(out_bytes, dx);
-                og.store(out_bytes, dg);
-            }
-            ox.back();
-            og.back();
+            if (k == 0 && s.dh0 && w == 0) s.dh0[(long)b * s.dim + c] = R;
         }
-        if (k == 0 && s.dh0 && w == 0 && act) store_v<float, V>(s.dh0 + (long)b * s.dim + c, R);
+        if (!more) return;
+        at = then;
     }
 }
 
@@ -542,22 +505,23 @@ __global__ __launch_bounds__(256) void scan_few_bwd_k(ScanArgs s) {
     if (s.dh0) s.dh0[state] = R;
 }
 
-// How a call is laid out: channels a lane, channel groups, and whether its tiles go to blocks of their own.
+// How a call is laid out: channel groups, and the blocks that share the tiles of each sequence and group (0: one has
+// them all).
 struct Plan {
-    int groups;
-    bool split;
-    size_t blocks, channels;  // of a split call; its words' channels
+    int groups, sharing;
+    size_t lines, channels;  // sequences times groups; a split call's words' channels
 };
-Plan plan_of(const ScanArgs &s, int tile) {
+Plan plan_of(const ScanArgs &s, int tile, int waves) {
     Plan p;
     p.groups = (int)ceil_div(s.dim, 64);
-    const size_t rows = (size_t)p.groups * s.n_batch, tiles = (s.n_pos + tile - 1) / tile;
-    p.blocks = rows * tiles;
-    p.channels = p.blocks * 64;
-    p.split = s.n_pos > kFew && tiles > 1 && rows < 1024 && p.blocks < (1u << 20);
+    p.lines = (size_t)p.groups * s.n_batch;
+    const size_t tiles = (s.n_pos + tile - 1) / tile, resident = (size_t)cu_count() * kPerSimd * 4 / waves;
+    p.channels = p.lines * tiles * 64;
+    p.sharing = (int)std::min(tiles, resident / p.lines);
+    if (s.n_pos <= kFew || p.sharing < 2 || p.channels > kMostChannels) p.sharing = 0;
     return p;
 }
-size_t words_bytes(const Plan &p) { return p.split ? (64 + p.channels * 12 + 15) / 16 * 16 : 0; }
+size_t words_bytes(const Plan &p) { return p.sharing ? p.lines * kTicketBytes + (p.channels * 12 + 15) / 16 * 16 : 0; }
 
 template <class F>
 void by_form(const ScanArgs &s, F f) {
@@ -574,16 +538,16 @@ void by_form(const ScanArgs &s, F f) {
 }
 
 // The plan of a call, its workspace ready
-Plan ready(const ScanArgs &s, int tile, hipStream_t st) {
-    Plan p = plan_of(s, tile);
-    if (!s.ws) p.split = false;
+Plan ready(const ScanArgs &s, int tile, int waves, hipStream_t st) {
+    Plan p = plan_of(s, tile, waves);
+    if (!s.ws) p.sharing = 0;
     const size_t n = words_bytes(p) / 16;
-    if (p.split) hipLaunchKernelGGL(scan_clear_k, dim3((unsigned)std::min<size_t>((n + 255) / 256, 1024)), dim3(256), 0, st, (uint4 *)s.ws, n);
+    if (n)
+        hipLaunchKernelGGL(scan_clear_k, dim3((unsigned)std::min<size_t>((n + 255) / 256, 1024)), dim3(256), 0, st, (uint4 *)s.ws,
+                           p.lines * kTicketBytes / 16, n);
     return p;
 }
-dim3 grid_of(const ScanArgs &s, const Plan &p, int waves) {
-    return p.split ? dim3((unsigned)std::min<size_t>(p.blocks, (size_t)cu_count() * kPerSimd * 4 / waves)) : dim3(p.groups, s.n_batch);
-}
+dim3 grid_of(const Plan &p) { return p.sharing ? dim3((unsigned)p.lines * p.sharing) : long_grid((long)p.lines); }
 
 }  // namespace
 
@@ -591,7 +555,7 @@ size_t scan_states_floats(const ScanArgs &s) {
     return (size_t)s.n_batch * ((s.n_pos + kScanTile - 1) / kScanTile) * s.dim;
 }
 size_t scan_ws_bytes(const ScanArgs &s) {
-    return std::max(words_bytes(plan_of(s, kFwdTile)), words_bytes(plan_of(s, kBwdTile)));
+    return std::max(words_bytes(plan_of(s, kFwdTile, kFwdWaves)), words_bytes(plan_of(s, kBwdTile, kBwdWaves)));
 }
 
 hipError_t scan_forward(const ScanArgs &s, hipStream_t st) {
@@ -605,9 +569,9 @@ hipError_t scan_forward(const ScanArgs &s, hipStream_t st) {
             hipLaunchKernelGGL(k, dim3(ceil_div(s.dim, 256 * V), s.n_batch), dim3(256), 0, st, s);
             return;
         }
-        const Plan p = ready(s, kFwdTile, st);
-        auto k = p.split ? scan_fwd_k<TI, TO, 1, SIG, COUP, true> : scan_fwd_k<TI, TO, 1, SIG, COUP, false>;
-        hipLaunchKernelGGL(k, grid_of(s, p, kFwdWaves), dim3(kFwdWaves * 64), 0, st, s, p.groups);
+        const Plan p = ready(s, kFwdTile, kFwdWaves, st);
+        auto k = p.sharing ? scan_fwd_k<TI, TO, SIG, COUP, true> : scan_fwd_k<TI, TO, SIG, COUP, false>;
+        hipLaunchKernelGGL(k, grid_of(p), dim3(kFwdWaves * 64), 0, st, s, p.groups);
     });
     return hipGetLastError();
 }
@@ -621,9 +585,9 @@ hipError_t scan_backward(const ScanArgs &s, hipStream_t st) {
             hipLaunchKernelGGL((scan_few_bwd_k<TI, TO, SIG, COUP>), dim3(ceil_div(s.dim, 256), s.n_batch), dim3(256), 0, st, s);
             return;
         }
-        const Plan p = ready(s, kBwdTile, st);
-        auto k = p.split ? scan_bwd_k<TI, TO, 1, SIG, COUP, true> : scan_bwd_k<TI, TO, 1, SIG, COUP, false>;
-        hipLaunchKernelGGL(k, grid_of(s, p, kBwdWaves), dim3(kBwdWaves * 64), 0, st, s, p.groups);
+        const Plan p = ready(s, kBwdTile, kBwdWaves, st);
+        auto k = p.sharing ? scan_bwd_k<TI, TO, SIG, COUP, true> : scan_bwd_k<TI, TO, SIG, COUP, false>;
+        hipLaunchKernelGGL(k, grid_of(p), dim3(kBwdWaves * 64), 0, st, s, p.groups);
     });
     return hipGetLastError();
 }
