@@ -32,9 +32,10 @@ namespace {
 constexpr int kFwdWaves = 8, kBwdWaves = 16;
 constexpr int kFwdRows = 16, kBwdRows = 8;  // a wave's
 constexpr int kFwdTile = kFwdWaves * kFwdRows, kBwdTile = kBwdWaves * kBwdRows;
-static_assert(kFwdTile == kScanTile && kBwdTile == kScanTile, "states");
+static_assert(kFwdTile % kScanTile == 0 && kScanTile % kFwdRows == 0 && kBwdTile == kScanTile, "states");
 constexpr int kFew = 16;  // rows of a short sequence
-constexpr int kPerSimd = 4;  // waves: registers for 16 a CU
+constexpr int kFwdPerSimd = 4, kBwdPerSimd = 4;  // waves: registers for 16 a CU
+constexpr int kFold = 16;
 constexpr int kLook = 4;  // tiles looked back over at a time
 constexpr size_t kMostChannels = 80l << 20;  // of a split call's words (12 bytes each)
 constexpr uint32_t kUnset = 0xffffffffu;
@@ -55,7 +56,12 @@ using Raw = std::conditional_t<V == 1, T, typename Vec<T, V>::type>;
 template <class T, int V>
 VKH_DEV Raw<T, V> load_raw(const T *p) { return *reinterpret_cast<const Raw<T, V> *>(p); }
 // A matrix's rows from `row` on: a pointer that is the same for all lanes, which add their channel's bytes to it in 32
-// bits.  (Both are kept from being joined into vector registers, two for each row of each matrix.)
+// bits.  (Both are kept from being joined into vector registers, two for each row of each matrix: the pointer here,
+// the bytes by here() at each row, after which they are a new value.)
+VKH_DEV unsigned here(unsigned bytes) {
+    asm volatile("" : "+v"(bytes));
+    return bytes;
+}
 typedef __attribute__((address_space(1))) char *Row;
 template <class T>
 struct Walk {
@@ -63,10 +69,7 @@ struct Walk {
     VKH_DEV Walk(const void *m, long row, long ld) : p((uintptr_t)m + row * ld * (long)sizeof(T)), step(ld * sizeof(T)) {
         asm volatile("" : "+s"(p));
     }
-    VKH_DEV Row at(unsigned bytes) const {
-        asm volatile("" : "+v"(bytes));
-        return (Row)p + bytes;
-    }
+    VKH_DEV Row at(unsigned bytes) const { return (Row)p + bytes; }
     VKH_DEV T load(unsigned bytes) const { return *(__attribute__((address_space(1))) T *)at(bytes); }
     VKH_DEV void store(unsigned bytes, float v) const { *(__attribute__((address_space(1))) T *)at(bytes) = (T)v; }
     VKH_DEV void next(bool more = true) { p += more ? step : 0; }
@@ -96,16 +99,24 @@ VKH_DEV Raw<T, V> raw_of(const float (&o)[V]) {
 }
 template <class T, int V>
 VKH_DEV void store_v(T *p, const float (&o)[V]) { *reinterpret_cast<Raw<T, V> *>(p) = raw_of<T, V>(o); }
-// a and 1 - a of a gate, each to its own last digits: e = exp(-|g|) from a product in two parts (one alone is
-// off by |g| steps), 1 / (1 + e) and e / (1 + e).
-template <bool SIG>
-VKH_DEV void gate(float g, float &a, float &rest) {
+// a and 1 - a of a gate, each to its own last digits: e = exp(-|g|), 1 / (1 + e) and e / (1 + e).  The exponential takes
+// its product with 1 / ln 2 in two parts (one alone is off by |g| steps): exact with the first 16 bits of it for a
+// bf16, the rounded one and what its rounding left for an fp32.
+template <bool SIG, class T>
+VKH_DEV void gate(T logit, float &a, float &rest) {
+    const float g = (float)logit;
     if constexpr (SIG) {
-        float m = fabsf(g);
-        m = m > 200.f ? 200.f : m;  // (a NaN stays)
-        const float p = m * -1.44269504f, lo = fmaf(m, -1.92596299e-8f, fmaf(m, -1.44269504f, -p));
+        float m = fabsf(g), p, less;  // e = 2^p (1 - less)
+        m = m > 200.f ? 200.f : m;    // (a NaN stays)
+        if constexpr (sizeof(T) == 2) {
+            p = m * -0x1.7154p+0f;
+            less = m * 4.88849537e-06f;
+        } else {
+            p = m * -1.44269502f;
+            less = fmaf(fmaf(m, 1.44269502f, p), 0.693147182f, m * 1.33497577e-08f);
+        }
         float e = __builtin_amdgcn_exp2f(p);
-        e = fmaf(e, lo * 0.693147181f, e);
+        e = fmaf(-e, less, e);
         const float s = __builtin_amdgcn_rcpf(1.0f + e), t = e * s;
         a = g >= 0.f ? s : t;
         rest = g >= 0.f ? t : s;
@@ -153,12 +164,12 @@ VKH_DEV float high_of(uint64_t w) { return __builtin_bit_cast(float, (uint32_t)(
 template <class T>
 VKH_DEV T peek(const void *at, unsigned bytes) {
     const Walk<T> w(at, 0, 0);
-    return __hip_atomic_load((__attribute__((address_space(1))) T *)w.at(bytes), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return __hip_atomic_load((__attribute__((address_space(1))) T *)w.at(here(bytes)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 template <class T>
 VKH_DEV void publish(void *at, unsigned bytes, T v) {
     const Walk<T> w(at, 0, 0);
-    __hip_atomic_store((__attribute__((address_space(1))) T *)w.at(bytes), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store((__attribute__((address_space(1))) T *)w.at(here(bytes)), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // By one wave, for the 64 channels at `base` of the words (tile s of the sequence at 64 s after it): publishes this
@@ -229,12 +240,12 @@ struct Tiles {
 };
 
 template <class TI, class TO, bool SIG, bool COUP, bool SPLIT>
-__global__ __launch_bounds__(kFwdWaves * 64, kPerSimd) void scan_fwd_k(ScanArgs s, int groups) {
+__global__ __launch_bounds__(kFwdWaves * 64, kFwdPerSimd) void scan_fwd_k(ScanArgs s, int groups) {
     constexpr int R = kFwdRows;
     __shared__ float shA[2][kFwdWaves][64], shB[2][kFwdWaves][64], shH[64];
     __shared__ unsigned ticket;
     const int lane = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int tiles = (s.n_pos + kFwdTile - 1) / kFwdTile;
+    const int tiles = (s.n_pos + kFwdTile - 1) / kFwdTile, marks = (s.n_pos + kScanTile - 1) / kScanTile;
     const long blk = SPLIT ? blockIdx.x % (groups * s.n_batch) : block_number();
     if (blk >= groups * s.n_batch) return;
     const int line = __builtin_amdgcn_readfirstlane((int)blk), b = __builtin_amdgcn_readfirstlane(line / groups);
@@ -244,25 +255,41 @@ __global__ __launch_bounds__(kFwdWaves * 64, kPerSimd) void scan_fwd_k(ScanArgs 
     const Words W = words_of(s.ws, (size_t)s.n_batch * groups, (size_t)s.n_batch * groups * tiles * 64);
     Tiles<SPLIT> order{(unsigned *)(W.tickets + (size_t)line * kTicketBytes), &ticket};
     TI xr[R], gr[R];
-    auto load = [&](int k) {
-        const int t0 = k * kFwdTile + w * R;
-        if (t0 >= len) return;
+    // FULL: all rows of the wave are in the sequence; else rows behind its end are the last one again
+    auto load = [&](int t0, auto full) {
+        constexpr bool FULL = decltype(full)::value;
         const long row0 = (long)b * s.n_pos + t0;
         Walk<TI> g(s.g, row0, s.ldg), x(s.x, row0, s.ldx);
+        unsigned at = in_bytes;
 #pragma unroll
-        for (int i = 0; i < R; ++i) {  // (rows behind the end: the last one again)
-            gr[i] = g.load(in_bytes);
-            xr[i] = x.load(in_bytes);
-            g.next(t0 + i + 1 < len);
-            x.next(t0 + i + 1 < len);
+        for (int i = 0; i < R; ++i) {
+            at = here(at);
+            gr[i] = g.load(at);
+            xr[i] = x.load(at);
+            g.next(FULL || t0 + i + 1 < len);
+            x.next(FULL || t0 + i + 1 < len);
+        }
+    };
+    auto store = [&](int t0, float h, const float (&a)[R], const float (&u)[R], auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        Walk<TO> out(s.h, (long)b * s.n_pos + t0, s.ldh);
+        unsigned at = c * sizeof(TO);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            h = fmaf(a[i], h, u[i]);
+            at = here(at);
+            if (FULL || t0 + i < s.n_pos) out.store(at, FULL || t0 + i < len ? h : 0.f);
+            out.next();
         }
     };
     float H = 0.f;
     int at = order.first();
     if (at >= tiles) return;
     for (int turn = 0;; turn ^= 1) {
-        load(at);
         const int k = at, t0 = k * kFwdTile + w * R;
+        const bool full = t0 + R <= len;
+        if (full) load(t0, std::true_type{});
+        else if (t0 < len) load(t0, std::false_type{});
         if (k == 0) {
             H = act && s.h0 ? s.h0[(long)b * s.dim + c] : 0.f;
             asm volatile("" : "+v"(H));  // (it has been read when the block meets at its barrier: h_last may be h0)
@@ -271,10 +298,10 @@ __global__ __launch_bounds__(kFwdWaves * 64, kPerSimd) void scan_fwd_k(ScanArgs 
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             float rest;
-            gate<SIG>((float)gr[i], a[i], rest);
+            gate<SIG>(gr[i], a[i], rest);
             u[i] = COUP ? rest * (float)xr[i] : (float)xr[i];
         }
-        if (t0 + R > len) {  // rows behind the end leave the state alone
+        if (!full) {  // rows behind the end leave the state alone
 #pragma unroll
             for (int i = 0; i < R; ++i)
                 if (t0 + i >= len) a[i] = 1.f, u[i] = 0.f;
@@ -293,7 +320,7 @@ __global__ __launch_bounds__(kFwdWaves * 64, kPerSimd) void scan_fwd_k(ScanArgs 
         const bool more = then < tiles;
         // of the waves before this one, and of the tile
         float pa = 1.f, pb = 0.f, ta = 1.f, tb = 0.f;
-#pragma unroll
+#pragma unroll kFold
         for (int j = 0; j < kFwdWaves; ++j) {
             if (j == w) pa = ta, pb = tb;
             ta *= A[j][lane];
@@ -310,15 +337,9 @@ __global__ __launch_bounds__(kFwdWaves * 64, kPerSimd) void scan_fwd_k(ScanArgs 
         float h = fmaf(pa, H, pb);
         H = fmaf(ta, H, tb);
         if (act) {
-            if (s.states && w == 0) s.states[((long)b * tiles + k) * s.dim + c] = h;
-            const long row0 = (long)b * s.n_pos + t0;
-            Walk<TO> out(s.h, row0, s.ldh);
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                h = fmaf(a[i], h, u[i]);
-                if (t0 + i < s.n_pos) out.store(c * sizeof(TO), t0 + i < len ? h : 0.f);
-                out.next();
-            }
+            if (s.states && w * R % kScanTile == 0 && t0 < s.n_pos) s.states[((long)b * marks + t0 / kScanTile) * s.dim + c] = h;
+            if (full) store(t0, h, a, u, std::true_type{});
+            else store(t0, h, a, u, std::false_type{});
             if (k + 1 == tiles && s.h_last && w == 0) s.h_last[(long)b * s.dim + c] = H;
         }
         if (!more) return;
@@ -327,7 +348,7 @@ __global__ __launch_bounds__(kFwdWaves * 64, kPerSimd) void scan_fwd_k(ScanArgs 
 }
 
 template <class TI, class TO, bool SIG, bool COUP, bool SPLIT>
-__global__ __launch_bounds__(kBwdWaves * 64, kPerSimd) void scan_bwd_k(ScanArgs s, int groups) {
+__global__ __launch_bounds__(kBwdWaves * 64, kBwdPerSimd) void scan_bwd_k(ScanArgs s, int groups) {
     constexpr int N = kBwdRows;
     __shared__ float shA[2][kBwdWaves][64], shB[2][kBwdWaves][64], shQ[2][kBwdWaves][64], shR[64];
     __shared__ unsigned ticket;
@@ -342,41 +363,45 @@ __global__ __launch_bounds__(kBwdWaves * 64, kPerSimd) void scan_bwd_k(ScanArgs 
     const Words W = words_of(s.ws, (size_t)s.n_batch * groups, (size_t)s.n_batch * groups * tiles * 64);
     Tiles<SPLIT> order{(unsigned *)(W.tickets + (size_t)line * kTicketBytes), &ticket};
     TI xr[N], gr[N], dr[N];
-    float hr = 0.f;  // the state before the tile (one behind the sequence's end has none, and needs none)
-    auto load = [&](int at) {
-        const int k = tiles - 1 - at, t0 = k * kBwdTile + w * N;
-        hr = act && k * kBwdTile < len ? s.states[((long)b * tiles + k) * s.dim + c] : 0.f;
-        if (t0 >= len) return;
+    // (FULL: as in the forward)
+    auto load = [&](int t0, auto full) {
+        constexpr bool FULL = decltype(full)::value;
         const long row0 = (long)b * s.n_pos + t0;
         Walk<TI> g(s.g, row0, s.ldg), d(s.dh, row0, s.lddh), x(s.x, row0, s.ldx);
+        unsigned at = in_bytes;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {  // (rows behind the end: the last one again)
-            gr[i] = g.load(in_bytes);
-            dr[i] = d.load(in_bytes);
-            xr[i] = x.load(in_bytes);
-            g.next(t0 + i + 1 < len);
-            d.next(t0 + i + 1 < len);
-            x.next(t0 + i + 1 < len);
+        for (int i = 0; i < N; ++i) {
+            at = here(at);
+            gr[i] = g.load(at);
+            dr[i] = d.load(at);
+            xr[i] = x.load(at);
+            g.next(FULL || t0 + i + 1 < len);
+            d.next(FULL || t0 + i + 1 < len);
+            x.next(FULL || t0 + i + 1 < len);
         }
     };
     float R = 0.f;
     int at = order.first();
     if (at >= tiles) return;
     for (int turn = 0;; turn ^= 1) {
-        load(at);
         const int k = tiles - 1 - at, t0 = k * kBwdTile + w * N;
+        const bool full = t0 + N <= len;
+        if (full) load(t0, std::true_type{});
+        else if (t0 < len) load(t0, std::false_type{});
+        // the state before the tile (one behind the sequence's end has none, and needs none)
+        float h = act && k * kBwdTile < len ? s.states[((long)b * tiles + k) * s.dim + c] : 0.f;
         if (at == 0) {
             R = act && s.dh_last ? s.dh_last[(long)b * s.dim + c] : 0.f;
             asm volatile("" : "+v"(R));  // (as in the forward: dh0 may be dh_last)
         }
-        float a[N], rest[N], x[N], d[N], h = hr;
+        float a[N], rest[N], x[N], d[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            gate<SIG>((float)gr[i], a[i], rest[i]);
+            gate<SIG>(gr[i], a[i], rest[i]);
             x[i] = (float)xr[i];
             d[i] = (float)dr[i];
         }
-        if (t0 + N > len) {  // rows behind the end leave state and gradient alone
+        if (!full) {  // rows behind the end leave state and gradient alone
 #pragma unroll
             for (int i = 0; i < N; ++i)
                 if (t0 + i >= len) a[i] = 1.f, rest[i] = x[i] = d[i] = 0.f;
@@ -400,13 +425,13 @@ __global__ __launch_bounds__(kBwdWaves * 64, kPerSimd) void scan_bwd_k(ScanArgs 
         const bool more = then < tiles;
         // of the waves behind this one, and of the tile; and the state before this wave's rows
         float pa = 1.f, pb = 0.f, ta = 1.f, tb = 0.f;
-#pragma unroll
+#pragma unroll kFold
         for (int j = kBwdWaves - 1; j >= 0; --j) {
             if (j == w) pa = ta, pb = tb;
             ta *= A[j][lane];
             tb = fmaf(A[j][lane], tb, Q[j][lane]);
         }
-#pragma unroll
+#pragma unroll kFold
         for (int j = 0; j < kBwdWaves; ++j)
             if (j < w) h = fmaf(A[j][lane], h, B[j][lane]);
         if (SPLIT) {
@@ -425,21 +450,28 @@ __global__ __launch_bounds__(kBwdWaves * 64, kPerSimd) void scan_bwd_k(ScanArgs 
             h = fmaf(a[i], h, u(i));
         }
         if (act) {
-            const long row0 = (long)b * s.n_pos + t0;
-            Walk<TO> ox(s.dx, row0 + N - 1, s.lddx), og(s.dg, row0 + N - 1, s.lddg);
+            auto store = [&](auto full) {
+                constexpr bool FULL = decltype(full)::value;
+                const long row = (long)b * s.n_pos + t0 + N - 1;
+                Walk<TO> ox(s.dx, row, s.lddx), og(s.dg, row, s.lddg);
+                unsigned at = c * sizeof(TO);
 #pragma unroll
-            for (int i = N - 1; i >= 0; --i) {
-                const float G = d[i] + e;
-                e = a[i] * G;
-                float dx = COUP ? rest[i] * G : G, dg = COUP ? G * (hp[i] - x[i]) : G * hp[i];
-                if (SIG) dg *= a[i] * rest[i];
-                if (t0 + i < s.n_pos) {
-                    ox.store(c * sizeof(TO), t0 + i < len ? dx : 0.f);
-                    og.store(c * sizeof(TO), t0 + i < len ? dg : 0.f);
+                for (int i = N - 1; i >= 0; --i) {
+                    const float G = d[i] + e;
+                    e = a[i] * G;
+                    float dx = COUP ? rest[i] * G : G, dg = COUP ? G * (hp[i] - x[i]) : G * hp[i];
+                    if (SIG) dg *= a[i] * rest[i];
+                    at = here(at);
+                    if (FULL || t0 + i < s.n_pos) {
+                        ox.store(at, FULL || t0 + i < len ? dx : 0.f);
+                        og.store(at, FULL || t0 + i < len ? dg : 0.f);
+                    }
+                    ox.back();
+                    og.back();
                 }
-                ox.back();
-                og.back();
-            }
+            };
+            if (full) store(std::true_type{});
+            else store(std::false_type{});
             if (k == 0 && s.dh0 && w == 0) s.dh0[(long)b * s.dim + c] = R;
         }
         if (!more) return;
@@ -458,14 +490,15 @@ __global__ __launch_bounds__(256) void scan_few_fwd_k(ScanArgs s) {
     if (s.states && s.n_pos) store_v<float, V>(s.states + state, h);
 #pragma unroll 4
     for (int t = 0; t < s.n_pos; ++t) {
-        float g[V], x[V], o[V] = {};
+        float x[V], o[V] = {};
         if (t < len) {
-            load_v<TI, V>((const TI *)s.g + (row0 + t) * s.ldg + c, g);
+            const Raw<TI, V> g = load_raw<TI, V>((const TI *)s.g + (row0 + t) * s.ldg + c);
             load_v<TI, V>((const TI *)s.x + (row0 + t) * s.ldx + c, x);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 float a, rest;
-                gate<SIG>(g[v], a, rest);
+                if constexpr (V == 1) gate<SIG>(g, a, rest);
+                else gate<SIG>((TI)g[v], a, rest);
                 o[v] = h[v] = fmaf(a, h[v], COUP ? rest * x[v] : x[v]);
             }
         }
@@ -483,7 +516,7 @@ __global__ __launch_bounds__(256) void scan_few_bwd_k(ScanArgs s) {
 #pragma unroll
     for (int t = 0; t < kFew; ++t) {
         if (t >= len) continue;
-        gate<SIG>(to_f32(((const TI *)s.g)[(row0 + t) * s.ldg + c]), a[t], rest[t]);
+        gate<SIG>(((const TI *)s.g)[(row0 + t) * s.ldg + c], a[t], rest[t]);
         x[t] = to_f32(((const TI *)s.x)[(row0 + t) * s.ldx + c]);
         hp[t] = h;
         h = fmaf(a[t], h, COUP ? rest[t] * x[t] : x[t]);
@@ -511,11 +544,11 @@ struct Plan {
     int groups, sharing;
     size_t lines, channels;  // sequences times groups; a split call's words' channels
 };
-Plan plan_of(const ScanArgs &s, int tile, int waves) {
+Plan plan_of(const ScanArgs &s, int tile, int waves, int per_simd) {
     Plan p;
     p.groups = (int)ceil_div(s.dim, 64);
     p.lines = (size_t)p.groups * s.n_batch;
-    const size_t tiles = (s.n_pos + tile - 1) / tile, resident = (size_t)cu_count() * kPerSimd * 4 / waves;
+    const size_t tiles = (s.n_pos + tile - 1) / tile, resident = (size_t)cu_count() * (per_simd * 4 / waves);
     p.channels = p.lines * tiles * 64;
     p.sharing = (int)std::min(tiles, resident / p.lines);
     if (s.n_pos <= kFew || p.sharing < 2 || p.channels > kMostChannels) p.sharing = 0;
@@ -538,8 +571,8 @@ void by_form(const ScanArgs &s, F f) {
 }
 
 // The plan of a call, its workspace ready
-Plan ready(const ScanArgs &s, int tile, int waves, hipStream_t st) {
-    Plan p = plan_of(s, tile, waves);
+Plan ready(const ScanArgs &s, int tile, int waves, int per_simd, hipStream_t st) {
+    Plan p = plan_of(s, tile, waves, per_simd);
     if (!s.ws) p.sharing = 0;
     const size_t n = words_bytes(p) / 16;
     if (n)
@@ -555,7 +588,7 @@ size_t scan_states_floats(const ScanArgs &s) {
     return (size_t)s.n_batch * ((s.n_pos + kScanTile - 1) / kScanTile) * s.dim;
 }
 size_t scan_ws_bytes(const ScanArgs &s) {
-    return std::max(words_bytes(plan_of(s, kFwdTile, kFwdWaves)), words_bytes(plan_of(s, kBwdTile, kBwdWaves)));
+    return std::max(words_bytes(plan_of(s, kFwdTile, kFwdWaves, kFwdPerSimd)), words_bytes(plan_of(s, kBwdTile, kBwdWaves, kBwdPerSimd)));
 }
 
 hipError_t scan_forward(const ScanArgs &s, hipStream_t st) {
@@ -569,7 +602,7 @@ hipError_t scan_forward(const ScanArgs &s, hipStream_t st) {
             hipLaunchKernelGGL(k, dim3(ceil_div(s.dim, 256 * V), s.n_batch), dim3(256), 0, st, s);
             return;
         }
-        const Plan p = ready(s, kFwdTile, kFwdWaves, st);
+        const Plan p = ready(s, kFwdTile, kFwdWaves, kFwdPerSimd, st);
         auto k = p.sharing ? scan_fwd_k<TI, TO, SIG, COUP, true> : scan_fwd_k<TI, TO, SIG, COUP, false>;
         hipLaunchKernelGGL(k, grid_of(p), dim3(kFwdWaves * 64), 0, st, s, p.groups);
     });
@@ -585,7 +618,7 @@ hipError_t scan_backward(const ScanArgs &s, hipStream_t st) {
             hipLaunchKernelGGL((scan_few_bwd_k<TI, TO, SIG, COUP>), dim3(ceil_div(s.dim, 256), s.n_batch), dim3(256), 0, st, s);
             return;
         }
-        const Plan p = ready(s, kBwdTile, kBwdWaves, st);
+        const Plan p = ready(s, kBwdTile, kBwdWaves, kBwdPerSimd, st);
         auto k = p.sharing ? scan_bwd_k<TI, TO, SIG, COUP, true> : scan_bwd_k<TI, TO, SIG, COUP, false>;
         hipLaunchKernelGGL(k, grid_of(p), dim3(kBwdWaves * 64), 0, st, s, p.groups);
     });
