@@ -67,11 +67,13 @@ template <class T>
 struct Walk {
     uintptr_t p, step;
     VKH_DEV Walk(const void *m, long row, long ld) : p((uintptr_t)m + row * ld * (long)sizeof(T)), step(ld * sizeof(T)) {
+        p = (uintptr_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)p);
         asm volatile("" : "+s"(p));
     }
     VKH_DEV Row at(unsigned bytes) const { return (Row)p + bytes; }
     VKH_DEV T load(unsigned bytes) const { return *(__attribute__((address_space(1))) T *)at(bytes); }
-    VKH_DEV void store(unsigned bytes, float v) const { *(__attribute__((address_space(1))) T *)at(bytes) = (T)v; }
+    // past the caches: what is written is read by another kernel
+    VKH_DEV void store(unsigned bytes, float v) const { __builtin_nontemporal_store((T)v, (__attribute__((address_space(1))) T *)at(bytes)); }
     VKH_DEV void next(bool more = true) { p += more ? step : 0; }
     VKH_DEV void back() { p -= step; }
 };
