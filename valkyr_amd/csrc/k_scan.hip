@@ -35,7 +35,7 @@ constexpr int kFwdTile = kFwdWaves * kFwdRows, kBwdTile = kBwdWaves * kBwdRows;
 static_assert(kFwdTile % kScanTile == 0 && kScanTile % kFwdRows == 0 && kBwdTile == kScanTile, "states");
 constexpr int kFew = 16;  // rows of a short sequence
 constexpr int kFwdPerSimd = 4, kBwdPerSimd = 4;  // waves: registers for 16 a CU
-constexpr int kFold = 16;
+constexpr int kFold = 4;  // waves whose A and B are read at a time
 constexpr int kLook = 4;  // tiles looked back over at a time
 constexpr size_t kMostChannels = 80l << 20;  // of a split call's words (12 bytes each)
 constexpr uint32_t kUnset = 0xffffffffu;
@@ -287,11 +287,15 @@ __global__ __launch_bounds__(kFwdWaves * 64, kFwdPerSimd) void scan_fwd_k(ScanAr
     float H = 0.f;
     int at = order.first();
     if (at >= tiles) return;
+    auto ask = [&](int tile) {
+        const int t0 = tile * kFwdTile + w * R;
+        if (t0 + R <= len) load(t0, std::true_type{});
+        else if (t0 < len) load(t0, std::false_type{});
+    };
+    ask(at);
     for (int turn = 0;; turn ^= 1) {
         const int k = at, t0 = k * kFwdTile + w * R;
         const bool full = t0 + R <= len;
-        if (full) load(t0, std::true_type{});
-        else if (t0 < len) load(t0, std::false_type{});
         if (k == 0) {
             H = act && s.h0 ? s.h0[(long)b * s.dim + c] : 0.f;
             asm volatile("" : "+v"(H));  // (it has been read when the block meets at its barrier: h_last may be h0)
@@ -320,6 +324,7 @@ __global__ __launch_bounds__(kFwdWaves * 64, kFwdPerSimd) void scan_fwd_k(ScanAr
         __syncthreads();
         const int then = order.take(at);
         const bool more = then < tiles;
+        if (more && (!SPLIT || w)) ask(then);
         // of the waves before this one, and of the tile
         float pa = 1.f, pb = 0.f, ta = 1.f, tb = 0.f;
 #pragma unroll kFold
@@ -335,6 +340,7 @@ __global__ __launch_bounds__(kFwdWaves * 64, kFwdPerSimd) void scan_fwd_k(ScanAr
             }
             __syncthreads();
             H = shH[lane];
+            if (more && !w) ask(then);
         }
         float h = fmaf(pa, H, pb);
         H = fmaf(ta, H, tb);
@@ -385,11 +391,15 @@ __global__ __launch_bounds__(kBwdWaves * 64, kBwdPerSimd) void scan_bwd_k(ScanAr
     float R = 0.f;
     int at = order.first();
     if (at >= tiles) return;
+    auto ask = [&](int tile) {
+        const int t0 = (tiles - 1 - tile) * kBwdTile + w * N;
+        if (t0 + N <= len) load(t0, std::true_type{});
+        else if (t0 < len) load(t0, std::false_type{});
+    };
+    ask(at);
     for (int turn = 0;; turn ^= 1) {
         const int k = tiles - 1 - at, t0 = k * kBwdTile + w * N;
         const bool full = t0 + N <= len;
-        if (full) load(t0, std::true_type{});
-        else if (t0 < len) load(t0, std::false_type{});
         // the state before the tile (one behind the sequence's end has none, and needs none)
         float h = act && k * kBwdTile < len ? s.states[((long)b * tiles + k) * s.dim + c] : 0.f;
         if (at == 0) {
@@ -425,6 +435,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, kBwdPerSimd) void scan_bwd_k(ScanAr
         __syncthreads();
         const int then = order.take(at);
         const bool more = then < tiles;
+        if (more && (!SPLIT || w)) ask(then);
         // of the waves behind this one, and of the tile; and the state before this wave's rows
         float pa = 1.f, pb = 0.f, ta = 1.f, tb = 0.f;
 #pragma unroll kFold
@@ -443,6 +454,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, kBwdPerSimd) void scan_bwd_k(ScanAr
             }
             __syncthreads();
             R = shR[lane];
+            if (more && !w) ask(then);
         }
         float hp[N], e = fmaf(pa, R, pb);
         R = fmaf(ta, R, tb);
