@@ -211,3 +211,32 @@ def test_a_tensor_past_two_to_the_32_bytes():
         check(lib().vkh_memcpy_d2h(got.ctypes.data, big.offset(at * 4), got.nbytes))
         ref = ends.astype(np.float64) * 2.0 / want
         assert np.all(np.abs(got - ref) <= 1.01 * U * ref)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [3, 61, 200])
+def test_tensors_far_from_each_other(n):
+    """Every other tensor 9 GiB behind the one before it: more than 32 bits of an address apart."""
+    from valkyr_amd import kernels as K
+    from valkyr_amd._lib import check, lib
+    from valkyr_amd.device import DeviceBuffer
+
+    note(f"clip of {n} tensors 9 GiB apart")
+    far, step, size = 9 << 30, 4096, 777
+    big, norm = DeviceBuffer(far + (n + 1) * step), dev(np.zeros(1, np.float32))
+    rng = np.random.default_rng(2)
+    at = [(i % 2) * far + i * step + 4 * (i % 5) for i in range(n)]
+    vals = [rng.standard_normal(size).astype(np.float32) for _ in at]
+    for o, v in zip(at, vals):
+        check(lib().vkh_memcpy_h2d(big.offset(o), v.ctypes.data, v.nbytes))
+    want = math.sqrt(sum(float((v.astype(np.float64) ** 2).sum()) for v in vals))
+    grads = K.grad_list([(big.offset(o), size, K.F32) for o in at])
+    K.grad_norm(grads, norm)
+    assert abs(float(host(norm)[0]) - want) <= 1.0001 * U * want
+    K.grad_clip(grads, 1.5, norm)
+    assert abs(float(host(norm)[0]) - want) <= 1.0001 * U * want
+    for o, v in zip(at, vals):
+        got = np.empty_like(v)
+        check(lib().vkh_memcpy_d2h(got.ctypes.data, big.offset(o), got.nbytes))
+        ref = v.astype(np.float64) * (1.5 / want)
+        assert np.all(np.abs(got - ref) <= 1.01 * U * np.abs(ref) + 2e-45)

@@ -7,8 +7,8 @@
 //
 // The variance is that of the centred values (a row far from 0 keeps its digits), statistics and sums
 // are fp32, and the backward forms the statistics again from x, which it reads anyway.  Each row is read once
-// and held in registers, kHeld values a lane: by a wave where it has up to 64 kHeld values, by up to sixteen waves
-// beyond that, by a block that reads it several times where even those do not hold it.  Rows may start at any
+// and held in registers, 16 values a lane in the forward and 8 in the backward, which has the sums of two
+// gradients beside them: by a wave where that holds it, by up to sixteen waves beyond that, by a block that reads it several times where even those do not hold it.  Rows may start at any
 // value; their last values, less than a vector, are taken one by one.  Bound by HBM for long batches and by the launch
 // for a few tokens.
 #include <algorithm>
@@ -19,8 +19,8 @@
 namespace vkh {
 namespace {
 
-constexpr int kHeld = 16;          // values of a row in a lane
-constexpr int kWide = 1024 * kHeld;  // the longest row that is held
+constexpr int kFwdHeld = 16, kBwdHeld = 8;  // values of a row in a lane (the backward's longest rows: kFwdHeld)
+constexpr int kWide = 16384;  // the longest row that is held
 constexpr int LNT = 256;           // threads on a longer one
 
 template <class F>
@@ -43,31 +43,36 @@ VKH_DEV float lanes_sum(float v) {
 
 // A row's values from `e` on, what is past its end as 0: chunk k of thread t of the NT on a row starts at (k NT + t) W.
 // TAIL: the row's last chunk is not whole (dim % W), else a chunk is in the row or behind it.
-template <bool TAIL, class T, int W>
-VKH_DEV void load_chunk(const T *p, int e, int dim, float (&o)[W]) {
-    if constexpr (!TAIL) {
+template <int W, bool TAIL, class T>
+VKH_DEV typename Vec<T, W>::type raw_chunk(const T *p, int e, int dim) {
+    typename Vec<T, W>::type v = {};
+    if (e + W <= dim) {
+        v = *reinterpret_cast<const typename Vec<T, W>::type *>(p + e);
+    } else if constexpr (TAIL) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) o[i] = 0.f;
-        if (e >= dim) return;
+        for (int i = 0; i < W; ++i)
+            if (e + i < dim) v[i] = p[e + i];
     }
-    if (!TAIL || e + W <= dim) {
-        const auto v = *reinterpret_cast<const typename Vec<T, W>::type *>(p + e);
+    return v;
+}
+template <class T, int W>
+VKH_DEV void widen(T v, float (&o)[W]) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) o[i] = (float)v[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < W; ++i) o[i] = e + i < dim ? to_f32(p[e + i]) : 0.f;
-    }
+    for (int i = 0; i < W; ++i) o[i] = (float)v[i];
 }
 template <bool TAIL, class T, int W>
+VKH_DEV void load_chunk(const T *p, int e, int dim, float (&o)[W]) { widen(raw_chunk<W, TAIL>(p, e, dim), o); }
+// Results go past the caches: they are read by another kernel, and each store covers whole lines over its lanes (16384
+// rows of 4096 bf16, forward: 65 us through the caches, 46 past them).
+template <bool TAIL, bool PAST = true, class T, int W>
 VKH_DEV void store_chunk(T *p, int e, int dim, const float (&o)[W]) {
-    if (!TAIL && e >= dim) return;
-    if (!TAIL || e + W <= dim) {
+    if (e + W <= dim) {
         typename Vec<T, W>::type v;
 #pragma unroll
         for (int i = 0; i < W; ++i) v[i] = (T)o[i];
-        *reinterpret_cast<typename Vec<T, W>::type *>(p + e) = v;
-    } else {
+        if constexpr (PAST) __builtin_nontemporal_store(v, reinterpret_cast<typename Vec<T, W>::type *>(p + e));
+        else *reinterpret_cast<typename Vec<T, W>::type *>(p + e) = v;
+    } else if (TAIL) {
 #pragma unroll
         for (int i = 0; i < W; ++i)
             if (e + i < dim) p[e + i] = (T)o[i];
@@ -76,7 +81,7 @@ VKH_DEV void store_chunk(T *p, int e, int dim, const float (&o)[W]) {
 
 // The NT threads on a row (BT in the block).  Lane j of each 16 takes wave j's part of an exchange: sums over the waves are
 // sums over a row of lanes.
-template <int NT, int BT, int W>
+template <int NT, int BT, int W, int HELD>
 struct Group {
     static constexpr int waves = NT / 64;
     float2 (*sh)[BT / 64];    // two, in turn: one barrier an exchange
@@ -88,7 +93,7 @@ struct Group {
             auto held = [&](int w) {
                 int n = 0;
 #pragma unroll
-                for (int k = 0; k < kHeld / W; ++k) n += min(max(dim - (k * NT + w * 64) * W, 0), 64 * W);
+                for (int k = 0; k < HELD / W; ++k) n += min(max(dim - (k * NT + w * 64) * W, 0), 64 * W);
                 return n;
             };
             const int j = threadIdx.x % 16, n = j < waves ? held(j) : 0, m = held(threadIdx.x % NT / 64);
@@ -110,18 +115,18 @@ struct Group {
 
 // 1 / deviation of the row in x; leaves x centred and scaled (0 past its end).  Each wave centres its values about its
 // own mean; the waves' sums of squares are joined with n (mean_w - mean)^2 each.
-template <bool TAIL, int NT, int BT, int W>
-VKH_DEV float normalise(float (&x)[kHeld / W][W], int t, int dim, float inv_dim, float eps, Group<NT, BT, W> &g) {
+template <bool TAIL, int NT, int BT, int W, int HELD>
+VKH_DEV float normalise(float (&x)[HELD / W][W], int t, int dim, float inv_dim, float eps, Group<NT, BT, W, HELD> &g) {
     auto centred = [&](int k, int i, float m) { return (k * NT + t) * W + (TAIL ? i : 0) < dim ? x[k][i] - m : 0.f; };
     float s = 0.f, q = 0.f;
 #pragma unroll
-    for (int k = 0; k < kHeld / W; ++k)
+    for (int k = 0; k < HELD / W; ++k)
 #pragma unroll
         for (int i = 0; i < W; ++i) s += x[k][i];
     s = lanes_sum(s);
     float mu = s * (NT == 64 ? inv_dim : g.mine);
 #pragma unroll
-    for (int k = 0; k < kHeld / W; ++k)
+    for (int k = 0; k < HELD / W; ++k)
 #pragma unroll
         for (int i = 0; i < W; ++i) {
             const float c = centred(k, i, mu);
@@ -136,7 +141,7 @@ VKH_DEV float normalise(float (&x)[kHeld / W][W], int t, int dim, float inv_dim,
     }
     const float r = 1.0f / sqrtf(fmaf(q, inv_dim, eps));
 #pragma unroll
-    for (int k = 0; k < kHeld / W; ++k)
+    for (int k = 0; k < HELD / W; ++k)
 #pragma unroll
         for (int i = 0; i < W; ++i) x[k][i] = centred(k, i, mu) * r;
     return r;
@@ -144,16 +149,19 @@ VKH_DEV float normalise(float (&x)[kHeld / W][W], int t, int dim, float inv_dim,
 
 template <class TX, class TY, int NT, bool TAIL>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void layernorm_fwd_held_k(LayernormArgs a) {
-    constexpr int BT = NT < 256 ? 256 : NT, W = 16 / (int)sizeof(TX), NI = kHeld / W;
+    constexpr int BT = NT < 256 ? 256 : NT, W = 16 / (int)sizeof(TX), NI = kFwdHeld / W;
     __shared__ float2 sh[2][BT / 64];
     const int t = threadIdx.x % NT, dim = a.dim;
     const long row = block_number() * (BT / NT) + __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
     const bool live = row < a.n_rows;
-    Group<NT, BT, W> g(sh, threadIdx.x / NT, dim);
+    Group<NT, BT, W, kFwdHeld> g(sh, threadIdx.x / NT, dim);
+    typename Vec<TX, W>::type xr[NI];  // (all asked for before the first is used)
     float x[NI][W];
 #pragma unroll
-    for (int k = 0; k < NI; ++k) load_chunk<TAIL>((const TX *)a.x + (live ? row : 0) * a.ldx, (k * NT + t) * W, dim, x[k]);
-    normalise<TAIL, NT, BT, W>(x, t, dim, 1.0f / (float)dim, a.eps, g);
+    for (int k = 0; k < NI; ++k) xr[k] = raw_chunk<W, TAIL>((const TX *)a.x + (live ? row : 0) * a.ldx, (k * NT + t) * W, dim);
+#pragma unroll
+    for (int k = 0; k < NI; ++k) widen(xr[k], x[k]);
+    normalise<TAIL>(x, t, dim, 1.0f / (float)dim, a.eps, g);
     if (!live) return;
 #pragma unroll
     for (int k = 0; k < NI; ++k) {
@@ -182,14 +190,14 @@ constexpr int bwd_vector() {
 // Rows are dealt to the blocks' groups of NT threads in turn.  A lane sums its columns' gradients of w and b over its
 // rows; the groups of a block add theirs through LDS, one after the other, and the block writes them to its row of
 // `partial` ([blocks][2][dim]), which layernorm_dw_k adds in block order.
-template <class TX, class TG, class TD, int NT, int BT, bool TAIL>
+template <class TX, class TG, class TD, int NT, int BT, int HELD, bool TAIL>
 __global__ __launch_bounds__(BT) void layernorm_bwd_held_k(LayernormArgs a) {
-    constexpr int W = bwd_vector<TX, TG, TD>(), NI = kHeld / W, GR = BT / NT;
+    constexpr int W = bwd_vector<TX, TG, TD>(), NI = HELD / W, GR = BT / NT;
     __shared__ float2 sh[2][BT / 64];
     extern __shared__ float sums[];  // [2][dim] with more than one group
     const int grp = __builtin_amdgcn_readfirstlane(threadIdx.x / NT), t = threadIdx.x % NT, dim = a.dim;
     const long stride = (long)gridDim.x * GR;
-    Group<NT, BT, W> g(sh, grp, dim);
+    Group<NT, BT, W, HELD> g(sh, grp, dim);
     const float inv_dim = 1.0f / (float)dim;
     float dw[NI][W] = {}, db[NI][W] = {}, w[NI][W];
 #pragma unroll
@@ -204,17 +212,22 @@ __global__ __launch_bounds__(BT) void layernorm_bwd_held_k(LayernormArgs a) {
     for (long row0 = (long)blockIdx.x * GR; row0 < a.n_rows; row0 += stride) {  // (all groups of a block take every barrier)
         const bool live = row0 + grp < a.n_rows;
         const long row = live ? row0 + grp : row0;
-        float x[NI][W], d[NI][W], o[NI][W] = {};
+        typename Vec<TX, W>::type xr[NI];  // (all asked for before the first is used)
+        typename Vec<TG, W>::type dr[NI];
+        typename Vec<TD, W>::type rr[NI] = {};
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
-            load_chunk<TAIL>((const TX *)a.x + row * a.ldx, (k * NT + t) * W, dim, x[k]);
-            load_chunk<TAIL>((const TG *)a.dy + row * a.lddy, (k * NT + t) * W, dim, d[k]);
+            xr[k] = raw_chunk<W, TAIL>((const TX *)a.x + row * a.ldx, (k * NT + t) * W, dim);
+            dr[k] = raw_chunk<W, TAIL>((const TG *)a.dy + row * a.lddy, (k * NT + t) * W, dim);
         }
         if (a.res) {
 #pragma unroll
-            for (int k = 0; k < NI; ++k) load_chunk<TAIL>((const TD *)a.res + row * a.lddx, (k * NT + t) * W, dim, o[k]);
+            for (int k = 0; k < NI; ++k) rr[k] = raw_chunk<W, TAIL>((const TD *)a.res + row * a.lddx, (k * NT + t) * W, dim);
         }
-        const float r = normalise<TAIL, NT, BT, W>(x, t, dim, inv_dim, a.eps, g);
+        float x[NI][W], d[NI][W];
+#pragma unroll
+        for (int k = 0; k < NI; ++k) widen(xr[k], x[k]), widen(dr[k], d[k]);
+        const float r = normalise<TAIL>(x, t, dim, inv_dim, a.eps, g);
         float s = 0.f, q = 0.f;
 #pragma unroll
         for (int k = 0; k < NI; ++k)
@@ -240,10 +253,11 @@ __global__ __launch_bounds__(BT) void layernorm_bwd_held_k(LayernormArgs a) {
         if (!live) continue;
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
-            const int e = (k * NT + t) * W;
+            float o[W];
+            widen(rr[k], o);
 #pragma unroll
-            for (int i = 0; i < W; ++i) o[k][i] = fmaf(d[k][i] - s - x[k][i] * q, r, o[k][i]);
-            store_chunk<TAIL>((TD *)a.dx + row * a.lddx, e, dim, o[k]);
+            for (int i = 0; i < W; ++i) o[i] = fmaf(d[k][i] - s - x[k][i] * q, r, o[i]);
+            store_chunk<TAIL>((TD *)a.dx + row * a.lddx, (k * NT + t) * W, dim, o);
         }
     }
     if (!a.partial) return;
@@ -262,8 +276,8 @@ __global__ __launch_bounds__(BT) void layernorm_bwd_held_k(LayernormArgs a) {
 #pragma unroll
                 for (int i = 0; i < W; ++i) dw[k][i] += u[i], db[k][i] += v[i];
             }
-            store_chunk<TAIL>(j + 1 < GR ? sums : out, e, dim, dw[k]);
-            store_chunk<TAIL>((j + 1 < GR ? sums : out) + dim, e, dim, db[k]);
+            store_chunk<TAIL, false>(j + 1 < GR ? sums : out, e, dim, dw[k]);
+            store_chunk<TAIL, false>((j + 1 < GR ? sums : out) + dim, e, dim, db[k]);
         }
     }
 }
@@ -348,9 +362,9 @@ __global__ __launch_bounds__(1024) void layernorm_dw_k(const float *partial, int
 }
 
 // Threads on a row: as many as hold it.
-int threads_of(int dim) {
+int threads_of(int dim, int held) {
     int n = 64;
-    while (n * kHeld < dim) n *= 2;
+    while (n * held < dim) n *= 2;
     return n;
 }
 template <class F>
@@ -364,7 +378,10 @@ void by_threads(int n, F f) {
     }
 }
 
-// The backward's threads a block and blocks.
+// The backward's threads a block and blocks: 512 threads where there are rows for more than 512 blocks of 256, and as
+// many blocks as give every CU sixteen waves.  Two blocks of 512 threads a CU work while the other waits (16384
+// rows of 4096 bf16: 106 us; one block of 1024 threads 118, three of 512 119, with the partial sums of half as many more
+// blocks; 16 values a lane 135 to 181).
 struct Bwd {
     int threads, blocks;
 };
@@ -373,11 +390,8 @@ Bwd bwd_of(const LayernormArgs &a) {
         const long most = std::min(512l, std::max(1l, (8l << 20) / a.dim));
         return {LNT, (int)std::min(a.n_rows, most)};
     }
-    const int nt = threads_of(a.dim);
-    int bt = std::max(nt, 256);
-    while (bt < 1024 && a.n_rows * nt / bt > 512) bt *= 2;
-    const long need = (a.n_rows * nt + bt - 1) / bt;
-    return {bt, (int)std::min(need, 256l * 1024 / bt)};
+    const int nt = std::min(1024, threads_of(a.dim, kBwdHeld)), bt = std::max(nt, a.n_rows * nt / 256 > 512 ? 512 : 256);
+    return {bt, (int)std::min((a.n_rows * nt + bt - 1) / bt, 256l * 1024 / bt)};
 }
 
 }  // namespace
@@ -394,7 +408,7 @@ hipError_t layernorm_forward(const LayernormArgs &a, DType xt, DType yt, hipStre
                 hipLaunchKernelGGL((layernorm_fwd_k<X, Y>), long_grid(a.n_rows), dim3(LNT), 0, st, a);
                 return;
             }
-            by_threads(threads_of(a.dim), [&](auto nt) {
+            by_threads(threads_of(a.dim, kFwdHeld), [&](auto nt) {
                 constexpr int NT = decltype(nt)::value, BT = std::max(NT, 256), per = BT / NT;
                 auto k = a.dim % (16 / sizeof(X)) ? layernorm_fwd_held_k<X, Y, NT, true> : layernorm_fwd_held_k<X, Y, NT, false>;
                 hipLaunchKernelGGL(k, long_grid((a.n_rows + per - 1) / per), dim3(BT), 0, st, a);
@@ -417,18 +431,24 @@ hipError_t layernorm_backward(const LayernormArgs &a, DType xt, DType gt, DType 
                     hipLaunchKernelGGL((layernorm_bwd_k<X, G, D>), dim3(n.blocks), dim3(LNT), 0, st, a);
                     return;
                 }
-                by_threads(threads_of(a.dim), [&](auto nt) {
+                by_threads(std::min(1024, threads_of(a.dim, kBwdHeld)), [&](auto nt) {
                     constexpr int NT = decltype(nt)::value;
                     auto go = [&](auto bt) {
                         constexpr int BT = std::max(NT, decltype(bt)::value);
                         const size_t lds = BT > NT && a.partial ? 2 * a.dim * sizeof(float) : 0;
-                        auto k = a.dim % bwd_vector<X, G, D>() ? layernorm_bwd_held_k<X, G, D, NT, BT, true>
-                                                               : layernorm_bwd_held_k<X, G, D, NT, BT, false>;
-                        hipLaunchKernelGGL(k, dim3(n.blocks), dim3(BT), lds, st, a);
+                        auto pick = [&](auto held) {
+                            constexpr int H = decltype(held)::value;
+                            auto k = a.dim % bwd_vector<X, G, D>() ? layernorm_bwd_held_k<X, G, D, NT, BT, H, true>
+                                                                   : layernorm_bwd_held_k<X, G, D, NT, BT, H, false>;
+                            hipLaunchKernelGGL(k, dim3(n.blocks), dim3(BT), lds, st, a);
+                        };
+                        if constexpr (NT == 1024) {
+                            if (a.dim > 1024 * kBwdHeld) return pick(std::integral_constant<int, kFwdHeld>{});
+                        }
+                        pick(std::integral_constant<int, kBwdHeld>{});
                     };
-                    if (n.threads <= 256) go(std::integral_constant<int, 256>{});
-                    else if (n.threads <= 512) go(std::integral_constant<int, 512>{});
-                    else go(std::integral_constant<int, 1024>{});
+                    if (n.threads == 256) go(std::integral_constant<int, 256>{});
+                    else go(std::integral_constant<int, 512>{});
                 });
             });
         });

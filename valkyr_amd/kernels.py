@@ -21,13 +21,15 @@ SCAN_SIGMOID, SCAN_DECAY = 0, 1
 
 
 def _p(x):
-    if x is None:
-        return None
-    if isinstance(x, C.c_void_p):
+    if x is None or isinstance(x, (int, C.c_void_p)):
         return x
-    if isinstance(x, int):
-        return C.c_void_p(x)
     return x.ptr
+
+
+def _addr(x):
+    """x as a field of a struct."""
+    p = _p(x)
+    return p.value if isinstance(p, C.c_void_p) else p
 
 
 def _s(stream):
@@ -185,14 +187,10 @@ def lora_backward(dy, x, w, a, b, inter, dx, dA, dB, M, N, K, r, alpha_over_r,
 def lora_adapters(specs):
     """ctypes array of vkh_lora_adapter from dicts with keys col, n, k, a, b,
     inter, dyb, da, db (buffers or None)."""
-    def addr(x):
-        p = _p(x)
-        return None if p is None else p.value
-
     arr = (LoraAdapter * len(specs))()
     for i, d in enumerate(specs):
         arr[i] = LoraAdapter(d["col"], d["n"], d["k"],
-                             *(addr(d.get(f)) for f in ("a", "b", "inter", "dyb", "da", "db")))
+                             *(_addr(d.get(f)) for f in ("a", "b", "inter", "dyb", "da", "db")))
     return arr
 
 
@@ -296,13 +294,9 @@ def gated_scan_backward(p, x, g, states, dh, dx, dg, dh_last=None, dh0=None, len
 
 def grad_list(tensors):
     """ctypes array of vkh_grad from (gradient, values, dtype) or (gradient, values, dtype, out)."""
-    def addr(x):
-        p = _p(x)
-        return None if p is None else p.value
-
     arr = (Grad * len(tensors))()
     for i, (g, n, dtype, *out) in enumerate(tensors):
-        arr[i] = Grad(addr(g), n, dtype, addr(out[0]) if out else None)
+        arr[i] = Grad(_addr(g), n, dtype, _addr(out[0]) if out else None)
     return arr
 
 
