@@ -207,6 +207,12 @@ uint32_t vkh_runner_step_t(const vkh_runner *r);
 vkh_status vkh_runner_set_step_t(vkh_runner *r, uint32_t step_t);
 float vkh_runner_get_lr(const vkh_runner *r);
 vkh_status vkh_runner_set_lr(vkh_runner *r, float lr); /* cfg.lr is mutable between steps */
+/* Clipping by the norm of all trainable gradients (vkh_grad_clip) in every later step, ahead of Adam: 0, as at the
+ * start, for none.  The gradients that vkh_runner_get_tensor then reads behind a step are the clipped ones; a step whose
+ * norm is not finite is not clipped.  The reference has no clipping. */
+vkh_status vkh_runner_set_grad_clip(vkh_runner *r, float max_norm);
+/* The gradients' norm in the last step with clipping, before it was clipped (waits for the step). */
+vkh_status vkh_runner_last_grad_norm(vkh_runner *r, float *norm);
 vkh_status vkh_runner_get_config(const vkh_runner *r, vkh_config *out);
 size_t vkh_runner_param_count(const vkh_runner *r);          /* trainable params */
 size_t vkh_runner_device_bytes(const vkh_runner *r);

@@ -196,6 +196,8 @@ SIGNATURES = [
     ("vkh_runner_set_step_t", ST, [P, U32]),
     ("vkh_runner_get_lr", F, [P]),
     ("vkh_runner_set_lr", ST, [P, F]),
+    ("vkh_runner_set_grad_clip", ST, [P, F]),
+    ("vkh_runner_last_grad_norm", ST, [P, C.POINTER(F)]),
     ("vkh_runner_get_config", ST, [P, C.POINTER(Config)]),
     ("vkh_runner_param_count", SZ, [P]),
     ("vkh_runner_device_bytes", SZ, [P]),

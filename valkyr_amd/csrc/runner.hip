@@ -230,6 +230,10 @@ struct vkh_runner {
     hipStream_t last_st = nullptr;
     uint32_t step_t = 1;  // transformer.zig:940
     float loss_target = 0.f;
+    // gradient clipping (0: none): the largest norm, the last step's norm and the call's workspace
+    float clip_norm = 0.f, *grad_norm_d = nullptr;
+    void *clip_ws = nullptr;
+    bool norm_pending = false;
     bool loss_pending = false, tick_loss_pending = false, batch_ready = false;
     // the tick API's cached last loss (runner.zig:932-945)
     bool has_last = false;
@@ -1666,13 +1670,25 @@ struct vkh_runner {
         return record_tick_loss();
     }
 
-    vkh_status step_enqueue(bool with_adam) {
-        VKH_TRY(forward_backward_enqueue(with_adam));
-        VKH_TRY(record_loss());
-        if (with_adam) {
-            if (!concurrent) VKH_TRY(adam_enqueue());
-            step_t += 1;  // transformer.zig:1318
+    // A training step's forward, backward and Adam.  Clipping needs the norm of all gradients before the first is
+    // used: Adam then follows the whole backward in place of running beside it.
+    vkh_status train_enqueue() {
+        const bool clip = clip_norm > 0.f;
+        VKH_TRY(forward_backward_enqueue(!clip));
+        if (clip) {
+            const GradTensor g{G, G, te - tb, DType::F32};  // (what lies between the tensors is zero)
+            VKH_HIP(grad_clip(&g, 1, true, clip_norm, grad_norm_d, clip_ws, cur));
+            VKH_HIP(hipMemcpyAsync(loss_h + 2, grad_norm_d, 4, hipMemcpyDeviceToHost, cur));
+            norm_pending = true;
         }
+        if (clip || !concurrent) VKH_TRY(adam_enqueue());
+        return VKH_OK;
+    }
+
+    vkh_status step_enqueue(bool with_adam) {
+        VKH_TRY(with_adam ? train_enqueue() : forward_backward_enqueue(false));
+        VKH_TRY(record_loss());
+        if (with_adam) step_t += 1;  // transformer.zig:1318
         return VKH_OK;
     }
 };
@@ -2007,6 +2023,27 @@ vkh_status vkh_runner_set_lr(vkh_runner *r, float lr) {
     return VKH_OK;
 }
 
+vkh_status vkh_runner_set_grad_clip(vkh_runner *r, float max_norm) {
+    if (!r) return fail(VKH_ERR_INVALID_ARGUMENT, "null runner");
+    if (!(max_norm >= 0.f)) return fail(VKH_ERR_INVALID_ARGUMENT, "max_norm is negative or not a number");
+    if (max_norm > 0.f && !r->clip_ws) {
+        char *ws = nullptr;
+        if (!r->grad_norm_d) VKH_TRY(r->alloc(r->grad_norm_d, 4));
+        VKH_TRY(r->alloc(ws, grad_ws_bytes(1)));
+        r->clip_ws = ws;
+    }
+    r->clip_norm = max_norm;
+    return VKH_OK;
+}
+
+vkh_status vkh_runner_last_grad_norm(vkh_runner *r, float *norm) {
+    if (!r || !norm) return fail(VKH_ERR_INVALID_ARGUMENT, "null argument");
+    if (!r->norm_pending) return fail(VKH_ERR_INVALID_ARGUMENT, "no step with clipping has run");
+    VKH_TRY(r->host_wait());
+    *norm = r->loss_h[2];
+    return VKH_OK;
+}
+
 vkh_status vkh_runner_get_config(const vkh_runner *r, vkh_config *out) {
     if (!r || !out) return fail(VKH_ERR_INVALID_ARGUMENT, "null argument");
     *out = r->cfg;
@@ -2222,8 +2259,7 @@ vkh_status vkh_runner_tick_frame_train(vkh_runner *r, vkh_stream stream,
     vkh_status st = VKH_OK;
     uint32_t n = 0;
     while (should_train && n < max_steps) {
-        st = r->forward_backward_enqueue(true);
-        if (st == VKH_OK && !r->concurrent) st = r->adam_enqueue();
+        st = r->train_enqueue();
         if (st != VKH_OK) break;
         r->step_t += 1;
         ++n;

@@ -198,6 +198,16 @@ class Runner:
     def lr(self, v: float):
         check(lib().vkh_runner_set_lr(self._h, v))
 
+    def set_grad_clip(self, max_norm: float) -> None:
+        """Scale all gradients of a step down to this norm ahead of Adam (0: no clipping)."""
+        check(lib().vkh_runner_set_grad_clip(self._h, max_norm))
+
+    def last_grad_norm(self) -> float:
+        """The gradients' norm in the last step with clipping, before it was clipped."""
+        v = C.c_float()
+        check(lib().vkh_runner_last_grad_norm(self._h, C.byref(v)))
+        return v.value
+
     def param_count(self) -> int:
         return lib().vkh_runner_param_count(self._h)
 
