@@ -29,16 +29,22 @@
 namespace vkh {
 namespace {
 
+// 16 rows a wave in the forward, whose values, gates and inputs fit 128 registers so; 8 in the backward, which holds five
+// numbers of each, and twice the waves, so that a tile has as many rows: fewer tiles have fewer words to publish and to
+// look back over (16384 x 4096 bf16, a forward of 64 rows a tile 120 us beside 113, a backward of 8 waves and 64 rows 196
+// beside 185).  Registers for three blocks a CU spill and are slower (128 and 210).
 constexpr int kFwdWaves = 8, kBwdWaves = 16;
-constexpr int kFwdRows = 16, kBwdRows = 8;  // a wave's
+constexpr int kFwdRows = 16, kBwdRows = 8;
 constexpr int kFwdTile = kFwdWaves * kFwdRows, kBwdTile = kBwdWaves * kBwdRows;
-static_assert(kFwdTile % kScanTile == 0 && kScanTile % kFwdRows == 0 && kBwdTile == kScanTile, "states");
-constexpr int kFew = 16;  // rows of a short sequence
-constexpr int kFwdPerSimd = 4, kBwdPerSimd = 4;  // waves: registers for 16 a CU
-constexpr int kFold = 4;  // waves whose A and B are read at a time
-constexpr int kLook = 4;  // tiles looked back over at a time
+static_assert(kFwdTile == kScanTile && kBwdTile == kScanTile, "states");
+constexpr int kPerSimd = 4;  // waves: 128 registers
+constexpr int kFold = 4;     // waves whose A and B are read at a time
+constexpr int kLook = 4;     // tiles looked back over at a time (one: a forward of 131 us beside 118; eight: 114 beside 113)
 constexpr size_t kMostChannels = 80l << 20;  // of a split call's words (12 bytes each)
 constexpr uint32_t kUnset = 0xffffffffu;
+// Rows of a sequence that a thread takes alone.  64 sequences of 16 rows of 4096 bf16, forward and backward: 14 and 17 us,
+// 30 and 66 in tiles; 8 of them, 10 and 9, in tiles 8 and 10.
+constexpr int kFew = 16;
 
 template <class F>
 void by_type(DType d, F f) {
@@ -241,13 +247,20 @@ struct Tiles {
     }
 };
 
+// Both kernels: a tile's values are asked for as soon as the one before is in use, by the wave that looks back once it
+// has (a wave's loads return in order), so they arrive while that tile is joined and stored.  (Backward of 16384 x 4096
+// bf16: 208 us without, 185 with; the forward, 16 blocks' loads deep already, 113 and 111.)
+//
+// 16384 x 4096 bf16 (0.40 and 0.67 GB): forward 105 us, 3.8 TB/s, backward 179, 3.75, and 6 each to make the words
+// ready; fp32, 8192 rows (the same bytes): 81 and 130, 4.9 and 5.2.  Half the values of bf16 lie between it and HBM: about
+// 26 vector instructions each, and the joins.  16 sequences of 1024 rows, a block each: 90 and 162.
 template <class TI, class TO, bool SIG, bool COUP, bool SPLIT>
-__global__ __launch_bounds__(kFwdWaves * 64, kFwdPerSimd) void scan_fwd_k(ScanArgs s, int groups) {
+__global__ __launch_bounds__(kFwdWaves * 64, kPerSimd) void scan_fwd_k(ScanArgs s, int groups) {
     constexpr int R = kFwdRows;
     __shared__ float shA[2][kFwdWaves][64], shB[2][kFwdWaves][64], shH[64];
     __shared__ unsigned ticket;
     const int lane = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int tiles = (s.n_pos + kFwdTile - 1) / kFwdTile, marks = (s.n_pos + kScanTile - 1) / kScanTile;
+    const int tiles = (s.n_pos + kFwdTile - 1) / kFwdTile;
     const long blk = SPLIT ? blockIdx.x % (groups * s.n_batch) : block_number();
     if (blk >= groups * s.n_batch) return;
     const int line = __builtin_amdgcn_readfirstlane((int)blk), b = __builtin_amdgcn_readfirstlane(line / groups);
@@ -345,7 +358,7 @@ __global__ __launch_bounds__(kFwdWaves * 64, kFwdPerSimd) void scan_fwd_k(ScanAr
         float h = fmaf(pa, H, pb);
         H = fmaf(ta, H, tb);
         if (act) {
-            if (s.states && w * R % kScanTile == 0 && t0 < s.n_pos) s.states[((long)b * marks + t0 / kScanTile) * s.dim + c] = h;
+            if (s.states && w == 0) s.states[((long)b * tiles + k) * s.dim + c] = h;
             if (full) store(t0, h, a, u, std::true_type{});
             else store(t0, h, a, u, std::false_type{});
             if (k + 1 == tiles && s.h_last && w == 0) s.h_last[(long)b * s.dim + c] = H;
@@ -356,7 +369,7 @@ __global__ __launch_bounds__(kFwdWaves * 64, kFwdPerSimd) void scan_fwd_k(ScanAr
 }
 
 template <class TI, class TO, bool SIG, bool COUP, bool SPLIT>
-__global__ __launch_bounds__(kBwdWaves * 64, kBwdPerSimd) void scan_bwd_k(ScanArgs s, int groups) {
+__global__ __launch_bounds__(kBwdWaves * 64, kPerSimd) void scan_bwd_k(ScanArgs s, int groups) {
     constexpr int N = kBwdRows;
     __shared__ float shA[2][kBwdWaves][64], shB[2][kBwdWaves][64], shQ[2][kBwdWaves][64], shR[64];
     __shared__ unsigned ticket;
@@ -558,14 +571,18 @@ struct Plan {
     int groups, sharing;
     size_t lines, channels;  // sequences times groups; a split call's words' channels
 };
-Plan plan_of(const ScanArgs &s, int tile, int waves, int per_simd) {
+Plan plan_of(const ScanArgs &s, bool back) {
     Plan p;
     p.groups = (int)ceil_div(s.dim, 64);
     p.lines = (size_t)p.groups * s.n_batch;
-    const size_t tiles = (s.n_pos + tile - 1) / tile, resident = (size_t)cu_count() * (per_simd * 4 / waves);
+    const int tile = back ? kBwdTile : kFwdTile;
+    const size_t tiles = (s.n_pos + tile - 1) / tile, resident = (size_t)cu_count() * (kPerSimd * 4 / (back ? kBwdWaves : kFwdWaves));
     p.channels = p.lines * tiles * 64;
     p.sharing = (int)std::min(tiles, resident / p.lines);
-    if (s.n_pos <= kFew || p.sharing < 2 || p.channels > kMostChannels) p.sharing = 0;
+    // Two tiles (forward: three) one after the other cost less than the launch that makes the words ready: 200 x 1024
+    // bf16, forward and backward, 8.3 and 8.8 us in one block a line, 10.6 and 10.4 shared; 512 x 1024 mixed, of four tiles,
+    // 11.6 and 17.8, shared 10.2 and 11.7.
+    if (s.n_pos <= kFew || p.sharing < 2 || tiles < (back ? 3 : 4) || p.channels > kMostChannels) p.sharing = 0;
     return p;
 }
 size_t words_bytes(const Plan &p) { return p.sharing ? p.lines * kTicketBytes + (p.channels * 12 + 15) / 16 * 16 : 0; }
@@ -585,8 +602,8 @@ void by_form(const ScanArgs &s, F f) {
 }
 
 // The plan of a call, its workspace ready
-Plan ready(const ScanArgs &s, int tile, int waves, int per_simd, hipStream_t st) {
-    Plan p = plan_of(s, tile, waves, per_simd);
+Plan ready(const ScanArgs &s, bool back, hipStream_t st) {
+    Plan p = plan_of(s, back);
     if (!s.ws) p.sharing = 0;
     const size_t n = words_bytes(p) / 16;
     if (n)
@@ -602,7 +619,7 @@ size_t scan_states_floats(const ScanArgs &s) {
     return (size_t)s.n_batch * ((s.n_pos + kScanTile - 1) / kScanTile) * s.dim;
 }
 size_t scan_ws_bytes(const ScanArgs &s) {
-    return std::max(words_bytes(plan_of(s, kFwdTile, kFwdWaves, kFwdPerSimd)), words_bytes(plan_of(s, kBwdTile, kBwdWaves, kBwdPerSimd)));
+    return std::max(words_bytes(plan_of(s, false)), words_bytes(plan_of(s, true)));
 }
 
 hipError_t scan_forward(const ScanArgs &s, hipStream_t st) {
@@ -616,7 +633,7 @@ hipError_t scan_forward(const ScanArgs &s, hipStream_t st) {
             hipLaunchKernelGGL(k, dim3(ceil_div(s.dim, 256 * V), s.n_batch), dim3(256), 0, st, s);
             return;
         }
-        const Plan p = ready(s, kFwdTile, kFwdWaves, kFwdPerSimd, st);
+        const Plan p = ready(s, false, st);
         auto k = p.sharing ? scan_fwd_k<TI, TO, SIG, COUP, true> : scan_fwd_k<TI, TO, SIG, COUP, false>;
         hipLaunchKernelGGL(k, grid_of(p), dim3(kFwdWaves * 64), 0, st, s, p.groups);
     });
@@ -632,7 +649,7 @@ hipError_t scan_backward(const ScanArgs &s, hipStream_t st) {
             hipLaunchKernelGGL((scan_few_bwd_k<TI, TO, SIG, COUP>), dim3(ceil_div(s.dim, 256), s.n_batch), dim3(256), 0, st, s);
             return;
         }
-        const Plan p = ready(s, kBwdTile, kBwdWaves, kBwdPerSimd, st);
+        const Plan p = ready(s, true, st);
         auto k = p.sharing ? scan_bwd_k<TI, TO, SIG, COUP, true> : scan_bwd_k<TI, TO, SIG, COUP, false>;
         hipLaunchKernelGGL(k, grid_of(p), dim3(kBwdWaves * 64), 0, st, s, p.groups);
     });
