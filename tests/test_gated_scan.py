@@ -291,6 +291,34 @@ def test_what_is_not_finite_stays_in_its_channel():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("types", ["ff", "bb"])
+def test_a_nan_whose_bits_are_all_ones(types):
+    """The word that a split call's tiles hold before they are published is such a NaN; one among the values is passed
+    on as another."""
+    note(f"scan of a NaN of ones {types}")
+    n, d = 1500, 66
+    c = Call(1, n, d, types)
+    c.run()
+    good = c.read()
+    word = np.uint16 if c.bin else np.uint32
+    for k, row, ch in (("x", 200, 3), ("g", 700, 4), ("dh", 900, 5)):
+        buf = getattr(c, k)
+        bits = buf.to_numpy(word).reshape(n, d)
+        bits[row, ch] = np.iinfo(word).max
+        buf.upload(bits)
+    h0 = c.h0.to_numpy(np.uint32)
+    h0[6] = 0xFFFFFFFF
+    c.h0.upload(h0)
+    c.run()
+    got = c.read()
+    rest = np.setdiff1d(np.arange(d), [3, 4, 5, 6])
+    for k in got:
+        assert np.array_equal(got[k][..., rest], good[k][..., rest]), k
+    assert np.isnan(got["h"][0, 200:, 3]).all() and np.isnan(got["h"][0, 700:, 4]).all() and np.isnan(got["h"][0, :, 6]).all()
+    assert np.isnan(got["dx"][0, :901, 5]).all() and np.isnan(got["last"][0, [3, 4, 6]]).all()
+
+
+@pytest.mark.gpu
 def test_no_rows():
     """The states go through."""
     c = Call(2, 1, 70)
@@ -373,6 +401,29 @@ def test_the_same_every_time_on_two_streams_and_replayed(b, n, d, lens):
 
         shrink()
         _replays(lib(), st[0], lambda: c.run(st[0], **kw), check, between)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types,b,n,d,lens", [("bb", 1, 4000, 192, None), ("ff", 2, 1001, 130, [1001, 400]), ("fb", 3, 640, 64, [640, 0, 513])])
+def test_split_and_whole_sequences_give_the_same_bits(types, b, n, d, lens):
+    """A call on a captured stream without a workspace takes each sequence in one block."""
+    from test_gpu_kernels import _replays
+    from valkyr_amd import lib
+    from valkyr_amd.device import Stream, synchronize
+
+    note(f"scan split and whole {types} {b} {n} {d}")
+    c, st = Call(b, n, d, types, coupled=True, lens=lens), Stream()
+    assert c.K.gated_scan_workspace_bytes(c.p) > 0
+    synchronize()
+    c.run(st)
+    want = c.read()
+    c.check(want)
+
+    def check():
+        got = c.read()
+        assert all(np.array_equal(got[k], want[k]) for k in want)
+
+    _replays(lib(), st, lambda: c.run(st), check, lambda: None)
 
 
 @pytest.mark.gpu

@@ -348,7 +348,9 @@ __global__ __launch_bounds__(kFwdWaves * 64, kPerSimd) void scan_fwd_k(ScanArgs 
         }
         if (SPLIT) {
             if (w == 0) {
+                __builtin_amdgcn_s_setprio(3);  // (others wait for it: 1 % of a long scan)
                 look_back(W, (size_t)line * tiles * 64, at, lane, ta, tb, H);
+                __builtin_amdgcn_s_setprio(0);
                 shH[lane] = H;
             }
             __syncthreads();
@@ -462,7 +464,9 @@ __global__ __launch_bounds__(kBwdWaves * 64, kPerSimd) void scan_bwd_k(ScanArgs 
             if (j < w) h = fmaf(A[j][lane], h, B[j][lane]);
         if (SPLIT) {
             if (w == 0) {
+                __builtin_amdgcn_s_setprio(3);
                 look_back(W, (size_t)line * tiles * 64, at, lane, ta, tb, R);
+                __builtin_amdgcn_s_setprio(0);
                 shR[lane] = R;
             }
             __syncthreads();
