@@ -225,16 +225,18 @@ VKH_DEV void look_back(const Words &W, size_t base, int s, unsigned lane, float 
 // address wait for each other.)
 template <bool SPLIT>
 struct Tiles {
-    unsigned *ticket, *sh, next = 0;
+    unsigned *ticket, *sh, next = 0;  // sh: two, in turn, as a wave may still read one when the next is handed round
+    int turn = 0;
     VKH_DEV void fetch() {
         if (SPLIT && threadIdx.x == 0) next = atomicAdd(ticket, 1u);
     }
     VKH_DEV void hand_round() {  // ahead of a barrier
-        if (SPLIT && threadIdx.x == 0) *sh = next;
+        if (SPLIT && threadIdx.x == 0) sh[turn] = next;
     }
     VKH_DEV int take(int now) {  // behind it
         if (!SPLIT) return now + 1;
-        const int t = __builtin_amdgcn_readfirstlane(*sh);
+        const int t = __builtin_amdgcn_readfirstlane(sh[turn]);
+        turn ^= 1;
         fetch();
         return t;
     }
@@ -249,16 +251,16 @@ struct Tiles {
 
 // Both kernels: a tile's values are asked for as soon as the one before is in use, by the wave that looks back once it
 // has (a wave's loads return in order), so they arrive while that tile is joined and stored.  (Backward of 16384 x 4096
-// bf16: 208 us without, 185 with; the forward, 16 blocks' loads deep already, 113 and 111.)
+// bf16: 208 us without, 185 with; the forward 113 and 111.)
 //
 // 16384 x 4096 bf16 (0.40 and 0.67 GB): forward 105 us, 3.8 TB/s, backward 179, 3.75, and 6 each to make the words
-// ready; fp32, 8192 rows (the same bytes): 81 and 130, 4.9 and 5.2.  Half the values of bf16 lie between it and HBM: about
-// 26 vector instructions each, and the joins.  16 sequences of 1024 rows, a block each: 90 and 162.
+// ready; fp32, 8192 rows (the same bytes): 81 and 130, 4.9 and 5.2.  What keeps bf16, of twice the values, from HBM's
+// rate: 26 and 46 vector instructions for each, and the joins.  16 sequences of 1024 rows, a block each: 90 and 162.
 template <class TI, class TO, bool SIG, bool COUP, bool SPLIT>
 __global__ __launch_bounds__(kFwdWaves * 64, kPerSimd) void scan_fwd_k(ScanArgs s, int groups) {
     constexpr int R = kFwdRows;
     __shared__ float shA[2][kFwdWaves][64], shB[2][kFwdWaves][64], shH[64];
-    __shared__ unsigned ticket;
+    __shared__ unsigned ticket[2];
     const int lane = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int tiles = (s.n_pos + kFwdTile - 1) / kFwdTile;
     const long blk = SPLIT ? blockIdx.x % (groups * s.n_batch) : block_number();
@@ -268,7 +270,7 @@ __global__ __launch_bounds__(kFwdWaves * 64, kPerSimd) void scan_fwd_k(ScanArgs 
     const bool act = c < s.dim;
     const unsigned in_bytes = min(c, s.dim - 1) * sizeof(TI);  // (lanes past the channels: the last one)
     const Words W = words_of(s.ws, (size_t)s.n_batch * groups, (size_t)s.n_batch * groups * tiles * 64);
-    Tiles<SPLIT> order{(unsigned *)(W.tickets + (size_t)line * kTicketBytes), &ticket};
+    Tiles<SPLIT> order{(unsigned *)(W.tickets + (size_t)line * kTicketBytes), ticket};
     TI xr[R], gr[R];
     // FULL: all rows of the wave are in the sequence; else rows behind its end are the last one again
     auto load = [&](int t0, auto full) {
@@ -374,7 +376,7 @@ template <class TI, class TO, bool SIG, bool COUP, bool SPLIT>
 __global__ __launch_bounds__(kBwdWaves * 64, kPerSimd) void scan_bwd_k(ScanArgs s, int groups) {
     constexpr int N = kBwdRows;
     __shared__ float shA[2][kBwdWaves][64], shB[2][kBwdWaves][64], shQ[2][kBwdWaves][64], shR[64];
-    __shared__ unsigned ticket;
+    __shared__ unsigned ticket[2];
     const int lane = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int tiles = (s.n_pos + kBwdTile - 1) / kBwdTile;
     const long blk = SPLIT ? blockIdx.x % (groups * s.n_batch) : block_number();
@@ -384,7 +386,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, kPerSimd) void scan_bwd_k(ScanArgs 
     const bool act = c < s.dim;
     const unsigned in_bytes = min(c, s.dim - 1) * sizeof(TI);  // (lanes past the channels: the last one)
     const Words W = words_of(s.ws, (size_t)s.n_batch * groups, (size_t)s.n_batch * groups * tiles * 64);
-    Tiles<SPLIT> order{(unsigned *)(W.tickets + (size_t)line * kTicketBytes), &ticket};
+    Tiles<SPLIT> order{(unsigned *)(W.tickets + (size_t)line * kTicketBytes), ticket};
     TI xr[N], gr[N], dr[N];
     // (FULL: as in the forward)
     auto load = [&](int t0, auto full) {
