@@ -1671,10 +1671,12 @@ struct vkh_runner {
     }
 
     // A training step's forward, backward and Adam.  Clipping needs the norm of all gradients before the first is
-    // used: Adam then follows the whole backward in place of running beside it.
-    vkh_status train_enqueue() {
+    // used: Adam then follows the whole backward in place of running beside it.  With `loss` the loss is recorded
+    // as soon as the backward is done: a caller who waits for it does not wait for an Adam that follows.
+    vkh_status train_enqueue(bool loss) {
         const bool clip = clip_norm > 0.f;
         VKH_TRY(forward_backward_enqueue(!clip));
+        if (loss) VKH_TRY(record_loss());
         if (clip) {
             const GradTensor g{G, G, te - tb, DType::F32};  // (what lies between the tensors is zero)
             VKH_HIP(grad_clip(&g, 1, true, clip_norm, grad_norm_d, clip_ws, cur));
@@ -1686,9 +1688,12 @@ struct vkh_runner {
     }
 
     vkh_status step_enqueue(bool with_adam) {
-        VKH_TRY(with_adam ? train_enqueue() : forward_backward_enqueue(false));
-        VKH_TRY(record_loss());
-        if (with_adam) step_t += 1;  // transformer.zig:1318
+        if (!with_adam) {
+            VKH_TRY(forward_backward_enqueue(false));
+            return record_loss();
+        }
+        VKH_TRY(train_enqueue(true));
+        step_t += 1;  // transformer.zig:1318
         return VKH_OK;
     }
 };
@@ -2259,7 +2264,7 @@ vkh_status vkh_runner_tick_frame_train(vkh_runner *r, vkh_stream stream,
     vkh_status st = VKH_OK;
     uint32_t n = 0;
     while (should_train && n < max_steps) {
-        st = r->train_enqueue();
+        st = r->train_enqueue(false);
         if (st != VKH_OK) break;
         r->step_t += 1;
         ++n;
