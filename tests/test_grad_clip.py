@@ -240,3 +240,52 @@ def test_tensors_far_from_each_other(n):
         check(lib().vkh_memcpy_d2h(got.ctypes.data, big.offset(o), got.nbytes))
         ref = v.astype(np.float64) * (1.5 / want)
         assert np.all(np.abs(got - ref) <= 1.01 * U * np.abs(ref) + 2e-45)
+
+
+@pytest.mark.gpu
+def test_a_norm_does_not_depend_on_where_the_tensors_lie():
+    """200 tensors of 64 chunks (8192 values), each list of the same values at three places: all tensors one behind the
+    other, one of them 9 GiB behind the rest, and outputs that far from each other.
+
+    A chunk that holds 2^24, 2^12, 2^12 and 1, whose squares add up to m^2, m = 2^24 + 1, is followed by one whose eight
+    values at one lane's first place have squares of 0.029 and are all that lane adds to the 2^48 there if one block
+    takes both chunks: each is under half a step of 2^48 in 64 bits (2^-5), so the norm is m, halfway between two fp32
+    numbers, and rounds to 2^24.  Where two blocks take them, the second's sum (0.23) counts and the norm rounds to
+    2^24 + 2.  Which blocks take them follows from the sizes alone, so the three places give the same bits."""
+    from valkyr_amd import kernels as K
+    from valkyr_amd._lib import check, lib
+    from valkyr_amd.device import DeviceBuffer
+
+    note("norm of near and far tensors")
+    chunk, chunks, n, far = 8192, 64, 200, 9 << 30
+    size = chunk * chunks
+    whole, apart = DeviceBuffer.zeros(n * size * 4), DeviceBuffer(far + n * size * 4)
+    norm = dev(np.zeros(1, np.float32))
+    near = [(whole.offset(i * size * 4), size, K.F32) for i in range(n)]
+    moved = 100
+    check(lib().vkh_memset(apart.offset(far), 0, size * 4))
+    distant = list(near)
+    distant[moved] = (apart.offset(far), size, K.F32)
+    outs = [(g, k, t, apart.offset(i * size * 4 + (far if i % 2 else 0))) for i, (g, k, t) in enumerate(near)]
+    lists = [K.grad_list(v) for v in (near, distant, outs)]
+    big, small, none = (np.zeros(chunk, np.float32) for _ in range(3))
+    big[:4] = 2.0**24, 2.0**12, 2.0**12, 1.0
+    small[::1024] = 0.17
+    seen = set()
+    for at in range(64 * 3 + 5, 64 * n - 1, 197):
+        if at % 64 == 63 or at // 64 == moved:  # (both chunks in one tensor)
+            continue
+        check(lib().vkh_memcpy_h2d(whole.offset(at * chunk * 4), big.ctypes.data, big.nbytes))
+        check(lib().vkh_memcpy_h2d(whole.offset((at + 1) * chunk * 4), small.ctypes.data, small.nbytes))
+        got = []
+        for lst in lists[:2]:
+            K.grad_norm(lst, norm)
+            got.append(float(host(norm)[0]))
+        for lst in lists[2:]:
+            K.grad_clip(lst, 1e9, norm)
+            got.append(float(host(norm)[0]))
+        assert got == got[:1] * 3, (at, got)
+        seen.add(got[0])
+        for k in (at, at + 1):
+            check(lib().vkh_memcpy_h2d(whole.offset(k * chunk * 4), none.ctypes.data, none.nbytes))
+    assert seen == {2.0**24, 2.0**24 + 2}  # (both kinds of pairs were among them)

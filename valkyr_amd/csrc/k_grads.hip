@@ -4,8 +4,8 @@
 //
 // Squares are formed and summed in 64 bits: gradients near either end of fp32 neither overflow nor vanish, and
 // long sums lose nothing.  Two passes: the squares, one partial sum a block; then every block adds the partial
-// sums (in their order) and scales its part.  Which values a block takes follows from the sizes alone, so results
-// do not change from run to run.
+// sums (in their order) and scales its part.  Which values a block takes follows from the sizes of the list's tensors
+// alone, wherever they and their outputs lie, so results do not change from run to run.
 #include <algorithm>
 #include <type_traits>
 
@@ -16,19 +16,22 @@ namespace {
 
 constexpr int GNT = 256;
 constexpr int kChunk = 8192;    // values: a block's unit of work, of one tensor
-constexpr int kParts = 2048;    // partial sums of all launches, but for one more a launch
+constexpr int kParts = 2048;    // partial sums of all sections, but for one more a section
+// Tensors whose chunks are shared by blocks of their own: a launch takes two or three whole sections, as its table holds
+// by where the tensors lie, and the partial sums are the same in either case.
+constexpr int kSection = 90;
 
 // The tensors of one launch, an argument of the kernel.  Tensor i takes chunks first[i] .. first[i + 1], the last of them
-// of (tail & 0x7fff) + 1 values.  NEAR: addresses are 32-bit numbers of 2-byte units past the lowest one, so that a
-// launch holds more tensors (224 adapters in one launch a pass in place of two: 16 us, not 24); for gradients, and
-// outputs, within 8 GiB of each other.
+// of (tail & 0x7fff) + 1 values; section s has the blocks from block[s] on.  NEAR: addresses are 32-bit numbers of 2-byte
+// units past the lowest one, so that a launch holds more tensors (224 adapters in one launch a pass in place of two: 16
+// us, not 24); for gradients, and outputs, within 8 GiB of each other.
 template <bool NEAR>
 struct Table {
     static constexpr bool near = NEAR;
-    static constexpr int most = NEAR ? 276 : 180;
+    static constexpr int sections = NEAR ? 3 : 2, most = sections * kSection;
     typedef std::conditional_t<NEAR, unsigned, uintptr_t> At;
     int n;
-    unsigned chunks;
+    unsigned block[sections];
     uintptr_t g0, out0;
     At g[most], out[most];
     unsigned first[most + 1];
@@ -38,18 +41,27 @@ struct Table {
 };
 static_assert(sizeof(Table<true>) + 64 <= 4096 && sizeof(Table<false>) + 64 <= 4096, "kernel arguments");
 
-// The chunks of this block: an equal share, one after the other.
+// The chunks of this block: an equal share of its section's, one after the other.
 struct Share {
     unsigned c, end;
     int t;
 };
 template <bool NEAR>
 VKH_DEV Share share(const Table<NEAR> &T) {
-    const unsigned per = T.chunks / gridDim.x, more = T.chunks % gridDim.x, b = blockIdx.x;
+    int s0 = 0;
+    unsigned b0 = 0, b1 = gridDim.x;
+#pragma unroll
+    for (int i = 1; i < Table<NEAR>::sections; ++i) {  // (a section that the launch does not have: block[i] = gridDim.x)
+        if (blockIdx.x >= T.block[i]) s0 = i, b0 = T.block[i];
+        else b1 = min(b1, T.block[i]);
+    }
+    const int t0 = s0 * kSection, t1 = min(t0 + kSection, T.n);
+    const unsigned c0 = T.first[t0], chunks = T.first[t1] - c0, blocks = b1 - b0;
+    const unsigned per = chunks / blocks, more = chunks % blocks, b = blockIdx.x - b0;
     Share s;
-    s.c = b * per + (b < more ? b : more);
+    s.c = c0 + b * per + (b < more ? b : more);
     s.end = s.c + per + (b < more ? 1 : 0);
-    int lo = 0, hi = T.n - 1;  // the last tensor that starts at or before c
+    int lo = t0, hi = t1 - 1;  // the last tensor that starts at or before c
     while (lo < hi) {
         const int m = (lo + hi + 1) / 2;
         if (T.first[m] <= s.c) lo = m;
@@ -188,7 +200,7 @@ unsigned chunks_of(const GradTensor &t) { return (unsigned)((t.n + kChunk - 1) /
 
 }  // namespace
 
-size_t grad_ws_bytes(size_t n) { return (kParts + n / Table<false>::most + 1) * sizeof(double); }
+size_t grad_ws_bytes(size_t n) { return (kParts + n / kSection + 1) * sizeof(double); }
 
 hipError_t grad_clip(const GradTensor *t, size_t n, bool clip, float max_norm, float *norm, void *ws, hipStream_t st) {
     double *part = (double *)ws;
@@ -198,10 +210,10 @@ hipError_t grad_clip(const GradTensor *t, size_t n, bool clip, float max_norm, f
     // them, 1366 past them; 128 MB: 68 and 77).  Results always do (2.4 GB: 1448 through them; 128 MB: 86).
     const bool past = bytes > (256ull << 20);
     if (!total) return norm ? fill_f32(norm, 1, 0.f, st) : hipSuccess;
-    // f(table, blocks) for each launch: its share of kParts blocks, at most one a chunk
+    // f(table, blocks) for each launch of whole sections, each with its share of kParts blocks, at most one a chunk
     auto each = [&](auto f) {
         for (size_t i = 0; i < n;) {
-            // how many of the next tensors are near each other
+            // how many of the next tensors are near each other, in whole sections
             uintptr_t g0 = (uintptr_t)t[i].g, g1 = g0, o0 = (uintptr_t)t[i].out, o1 = o0;
             size_t near = i;
             for (; near < n && near - i < (size_t)Table<true>::most; ++near) {
@@ -212,20 +224,26 @@ hipError_t grad_clip(const GradTensor *t, size_t n, bool clip, float max_norm, f
             }
             auto go = [&](auto T, size_t end, uintptr_t gb, uintptr_t ob, unsigned unit) {
                 T.n = (int)(end - i);
-                T.chunks = 0;
                 T.g0 = gb;
                 T.out0 = ob;
-                for (int k = 0; i < end; ++i, ++k) {
-                    T.first[k] = T.chunks;
-                    T.tail[k] = (uint16_t)((t[i].n - 1) % kChunk | (t[i].dt == DType::BF16 ? 0x8000 : 0));
-                    T.g[k] = (typename decltype(T)::At)(((uintptr_t)t[i].g - gb) / unit);
-                    T.out[k] = (typename decltype(T)::At)(((uintptr_t)t[i].out - ob) / unit);
-                    T.chunks += chunks_of(t[i]);
+                unsigned c = 0, blocks = 0;
+                for (int s = 0; s < decltype(T)::sections; ++s) {
+                    T.block[s] = blocks;
+                    const unsigned c0 = c;
+                    for (int k = s * kSection; k < (s + 1) * kSection && i < end; ++i, ++k) {
+                        T.first[k] = c;
+                        T.tail[k] = (uint16_t)((t[i].n - 1) % kChunk | (t[i].dt == DType::BF16 ? 0x8000 : 0));
+                        T.g[k] = (typename decltype(T)::At)(((uintptr_t)t[i].g - gb) / unit);
+                        T.out[k] = (typename decltype(T)::At)(((uintptr_t)t[i].out - ob) / unit);
+                        c += chunks_of(t[i]);
+                    }
+                    if (c > c0) blocks += (unsigned)std::min<size_t>(c - c0, (size_t)kParts * (c - c0) / total + 1);
                 }
-                T.first[T.n] = T.chunks;
-                f(T, (int)std::min<size_t>(T.chunks, (size_t)kParts * T.chunks / total + 1));
+                T.first[T.n] = c;
+                f(T, (int)blocks);
             };
             const size_t far = std::min(n, i + Table<false>::most);
+            if (near < n) near -= (near - i) % kSection;
             if (near >= far) go(Table<true>(), near, g0, o0, 2);
             else go(Table<false>(), far, 0, 0, 1);
         }
