@@ -338,3 +338,35 @@ def test_rows_past_two_to_the_31_bytes_and_past_a_launch(dim, rows):
             assert close(rows_at(at), ref, off, True), (name, at)
         rest = rows_at(rows // 3)
         assert np.all(rest == bf16_bits_to_f32(f32_to_bf16_bits(B)).astype(np.float64)) if name == "y" else not rest.any()
+
+
+@pytest.mark.gpu
+def test_more_wide_rows_than_threads_of_a_launch():
+    """2^22 + 3 bf16 rows of 8200 values, each a block of 1024 threads: more threads than one axis of a launch takes.
+    In place; rows at both ends and around 2^21 blocks hold numbers, the others zeros, whose result is the bias."""
+    from valkyr_amd import kernels as K
+    from valkyr_amd._lib import check, lib
+    from valkyr_amd.device import DeviceBuffer, bf16_bits_to_f32, f32_to_bf16_bits
+
+    rows, dim, n = (1 << 22) + 3, 8200, 4
+    row = dim * 2
+    note(f"layernorm of {rows} rows of {dim}")
+    x, rng = DeviceBuffer.zeros(rows * row), np.random.default_rng(10)
+    W, B = rng.uniform(0.5, 1.5, dim).astype(np.float32), rng.standard_normal(dim).astype(np.float32)
+    starts, vals = (0, (1 << 21) - 2, rows - n), []
+    for at in starts:
+        bits = f32_to_bf16_bits(rng.standard_normal((n, dim)).astype(np.float32))
+        check(lib().vkh_memcpy_h2d(x.offset(at * row), bits.ctypes.data, bits.nbytes))
+        vals.append(bf16_bits_to_f32(bits).astype(np.float64).reshape(n, dim))
+
+    def rows_at(at):
+        got = np.empty((n, dim), np.uint16)
+        check(lib().vkh_memcpy_d2h(got.ctypes.data, x.offset(at * row), got.nbytes))
+        return bf16_bits_to_f32(got).astype(np.float64).reshape(n, dim)
+
+    K.layernorm_forward(K.layernorm_params(rows, dim, 1e-5, 1, 1), x, dev(W), dev(B), x)
+    for at, X in zip(starts, vals):
+        ref, off = formulas(X, W.astype(np.float64), B.astype(np.float64), 1e-5)["y"]
+        assert close(rows_at(at), ref, off, True), at
+    for at in (4, rows // 3, rows - 2 * n):
+        assert np.all(rows_at(at) == bf16_bits_to_f32(f32_to_bf16_bits(B)).astype(np.float64)), at

@@ -104,13 +104,16 @@ VKH_DEV float block_sum(float v, float *sh) {
 
 inline unsigned ceil_div(size_t a, size_t b) { return (unsigned)((a + b - 1) / b); }
 
-// A grid of at least `blocks` blocks (up to 2^38) as block_number() counts them: a launch takes fewer than
-// 2^32 threads along x, so blocks past 2^22 go on along y.  The kernel leaves what is beyond the last one.
-inline dim3 long_grid(long blocks) {
-    const long x = blocks < (1l << 22) ? blocks : 1l << 22;
+// A grid of at least `blocks` blocks (up to 2^37) of `threads` threads as block_number<threads>() counts them: a launch
+// takes fewer than 2^32 threads along x, so blocks past 2^22 (of more than 512 threads: past 2^21) go on along y.
+// The kernel leaves what is beyond the last one.
+constexpr int blocks_along_x(int threads) { return threads > 512 ? 21 : 22; }  // their number's logarithm
+inline dim3 long_grid(long blocks, int threads = 512) {
+    const long most = 1l << blocks_along_x(threads), x = blocks < most ? blocks : most;
     return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
 }
-VKH_DEV long block_number() { return (long)blockIdx.y << 22 | blockIdx.x; }
+template <int THREADS = 512>
+VKH_DEV long block_number() { return (long)blockIdx.y << blocks_along_x(THREADS) | blockIdx.x; }
 
 // Causal grids with row 0 the heaviest: the block row of grid row y (of n)
 // when the whole grid is resident at once with two blocks per CU.  The first

@@ -152,7 +152,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void layernorm_fwd_held_k(Laye
     constexpr int BT = NT < 256 ? 256 : NT, W = 16 / (int)sizeof(TX), NI = kFwdHeld / W;
     __shared__ float2 sh[2][BT / 64];
     const int t = threadIdx.x % NT, dim = a.dim;
-    const long row = block_number() * (BT / NT) + __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
+    const long row = block_number<BT>() * (BT / NT) + __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
     const bool live = row < a.n_rows;
     Group<NT, BT, W, kFwdHeld> g(sh, threadIdx.x / NT, dim);
     typename Vec<TX, W>::type xr[NI];  // (all asked for before the first is used)
@@ -411,7 +411,7 @@ hipError_t layernorm_forward(const LayernormArgs &a, DType xt, DType yt, hipStre
             by_threads(threads_of(a.dim, kFwdHeld), [&](auto nt) {
                 constexpr int NT = decltype(nt)::value, BT = std::max(NT, 256), per = BT / NT;
                 auto k = a.dim % (16 / sizeof(X)) ? layernorm_fwd_held_k<X, Y, NT, true> : layernorm_fwd_held_k<X, Y, NT, false>;
-                hipLaunchKernelGGL(k, long_grid((a.n_rows + per - 1) / per), dim3(BT), 0, st, a);
+                hipLaunchKernelGGL(k, long_grid((a.n_rows + per - 1) / per, BT), dim3(BT), 0, st, a);
             });
         });
     });
