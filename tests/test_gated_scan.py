@@ -461,3 +461,48 @@ def test_rows_past_two_to_the_31_bytes():
         for k, buf in (("dx", out), ("dg", dg)):
             ref, off = w[k]
             assert np.all(np.abs(rows_at(buf, at) - ref) <= off + (U16 + U) * (np.abs(ref) + off) + 1e-37), (k, at)
+
+
+@pytest.mark.gpu
+def test_more_groups_than_threads_of_a_launch():
+    """65535 bf16 sequences of 17 rows and 65 groups of channels, over 2^22 groups in all, each a block of 1024 threads
+    in the backward: more threads than one axis of a launch takes.  Zeros (gates of 1/2) but for some sequences."""
+    from valkyr_amd import kernels as K
+    from valkyr_amd._lib import check, lib
+    from valkyr_amd.device import DeviceBuffer, bf16_bits_to_f32, f32_to_bf16_bits
+
+    b, n, d = 65535, 17, 64 * 64 + 1
+    note(f"scan of {b} x {n} x {d}")
+    rng, seq = np.random.default_rng(7), n * d * 2
+    x, g, c = (DeviceBuffer.zeros(b * seq) for _ in range(3))  # c: h, and then dh
+    some, vals = (0, 32262, 32264, 64526, 64528, b - 1), {}
+
+    def put(k, buf):
+        for i in some:
+            bits = f32_to_bf16_bits(rng.standard_normal((n, d)).astype(np.float32))
+            check(lib().vkh_memcpy_h2d(buf.offset(i * seq), bits.ctypes.data, bits.nbytes))
+            vals[k, i] = bf16_bits_to_f32(bits).astype(np.float64).reshape(1, n, d)
+
+    def at(buf, i):
+        got = np.empty((n, d), np.uint16)
+        check(lib().vkh_memcpy_d2h(got.ctypes.data, buf.offset(i * seq), got.nbytes))
+        return bf16_bits_to_f32(got).astype(np.float64).reshape(1, n, d)
+
+    put("x", x)
+    put("g", g)
+    p = K.scan_params(n, d, b, dtype=K.BF16)
+    states = DeviceBuffer.zeros(K.gated_scan_states_floats(p) * 4)
+    K.gated_scan_forward(p, x, g, c, states=states)
+    for i in some:
+        ref, off = formulas(vals["x", i], vals["g", i])["h"]
+        assert np.all(np.abs(at(c, i) - ref) <= off + (U16 + U) * (np.abs(ref) + off) + 1e-37), i
+        assert not at(c, min(i + 1, b - 2)).any()
+    c.fill_zero()
+    put("dh", c)
+    K.gated_scan_backward(p, x, g, states, c, c, g)
+    for i in some:
+        w = formulas(vals["x", i], vals["g", i], dh=vals["dh", i])
+        for k, buf in (("dx", c), ("dg", g)):
+            ref, off = w[k]
+            assert np.all(np.abs(at(buf, i) - ref) <= off + (U16 + U) * (np.abs(ref) + off) + 1e-37), (k, i)
+            assert not at(buf, min(i + 1, b - 2)).any()

@@ -263,7 +263,7 @@ __global__ __launch_bounds__(kFwdWaves * 64, kPerSimd) void scan_fwd_k(ScanArgs 
     __shared__ unsigned ticket[2];
     const int lane = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int tiles = (s.n_pos + kFwdTile - 1) / kFwdTile;
-    const long blk = SPLIT ? blockIdx.x % (groups * s.n_batch) : block_number();
+    const long blk = SPLIT ? blockIdx.x % (groups * s.n_batch) : block_number<kFwdWaves * 64>();
     if (blk >= groups * s.n_batch) return;
     const int line = __builtin_amdgcn_readfirstlane((int)blk), b = __builtin_amdgcn_readfirstlane(line / groups);
     const int c = (line - b * groups) * 64 + lane, len = __builtin_amdgcn_readfirstlane(rows_of(s, b));
@@ -379,7 +379,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, kPerSimd) void scan_bwd_k(ScanArgs 
     __shared__ unsigned ticket[2];
     const int lane = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int tiles = (s.n_pos + kBwdTile - 1) / kBwdTile;
-    const long blk = SPLIT ? blockIdx.x % (groups * s.n_batch) : block_number();
+    const long blk = SPLIT ? blockIdx.x % (groups * s.n_batch) : block_number<kBwdWaves * 64>();
     if (blk >= groups * s.n_batch) return;
     const int line = __builtin_amdgcn_readfirstlane((int)blk), b = __builtin_amdgcn_readfirstlane(line / groups);
     const int c = (line - b * groups) * 64 + lane, len = __builtin_amdgcn_readfirstlane(rows_of(s, b));
@@ -617,7 +617,7 @@ Plan ready(const ScanArgs &s, bool back, hipStream_t st) {
                            p.lines * kTicketBytes / 16, n);
     return p;
 }
-dim3 grid_of(const Plan &p) { return p.sharing ? dim3((unsigned)p.lines * p.sharing) : long_grid((long)p.lines); }
+dim3 grid_of(const Plan &p, int threads) { return p.sharing ? dim3((unsigned)p.lines * p.sharing) : long_grid((long)p.lines, threads); }
 
 }  // namespace
 
@@ -641,7 +641,7 @@ hipError_t scan_forward(const ScanArgs &s, hipStream_t st) {
         }
         const Plan p = ready(s, false, st);
         auto k = p.sharing ? scan_fwd_k<TI, TO, SIG, COUP, true> : scan_fwd_k<TI, TO, SIG, COUP, false>;
-        hipLaunchKernelGGL(k, grid_of(p), dim3(kFwdWaves * 64), 0, st, s, p.groups);
+        hipLaunchKernelGGL(k, grid_of(p, kFwdWaves * 64), dim3(kFwdWaves * 64), 0, st, s, p.groups);
     });
     return hipGetLastError();
 }
@@ -657,7 +657,7 @@ hipError_t scan_backward(const ScanArgs &s, hipStream_t st) {
         }
         const Plan p = ready(s, true, st);
         auto k = p.sharing ? scan_bwd_k<TI, TO, SIG, COUP, true> : scan_bwd_k<TI, TO, SIG, COUP, false>;
-        hipLaunchKernelGGL(k, grid_of(p), dim3(kBwdWaves * 64), 0, st, s, p.groups);
+        hipLaunchKernelGGL(k, grid_of(p, kBwdWaves * 64), dim3(kBwdWaves * 64), 0, st, s, p.groups);
     });
     return hipGetLastError();
 }
