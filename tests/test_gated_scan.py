@@ -464,6 +464,86 @@ def test_rows_past_two_to_the_31_bytes():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("types", ["ff", "bb"])
+@pytest.mark.parametrize("n", [1, 5, 16])
+@pytest.mark.parametrize("d", [64, 65])
+def test_a_few_rows_in_place(n, d, types):
+    """Sequences of up to 16 rows, one of them with fewer: states over each other, h over x or g, dx and dg over the
+    inputs give the bits of a call with places of its own."""
+    note(f"scan of a few rows in place {n} {d} {types}")
+    bf, shape = types == "bb", (3, n, d)
+    for sig, coupled, lens in ((True, True, None), (False, False, [n, n // 2, 0])):
+        make = lambda: Call(3, n, d, types, sig, coupled, lens=lens)  # noqa: E731
+        c = make()
+        c.run()
+        want = c.read()
+        c.check(want)
+        c = make()
+        c.K.gated_scan_forward(c.p, c.x, c.g, c.out["h"], c.h0, c.h0, c.states, c.length)
+        c.K.gated_scan_backward(c.p, c.x, c.g, c.states, c.dh, c.out["dx"], c.out["dg"], c.dl, c.dl, c.length)
+        c.out.update(last=c.h0, dh0=c.dl)
+        assert all(np.array_equal(v, want[k]) for k, v in c.read().items())
+        for over in ("x", "g"):
+            c = make()
+            c.K.gated_scan_forward(c.p, c.x, c.g, getattr(c, over), c.h0, length=c.length)
+            assert np.array_equal(down(getattr(c, over), shape, bf), want["h"])
+        for dx, dg in (("x", "g"), ("dh", "x"), ("g", "dh"), ("x", "dh"), ("dh", "g"), ("g", "x")):
+            c = make()
+            c.forward()
+            c.K.gated_scan_backward(c.p, c.x, c.g, c.states, c.dh, getattr(c, dx), getattr(c, dg), c.dl, length=c.length)
+            assert np.array_equal(down(getattr(c, dx), shape, bf), want["dx"])
+            assert np.array_equal(down(getattr(c, dg), shape, bf), want["dg"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sig", [True, False])
+@pytest.mark.parametrize("coupled", [True, False])
+@pytest.mark.parametrize("types,b,n,d,lens", [("bb", 1, 2500, 130, None), ("ff", 2, 900, 64, [900, 515])])
+def test_split_and_whole_sequences_give_the_same_bits_for_every_gate(types, b, n, d, lens, sig, coupled):
+    same_bits_whole(Call(b, n, d, types, sig, coupled, lens=lens), True)
+
+
+def same_bits_whole(c, split, want=None):
+    """A call, against 64 bits, and the same one on a captured stream without a workspace, where each sequence is one
+    block's: the same bits."""
+    from test_gpu_kernels import _replays
+    from valkyr_amd import lib
+    from valkyr_amd.device import Stream, synchronize
+
+    st = Stream()
+    if split is not None:
+        assert (c.K.gated_scan_workspace_bytes(c.p) > 0) == split
+    synchronize()
+    c.run(st)
+    got = c.read()
+    c.check(got, want)
+
+    def check():
+        now = c.read()
+        assert all(np.array_equal(now[k], got[k]) for k in got)
+
+    def clear():
+        for buf in c.out.values():
+            buf.upload(np.full(buf.nbytes // 2, 0x40E0, np.uint16))  # (7 in bf16)
+
+    clear()
+    _replays(lib(), st, lambda: c.run(st), check, clear, 2)
+
+
+# 64-channel groups of all sequences: where a sequence's tiles stop being shared between blocks (256 blocks
+# are resident in the backward, 512 in the forward), and more groups than there are blocks
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", ["ff", "bb"])
+@pytest.mark.parametrize("b,groups,lens", [(2, 64, None), (3, 43, [400, 31, 300]), (4, 40, None), (1, 256, None), (1, 257, None), (5, 64, [400, 0, 399, 129, 128]),
+                                           (10, 60, None)])
+def test_groups_around_the_blocks_that_are_resident(b, groups, lens, types):
+    n = 400
+    d = 64 * groups - (7 if groups % 2 else 0)
+    note(f"scan of {b * groups} groups {types} {lens}")
+    same_bits_whole(Call(b, n, d, types, coupled=b % 2 == 0, lens=lens), None)
+
+
+@pytest.mark.gpu
 def test_more_groups_than_threads_of_a_launch():
     """65535 bf16 sequences of 17 rows and 65 groups of channels, over 2^22 groups in all, each a block of 1024 threads
     in the backward: more threads than one axis of a launch takes.  Zeros (gates of 1/2) but for some sequences."""
@@ -506,3 +586,47 @@ def test_more_groups_than_threads_of_a_launch():
             ref, off = w[k]
             assert np.all(np.abs(at(buf, i) - ref) <= off + (U16 + U) * (np.abs(ref) + off) + 1e-37), (k, i)
             assert not at(buf, min(i + 1, b - 2)).any()
+
+
+@pytest.mark.gpu
+def test_a_sequence_whose_words_would_be_too_many():
+    """128 groups of a sequence of 1.3 million rows: the words of its tiles would take a GB, so it stays whole.  Zeros
+    (gates of 1/2) but for its first rows and its last."""
+    from valkyr_amd import kernels as K
+    from valkyr_amd._lib import check, lib
+    from valkyr_amd.device import DeviceBuffer, bf16_bits_to_f32, f32_to_bf16_bits
+
+    n, d, m = 128 * 10240 + 77, 64 * 128, 40
+    note(f"scan of {n} x {d}")
+    p = K.scan_params(n, d, dtype=K.BF16)
+    assert K.gated_scan_workspace_bytes(p) == 0 and K.gated_scan_workspace_bytes(K.scan_params(n // 2, d, dtype=K.BF16)) > 0
+    rng, row = np.random.default_rng(8), d * 2
+    x, g, c = (DeviceBuffer.zeros(n * row) for _ in range(3))  # c: h, and then dh
+    vals = {}
+
+    def put(k, buf):
+        for at in (0, n - m):
+            bits = f32_to_bf16_bits(rng.standard_normal((m, d)).astype(np.float32))
+            check(lib().vkh_memcpy_h2d(buf.offset(at * row), bits.ctypes.data, bits.nbytes))
+            vals[k, at] = bf16_bits_to_f32(bits).astype(np.float64).reshape(1, m, d)
+
+    def rows_at(buf, at):
+        got = np.empty((m, d), np.uint16)
+        check(lib().vkh_memcpy_d2h(got.ctypes.data, buf.offset(at * row), got.nbytes))
+        return bf16_bits_to_f32(got).astype(np.float64).reshape(1, m, d)
+
+    put("x", x)
+    put("g", g)
+    states = DeviceBuffer.zeros(K.gated_scan_states_floats(p) * 4)
+    K.gated_scan_forward(p, x, g, c, states=states)
+    for at in (0, n - m):  # (gates of 1/2 between them: nothing is left of the state)
+        ref, off = formulas(vals["x", at], vals["g", at])["h"]
+        assert np.all(np.abs(rows_at(c, at) - ref) <= off + (U16 + U) * (np.abs(ref) + off) + 1e-37), at
+    c.fill_zero()
+    put("dh", c)
+    K.gated_scan_backward(p, x, g, states, c, c, g)
+    for at in (0, n - m):
+        w = formulas(vals["x", at], vals["g", at], dh=vals["dh", at])
+        for k, buf in (("dx", c), ("dg", g)):
+            ref, off = w[k]
+            assert np.all(np.abs(rows_at(buf, at) - ref) <= off + (U16 + U) * (np.abs(ref) + off) + 1e-37), (k, at)

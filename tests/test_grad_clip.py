@@ -289,3 +289,70 @@ def test_a_norm_does_not_depend_on_where_the_tensors_lie():
         for k in (at, at + 1):
             check(lib().vkh_memcpy_h2d(whole.offset(k * chunk * 4), none.ctypes.data, none.nbytes))
     assert seen == {2.0**24, 2.0**24 + 2}  # (both kinds of pairs were among them)
+
+
+class Spread:
+    """Tensors at given places of a stretch of memory, outputs at the same places of another."""
+
+    def __init__(self, places, span, seed):
+        from valkyr_amd import kernels as K
+        from valkyr_amd._lib import check, lib
+        from valkyr_amd.device import DeviceBuffer, bf16_bits_to_f32, f32_to_bf16_bits
+
+        self.K, self.lib, self.check, self.places = K, lib(), check, places
+        self.src, self.out = DeviceBuffer(span), DeviceBuffer(span)
+        rng, self.val = np.random.default_rng(seed), []
+        for at, n, t in places:
+            v = rng.standard_normal(n, dtype=np.float32)
+            raw = f32_to_bf16_bits(v) if t else v
+            check(self.lib.vkh_memcpy_h2d(self.src.offset(at), raw.ctypes.data, raw.nbytes))
+            self.val.append((bf16_bits_to_f32(raw) if t else v).astype(np.float64))
+        self.norm = dev(np.zeros(1, np.float32))
+        self.want = math.sqrt(sum(float((v ** 2).sum()) for v in self.val))
+
+    def clip(self, limit, inplace):
+        self.K.grad_clip(self.K.grad_list([(self.src.offset(at), n, t) + (() if inplace else (self.out.offset(at),))
+                                           for at, n, t in self.places]), limit, self.norm)
+        assert abs(float(host(self.norm)[0]) - self.want) <= 1.0001 * U * self.want
+        return self.src if inplace else self.out
+
+    def check_scaled(self, buf, c):
+        from valkyr_amd.device import bf16_bits_to_f32
+
+        for (at, n, t), v in zip(self.places, self.val):
+            got = np.empty(n, np.uint16 if t else np.float32)
+            self.check(self.lib.vkh_memcpy_d2h(got.ctypes.data, buf.offset(at), got.nbytes))
+            ref = v * c
+            off = np.abs(ref) * (U16 + 1.01 * U if t else 1.01 * U) + (1e-40 if t else 2e-45)
+            assert np.all(np.abs((bf16_bits_to_f32(got) if t else got) - ref) <= off), (at, n, t)
+
+
+@pytest.mark.gpu
+def test_more_than_the_last_cache_holds_in_both_types():
+    """410 MB at odd places, which are read past the caches, with whole chunks and rests of each type."""
+    note("clip of 410 MB, both types")
+    sizes, places, at = [(50000001, 1), (3, 0), (40000011, 0), (8192, 1), (12345, 0), (70000000, 1), (1, 1), (2 * 8192 + 5, 0)], [], 4
+    for n, t in sizes:
+        at += 2 if t else -at % 4
+        places.append((at, n, t))
+        at += n * (2 if t else 4) + 2
+    assert sum(n * (2 if t else 4) for n, t in sizes) > 256 << 20
+    g = Spread(places, at, 11)
+    limit = float(np.float32(g.want / 3))
+    g.check_scaled(g.clip(limit, False), limit / g.want)
+    g.check_scaled(g.clip(limit, True), limit / g.want)
+
+
+@pytest.mark.gpu
+def test_both_types_far_from_each_other():
+    """Tensors of both types in turn 9 GiB behind each other, more of them than one launch takes."""
+    note("clip of both types, 9 GiB apart")
+    far, places = 9 << 30, []
+    for i in range(230):
+        n = 1 + (53 * i) % 9001
+        places.append(((i % 3 % 2) * far + i * 40000 + 4 * (i % 7) + 2 * (i % 2), n, i % 2))
+    places = [(at - at % (2 if t else 4), n, t) for at, n, t in places]
+    g = Spread(places, far + 230 * 40000 + 40000, 12)
+    limit = float(np.float32(g.want / 5))
+    g.check_scaled(g.clip(limit, False), limit / g.want)
+    g.check_scaled(g.clip(limit, True), limit / g.want)

@@ -341,6 +341,25 @@ def test_rows_past_two_to_the_31_bytes_and_past_a_launch(dim, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("types", ["ffff", "bbbb"])
+@pytest.mark.parametrize("rows,dim", [(700, 5000), (600, 8200), (515, 16384), (530, 16400), (450, 40001)])
+def test_more_wide_rows_than_blocks(rows, dim, types):
+    """Rows of which a block takes several in turn, the last of them not by every block: up to 256 blocks for these
+    widths up to 16384, min(512, 2^23 / dim) beyond them.  A gain's gradient then adds at most 3 rows one after the other and
+    up to 256 / 16 + 16 (512 / 16 + 16) partial sums, within what formulas() allows.  The same bits each time."""
+    note(f"layernorm of many wide rows {rows} x {dim} {types}")
+    c = Call(rows, dim, types, res=True, pad=dim % 2)
+    c.run()
+    got = c.read()
+    c.check(got)
+    for n in ("dw", "db"):
+        getattr(c, n).upload(np.full(dim, 7.0, np.float32))
+    c.run()
+    again = c.read()
+    assert all(np.array_equal(again[n], got[n]) for n in got)
+
+
+@pytest.mark.gpu
 def test_more_wide_rows_than_threads_of_a_launch():
     """2^22 + 3 bf16 rows of 8200 values, each a block of 1024 threads: more threads than one axis of a launch takes.
     In place; rows at both ends and around 2^21 blocks hold numbers, the others zeros, whose result is the bias."""
