@@ -82,17 +82,14 @@ VKH_DEV double block_sum64(double v, double *sh) {
 
 // 16 bytes of a tensor, which may start at any of its values: two neighbouring lines at most take a lane's load, and
 // the lanes of a wave whole lines but for the first and last.
-typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
-typedef bf16 bf16x8u __attribute__((ext_vector_type(8), aligned(2)));
-template <class T> struct Vec;
-template <> struct Vec<float> { typedef f32x4u type; };
-template <> struct Vec<bf16> { typedef bf16x8u type; };
+template <class T>
+using Bytes16 = typename Vec<T, 16 / (int)sizeof(T)>::type;
 
 // f(vector of U at i) over the chunk's n values, 16 bytes a lane and 32 KiB under way, and f1(value) behind the last
 // whole vector.
 template <bool PAST, class T, class F, class F1>
 VKH_DEV void over_chunk(const T *g, int n, F f, F1 f1) {
-    typedef typename Vec<T>::type V;
+    typedef Bytes16<T> V;
     constexpr int W = 16 / sizeof(T), U = kChunk / W / GNT;
     if (n == kChunk) {
         V v[U];
@@ -122,7 +119,7 @@ VKH_DEV void squares_of(const T *g, int n, double (&s)[4]) {
     constexpr int W = 16 / sizeof(T);
     over_chunk<PAST>(
         g, n,
-        [&](int, typename Vec<T>::type v) {
+        [&](int, Bytes16<T> v) {
 #pragma unroll
             for (int i = 0; i < W; ++i) {
                 const double d = (float)v[i];
@@ -166,7 +163,7 @@ __global__ __launch_bounds__(GNT) void grad_norm_k(const double *part, int n_par
 // (scaled = false: the bits as they are)
 template <bool PAST, class T>
 VKH_DEV void scale_of(const T *g, T *out, int n, bool scaled, double c) {
-    typedef typename Vec<T>::type V;
+    typedef Bytes16<T> V;
     auto one = [&](T v) { return scaled ? (T)(float)((double)(float)v * c) : v; };
     over_chunk<PAST>(
         g, n,

@@ -23,17 +23,6 @@ constexpr int kFwdHeld = 16, kBwdHeld = 8;  // values of a row in a lane (the ba
 constexpr int kWide = 16384;  // the longest row that is held
 constexpr int LNT = 256;           // threads on a longer one
 
-template <class F>
-void by_type(DType d, F f) {
-    if (d == DType::F32) f(float{});
-    else f(bf16{});
-}
-
-// W values from any address of T
-template <class T, int W> struct Vec;
-template <int W> struct Vec<float, W> { typedef float type __attribute__((ext_vector_type(W), aligned(4))); };
-template <int W> struct Vec<bf16, W> { typedef bf16 type __attribute__((ext_vector_type(W), aligned(2))); };
-
 // The sum over a wave, in its lanes' order by halves of 16 and then row by row.
 VKH_DEV float lanes_sum(float v) {
     v = row16_sum(v);

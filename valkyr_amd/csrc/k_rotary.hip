@@ -483,12 +483,6 @@ int lanes(int hd, int V) {
     return l;
 }
 
-template <class F>
-void by_type(DType d, F f) {
-    if (d == DType::F32) f(float{});
-    else f(bf16{});
-}
-
 }  // namespace
 
 // Blocks of each side: five a CU in all (as many as fit at 4-value chunks), shared by the sides'

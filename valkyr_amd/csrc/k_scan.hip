@@ -46,16 +46,7 @@ constexpr uint32_t kUnset = 0xffffffffu;
 // 30 and 66 in tiles; 8 of them, 10 and 9, in tiles 8 and 10.
 constexpr int kFew = 16;
 
-template <class F>
-void by_type(DType d, F f) {
-    if (d == DType::F32) f(float{});
-    else f(bf16{});
-}
-
 // V values from any address of T
-template <class T, int V> struct Vec;
-template <int V> struct Vec<float, V> { typedef float type __attribute__((ext_vector_type(V), aligned(4))); };
-template <int V> struct Vec<bf16, V> { typedef bf16 type __attribute__((ext_vector_type(V), aligned(2))); };
 template <class T, int V>
 using Raw = std::conditional_t<V == 1, T, typename Vec<T, V>::type>;
 

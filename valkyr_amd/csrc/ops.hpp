@@ -11,6 +11,18 @@ namespace vkh {
 enum class DType : int { F32 = 0, BF16 = 1 };
 enum class Precision : int { FP32 = 0, BF16 = 1 };
 
+// f(a value of the type d)
+template <class F>
+void by_type(DType d, F f) {
+    if (d == DType::F32) f(float{});
+    else f(bf16{});
+}
+
+// W values at any address of T
+template <class T, int W> struct Vec;
+template <int W> struct Vec<float, W> { typedef float type __attribute__((ext_vector_type(W), aligned(4))); };
+template <int W> struct Vec<bf16, W> { typedef bf16 type __attribute__((ext_vector_type(W), aligned(2))); };
+
 struct Mat {
     const void *p;
     long ld;
