@@ -208,10 +208,11 @@ vkh_status vkh_runner_set_step_t(vkh_runner *r, uint32_t step_t);
 float vkh_runner_get_lr(const vkh_runner *r);
 vkh_status vkh_runner_set_lr(vkh_runner *r, float lr); /* cfg.lr is mutable between steps */
 /* Clipping by the norm of all trainable gradients (vkh_grad_clip) in every later step, ahead of Adam: 0, as at the
- * start, for none.  The gradients that vkh_runner_get_tensor then reads behind a step are the clipped ones; a step whose
- * norm is not finite is not clipped.  The reference has no clipping. */
+ * start, for none.  The gradients that vkh_runner_get_tensor then reads behind a step are the clipped ones; a step with
+ * gradients that are not finite is not clipped.  The reference has no clipping. */
 vkh_status vkh_runner_set_grad_clip(vkh_runner *r, float max_norm);
-/* The gradients' norm in the last step with clipping, before it was clipped (waits for the step). */
+/* The gradients' norm in the last step with clipping, before it was clipped (waits for the step); infinity for one past
+ * fp32's range. */
 vkh_status vkh_runner_last_grad_norm(vkh_runner *r, float *norm);
 vkh_status vkh_runner_get_config(const vkh_runner *r, vkh_config *out);
 size_t vkh_runner_param_count(const vkh_runner *r);          /* trainable params */
@@ -919,7 +920,8 @@ typedef struct vkh_grad {
     uint32_t dtype; /* vkh_dtype */
     void *out;      /* vkh_grad_clip: where the clipped gradient goes; NULL: in place */
 } vkh_grad;
-/* norm[0] (fp32) = the root of the sum of all squares, summed in 64 bits in a fixed order.  `grads`
+/* norm[0] (fp32) = the root of the sum of all squares, summed in 64 bits in an order that follows from the
+ * tensors' sizes alone.  `grads`
  * is a host array, read before the call returns.  `workspace` (16-byte aligned) holds
  * vkh_grad_clip_workspace_bytes(n_grads) bytes; NULL takes the library's per-stream scratch, which
  * a call on a stream under capture may not (VKH_ERR_INVALID_ARGUMENT). */
@@ -927,8 +929,10 @@ size_t vkh_grad_clip_workspace_bytes(size_t n_grads);
 vkh_status vkh_grad_norm(const vkh_grad *grads, size_t n_grads, float *norm, void *workspace,
                          vkh_stream stream);
 /* The same norm (norm may be NULL), and every gradient times max_norm / norm where the norm is over
- * max_norm (at least 0) and finite; elsewhere they stay as they are, so a caller finds a step that overflowed in
- * its norm.  No output may overlap another tensor of the list (VKH_ERR_INVALID_ARGUMENT). */
+ * max_norm (at least 0) and finite; elsewhere they stay as they are.  That norm is the 64-bit one, which is
+ * finite as long as every gradient is: a step that overflowed keeps its gradients and has a norm[0] of NaN or
+ * infinity, but finite gradients whose norm is past fp32's range are clipped, and norm[0] is infinity.
+ * No output may overlap another tensor of the list (VKH_ERR_INVALID_ARGUMENT). */
 vkh_status vkh_grad_clip(const vkh_grad *grads, size_t n_grads, float max_norm, float *norm,
                          void *workspace, vkh_stream stream);
 /* shaders/add_in_place.comp, vec_add.comp, scale.comp */

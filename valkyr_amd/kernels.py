@@ -310,7 +310,8 @@ def grad_norm(grads, norm, workspace=None, stream=None):
 
 
 def grad_clip(grads, max_norm, norm=None, workspace=None, stream=None):
-    """Every gradient scaled by max_norm / norm where the norm of all is over max_norm and finite."""
+    """Every gradient scaled by max_norm / norm where the norm of all is over max_norm and finite (in 64 bits: wherever
+    the gradients are; norm is infinity past fp32's range)."""
     check(lib().vkh_grad_clip(grads, len(grads), max_norm, _p(norm), _p(workspace), _s(stream)))
 
 
