@@ -42,8 +42,8 @@ constexpr int kFold = 4;     // waves whose A and B are read at a time
 constexpr int kLook = 4;     // tiles looked back over at a time (one: a forward of 131 us beside 118; eight: 114 beside 113)
 constexpr size_t kMostChannels = 80l << 20;  // of a split call's words (12 bytes each)
 constexpr uint32_t kUnset = 0xffffffffu;
-// Rows of a sequence that a thread takes alone.  64 sequences of 16 rows of 4096 bf16, forward and backward: 14 and 17 us,
-// 30 and 66 in tiles; 8 of them, 10 and 9, in tiles 8 and 10.
+// Rows of a sequence that a thread takes alone.  64 sequences of 16 rows of 4096 bf16, forward and backward, their inputs
+// in the last cache: 14 and 17 us (22 and 25 where they are not), 30 and 66 in tiles; 8 of them, 10 and 9, in tiles 8 and 10.
 constexpr int kFew = 16;
 
 // V values from any address of T
@@ -98,7 +98,8 @@ VKH_DEV Raw<T, V> raw_of(const float (&o)[V]) {
 }
 template <class T, int V>
 VKH_DEV void store_v(T *p, const float (&o)[V]) { *reinterpret_cast<Raw<T, V> *>(p) = raw_of<T, V>(o); }
-// a and 1 - a of a gate, each to its own last digits: e = exp(-|g|), 1 / (1 + e) and e / (1 + e).  The exponential takes
+// a and 1 - a of a gate, each to its own last digits (the smaller one may be 0 past |g| = 87, where it would be less than
+// fp32's normal numbers): e = exp(-|g|), 1 / (1 + e) and e / (1 + e).  The exponential takes
 // its product with 1 / ln 2 in two parts (one alone is off by |g| steps): exact with the first 16 bits of it for a
 // bf16, the rounded one and what its rounding left for an fp32.
 template <bool SIG, class T>
@@ -244,9 +245,12 @@ struct Tiles {
 // has (a wave's loads return in order), so they arrive while that tile is joined and stored.  (Backward of 16384 x 4096
 // bf16: 208 us without, 185 with; the forward 113 and 111.)
 //
-// 16384 x 4096 bf16 (0.40 and 0.67 GB): forward 105 us, 3.8 TB/s, backward 179, 3.75, and 6 each to make the words
-// ready; fp32, 8192 rows (the same bytes): 81 and 130, 4.9 and 5.2.  What keeps bf16, of twice the values, from HBM's
-// rate: 26 and 46 vector instructions for each, and the joins.  16 sequences of 1024 rows, a block each: 90 and 162.
+// 16384 x 4096 bf16 (0.40 and 0.67 GB): forward 105 us, 3.8 TB/s, backward 179, 3.75, and 5 or 6 each for the launch that
+// makes the words ready; fp32, 8192 rows (the same bytes): 84 and 128, 4.8 and 5.2, and the same launch (with it, back to
+// back: 110 and 185, 90 and 137).  bf16 has twice the values of its bytes and reaches neither HBM's rate nor that of the
+// vector instructions (26 and 46 for each value, 40 % of the cycles): all waves of a block wait while one looks back, a
+// third of a tile's time, and a CU has two blocks to go on with in the forward and none in the backward.  16 sequences of
+// 1024 rows, a block each: 90 and 162.
 template <class TI, class TO, bool SIG, bool COUP, bool SPLIT>
 __global__ __launch_bounds__(kFwdWaves * 64, kPerSimd) void scan_fwd_k(ScanArgs s, int groups) {
     constexpr int R = kFwdRows;
@@ -575,6 +579,9 @@ Plan plan_of(const ScanArgs &s, bool back) {
     const int tile = back ? kBwdTile : kFwdTile;
     const size_t tiles = (s.n_pos + tile - 1) / tile, resident = (size_t)cu_count() * (kPerSimd * 4 / (back ? kBwdWaves : kFwdWaves));
     p.channels = p.lines * tiles * 64;
+    // The same number of blocks for every line: what is left of the resident ones has no work, and lines past half of them
+    // are a block's each.  4 x 4096 x 2560 bf16, of 160 lines, 72 and 160 us (3.5 and 2.6 TB/s), 5 x 4096 x 4096, of 320 lines and
+    // more than one round of blocks, 160 and 291 (3.1 and 2.9); of 256 lines, 4 x 4096 x 4096, 102 and 162 (4.0 and 4.1).
     p.sharing = (int)std::min(tiles, resident / p.lines);
     // Two tiles (forward: three) one after the other cost less than the launch that makes the words ready: 200 x 1024
     // bf16, forward and backward, 8.3 and 8.8 us in one block a line, 10.6 and 10.4 shared; 512 x 1024 mixed, of four tiles,
