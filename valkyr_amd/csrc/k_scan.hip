@@ -249,7 +249,7 @@ struct Tiles {
 // makes the words ready; fp32, 8192 rows (the same bytes): 84 and 128, 4.8 and 5.2, and the same launch (with it, back to
 // back: 110 and 185, 90 and 137).  bf16 has twice the values of its bytes and reaches neither HBM's rate nor that of the
 // vector instructions (26 and 46 for each value, 40 % of the cycles): all waves of a block wait while one looks back, a
-// third of a tile's time, and a CU has two blocks to go on with in the forward and none in the backward.  16 sequences of
+// third of a tile's time, and a CU has one other block to go on with in the forward and none in the backward.  16 sequences of
 // 1024 rows, a block each: 90 and 162.
 template <class TI, class TO, bool SIG, bool COUP, bool SPLIT>
 __global__ __launch_bounds__(kFwdWaves * 64, kPerSimd) void scan_fwd_k(ScanArgs s, int groups) {
